@@ -26,14 +26,18 @@ EXPORTS = ("hexkv_version", "hexkv_last_error", "hexkv_pack", "hexkv_unpack", "h
            "hexkv_attend_noalloc", "hexkv_attend_plan", "hexkv_attend_plan_chunk", "hexkv_attend_plan_kernel",
            "hexkv_device_status", "hexkv_device_xcds", "hexkv_add_rms_norm", "hexkv_rope_split", "hexkv_silu_mul", "hexkv_norm_linear", "hexkv_norm_rope_linear",
            "hexkv_attend_layers", "hexkv_attend_layers_workspace_bytes", "hexkv_attend_layers_independent",
-           "hexkv_attend_plan_layers")
+           "hexkv_attend_plan_layers", "hexkv_mx_store", "hexkv_mx_load", "hexkv_mx_quantize", "hexkv_mx_dequantize",
+           "hexkv_mx_attend", "hexkv_mx_attend_workspace_bytes", "hexkv_mx_linear", "hexkv_token_logprobs",
+           "hexkv_token_logprobs_workspace_bytes")
 NOALLOC_SCRATCH_BYTES = 32 << 20
 # Arrival counters at the front of every attention workspace (zero them once).
 ATTEND_COUNTER_BYTES = 256 << 10
 ATTEND_COUNTER_WORDS = ATTEND_COUNTER_BYTES // 8  # one 64-bit counter per (row, head group)
 # Device status flags (hexkv_device_status).
 STATUS_APPEND_SKIPPED, STATUS_LENGTH_CLAMPED, STATUS_PLACEMENT, STATUS_DISPATCH, STATUS_LIST = 1, 2, 4, 8, 16
-STATUS_ERRORS = STATUS_APPEND_SKIPPED | STATUS_LENGTH_CLAMPED | STATUS_PLACEMENT | STATUS_LIST
+STATUS_LOAD_SKIPPED = 32
+STATUS_ERRORS = STATUS_APPEND_SKIPPED | STATUS_LENGTH_CLAMPED | STATUS_PLACEMENT | STATUS_LIST | STATUS_LOAD_SKIPPED
+MAX_TOP = 64  # most alternatives of hexkv_token_logprobs
 
 
 class AttendParams(ctypes.Structure):
@@ -80,6 +84,21 @@ class FtAttendParams(ctypes.Structure):
         ("positions_dev", ctypes.c_void_p), ("position_bias", ctypes.c_int32), ("max_position", ctypes.c_int32),
         ("rotary_dim", ctypes.c_int), ("rotary_base", ctypes.c_float), ("rotary_neox", ctypes.c_int),
         ("partition", ctypes.c_int),
+    ]
+
+
+class MxAttendParams(ctypes.Structure):
+    """Mirror of ``hexkv_mx_attend_params``."""
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("batch", ctypes.c_int), ("q_len", ctypes.c_int), ("q_heads", ctypes.c_int),
+        ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("causal", ctypes.c_int),
+        ("softmax_scale", ctypes.c_float),
+        ("q", ctypes.c_void_p), ("q_batch_stride", ctypes.c_int64), ("q_row_stride", ctypes.c_int64),
+        ("cache", ctypes.c_void_p), ("cache_batch_bytes", ctypes.c_int64), ("cache_row_bytes", ctypes.c_int64),
+        ("capacity", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("out_batch_stride", ctypes.c_int64), ("out_row_stride", ctypes.c_int64),
+        ("seqlens_dev", ctypes.c_void_p), ("seqlen_bias", ctypes.c_int32), ("max_seqlen", ctypes.c_int32),
+        ("kv_new", ctypes.c_void_p), ("partition", ctypes.c_int),
     ]
 
 
@@ -184,6 +203,25 @@ def load() -> ctypes.CDLL:
     lib.hexkv_rope_split.argtypes = [vp, i64, vp, vp, ci, vp, vp, i64, ci, ci, ci, ci, ci, vp]
     lib.hexkv_silu_mul.restype = ci
     lib.hexkv_silu_mul.argtypes = [vp, vp, i64, ci, ci, vp]
+    for name, kv_first in (("hexkv_mx_store", True), ("hexkv_mx_load", False)):
+        fn = getattr(lib, name)
+        rows, cache = [vp, i64, i64, i64], [vp, i64, i64, i64]
+        fn.restype = ci
+        fn.argtypes = (rows + cache if kv_first else cache + rows) + [ci, ci, ci, ci, ci, vp, i32, vp]
+    lib.hexkv_mx_quantize.restype = ci
+    lib.hexkv_mx_quantize.argtypes = [vp, i64, vp, vp, i64, ci, ci, vp]
+    lib.hexkv_mx_dequantize.restype = ci
+    lib.hexkv_mx_dequantize.argtypes = [vp, vp, vp, i64, i64, ci, ci, vp]
+    lib.hexkv_mx_attend_workspace_bytes.restype = ctypes.c_size_t
+    lib.hexkv_mx_attend_workspace_bytes.argtypes = [ctypes.POINTER(MxAttendParams)]
+    lib.hexkv_mx_attend.restype = ci
+    lib.hexkv_mx_attend.argtypes = [ctypes.POINTER(MxAttendParams), vp, ctypes.c_size_t, vp]
+    lib.hexkv_mx_linear.restype = ci
+    lib.hexkv_mx_linear.argtypes = [vp, i64, vp, vp, vp, ci, ci, ci, ci, vp]
+    lib.hexkv_token_logprobs_workspace_bytes.restype = ctypes.c_size_t
+    lib.hexkv_token_logprobs_workspace_bytes.argtypes = [i64, ci, ci]
+    lib.hexkv_token_logprobs.restype = ci
+    lib.hexkv_token_logprobs.argtypes = [vp, i64, i64, ci, ci, vp, ci, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
     _lib = lib
     return lib
 

@@ -1,0 +1,624 @@
+// Attention over a 4-bit cache: hexkv_mx_attend.
+//
+// One wave takes up to 16 query rows that share a KV head (the heads of a
+// group, and several positions' where there are) over one partition of the
+// keys, 32 of them at a time:
+//   S^T = K Q^T    v_mfma_f32_16x16x32_bf16.  Lane (c, g) holds a quarter of
+//                  key c's elements, the query's operand the same quarter in
+//                  the same order, so a lane's vector of elements is its
+//                  operand as it stands: no exchange, no LDS.  The conversion
+//                  from 4 bits takes the power with it and is exact in bf16
+//                  for every power (fp16 would end at 2^15); the query enters
+//                  as one (bf16), two (fp16) or three (fp32) bf16 terms that
+//                  add up to it exactly.
+//   softmax        per lane (its query row), in the log2 domain; the running
+//                  maximum moves only when a score exceeds it by 2^kSlack.
+//   O^T += V^T P^T the scores' layout is the operand as it stands; V^T comes
+//                  from row-major LDS (bf16, written by the lanes that
+//                  converted it) by transposing reads.  Probabilities enter as two
+//                  bf16 terms (2^-16 of the largest; three for fp32), both
+//                  products in fp32.
+// A lane's accumulators belong to its own row, so rescaling and the final
+// division need no exchange.  Rows split over partitions leave (sum, maximum,
+// unscaled output) in the workspace and a second kernel joins them.
+//
+// A NaN block of V is taken out of the product (0 times NaN would reach rows
+// that do not attend it) and put into the outputs of the rows that do.
+#include "hexkv_mx.h"
+
+#include <algorithm>
+
+namespace hexkv {
+
+constexpr int kMxaThreads = 256;
+constexpr int kMxaWaves = kMxaThreads / 64;
+constexpr int kMxaRows = 16;  // query rows of a wave
+constexpr int kMxaKeys = 32;  // keys of one step
+constexpr float kMxaLowest = -1e30f;  // finite "minus infinity" of the running maximum
+constexpr float kMxaSlack = 8.f;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+struct MxAttendArgs {
+  const void *q;
+  int64_t q_bs, q_rs;  // elements
+  unsigned char *cache;
+  int64_t c_bs, c_ps;  // bytes
+  void *out;
+  int64_t o_bs, o_rs;  // elements
+  const int32_t *seqlens;
+  int32_t bias, max_seqlen, q_len, causal;
+  int32_t q_heads, kv_heads, group, tiles;  // tiles: row tiles of one (sequence, KV head)
+  int32_t part, max_parts;
+  int64_t units;  // (sequence, partition, row tile, KV head): one wave each
+  const void *kv_new;
+  float scale_log2;
+  float *ws_o, *ws_ml;
+  unsigned int *status;
+  bool q_vec;
+};
+
+// Terms whose sum is an element of T (query), and of a probability.
+template <typename T>
+struct MxTerms;
+template <>
+struct MxTerms<__bf16> { static constexpr int kQ = 1, kP = 2; };
+template <>
+struct MxTerms<_Float16> { static constexpr int kQ = 2, kP = 2; };
+template <>
+struct MxTerms<float> { static constexpr int kQ = 3, kP = 3; };
+
+__device__ __forceinline__ f32x4 mx_mma(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// The bf16 terms of (x0, x1), each the truncated rest of those before: 8 bits
+// of the significand a term, and never past the largest bf16.
+template <int N>
+__device__ __forceinline__ void mx_split(float x0, float x1, unsigned int *terms) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const unsigned int u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
+    terms[n] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);  // the upper halves
+    if (n + 1 < N) {
+      const float r0 = x0 - __uint_as_float(u0 & 0xffff0000u), r1 = x1 - __uint_as_float(u1 & 0xffff0000u);
+      x0 = r0 == r0 ? r0 : 0.f;  // an infinity is its first term alone
+      x1 = r1 == r1 ? r1 : 0.f;
+    }
+  }
+}
+
+// Orders this wave's LDS writes before its later reads of other lanes' data.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+template <int D>
+struct MxTile {
+  static constexpr int NW = D / 32, NB = D < 128 ? 1 : D / 128;
+  unsigned int k[2][NW], v[2][NW];
+  unsigned char kp[2][NB], vp[2][NB];
+};
+
+template <int NW>
+__device__ __forceinline__ void mx_read_words(const unsigned char *p, unsigned int *w) {
+  if constexpr (NW >= 4) {
+#pragma unroll
+    for (int i = 0; i < NW; i += 4) {
+      const u32x4 v = *reinterpret_cast<const u32x4 *>(p + 4 * i);
+      w[i] = v[0], w[i + 1] = v[1], w[i + 2] = v[2], w[i + 3] = v[3];
+    }
+  } else if constexpr (NW == 2) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const unsigned int *>(p);
+  }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kMxaThreads, 2) void mx_attend_kernel(const MxAttendArgs a) {
+  constexpr int NQ = MxTerms<T>::kQ, NP = MxTerms<T>::kP;
+  constexpr int NW = MxTile<D>::NW;  // words of elements a lane holds of a key, = products of a score
+  constexpr int NB = MxTile<D>::NB;  // blocks they lie in
+  constexpr int ND = D / 16;         // output tiles
+  constexpr int VP = 2 * D + 32;     // LDS bytes per V row: a transposed read's four rows over all banks
+  constexpr int NEW = 2 * (D / 8) + 2 * (D / 32);
+  __shared__ __attribute__((aligned(16))) char s_v[kMxaWaves][kMxaKeys * VP];
+  __shared__ unsigned int s_new[kMxaWaves][NEW];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  int64_t unit = static_cast<int64_t>(blockIdx.x) * kMxaWaves + wave;
+  if (unit >= a.units) return;
+  const unsigned u = static_cast<unsigned>(unit);
+  const int h = static_cast<int>(u % static_cast<unsigned>(a.kv_heads));
+  unsigned rest = u / static_cast<unsigned>(a.kv_heads);
+  const int tile = static_cast<int>(rest % static_cast<unsigned>(a.tiles));
+  rest /= static_cast<unsigned>(a.tiles);
+  const int part = static_cast<int>(rest % static_cast<unsigned>(a.max_parts));
+  const int64_t b = rest / static_cast<unsigned>(a.max_parts);
+
+  // Lengths: `base` keys as asked for, no more than max_seqlen of them.
+  int64_t want = static_cast<int64_t>(a.bias) + (a.kv_new ? 1 : 0);
+  if (a.seqlens) want += a.seqlens[b];
+  const int len = static_cast<int>(want < 0 ? 0 : want > a.max_seqlen ? a.max_seqlen : want);
+  if (want > a.max_seqlen && lane == 0 && h == 0 && tile == 0 && part == 0)
+    raise_status(a.status, HEXKV_STATUS_LENGTH_CLAMPED);
+  const int fresh = a.kv_new && want > 0 && want <= a.max_seqlen ? len - 1 : -1;  // the new row's position
+  const int nparts = len > 0 ? (len + a.part - 1) / a.part : 1;
+  if (part >= nparts) return;
+  const int p0 = part * a.part, p1 = min(len, p0 + a.part);
+
+  // This lane's query row, and the tile's first and last.
+  const int rows = a.q_len * a.group;
+  const int row = tile * kMxaRows + c;
+  const bool live = row < rows;
+  const int t = live ? row / a.group : 0, qh = h * a.group + (live ? row - t * a.group : 0);
+  const auto keys_of = [&](int tt) {
+    const int64_t n = a.causal ? want - a.q_len + tt + 1 : want;
+    return static_cast<int>(n < 0 ? 0 : n > a.max_seqlen ? a.max_seqlen : n);
+  };
+  const int lim = keys_of(t);
+  const int first_lim = keys_of(tile * kMxaRows / a.group);
+  const int end = min(p1, keys_of((min(rows, (tile + 1) * kMxaRows) - 1) / a.group));
+
+  const unsigned char *seq = a.cache + b * a.c_bs + static_cast<int64_t>(p0) * a.c_ps;
+  const int blk = NB > 1 ? g * NB : g * D / 128;  // the lane's first block within a head
+  const unsigned char *k_base = seq + h * (D / 2);
+  const unsigned char *v_base = k_base + static_cast<int64_t>(a.kv_heads) * (D / 2);
+  const unsigned char *kp_base = seq + static_cast<int64_t>(a.kv_heads) * D + h * (D / 32);
+  const unsigned char *vp_base = kp_base + a.kv_heads * (D / 32);
+  const unsigned int pitch = static_cast<unsigned int>(a.c_ps);
+
+  // The new row: converted once by this wave, written to the cache, and put
+  // in place of what the tile that holds its position has loaded.
+  const bool holds_new = fresh >= p0 && fresh < p1;
+  if (holds_new) {
+    const int half = lane / (D / 8), at = lane % (D / 8);
+    if (half < 2) {
+      float f[8];
+      mx_read8(static_cast<const T *>(a.kv_new) + ((b * 2 + half) * a.kv_heads + h) * D + at * 8, true, f);
+      const unsigned int byte = mx_power(mx_block_bits(mx_bits(f))), w = mx_encode(f, byte);
+      unsigned char *dst = a.cache + b * a.c_bs + static_cast<int64_t>(fresh) * a.c_ps;
+      const int64_t head = static_cast<int64_t>(half) * a.kv_heads + h;
+      *reinterpret_cast<unsigned int *>(dst + head * (D / 2) + at * 4) = w;
+      s_new[wave][half * (D / 8) + at] = w;
+      if (at % 4 == 0) {
+        dst[static_cast<int64_t>(a.kv_heads) * D + head * (D / 32) + at / 4] = static_cast<unsigned char>(byte);
+        s_new[wave][2 * (D / 8) + half * (D / 32) + at / 4] = byte;
+      }
+    }
+    wave_lds_fence();
+  }
+
+  u32x4 q[NQ][NW];
+#pragma unroll
+  for (int j = 0; j < NW; ++j) {
+    float f[8] = {};
+    if (live)
+      mx_read8(static_cast<const T *>(a.q) + b * a.q_bs + t * a.q_rs + static_cast<int64_t>(qh) * D + g * (D / 4) + 8 * j,
+               a.q_vec, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      unsigned int terms[NQ];
+      mx_split<NQ>(f[2 * i], f[2 * i + 1], terms);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) q[n][j][i] = terms[n];
+    }
+  }
+
+  float m = kMxaLowest, l = 0.f;
+  f32x4 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acc[d] = f32x4{};
+  unsigned int nan_blocks = 0;
+
+  const auto fetch = [&](int k0, MxTile<D> &x) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const unsigned int at = static_cast<unsigned int>(min(k0 + s * 16 + c, end - 1) - p0) * pitch;
+      mx_read_words<NW>(k_base + (at + g * (D / 8)), x.k[s]);
+      mx_read_words<NW>(v_base + (at + g * (D / 8)), x.v[s]);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        x.kp[s][n] = kp_base[at + blk + n];
+        x.vp[s][n] = vp_base[at + blk + n];
+      }
+    }
+  };
+
+  const auto compute = [&](int k0, MxTile<D> &x) {
+    const bool whole = k0 + kMxaKeys <= end;
+    if (holds_new && fresh >= k0 && fresh < k0 + kMxaKeys) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (k0 + s * 16 + c == fresh) {
+#pragma unroll
+          for (int i = 0; i < NW; ++i) {
+            x.k[s][i] = s_new[wave][g * NW + i];
+            x.v[s][i] = s_new[wave][D / 8 + g * NW + i];
+          }
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            x.kp[s][n] = static_cast<unsigned char>(s_new[wave][2 * (D / 8) + blk + n]);
+            x.vp[s][n] = static_cast<unsigned char>(s_new[wave][2 * (D / 8) + D / 32 + blk + n]);
+          }
+        }
+    }
+    if (!whole) {  // keys past the end repeat the last one: their values are zero, their scores masked
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (k0 + s * 16 + c >= end) {
+#pragma unroll
+          for (int i = 0; i < NW; ++i) x.v[s][i] = 0;
+#pragma unroll
+          for (int n = 0; n < NB; ++n) x.vp[s][n] = 127;
+        }
+    }
+    bool bad = false;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) bad |= x.vp[s][n] == 255;
+    if (__ballot(bad)) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        unsigned int bits = 0;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+          if (x.vp[s][n] == 255) {
+            bits |= 1u << (blk + n);
+            x.vp[s][n] = 127;
+#pragma unroll
+            for (int i = 0; i < NW / NB; ++i) x.v[s][n * (NW / NB) + i] = 0;
+          }
+        uint64_t from = __ballot(bits != 0);
+        while (from) {
+          const int r = __builtin_ctzll(from);
+          from &= from - 1;
+          const unsigned int theirs = __shfl(bits, r);
+          if (k0 + s * 16 + (r & 15) < lim) nan_blocks |= theirs;
+        }
+      }
+    }
+
+    // V into LDS, as the transposed reads want it
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < NW; ++i)
+        *reinterpret_cast<u32x4 *>(&s_v[wave][(s * 16 + c) * VP + g * (D / 2) + i * 16]) =
+            mx_bf16(x.v[s][i], mx_scale(x.vp[s][i * NB / NW]));
+
+    f32x4 sc[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      sc[s] = f32x4{};
+#pragma unroll
+      for (int j = 0; j < NW; ++j) {
+        const u32x4 k = mx_bf16(x.k[s][j], mx_scale(x.kp[s][j * NB / NW]));
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) sc[s] = mx_mma(k, q[n][j], sc[s]);
+      }
+    }
+    float top = -INFINITY;
+    const bool open = k0 + kMxaKeys <= first_lim && whole;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sc[s][i] *= a.scale_log2;
+        if (!open && k0 + s * 16 + 4 * g + i >= min(lim, end)) sc[s][i] = -INFINITY;
+        top = fmaxf(top, sc[s][i]);
+      }
+    top = max_from<16>(top);
+    if (__ballot(top > m + kMxaSlack)) {
+      const float moved = top > m + kMxaSlack ? top : m;
+      const float by = __builtin_amdgcn_exp2f(m - moved);
+      m = moved;
+      l *= by;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) acc[d] *= by;
+    }
+    u32x4 p[NP];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const float e0 = __builtin_amdgcn_exp2f(sc[s][i] - m), e1 = __builtin_amdgcn_exp2f(sc[s][i + 1] - m);
+        l += e0 + e1;
+        unsigned int terms[NP];
+        mx_split<NP>(e0, e1, terms);
+#pragma unroll
+        for (int n = 0; n < NP; ++n) p[n][s * 2 + i / 2] = terms[n];
+      }
+    wave_lds_fence();
+    const auto *shared = (const __attribute__((address_space(3))) char *)&s_v[wave][0];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const int at = (4 * g + c / 4) * VP + (c % 4) * 8 + d * 32;
+      const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(shared + at));
+      const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(shared + at + 16 * VP));
+      const u32x4 v = __builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+      for (int n = 0; n < NP; ++n) acc[d] = mx_mma(v, p[n], acc[d]);
+    }
+    wave_lds_fence();
+  };
+
+  if (end > p0) {
+    MxTile<D> x;
+    for (int k0 = p0; k0 < end; k0 += kMxaKeys) {
+      fetch(k0, x);
+      compute(k0, x);
+    }
+  }
+
+  l = sum_from<16>(l);
+  nan_blocks |= __shfl_xor(nan_blocks, 16);
+  nan_blocks |= __shfl_xor(nan_blocks, 32);
+  if (!live) return;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+    if (nan_blocks >> (d / 2) & 1) acc[d] = f32x4{} + NAN;
+  if (nparts == 1) {
+    // A row without keys is zero; one whose scores are all minus infinity has
+    // no softmax (0 / 0).
+    const float inv = 1.f / l;
+    T *out = static_cast<T *>(a.out) + b * a.o_bs + t * a.o_rs + static_cast<int64_t>(qh) * D + 4 * g;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) store4(out + d * 16, lim > 0 ? acc[d] * inv : f32x4{});
+  } else {
+    const int64_t slot = ((b * a.q_len + t) * a.q_heads + qh) * a.max_parts + part;
+    float *o = a.ws_o + slot * D + 4 * g;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4 *>(o + d * 16) = acc[d];
+    if (g == 0) *reinterpret_cast<float2 *>(a.ws_ml + slot * 2) = float2{m, l};
+  }
+}
+
+// Joins a row's partitions: one wave per (sequence, position, query head).
+template <typename T, int D>
+__global__ __launch_bounds__(kMxaThreads) void mx_join_kernel(const MxAttendArgs a, int64_t heads_rows) {
+  constexpr int E = D < 64 ? 1 : D / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * kMxaWaves + (threadIdx.x >> 6);
+  if (r >= heads_rows) return;
+  const unsigned qh = static_cast<unsigned>(r) % static_cast<unsigned>(a.q_heads);
+  const unsigned bt = static_cast<unsigned>(r) / static_cast<unsigned>(a.q_heads);
+  const int t = static_cast<int>(bt % static_cast<unsigned>(a.q_len));
+  const int64_t b = bt / static_cast<unsigned>(a.q_len);
+  int64_t want = static_cast<int64_t>(a.bias) + (a.kv_new ? 1 : 0);
+  if (a.seqlens) want += a.seqlens[b];
+  const int len = static_cast<int>(want < 0 ? 0 : want > a.max_seqlen ? a.max_seqlen : want);
+  const int nparts = len > 0 ? (len + a.part - 1) / a.part : 1;
+  if (nparts == 1) return;  // written by the attention kernel
+  const bool empty = a.causal && want - a.q_len + t + 1 <= 0;
+  const float *ml = a.ws_ml + r * a.max_parts * 2, *o = a.ws_o + r * a.max_parts * D + lane * E;
+  float m = kMxaLowest;
+  for (int p = lane; p < nparts; p += 64) m = fmaxf(m, ml[2 * p]);
+  m = wave_max(m);
+  float l = 0.f, sum[E] = {};
+  if (lane * E < D) {
+    for (int p = 0; p < nparts; ++p) {
+      const float w = __builtin_amdgcn_exp2f(ml[2 * p] - m);
+      l = fmaf(w, ml[2 * p + 1], l);
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum[e] = fmaf(w, o[static_cast<int64_t>(p) * D + e], sum[e]);
+    }
+    T *out = static_cast<T *>(a.out) + b * a.o_bs + t * a.o_rs + static_cast<int64_t>(qh) * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[e] = Elem<T>::from_float(empty ? 0.f : sum[e] / l);
+  }
+}
+
+static int elem_bytes(int dtype) { return dtype == HEXKV_F32 ? 4 : 2; }
+
+static int mx_validate(const hexkv_mx_attend_params *p, const char *what) {
+  if (!p) return fail(HEXKV_EINVAL, "%s: null params", what);
+  if (p->dtype != HEXKV_F16 && p->dtype != HEXKV_BF16 && p->dtype != HEXKV_F32)
+    return fail(HEXKV_EINVAL, "%s: unknown dtype %d", what, p->dtype);
+  if (p->batch < 0 || p->q_len < 1 || p->q_heads < 1 || p->kv_heads < 1)
+    return fail(HEXKV_EINVAL, "%s: bad batch/q_len/heads", what);
+  if (p->q_heads % p->kv_heads)
+    return fail(HEXKV_EINVAL, "%s: q_heads %d not a multiple of kv_heads %d", what, p->q_heads, p->kv_heads);
+  if (p->q_heads > 65536) return fail(HEXKV_EINVAL, "%s: over 65536 heads", what);
+  if (p->head_dim != 32 && p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
+    return fail(HEXKV_EUNSUPPORTED, "%s: head_dim %d (compiled: 32, 64, 128, 256)", what, p->head_dim);
+  if (p->kv_new && p->q_len != 1) return fail(HEXKV_EINVAL, "%s: fused append needs q_len 1", what);
+  if (p->max_seqlen < 0 || p->max_seqlen > p->capacity)
+    return fail(HEXKV_ERANGE, "%s: max_seqlen %d outside [0, capacity %lld]", what, p->max_seqlen,
+                static_cast<long long>(p->capacity));
+  if (p->partition < 0 || p->partition % kMxaKeys || p->partition > 65536)
+    return fail(HEXKV_EINVAL, "%s: partition must be 0 or a multiple of %d up to 65536", what, kMxaKeys);
+  if (!(p->softmax_scale > 0.f) || p->softmax_scale > 3.0e38f)
+    return fail(HEXKV_EINVAL, "%s: softmax_scale must be positive and finite", what);
+  if (static_cast<int64_t>(p->q_len) * (p->q_heads / p->kv_heads) >= INT64_C(1) << 30 ||
+      static_cast<int64_t>(p->batch) * p->q_len * p->q_heads >= INT64_C(1) << 31)
+    return fail(HEXKV_ERANGE, "%s: 2^31 query rows or more", what);
+  if (p->cache_row_bytes < mx_row_bytes(p->kv_heads, p->head_dim) || p->cache_row_bytes % 16 ||
+      p->cache_batch_bytes % 16 || p->cache_row_bytes > (INT64_C(1) << 24) ||
+      (p->batch > 1 && p->cache_batch_bytes < p->capacity * p->cache_row_bytes))
+    return fail(HEXKV_EINVAL, "%s: cache rows must be multiples of 16 bytes, at least %lld apart (at most 2^24), and "
+                              "sequences capacity rows apart", what,
+                static_cast<long long>(mx_row_bytes(p->kv_heads, p->head_dim)));
+  return HEXKV_OK;
+}
+
+static int64_t row_tiles(const hexkv_mx_attend_params *p) {
+  return (static_cast<int64_t>(p->q_len) * (p->q_heads / p->kv_heads) + kMxaRows - 1) / kMxaRows;
+}
+
+// Positions per partition.  About 12 waves a CU, at least 64 positions each.
+static int mx_partition(const hexkv_mx_attend_params *p) {
+  int64_t part = p->partition;
+  if (!part) {
+    const int64_t units = std::max<int64_t>(1, static_cast<int64_t>(p->batch) * p->kv_heads * row_tiles(p));
+    const int64_t parts = std::min<int64_t>(256, std::max<int64_t>(1, 3072 / units));
+    part = std::max<int64_t>(64, (p->max_seqlen + parts - 1) / parts);
+  }
+  part = std::min<int64_t>((part + kMxaKeys - 1) / kMxaKeys * kMxaKeys, 65536);
+  // a partition's rows are addressed with 32-bit offsets
+  while (part > kMxaKeys && part * p->cache_row_bytes >= INT64_C(1) << 31) part = part / 2 / kMxaKeys * kMxaKeys;
+  return static_cast<int>(part);
+}
+
+static int64_t mx_parts(const hexkv_mx_attend_params *p, int part) {
+  return std::max<int64_t>(1, (static_cast<int64_t>(p->max_seqlen) + part - 1) / part);
+}
+
+static size_t mx_join_bytes(const hexkv_mx_attend_params *p) {
+  const int64_t parts = mx_parts(p, mx_partition(p));
+  if (parts == 1) return 0;
+  return static_cast<size_t>(p->batch) * p->q_len * p->q_heads * parts * (p->head_dim + 2) * sizeof(float);
+}
+
+// Many query rows (a prompt's chunk): the rows' keys and values are taken out
+// of the cache once and attended by hexkv_attend's query tiles, where those
+// are compiled.  Below kFewTiles row tiles the keys are read in four bits.
+constexpr int64_t kFewTiles = 4;
+static bool mx_unpacks(const hexkv_mx_attend_params *p) {
+  const int vec = 16 / elem_bytes(p->dtype);
+  return p->dtype != HEXKV_F32 && (p->head_dim == 64 || p->head_dim == 128) && p->q_len > 1 && p->partition == 0 &&
+         row_tiles(p) > kFewTiles && static_cast<int64_t>(p->batch) * p->q_len <= 65535 && p->max_seqlen > 0 &&
+         aligned16(p->q) && p->q_batch_stride % vec == 0 && p->q_row_stride % vec == 0 &&
+         static_cast<int64_t>(p->max_seqlen) * 2 * p->kv_heads * p->head_dim * 2 < INT64_C(0xffff0000);
+}
+
+static hexkv_attend_params mx_unpacked(const hexkv_mx_attend_params *p, void *kv) {
+  const int64_t row = static_cast<int64_t>(p->kv_heads) * p->head_dim;
+  hexkv_attend_params t = {};
+  t.dtype = p->dtype;
+  t.batch = p->batch;
+  t.q_len = p->q_len;
+  t.q_heads = p->q_heads;
+  t.kv_heads = p->kv_heads;
+  t.head_dim = p->head_dim;
+  t.causal = p->causal;
+  t.softmax_scale = p->softmax_scale;
+  t.q = p->q;
+  t.q_batch_stride = p->q_batch_stride;
+  t.q_row_stride = p->q_row_stride;
+  t.cache = kv;
+  t.cache_batch_stride = 2 * row * p->max_seqlen;
+  t.cache_pos_stride = 2 * row;
+  t.cache_kv_stride = row;
+  t.capacity = p->max_seqlen;
+  t.out = p->out;
+  t.out_batch_stride = p->out_batch_stride;
+  t.out_row_stride = p->out_row_stride;
+  t.seqlens_dev = p->seqlens_dev;
+  t.seqlen_bias = p->seqlen_bias;
+  t.max_seqlen = p->max_seqlen;
+  return t;
+}
+
+static size_t mx_unpacked_bytes(const hexkv_mx_attend_params *p) {
+  const size_t n = static_cast<size_t>(p->batch) * p->max_seqlen * 2 * p->kv_heads * p->head_dim * elem_bytes(p->dtype);
+  return (n + 255) / 256 * 256;
+}
+
+static size_t mx_workspace(const hexkv_mx_attend_params *p) {
+  if (!mx_unpacks(p)) return mx_join_bytes(p);
+  const hexkv_attend_params t = mx_unpacked(p, nullptr);
+  return mx_unpacked_bytes(p) + hexkv_attend_workspace_bytes(&t);
+}
+
+template <typename T, int D>
+static void mx_launch(const MxAttendArgs &a, int64_t rows, hipStream_t s) {
+  mx_attend_kernel<T, D><<<static_cast<unsigned>((a.units + kMxaWaves - 1) / kMxaWaves), kMxaThreads, 0, s>>>(a);
+  if (a.max_parts > 1)
+    mx_join_kernel<T, D><<<static_cast<unsigned>((rows + kMxaWaves - 1) / kMxaWaves), kMxaThreads, 0, s>>>(a, rows);
+}
+
+template <typename T>
+static void mx_launch_dim(const MxAttendArgs &a, int head_dim, int64_t rows, hipStream_t s) {
+  switch (head_dim) {
+    case 32: return mx_launch<T, 32>(a, rows, s);
+    case 64: return mx_launch<T, 64>(a, rows, s);
+    case 128: return mx_launch<T, 128>(a, rows, s);
+    default: return mx_launch<T, 256>(a, rows, s);
+  }
+}
+
+}  // namespace hexkv
+
+extern "C" size_t hexkv_mx_attend_workspace_bytes(const hexkv_mx_attend_params *p) {
+  using namespace hexkv;
+  clear_error();
+  return mx_validate(p, "hexkv_mx_attend_workspace_bytes") == HEXKV_OK && p->batch ? mx_workspace(p) : 0;
+}
+
+extern "C" int hexkv_mx_attend(const hexkv_mx_attend_params *p, void *workspace, size_t workspace_bytes,
+                               hexkv_stream_t stream) {
+  using namespace hexkv;
+  const char *what = "hexkv_mx_attend";
+  clear_error();
+  int rc = mx_validate(p, what);
+  if (rc != HEXKV_OK) return rc;
+  if (p->batch == 0) return HEXKV_OK;
+  if (!p->q || !p->cache || !p->out) return fail(HEXKV_EINVAL, "%s: null tensor", what);
+  const int elem = elem_bytes(p->dtype);
+  if (!aligned16(p->cache) || (p->kv_new && !aligned16(p->kv_new)))
+    return fail(HEXKV_EINVAL, "%s: cache/kv_new must be 16-byte aligned", what);
+  if ((reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->out)) & (elem - 1))
+    return fail(HEXKV_EINVAL, "%s: q/out misaligned", what);
+  const size_t need = mx_workspace(p);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(HEXKV_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace ? workspace_bytes : 0, need);
+  if (need && !aligned16(workspace)) return fail(HEXKV_EINVAL, "%s: workspace must be 16-byte aligned", what);
+
+  if (mx_unpacks(p)) {
+    const int64_t row = static_cast<int64_t>(p->kv_heads) * p->head_dim;
+    rc = hexkv_mx_load(p->cache, p->cache_batch_bytes, p->cache_row_bytes, p->capacity, workspace,
+                       2 * row * p->max_seqlen, 2 * row, row, p->batch, p->max_seqlen, p->kv_heads, p->head_dim, p->dtype,
+                       nullptr, 0, stream);
+    if (rc != HEXKV_OK) return rc;
+    const hexkv_attend_params t = mx_unpacked(p, workspace);
+    const size_t kv = mx_unpacked_bytes(p);
+    return hexkv_attend(&t, static_cast<char *>(workspace) + kv, workspace_bytes - kv, stream);
+  }
+
+  MxAttendArgs a = {};
+  a.q = p->q;
+  a.q_bs = p->q_batch_stride;
+  a.q_rs = p->q_row_stride;
+  a.cache = static_cast<unsigned char *>(p->cache);
+  a.c_bs = p->cache_batch_bytes;
+  a.c_ps = p->cache_row_bytes;
+  a.out = p->out;
+  a.o_bs = p->out_batch_stride;
+  a.o_rs = p->out_row_stride;
+  a.seqlens = p->seqlens_dev;
+  a.bias = p->seqlen_bias;
+  a.max_seqlen = p->max_seqlen;
+  a.q_len = p->q_len;
+  a.causal = p->causal && p->q_len > 1;
+  a.q_heads = p->q_heads;
+  a.kv_heads = p->kv_heads;
+  a.group = p->q_heads / p->kv_heads;
+  a.tiles = static_cast<int32_t>(row_tiles(p));
+  a.part = mx_partition(p);
+  a.max_parts = static_cast<int32_t>(mx_parts(p, a.part));
+  a.units = static_cast<int64_t>(p->batch) * a.max_parts * a.tiles * p->kv_heads;
+  if (a.units >= INT64_C(1) << 26) return fail(HEXKV_ERANGE, "%s: 2^24 workgroups or more; split the call", what);
+  a.kv_new = p->kv_new;
+  a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
+  const int64_t rows = static_cast<int64_t>(p->batch) * p->q_len * p->q_heads;
+  if (a.max_parts > 1) {
+    a.ws_o = static_cast<float *>(workspace);
+    a.ws_ml = a.ws_o + rows * a.max_parts * p->head_dim;
+  }
+  const int vec = 16 / elem;
+  a.q_vec = aligned16(p->q) && p->q_batch_stride % vec == 0 && p->q_row_stride % vec == 0;
+  rc = status_word(stream, &a.status, what);
+  if (rc != HEXKV_OK) return rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (p->dtype == HEXKV_BF16) mx_launch_dim<__bf16>(a, p->head_dim, rows, s);
+  else if (p->dtype == HEXKV_F16) mx_launch_dim<_Float16>(a, p->head_dim, rows, s);
+  else mx_launch_dim<float>(a, p->head_dim, rows, s);
+  return check_launch(what);
+}

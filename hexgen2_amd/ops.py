@@ -66,6 +66,8 @@ _STATUS_TEXT = {
                            "single-launch merge may have read stale partials",
     _lib.STATUS_LIST: "a work list planned for another attention kernel (another head-group size) was "
                       "launched, and its items were skipped",
+    _lib.STATUS_LOAD_SKIPPED: "a position read from device memory to load from a 4-bit cache fell outside it, so "
+                              "that row came back as zeros",
 }
 
 

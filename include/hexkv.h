@@ -103,6 +103,7 @@ const char *hexkv_last_error(void);
                                           planned for) */
 #define HEXKV_STATUS_LIST 16u          /* hexkv_attend: a work item planned for another head-group size (another
                                           kernel) was skipped, so its outputs were not written */
+#define HEXKV_STATUS_LOAD_SKIPPED 32u  /* hexkv_mx_load: a position outside [0, capacity); that row came back as zeros */
 
 /*
  * Waits for `stream`, then reads the status word of the stream's device into
@@ -657,6 +658,108 @@ int hexkv_rope_split(const void *qkv, int64_t qkv_stride, const float *inv_freq_
 /* out[r][i] = silu(gate_up[r][i]) * gate_up[r][width + i] (mlp.py:63-87).
  * One row's out may be either half of gate_up. */
 int hexkv_silu_mul(const void *gate_up, void *out, int64_t rows, int width, int dtype, hexkv_stream_t stream);
+
+/* ------------------------------------------------------ four-bit blocks ---
+ * Matrices and caches in blocks of 32 consecutive elements that share a power
+ * of two (the OCP microscaling format MXFP4, 4.25 bits an element): byte b is
+ * 2^(b - 127), 255 makes the block NaN; an element is a sign, two exponent bits
+ * and one fraction bit, 0, 0.5, 1, 1.5, 2, 3, 4 or 6 times the power, the
+ * earlier element in a byte's lower half.  What these calls write has
+ * the smallest power in [2^-125, 2^126] that leaves no element above 6, each
+ * element rounded to nearest (halfway: to the even code); a block that holds
+ * an infinity or a NaN becomes NaN.
+ *
+ * A 4-bit cache is one layer's [batch][capacity][row], a row one position's
+ * [2][kv_heads][head_dim / 2] bytes of elements, then their
+ * [2][kv_heads][head_dim / 32] powers, padded to a multiple of 16 bytes; rows
+ * and sequences lie cache_row_bytes and cache_batch_bytes apart (multiples of
+ * 16, the base 16-byte aligned).  hexkv_pack and hexkv_unpack move such rows as
+ * they are.  No counterpart in the reference, which holds weights and caches
+ * in the data type. */
+
+/* Rows kv [batch][seqlen][2][kv_heads][head_dim] (strides in elements, heads and
+ * head_dim contiguous, kv_stride from K to V) into cache positions
+ *   (positions_dev ? positions_dev[b] : 0) + position_bias + [0, seqlen),
+ * and back.  head_dim: a multiple of 32.  Positions from positions_dev outside
+ * [0, capacity) are skipped and raise HEXKV_STATUS_APPEND_SKIPPED (store), or
+ * come back as zeros and raise HEXKV_STATUS_LOAD_SKIPPED (load). */
+int hexkv_mx_store(const void *kv, int64_t kv_batch_stride, int64_t kv_pos_stride, int64_t kv_stride, void *cache,
+                   int64_t cache_batch_bytes, int64_t cache_row_bytes, int64_t capacity, int batch, int seqlen,
+                   int kv_heads, int head_dim, int dtype, const int32_t *positions_dev, int32_t position_bias,
+                   hexkv_stream_t stream);
+int hexkv_mx_load(const void *cache, int64_t cache_batch_bytes, int64_t cache_row_bytes, int64_t capacity, void *kv,
+                  int64_t kv_batch_stride, int64_t kv_pos_stride, int64_t kv_stride, int batch, int seqlen,
+                  int kv_heads, int head_dim, int dtype, const int32_t *positions_dev, int32_t position_bias,
+                  hexkv_stream_t stream);
+
+/* A matrix's rows [rows][width] (width a multiple of 32, rows x_stride
+ * elements apart) into contiguous elements [rows][width / 2] and powers
+ * [rows][width / 32], and back. */
+int hexkv_mx_quantize(const void *x, int64_t x_stride, void *codes, void *powers, int64_t rows, int width, int dtype,
+                      hexkv_stream_t stream);
+int hexkv_mx_dequantize(const void *codes, const void *powers, void *out, int64_t out_stride, int64_t rows, int width,
+                        int dtype, hexkv_stream_t stream);
+
+/* hexkv_attend over a 4-bit cache: the same rows, lengths, causal rule and
+ * fused append (kv_new is stored as hexkv_mx_store does and attended as
+ * stored).  q and out as there, at any element strides with heads contiguous.
+ * A call of many query rows first takes the cache's [0, max_seqlen) positions
+ * out into the workspace. */
+typedef struct hexkv_mx_attend_params {
+  int dtype;      /* enum hexkv_dtype of q, kv_new and out */
+  int batch;
+  int q_len;
+  int q_heads;
+  int kv_heads;   /* divides q_heads */
+  int head_dim;   /* 32, 64, 128 or 256 */
+  int causal;     /* q_len > 1 only: query t sees keys < len - q_len + t + 1 */
+  float softmax_scale;
+  const void *q;
+  int64_t q_batch_stride, q_row_stride;
+  void *cache;
+  int64_t cache_batch_bytes, cache_row_bytes;
+  int64_t capacity;
+  void *out;
+  int64_t out_batch_stride, out_row_stride;
+  const int32_t *seqlens_dev; /* lengths as in hexkv_attend_params */
+  int32_t seqlen_bias;
+  int32_t max_seqlen;
+  const void *kv_new; /* q_len 1 only: [batch][2][kv_heads][head_dim] contiguous, or NULL */
+  int partition;      /* positions per partition, a multiple of 32; 0: the library's choice */
+} hexkv_mx_attend_params;
+
+/* Scratch for these parameters; it need not be zeroed.  Calls sharing one
+ * workspace must not overlap. */
+size_t hexkv_mx_attend_workspace_bytes(const hexkv_mx_attend_params *p);
+int hexkv_mx_attend(const hexkv_mx_attend_params *p, void *workspace, size_t workspace_bytes, hexkv_stream_t stream);
+
+/* out [rows][n] = x W^T for W [n][k] in four-bit blocks (codes [n][k / 2],
+ * 16-byte aligned, powers [n][k / 32], contiguous; k a multiple of 32), x rows
+ * x_stride elements apart, out contiguous; sums in fp32, rounded once. */
+int hexkv_mx_linear(const void *x, int64_t x_stride, const void *codes, const void *powers, void *out, int rows, int n,
+                    int k, int dtype, hexkv_stream_t stream);
+
+/* ---------------------------------------------------------------- scoring ---
+ * What a step's logits say of its tokens (the reference reads no more than
+ * their argmax, hexgen2/model.py:79). */
+
+/* Largest `top` of hexkv_token_logprobs. */
+#define HEXKV_MAX_TOP 64
+
+/* Of each row of logits [rows][vocab] (row_stride elements apart):
+ *   logprob[r]   log softmax(logits[r])[tokens_dev[r]] (tokens_dev NULL: not
+ *                wanted); 0 for a negative token (padding), NaN for one that is
+ *                vocab or more
+ *   entropy[r]   - sum p log p (entropy NULL: not wanted)
+ *   top_ids, top_logprobs [rows][top]   the largest logits' ids and
+ *                log-probabilities from the largest down, ties by lowest id
+ * in fp32.  A logit of minus infinity has probability 0; a row of nothing else
+ * gives -inf log-probabilities and entropy 0; a NaN or plus infinity makes its
+ * row's NaN (NaN sorts as the largest). */
+size_t hexkv_token_logprobs_workspace_bytes(int64_t rows, int vocab, int top);
+int hexkv_token_logprobs(const void *logits, int64_t row_stride, int64_t rows, int vocab, int dtype,
+                         const int64_t *tokens_dev, int top, float *logprob, float *entropy, float *top_logprobs,
+                         int64_t *top_ids, void *workspace, size_t workspace_bytes, hexkv_stream_t stream);
 
 #ifdef __cplusplus
 }
