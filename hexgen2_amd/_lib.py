@@ -27,7 +27,8 @@ EXPORTS = ("hexkv_version", "hexkv_last_error", "hexkv_pack", "hexkv_unpack", "h
            "hexkv_device_status", "hexkv_device_xcds", "hexkv_add_rms_norm", "hexkv_rope_split", "hexkv_silu_mul", "hexkv_norm_linear", "hexkv_norm_rope_linear",
            "hexkv_attend_layers", "hexkv_attend_layers_workspace_bytes", "hexkv_attend_layers_independent",
            "hexkv_attend_plan_layers", "hexkv_mx_store", "hexkv_mx_load", "hexkv_mx_quantize", "hexkv_mx_dequantize",
-           "hexkv_mx_attend", "hexkv_mx_attend_workspace_bytes", "hexkv_mx_linear", "hexkv_token_logprobs",
+           "hexkv_mx_attend", "hexkv_mx_attend_workspace_bytes", "hexkv_mx_linear",
+           "hexkv_mx_linear_workspace_bytes", "hexkv_token_logprobs",
            "hexkv_token_logprobs_workspace_bytes")
 NOALLOC_SCRATCH_BYTES = 32 << 20
 # Arrival counters at the front of every attention workspace (zero them once).
@@ -217,7 +218,9 @@ def load() -> ctypes.CDLL:
     lib.hexkv_mx_attend.restype = ci
     lib.hexkv_mx_attend.argtypes = [ctypes.POINTER(MxAttendParams), vp, ctypes.c_size_t, vp]
     lib.hexkv_mx_linear.restype = ci
-    lib.hexkv_mx_linear.argtypes = [vp, i64, vp, vp, vp, ci, ci, ci, ci, vp]
+    lib.hexkv_mx_linear.argtypes = [vp, i64, vp, vp, vp, ci, ci, ci, ci, vp, ctypes.c_size_t, vp]
+    lib.hexkv_mx_linear_workspace_bytes.restype = ctypes.c_size_t
+    lib.hexkv_mx_linear_workspace_bytes.argtypes = [ci, ci, ci, ci]
     lib.hexkv_token_logprobs_workspace_bytes.restype = ctypes.c_size_t
     lib.hexkv_token_logprobs_workspace_bytes.argtypes = [i64, ci, ci]
     lib.hexkv_token_logprobs.restype = ci

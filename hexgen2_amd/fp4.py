@@ -294,6 +294,11 @@ def dequantize(weight: Fp4Tensor, dtype: torch.dtype) -> torch.Tensor:
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace(rows: int, n: int, k: int, dtype: int) -> int:
+    return int(_lib.load().hexkv_mx_linear_workspace_bytes(rows, n, k, dtype))
+
+
 def linear(x: torch.Tensor, weight: Fp4Tensor) -> torch.Tensor:
     """``x @ weight.T`` for ``x [..., k]`` and a 4-bit matrix ``[n, k]``: sums in
     fp32 over the weights' exact values, rounded once to ``x``'s type."""
@@ -306,6 +311,9 @@ def linear(x: torch.Tensor, weight: Fp4Tensor) -> torch.Tensor:
     n, k = codes.shape[0], x.shape[-1]
     stride = _matrix_rows(x, "x")
     out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-    _call("hexkv_mx_linear", x, x.data_ptr(), stride, codes.data_ptr(), powers.data_ptr(), out.data_ptr(),
-          x.numel() // max(k, 1), n, k, _DTYPES[x.dtype])
+    rows, dtype = x.numel() // max(k, 1), _DTYPES[x.dtype]
+    need = _linear_workspace(rows, n, k, dtype)
+    workspace = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _call("hexkv_mx_linear", x, x.data_ptr(), stride, codes.data_ptr(), powers.data_ptr(), out.data_ptr(), rows, n, k, dtype,
+          workspace.data_ptr() if need else None, need)
     return out

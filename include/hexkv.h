@@ -735,9 +735,12 @@ int hexkv_mx_attend(const hexkv_mx_attend_params *p, void *workspace, size_t wor
 
 /* out [rows][n] = x W^T for W [n][k] in four-bit blocks (codes [n][k / 2],
  * 16-byte aligned, powers [n][k / 32], contiguous; k a multiple of 32), x rows
- * x_stride elements apart, out contiguous; sums in fp32, rounded once. */
+ * x_stride elements apart, out contiguous; sums in fp32, rounded once.  The
+ * workspace (scratch, not shared with an overlapping call) holds partial sums
+ * where the inner dimension is split. */
+size_t hexkv_mx_linear_workspace_bytes(int rows, int n, int k, int dtype);
 int hexkv_mx_linear(const void *x, int64_t x_stride, const void *codes, const void *powers, void *out, int rows, int n,
-                    int k, int dtype, hexkv_stream_t stream);
+                    int k, int dtype, void *workspace, size_t workspace_bytes, hexkv_stream_t stream);
 
 /* ---------------------------------------------------------------- scoring ---
  * What a step's logits say of its tokens (the reference reads no more than

@@ -148,7 +148,7 @@ def test_attention_refuses_a_small_workspace_and_null_params():
     ((ADDRESS + 1, 64, ADDRESS, ADDRESS, ADDRESS, 4, 8, 64, 1), E), ((ADDRESS, 64, ADDRESS, ADDRESS, ADDRESS, 1 << 21, 8, 64, 1), R),
     ((ADDRESS, 64, ADDRESS, ADDRESS, ADDRESS, 0, 8, 64, 1), 0)])
 def test_linear_refuses(args, code):
-    assert _lib.load().hexkv_mx_linear(*args, None) == code
+    assert _lib.load().hexkv_mx_linear(*args, None, 0, None) == code
 
 
 def logprob_call(**change):
