@@ -1,16 +1,21 @@
 // Products with 4-bit matrices: hexkv_mx_linear.
 //
-// A wave takes 16 rows of the matrix and up to 64 tokens, 128 of the inner
-// dimension at a time: lane (c, g) holds one block (16 bytes, 32 elements) of
-// row c, and the tokens' operand the same 32 elements of each token in the
-// same order, so the converted block feeds four matrix instructions as it stands.
-// The four waves of a workgroup share the inner dimension and join through
-// LDS.
+// What bounds it: reading the matrix while tokens are few, 17/32 byte an element
+// (at the rate of a large copy, 4.85 TB/s), the matrix cores for a prompt.
+// Everywhere a lane loads whole blocks of a row (16 bytes, 32 elements, one
+// power) and converts them in registers; the matrix instructions' inner dimension is laid
+// out to fit what a lane holds, the tokens' operand in the same order, so a
+// converted block is an operand as it stands.  Three kernels, see mx_plan:
+//   mx_rows_kernel  one or two tokens: a wave reads rows from end to end;
+//   mx_few_kernel   up to 64: a wave holds the tokens' operands of its share of
+//                   the inner dimension in registers and walks the matrix;
+//   mx_tile_kernel  more: tiles, with the tokens in LDS.
 //
 // bf16 activations meet the matrix as bf16, exact for every power.  fp16 ones
-// meet it as fp16, exact for powers from 2^-23 to 2^13; a wave that meets
-// another power takes that step in bf16, with each activation as two terms.
-// fp32 activations are three bf16 terms.  All sums are fp32.
+// meet it as fp16, exact for powers from 2^-23 to 2^13; blocks with another
+// power are left out there and added afterwards in bf16, with each activation as two
+// terms (fp32 in mx_rows_kernel).  fp32 activations are three bf16 terms.  All
+// sums are fp32.
 #include "hexkv_mx.h"
 
 #include <algorithm>
@@ -18,7 +23,6 @@
 namespace hexkv {
 
 constexpr int kMxlThreads = 256;
-constexpr int kMxlWaves = kMxlThreads / 64;
 
 struct MxLinearArgs {
   const void *x;
@@ -67,93 +71,369 @@ __device__ __forceinline__ f32x4 mma_f16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Few tokens (up to 16): a wave takes 16 rows of the matrix, 128 of the inner
-// dimension at a time, the workgroup's waves in turn; kAhead of a wave's steps
-// are loaded before the first is used.  The activations come straight from the
-// caches.
-constexpr int kAhead = 4;
+// fp16 activations: the scale a block enters the fp16 product with, 0 for a
+// power that fp16 does not hold exactly (*far is raised), so that the block
+// adds nothing there.
+__device__ __forceinline__ float near_scale(unsigned int byte, bool *far) {
+  const bool out = byte - kMxF16Low > kMxF16High - kMxF16Low;
+  *far |= out;
+  return out ? 0.f : mx_scale(byte);
+}
 
-template <typename T>
-__global__ __launch_bounds__(kMxlThreads) void mx_few_kernel(const MxLinearArgs a) {
-  __shared__ f32x4 s_part[kMxlWaves][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4;
-  const int n0 = static_cast<int>(blockIdx.x) * 16;
-  const int64_t row = min(n0 + c, a.n - 1);
-  const unsigned char *codes = a.codes + row * (a.k / 2), *powers = a.powers + row * (a.k / kMxBlock);
-  const T *x = static_cast<const T *>(a.x) + static_cast<int64_t>(c < a.rows ? c : 0) * a.x_stride;
-  f32x4 acc = {};
-  for (int base = wave * 128; base < a.k; base += kAhead * kMxlWaves * 128) {
-    u32x4 w[kAhead];
-    unsigned int byte[kAhead];
+// Such a block alone, as bf16; any other is zero.
+struct FarBlock {
+  u32x4 w;
+  float scale;
+  bool any;
+  __device__ __forceinline__ void read(const MxLinearArgs &a, int64_t row, int block, bool live) {
+    const unsigned int byte = live ? a.powers[row * (a.k / kMxBlock) + block] : 127u;
+    any = byte - kMxF16Low > kMxF16High - kMxF16Low;
+    w = u32x4{};
+    if (any) w = *reinterpret_cast<const u32x4 *>(a.codes + row * (a.k / 2) + block * 16);
+    scale = any ? mx_scale(byte) : 1.f;
+  }
+  __device__ __forceinline__ unsigned int word(int j) const { return j < 2 ? (j == 0 ? w[0] : w[1]) : (j == 2 ? w[2] : w[3]); }
+  __device__ __forceinline__ u32x4 operand(int j) const { return mx_bf16(word(j), scale); }
+};
+// The two bf16 terms of 8 fp16 activations.
+__device__ __forceinline__ void far_terms(const _Float16 *p, bool live, u32x4 *terms) {
+  float f[8] = {};
+  if (live) mx_read8(p, false, f);
+  terms8<2>(f, terms);
+}
+
+// acc + the dot product of one block of the matrix and 32 fp32 activations.
+__device__ __forceinline__ float mx_dot(u32x4 w, unsigned int byte, const u32x4 *x, float acc) {
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s) {
-      const int k = base + s * kMxlWaves * 128 + g * kMxBlock;  // this lane's block
-      w[s] = u32x4{};
-      byte[s] = 127;
-      if (k < a.k) {
-        w[s] = *reinterpret_cast<const u32x4 *>(codes + k / 2);
-        byte[s] = powers[k / kMxBlock];
+  for (int j = 0; j < 4; ++j) {
+    float m[8], f[8];
+    mx_f32(w[j], mx_scale(byte), m);
+    Elem<float>::to_float(x[2 * j], f);
+    Elem<float>::to_float(x[2 * j + 1], f + 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc = fmaf(m[i], f[i], acc);
+  }
+  return acc;
+}
+
+// One or two tokens: a wave takes ROWS rows of the matrix, its lanes the
+// blocks of a row in turn (LOADS of them each), and the activations of those
+// blocks stay in registers.  No load is conditional: loads inside branches
+// waited for one another's latency (15.5 us where this takes 10.9, 1 x 22528 x 4096).
+template <typename T, int TOKENS, int LOADS, int ROWS, bool VEC>
+__global__ __launch_bounds__(kMxlThreads) void mx_rows_kernel(const MxLinearArgs a) {
+  constexpr int XW = sizeof(T) * 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int blocks = a.k / kMxBlock;
+  const int n0 = (static_cast<int>(blockIdx.x) * (kMxlThreads / 64) + wave) * ROWS;
+  if (n0 >= a.n) return;
+  u32x4 w[ROWS][LOADS];
+  unsigned int byte[ROWS][LOADS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int64_t row = min(n0 + r, a.n - 1);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int block = min(i * 64 + lane, blocks - 1);  // past the end: the last one again
+      w[r][i] = *reinterpret_cast<const u32x4 *>(a.codes + (row * blocks + block) * 16);
+      byte[r][i] = a.powers[row * blocks + block];
+    }
+  }
+  u32x4 x[TOKENS][LOADS][XW];
+#pragma unroll
+  for (int t = 0; t < TOKENS; ++t)
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const T *p = static_cast<const T *>(a.x) + t * a.x_stride + min(i * 64 + lane, blocks - 1) * kMxBlock;
+      if constexpr (VEC) {
+#pragma unroll
+        for (int j = 0; j < XW; ++j) x[t][i][j] = *reinterpret_cast<const u32x4 *>(p + j * 16 / sizeof(T));
+      } else {
+        T e[kMxBlock];
+#pragma unroll
+        for (int j = 0; j < kMxBlock; ++j) e[j] = p[j];
+        __builtin_memcpy(x[t][i], e, sizeof(e));
       }
     }
+  // the blocks past the end count as zero, in the matrix and in the tokens
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s) {
-      const int k = base + s * kMxlWaves * 128 + g * kMxBlock;
-      const bool live = c < a.rows && k < a.k;
-      const bool narrow = !__ballot(byte[s] - kMxF16Low > kMxF16High - kMxF16Low);
-      const float scale = mx_scale(byte[s]);
-      const T *at = x + (live ? k : 0);
-      if constexpr (sizeof(T) == 4) {
+  for (int i = 0; i < LOADS; ++i)
+    if (i * 64 + 64 > blocks && i * 64 + lane >= blocks) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        w[r][i] = u32x4{};
+        byte[r][i] = 127;
+      }
+#pragma unroll
+      for (int t = 0; t < TOKENS; ++t)
+#pragma unroll
+        for (int j = 0; j < XW; ++j) x[t][i][j] = u32x4{};
+    }
+  float sum[TOKENS][ROWS];
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int t = 0; t < TOKENS; ++t)
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        sum[t][r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) sum[t][r] = mx_dot(w[r][i], byte[r][i], x[t][i], sum[t][r]);
+      }
+  } else {
+    // The matrix instruction of what the lanes hold: entry (i, j) is the sum
+    // over g of lane (i, g)'s elements times lane (j, g)'s activations, so its
+    // diagonal adds up to the sum over all lanes.
+    f32x4 acc[TOKENS][ROWS];
+    bool far = false;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+      for (int t = 0; t < TOKENS; ++t) acc[t][r] = f32x4{};
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const float scale = Elem<T>::kDtype == HEXKV_F16 ? near_scale(byte[r][i], &far) : mx_scale(byte[r][i]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float f[8] = {};
-          if (live) mx_read8(at + 8 * j, a.vec, f);
-          u32x4 t[3];
-          terms8<3>(f, t);
-          const u32x4 m = mx_bf16(w[s][j], scale);
+          const u32x4 m = Elem<T>::kDtype == HEXKV_F16 ? mx_f16(w[r][i][j], scale) : mx_bf16(w[r][i][j], scale);
 #pragma unroll
-          for (int n = 0; n < 3; ++n) acc = mma_bf16(m, t[n], acc);
+          for (int t = 0; t < TOKENS; ++t)
+            acc[t][r] = Elem<T>::kDtype == HEXKV_F16 ? mma_f16(m, x[t][i][j], acc[t][r]) : mma_bf16(m, x[t][i][j], acc[t][r]);
         }
+      }
+    }
+    const int c = lane & 15;
+#pragma unroll
+    for (int t = 0; t < TOKENS; ++t)
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const f32x4 v = acc[t][r];
+        const float d = c & 2 ? (c & 1 ? v[3] : v[2]) : (c & 1 ? v[1] : v[0]);
+        sum[t][r] = c >> 2 == lane >> 4 ? d : 0.f;
+      }
+    if (Elem<T>::kDtype == HEXKV_F16 && __ballot(far)) {
+#pragma unroll 1
+      for (int b = lane; b < blocks; b += 64)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          FarBlock block;
+          block.read(a, min(n0 + r, a.n - 1), b, true);
+          if (!block.any) continue;
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j) {
+            float m[8], f[8];
+            mx_f32(block.word(j), block.scale, m);
+#pragma unroll
+            for (int t = 0; t < TOKENS; ++t) {
+              mx_read8(static_cast<const T *>(a.x) + t * a.x_stride + b * kMxBlock + 8 * j, false, f);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) sum[t][r] = fmaf(m[i], f[i], sum[t][r]);
+            }
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TOKENS; ++t) {
+    float mine = 0.f;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const float v = group_sum<64>(sum[t][r]);
+      if (lane == r) mine = v;
+    }
+    if (lane < ROWS && n0 + lane < a.n)
+      static_cast<T *>(a.out)[static_cast<int64_t>(t) * a.n + n0 + lane] = Elem<T>::from_float(mine);
+  }
+}
+
+// Words of 16 bytes that hold 32 activations of T as operands (fp32: three terms).
+template <typename T>
+constexpr int kOperandWords = sizeof(T) == 4 ? 12 : 4;
+
+// BL bytes at p.
+template <int BL>
+struct PowerBytes {
+  unsigned int v[BL <= 4 ? 1 : 2];
+  __device__ __forceinline__ void read(const unsigned char *p) {
+    if constexpr (BL == 1) {
+      v[0] = *p;
+    } else if constexpr (BL == 2) {
+      unsigned short u;
+      __builtin_memcpy(&u, p, 2);
+      v[0] = u;
+    } else {
+      __builtin_memcpy(v, p, BL);
+    }
+  }
+  __device__ __forceinline__ unsigned int operator[](int i) const { return v[i / 4] >> 8 * (i % 4) & 255; }
+};
+
+// Up to 16 MT tokens over one split of the inner dimension (1024 BL of it): each
+// of eight waves takes an eighth, its tokens' operands in registers (16 MT BL of
+// them), and walks the matrix 16 rows at a time; the waves join through LDS.  BL: consecutive blocks of a row that a lane holds; RING: matrix tiles a
+// wave has loaded or in flight; VEC: the activations' rows are 16-byte aligned.
+template <typename T, int MT, int BL, int RING, bool VEC>
+__global__ __launch_bounds__(512) void mx_few_kernel(const MxLinearArgs a) {
+  constexpr int XW = kOperandWords<T>, WAVES = 8;
+  __shared__ f32x4 s_part[2][WAVES][MT][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int row_blocks = a.k / kMxBlock, n_tiles = (a.n + 15) / 16;
+  const int split = static_cast<int>(blockIdx.y) % a.splits, m0 = static_cast<int>(blockIdx.y) / a.splits * 16 * MT;
+  const int block0 = split * (a.split_k / kMxBlock), blocks = min(row_blocks, block0 + a.split_k / kMxBlock);
+  const int first = block0 + (wave * 4 + g) * BL;  // this lane's blocks
+  // of the whole wave: none of its blocks exists, or not all of them
+  const bool idle = block0 + wave * 4 * BL >= blocks, ragged = block0 + (wave + 1) * 4 * BL > blocks;
+
+  // No load is conditional (the launch has rows of at least BL blocks): a lane
+  // whose blocks do not all exist reads BL before the end, and those
+  // that are not its own count as zero.
+  const int from = max(0, min(first, blocks - BL));
+  const auto foreign = [&](int s) { return from + s < first || from + s >= blocks; };
+  struct Tile {
+    u32x4 w[BL];
+    PowerBytes<BL> power;
+  };
+  Tile ring[RING];
+  const auto fetch = [&](int tile, Tile &t) {
+    const int64_t row = min(tile * 16 + c, a.n - 1);
+    const unsigned char *p = a.codes + (row * row_blocks + from) * 16;
+#pragma unroll
+    for (int i = 0; i < BL; ++i) t.w[i] = *reinterpret_cast<const u32x4 *>(p + i * 16);
+    t.power.read(a.powers + row * row_blocks + from);
+  };
+  const int stride = static_cast<int>(gridDim.x);
+  const int tile0 = static_cast<int>(blockIdx.x);
+  if (!idle) fetch(tile0, ring[0]);
+
+  // The activations of the wave's share stay in registers.  Columns behind the
+  // last token repeat it (they are not stored); past the inner dimension
+  // they are zero, as the matrix is.
+  u32x4 x[MT][BL][XW];
+  const T *tokens[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+    tokens[m] = static_cast<const T *>(a.x) + static_cast<int64_t>(min(m0 + 16 * m + c, a.rows - 1)) * a.x_stride + from * kMxBlock;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int s = 0; s < BL; ++s) {
+      const T *p = tokens[m] + s * kMxBlock;
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[m][s][j] = raw8(p + 8 * j, VEC);
       } else {
-        u32x4 r[4] = {};
-        if (live) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) r[j] = raw8(at + 8 * j, a.vec);
+        for (int j = 0; j < 4; ++j) {
+          float f[8];
+          mx_read8(p + 8 * j, VEC, f);
+          terms8<3>(f, &x[m][s][3 * j]);
         }
-        if constexpr (Elem<T>::kDtype == HEXKV_BF16) {
+      }
+    }
+  if (ragged) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc = mma_bf16(mx_bf16(w[s][j], scale), r[j], acc);
-        } else if (narrow) {
+    for (int s = 0; s < BL; ++s)
+      if (foreign(s)) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc = mma_f16(mx_f16(w[s][j], scale), r[j], acc);
-        } else {
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int j = 0; j < XW; ++j) x[m][s][j] = u32x4{};
+      }
+  }
+#pragma unroll
+  for (int r = 1; r < RING; ++r)
+    if (!idle && tile0 + r * stride < n_tiles) fetch(tile0 + r * stride, ring[r]);
+
+  for (int base = tile0, turn = 0; base < n_tiles; base += RING * stride) {
+#pragma unroll
+    for (int r = 0; r < RING; ++r, ++turn) {
+      const int tile = base + r * stride;
+      if (tile >= n_tiles) break;
+      f32x4 acc[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[m] = f32x4{};
+      bool far = false;
+      if (!idle) {
+        Tile &t = ring[r];
+        unsigned int byte[BL];
+#pragma unroll
+        for (int s = 0; s < BL; ++s) byte[s] = t.power[s];
+        if (ragged) {
+#pragma unroll
+          for (int s = 0; s < BL; ++s)
+            if (foreign(s)) {
+              t.w[s] = u32x4{};
+              byte[s] = 127;
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < BL; ++s) {
+          const float scale = Elem<T>::kDtype == HEXKV_F16 ? near_scale(byte[s], &far) : mx_scale(byte[s]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float f[8];
-            Elem<T>::to_float(r[j], f);
-            u32x4 t[2];
-            terms8<2>(f, t);
-            const u32x4 m = mx_bf16(w[s][j], scale);
-            acc = mma_bf16(m, t[1], mma_bf16(m, t[0], acc));
+            if constexpr (sizeof(T) == 4) {
+              const u32x4 w = mx_bf16(t.w[s][j], scale);
+#pragma unroll
+              for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < 3; ++n) acc[m] = mma_bf16(w, x[m][s][3 * j + n], acc[m]);
+            } else if constexpr (Elem<T>::kDtype == HEXKV_BF16) {
+              const u32x4 w = mx_bf16(t.w[s][j], scale);
+#pragma unroll
+              for (int m = 0; m < MT; ++m) acc[m] = mma_bf16(w, x[m][s][j], acc[m]);
+            } else {
+              const u32x4 w = mx_f16(t.w[s][j], scale);
+#pragma unroll
+              for (int m = 0; m < MT; ++m) acc[m] = mma_f16(w, x[m][s][j], acc[m]);
+            }
+          }
+        }
+        if (tile + RING * stride < n_tiles) fetch(tile + RING * stride, t);
+      }
+      if (Elem<T>::kDtype == HEXKV_F16 && __ballot(far)) {
+        const int64_t row = min(tile * 16 + c, a.n - 1);
+#pragma unroll 1
+        for (int s = 0; s < BL; ++s) {
+          FarBlock block;
+          block.read(a, row, from + s, !foreign(s));
+          if (!__ballot(block.any)) continue;
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j) {
+            const u32x4 w = block.operand(j);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              u32x4 terms[2];
+              far_terms(reinterpret_cast<const _Float16 *>(tokens[m]) + s * kMxBlock + 8 * j, !foreign(s), terms);
+              acc[m] = mma_bf16(w, terms[1], mma_bf16(w, terms[0], acc[m]));
+            }
           }
         }
       }
-    }
-  }
-  s_part[wave][lane] = acc;
-  __syncthreads();
-  // acc: column c is the token, rows 4 g + i are the matrix's
-  if (wave == 0) {
-    f32x4 sum = s_part[0][lane];
+      // Two halves of LDS in turn: a wave writes one again only after the
+      // barrier that follows the reading of it.
 #pragma unroll
-    for (int w = 1; w < kMxlWaves; ++w) sum += s_part[w][lane];
-    const int n = n0 + 4 * g;
-    if (c < a.rows && n < a.n) {
-      T *out = static_cast<T *>(a.out) + static_cast<int64_t>(c) * a.n + n;
-      if (n + 4 <= a.n) {
-        store4(out, sum);
-      } else {
-        for (int i = 0; i < a.n - n; ++i) out[i] = Elem<T>::from_float(sum[i]);
+      for (int m = 0; m < MT; ++m) s_part[turn & 1][wave][m][lane] = acc[m];
+      __syncthreads();
+      // acc: column c is the token, rows 4 g + i are the matrix's
+      const int m = (wave + turn * MT) % WAVES;
+      if (m < MT) {
+        f32x4 sum = s_part[turn & 1][0][m][lane];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) sum += s_part[turn & 1][i][m][lane];
+        const int token = m0 + 16 * m + c, n = tile * 16 + 4 * g;
+        if (token < a.rows && n < a.n) {
+          const int64_t at = static_cast<int64_t>(token) * a.n + n;
+          const int count = min(4, a.n - n);
+          if (a.splits > 1) {
+            float *o = a.partial + static_cast<int64_t>(split) * a.rows * a.n + at;
+            if (count == 4) store4(o, sum);
+            else for (int i = 0; i < count; ++i) o[i] = sum[i];
+          } else {
+            T *o = static_cast<T *>(a.out) + at;
+            if (count == 4) store4(o, sum);
+            else for (int i = 0; i < count; ++i) o[i] = Elem<T>::from_float(sum[i]);
+          }
+        }
       }
     }
   }
@@ -170,9 +450,10 @@ __global__ __launch_bounds__(kMxlThreads) void mx_few_kernel(const MxLinearArgs 
 // and the tokens' operand the same elements.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-template <typename T, int MT_, int NT_, int WM_, int WN_, int WK_, int STEPS_>
+template <typename T, int MT_, int NT_, int WM_, int WN_, int WK_, int STEPS_, int RING_, int XR_>
 struct MxTileShape {
-  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, WK = WK_, STEPS = STEPS_;
+  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, WK = WK_, STEPS = STEPS_, RING = RING_, XR = XR_;
+  static_assert(RING % XR == 0 && RING % 2 == 0, "the loop is unrolled by the ring");
   static constexpr int kWaves = WM * WN * WK, kThreads = 64 * kWaves;
   static constexpr int kTokens = 32 * MT * WM, kRows = 32 * NT * WN;
   static constexpr int kStep = 64 * WK * STEPS;            // inner dimension of one step
@@ -182,7 +463,7 @@ struct MxTileShape {
   static constexpr int kLoads = kPlane / kThreads;         // chunks a thread stages
   static constexpr size_t kLds = size_t{16} * 2 * kPlanes * kPlane;
   static_assert(kPlane % kThreads == 0, "every thread stages as much");
-  static_assert(static_cast<size_t>(WK - 1) * WM * WN * MT * NT * 16 * 64 * 4 <= kLds, "the join fits the stage");
+  static_assert(static_cast<size_t>(WK / 2) * WM * WN * MT * NT * 16 * 64 * 4 <= kLds, "the join fits the stage");
 };
 
 __device__ __forceinline__ f32x16 mma32_bf16(u32x4 a, u32x4 b, f32x16 c) {
@@ -192,7 +473,7 @@ __device__ __forceinline__ f32x16 mma32_f16(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-template <typename T, typename S>
+template <typename T, typename S, bool VEC>
 __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs a) {
   constexpr int MT = S::MT, NT = S::NT, CH = S::kChunks, PL = S::kPlanes;
   constexpr int kSpread = CH >= 16 ? 1 : 16 / CH;  // rows whose chunks fill the banks once
@@ -212,60 +493,95 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs
   const int n0 = group / a.splits * S::kRows, split = group % a.splits;
   const int k_first = split * a.split_k, k_last = min(a.k, k_first + a.split_k);
 
-  const unsigned char *codes[NT], *powers[NT];
+  // Every load is a uniform base that moves along the inner dimension plus a
+  // lane's constant 32-bit offset, and none is conditional: in the last step
+  // what lies past the end is the split's last piece again, and counts as zero.
+  const char *x_base = static_cast<const char *>(a.x) + static_cast<int64_t>(m0) * a.x_stride * sizeof(T);
+  const unsigned char *w_base = a.codes + static_cast<int64_t>(n0) * (a.k / 2);
+  const unsigned char *p_base = a.powers + static_cast<int64_t>(n0) * (a.k / kMxBlock);
+  unsigned int x_off[S::kLoads], w_off[NT], p_off[NT];
+#pragma unroll
+  for (int i = 0; i < S::kLoads; ++i) {
+    const int at = i * S::kThreads + tid, token = min(at / CH, a.rows - 1 - m0);
+    x_off[i] = (static_cast<unsigned int>(token) * static_cast<unsigned int>(a.x_stride) + at % CH * 8) * sizeof(T);
+  }
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int64_t row = min(n0 + (wn * NT + t) * 32 + c, a.n - 1);
-    codes[t] = a.codes + row * (a.k / 2);
-    powers[t] = a.powers + row * (a.k / kMxBlock);
+    const unsigned int row = min((wn * NT + t) * 32 + c, a.n - 1 - n0);
+    w_off[t] = row * (a.k / 2) + wk * S::STEPS * 32 + h * 16;
+    p_off[t] = row * (a.k / kMxBlock) + wk * S::STEPS * 2 + h;
   }
 
-  u32x4 stage[PL][S::kLoads];
-  const auto fetch_x = [&](int k0) {
+  struct Tokens {
+    u32x4 v[PL == 1 ? 1 : 2][S::kLoads];
+  };
+  const auto fetch_x = [&](int k0, Tokens &stage) {
+    const char *base = x_base + static_cast<int64_t>(k0) * sizeof(T);
+    const bool whole = k0 + S::kStep <= k_last;
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
-      const int at = i * S::kThreads + tid, token = m0 + at / CH, k = k0 + at % CH * 8;
-      const bool live = token < a.rows && k < k_last;
-      const T *p = static_cast<const T *>(a.x) + static_cast<int64_t>(live ? token : 0) * a.x_stride + (live ? k : 0);
+      unsigned int off = x_off[i];
+      if (!whole) off -= max(0, k0 + (i * S::kThreads + tid) % CH * 8 - (k_last - 8)) * sizeof(T);
+      const T *p = reinterpret_cast<const T *>(base + off);
       if constexpr (PL == 1) {
-        stage[0][i] = u32x4{};
-        if (live) stage[0][i] = raw8(p, a.vec);
+        stage.v[0][i] = raw8(p, VEC);
       } else {
-        float f[8] = {};
-        if (live) mx_read8(p, a.vec, f);
-        u32x4 t[3];
-        terms8<3>(f, t);
+        u32x4 f[2];
+        if constexpr (VEC) {
+          f[0] = *reinterpret_cast<const u32x4 *>(p);
+          f[1] = *reinterpret_cast<const u32x4 *>(p + 4);
+        } else {
+          float e[8];
 #pragma unroll
-        for (int n = 0; n < 3; ++n) stage[n][i] = t[n];
+          for (int j = 0; j < 8; ++j) e[j] = p[j];
+          __builtin_memcpy(f, e, sizeof(e));
+        }
+        stage.v[0][i] = f[0];
+        stage.v[1][i] = f[1];
       }
     }
   };
-  const auto store_x = [&](int buf) {
+  // (Tokens past the last repeat it and are not stored.)
+  const auto store_x = [&](int buf, int k0, const Tokens &stage) {
+    const bool whole = k0 + S::kStep <= k_last;
 #pragma unroll
-    for (int n = 0; n < PL; ++n)
-#pragma unroll
-      for (int i = 0; i < S::kLoads; ++i) {
-        const int at = i * S::kThreads + tid, token = at / CH, chunk = at % CH;
-        s_x[(buf * PL + n) * S::kPlane + token * CH + (chunk ^ (token / kSpread & kMask))] = stage[n][i];
+    for (int i = 0; i < S::kLoads; ++i) {
+      const int at = i * S::kThreads + tid, token = at / CH, chunk = at % CH;
+      u32x4 terms[PL];
+      if constexpr (PL == 1) {
+        terms[0] = stage.v[0][i];
+      } else {
+        float f[8];
+        Elem<float>::to_float(stage.v[0][i], f);
+        Elem<float>::to_float(stage.v[1][i], f + 4);
+        terms8<3>(f, terms);
       }
+      if (!whole && k0 + chunk * 8 >= k_last) {
+#pragma unroll
+        for (int n = 0; n < PL; ++n) terms[n] = u32x4{};
+      }
+#pragma unroll
+      for (int n = 0; n < PL; ++n)
+        s_x[(buf * PL + n) * S::kPlane + token * CH + (chunk ^ (token / kSpread & kMask))] = terms[n];
+    }
   };
   struct Weights {
     u32x4 w[S::STEPS][NT];
     unsigned int byte[S::STEPS][NT];
   };
   const auto fetch_w = [&](int k0, Weights &x) {
+    const unsigned char *w = w_base + k0 / 2, *p = p_base + k0 / kMxBlock;
+    const bool whole = k0 + S::kStep <= k_last;
 #pragma unroll
-    for (int s = 0; s < S::STEPS; ++s)
+    for (int s = 0; s < S::STEPS; ++s) {
+      // blocks this lane's lies past the last one
+      const int past = whole ? 0 : max(0, k0 / kMxBlock + (wk * S::STEPS + s) * 2 + h - (k_last / kMxBlock - 1));
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const int k = k0 + (wk * S::STEPS + s) * 64 + h * kMxBlock;
-        x.w[s][t] = u32x4{};
-        x.byte[s][t] = 127;
-        if (k < k_last) {
-          x.w[s][t] = *reinterpret_cast<const u32x4 *>(codes[t] + k / 2);
-          x.byte[s][t] = powers[t][k / kMxBlock];
-        }
+        x.w[s][t] = *reinterpret_cast<const u32x4 *>(w + (w_off[t] + s * 32 - past * 16));
+        x.byte[s][t] = p[p_off[t] + s * 2 - past];
       }
+    }
   };
 
   f32x16 acc[MT][NT];
@@ -274,55 +590,43 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[m][t] = f32x16{};
 
-  const auto compute = [&](int buf, const Weights &x) {
+  bool far = false;
+  const auto compute = [&](int buf, int k0, Weights &x) {
+    if (k0 + S::kStep > k_last) {  // what lies past the end counts as zero
 #pragma unroll
-    for (int s = 0; s < S::STEPS; ++s) {
-      bool far = false;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) far |= x.byte[s][t] - kMxF16Low > kMxF16High - kMxF16Low;
-      const auto tokens = [&](int n, int m, int j) {
-        const int token = (wm * MT + m) * 32 + c, chunk = (wk * S::STEPS + s) * 8 + h * 4 + j;
-        return s_x[(buf * PL + n) * S::kPlane + token * CH + (chunk ^ (token / kSpread & kMask))];
-      };
-      if (Elem<T>::kDtype == HEXKV_F16 && __ballot(far)) {
-        // (a loop that is not unrolled: the detour costs the main path no registers)
-#pragma unroll 1
-        for (int j = 0; j < 4; ++j) {
-          u32x4 w[NT];
+      for (int s = 0; s < S::STEPS; ++s)
+        if (k0 + (wk * S::STEPS + s) * 64 + h * kMxBlock >= k_last) {
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            const u32x4 v = x.w[s][t];
-            w[t] = mx_bf16(j < 2 ? (j == 0 ? v[0] : v[1]) : (j == 2 ? v[2] : v[3]), mx_scale(x.byte[s][t]));
-          }
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            float f[8];
-            Elem<_Float16>::to_float(tokens(0, m, j), f);
-            u32x4 terms[2];
-            terms8<2>(f, terms);
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int n = 0; n < 2; ++n) acc[m][t] = mma32_bf16(w[t], terms[n], acc[m][t]);
+            x.w[s][t] = u32x4{};
+            x.byte[s][t] = 127;
           }
         }
-        continue;
-      }
+    }
+#pragma unroll
+    for (int s = 0; s < S::STEPS; ++s) {
+      float scale[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        scale[t] = Elem<T>::kDtype == HEXKV_F16 ? near_scale(x.byte[s][t], &far) : mx_scale(x.byte[s][t]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         u32x4 b[PL][MT];
 #pragma unroll
         for (int n = 0; n < PL; ++n)
 #pragma unroll
-          for (int m = 0; m < MT; ++m) b[n][m] = tokens(n, m, j);
+          for (int m = 0; m < MT; ++m) {
+            const int token = (wm * MT + m) * 32 + c, chunk = (wk * S::STEPS + s) * 8 + h * 4 + j;
+            b[n][m] = s_x[(buf * PL + n) * S::kPlane + token * CH + (chunk ^ (token / kSpread & kMask))];
+          }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           if constexpr (Elem<T>::kDtype == HEXKV_F16) {
-            const u32x4 w = mx_f16(x.w[s][t][j], mx_scale(x.byte[s][t]));
+            const u32x4 w = mx_f16(x.w[s][t][j], scale[t]);
 #pragma unroll
             for (int m = 0; m < MT; ++m) acc[m][t] = mma32_f16(w, b[0][m], acc[m][t]);
           } else {
-            const u32x4 w = mx_bf16(x.w[s][t][j], mx_scale(x.byte[s][t]));
+            const u32x4 w = mx_bf16(x.w[s][t][j], scale[t]);
 #pragma unroll
             for (int n = 0; n < PL; ++n)
 #pragma unroll
@@ -333,52 +637,85 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs
     }
   };
 
-  if (k_first < k_last) {
-    Weights now, next;
-    fetch_x(k_first);
-    fetch_w(k_first, now);
-    store_x(0);
-    __syncthreads();
-    int buf = 0;
-    for (int k0 = k_first; k0 < k_last; k0 += S::kStep) {
-      const bool more = k0 + S::kStep < k_last;
-      if (more) {
-        fetch_x(k0 + S::kStep);
-        fetch_w(k0 + S::kStep, next);
-      }
-      compute(buf, now);
-      if (more) store_x(buf ^ 1);
-      buf ^= 1;
-      now = next;
+  Weights ring[S::RING];
+  Tokens xs[S::XR];
+  fetch_x(k_first, xs[0]);
+  fetch_w(k_first, ring[0]);
+#pragma unroll
+  for (int r = 1; r < S::RING; ++r) {  // in the order of their use
+    if (r < S::XR && k_first + r * S::kStep < k_last) fetch_x(k_first + r * S::kStep, xs[r]);
+    if (r < S::RING - 1 && k_first + r * S::kStep < k_last) fetch_w(k_first + r * S::kStep, ring[r]);
+  }
+  store_x(0, k_first, xs[0]);
+  __syncthreads();
+  for (int base = k_first; base < k_last; base += S::RING * S::kStep) {
+#pragma unroll
+    for (int r = 0; r < S::RING; ++r) {
+      const int k0 = base + r * S::kStep;
+      if (k0 >= k_last) break;
+      if (k0 + S::XR * S::kStep < k_last) fetch_x(k0 + S::XR * S::kStep, xs[r % S::XR]);
+      if (k0 + (S::RING - 1) * S::kStep < k_last) fetch_w(k0 + (S::RING - 1) * S::kStep, ring[(r + S::RING - 1) % S::RING]);
+      compute(r & 1, k0, ring[r]);
+      if (k0 + S::kStep < k_last) store_x((r + 1) & 1, k0 + S::kStep, xs[(r + 1) % S::XR]);
       __syncthreads();
     }
   }
 
-  // the waves that share the inner dimension join in the first of them
+  if (Elem<T>::kDtype == HEXKV_F16 && __ballot(far)) {
+#pragma unroll 1
+    for (int k0 = k_first; k0 < k_last; k0 += S::kStep)
+#pragma unroll 1
+      for (int s = 0; s < S::STEPS; ++s) {
+        const int k = k0 + (wk * S::STEPS + s) * 64 + h * kMxBlock;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          FarBlock block;
+          block.read(a, min(n0 + (wn * NT + t) * 32 + c, a.n - 1), k / kMxBlock, k < k_last);
+          if (!__ballot(block.any)) continue;
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const int token = min(m0 + (wm * MT + m) * 32 + c, a.rows - 1);
+            const _Float16 *p = static_cast<const _Float16 *>(a.x) + static_cast<int64_t>(token) * a.x_stride + k;
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) {
+              u32x4 terms[2];
+              far_terms(p + 8 * j, k < k_last, terms);
+              const u32x4 w = block.operand(j);
+              acc[m][t] = mma32_bf16(w, terms[1], mma32_bf16(w, terms[0], acc[m][t]));
+            }
+          }
+        }
+      }
+  }
+
+  // the waves that share the inner dimension join, half of them at a time
   if constexpr (S::WK > 1) {
     float *s_acc = reinterpret_cast<float *>(s_mem);
-    const int piece = (wm * S::WN + wn) * MT * NT * 16 * 64 + lane;
-    if (wk > 0) {
-      float *p = s_acc + (wk - 1) * S::WM * S::WN * MT * NT * 16 * 64 + piece;
+    constexpr int kPiece = MT * NT * 16 * 64;
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+    for (int half = S::WK / 2; half > 0; half /= 2) {
+      if (wk >= half && wk < 2 * half) {
+        float *p = s_acc + ((wk - half) * S::WM * S::WN + wm * S::WN + wn) * kPiece + lane;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) p[((m * NT + t) * 16 + i) * 64] = acc[m][t][i];
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[((m * NT + t) * 16 + i) * 64] = acc[m][t][i];
+      }
+      __syncthreads();
+      if (wk < half) {
+        const float *p = s_acc + (wk * S::WM * S::WN + wm * S::WN + wn) * kPiece + lane;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[m][t][i] += p[((m * NT + t) * 16 + i) * 64];
+      }
+      if (half > 1) __syncthreads();
     }
-    __syncthreads();
     if (wk > 0) return;
-#pragma unroll
-    for (int w = 0; w < S::WK - 1; ++w) {
-      const float *p = s_acc + w * S::WM * S::WN * MT * NT * 16 * 64 + piece;
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[m][t][i] += p[((m * NT + t) * 16 + i) * 64];
-    }
   }
   // acc: column c is the token, rows 8 i + 4 h + e the matrix's
 #pragma unroll
@@ -424,19 +761,38 @@ __global__ __launch_bounds__(kMxlThreads) void mx_sum_kernel(const MxLinearArgs 
   }
 }
 
-// The tile a call runs: its tokens and matrix rows, and what a split of the
-// inner dimension is a multiple of.
+// The kernels and tiles a call may run, by tokens (GPU time of a call on MI355X,
+// weights from memory, bf16 unless said):
+//   1, 2    kRows: 1 x 22528 x 4096 10.9 us (4.5 TB/s); kFew 12.7.
+//   3-16    kFew, 16 tokens a wave: 16 x 22528 x 4096 16.8 us; a tile 29.
+//   17-64   kFew where the matrix has kFewRows rows or more (32 tokens 21.0 us, a tile 29.6; 64
+//           tokens 30.8 against 37): each workgroup reads every token once,
+//           which many matrix tiles share.  Below that a tile: 64 x 4096 x
+//           11264 23.7 us against 37.
+//   65-     tiles of 64 tokens up to kNarrowTokens (128 x 22528 x 4096 54 us against
+//           62), of 128 above (611 x 4096 x 11264 fp16 96 us against 107, 590
+//           TFLOP/s).
+enum MxKind { kRows, kFew16, kFew32, kFew64, kTile32, kTile64, kTileNarrow, kTilePrompt };
+constexpr int kFewRows = 8192, kNarrowTokens = 192;
+
 struct MxPlan {
-  int kind;  // 0: few tokens
+  int kind;
+  int blocks;  // kRows: loads of a lane; kFew*: blocks of a lane
   int m_tiles, n_tiles, splits, split_k;
 };
 
-template <typename T> using TileDecode32 = MxTileShape<T, 1, 1, 1, 4, 2, sizeof(T) == 4 ? 1 : 2>;
-template <typename T> using TileDecode64 = MxTileShape<T, 2, 1, 1, 4, 2, sizeof(T) == 4 ? 1 : 2>;
-template <typename T> using TilePrompt = MxTileShape<T, 2, 2, 2, 2, 1, 1>;
+// fp32 tokens are three terms each: shorter steps and fewer waves on the inner dimension, so
+// that they fit LDS.
+constexpr int inner_waves(size_t elem) { return elem == 4 ? 2 : 4; }
+template <typename T> using Tile32 = MxTileShape<T, 1, 1, 1, 2, inner_waves(sizeof(T)), 1, 4, 4>;
+template <typename T> using Tile64 = MxTileShape<T, 2, 1, 1, 2, inner_waves(sizeof(T)), 1, 4, 2>;
+template <typename T> using TileNarrow = MxTileShape<T, 2, 2, 1, 2, 2, 1, 2, 2>;
+template <typename T> using TilePrompt = MxTileShape<T, 2, 2, 2, 2, 1, 1, 2, 1>;
 
+// Splits of the inner dimension: two workgroups a CU, at least four steps each.
 template <typename S>
-static void plan_tile(MxPlan *p, int rows, int n, int k) {
+static void plan_tile(MxPlan *p, int kind, int rows, int n, int k) {
+  p->kind = kind;
   p->m_tiles = (rows + S::kTokens - 1) / S::kTokens;
   p->n_tiles = (n + S::kRows - 1) / S::kRows;
   const int steps = (k + S::kStep - 1) / S::kStep;
@@ -445,13 +801,40 @@ static void plan_tile(MxPlan *p, int rows, int n, int k) {
   p->splits = (k + p->split_k - 1) / p->split_k;
 }
 
+// Blocks a lane holds of a row: a wave's share of eight, or as much of it as
+// leaves the activations 128 registers; more is further splits.
+static void plan_few(MxPlan *p, int kind, int most, int rows, int k) {
+  p->kind = kind;
+  p->blocks = 1;
+  while (p->blocks < most && k > 1024 * p->blocks) p->blocks *= 2;
+  p->m_tiles = kind == kFew16 ? 1 : (rows + 63) / 64;
+  p->split_k = 1024 * p->blocks;
+  p->splits = (k + p->split_k - 1) / p->split_k;
+}
+
 template <typename T>
 static MxPlan mx_plan(int rows, int n, int k) {
   MxPlan p = {};
-  if (rows <= 16) return p;
-  if (rows <= 32) { p.kind = 1; plan_tile<TileDecode32<T>>(&p, rows, n, k); }
-  else if (rows <= 64) { p.kind = 2; plan_tile<TileDecode64<T>>(&p, rows, n, k); }
-  else { p.kind = 3; plan_tile<TilePrompt<T>>(&p, rows, n, k); }
+  p.splits = 1;
+  // kRows: the registers hold 6 blocks a lane of one token, 4 of two (fp32: 4, 2)
+  const int loads = (k + 2047) / 2048, most = (rows == 1 ? 6 : 4) - (sizeof(T) == 4 ? 2 : 0);
+  if (rows <= 2 && loads <= most) {
+    p.kind = kRows;
+    p.blocks = loads <= 2 ? loads : loads <= 4 ? 4 : 6;
+  } else if (rows <= 16) {
+    plan_few(&p, kFew16, sizeof(T) == 4 ? 2 : 4, rows, k);
+  } else if (rows <= 64 && n >= kFewRows && sizeof(T) == 2) {
+    if (rows <= 32) plan_few(&p, kFew32, 4, rows, k);
+    else plan_few(&p, kFew64, 2, rows, k);
+  } else if (rows <= 32) {
+    plan_tile<Tile32<T>>(&p, kTile32, rows, n, k);
+  } else if (rows <= 64) {
+    plan_tile<Tile64<T>>(&p, kTile64, rows, n, k);
+  } else if (rows <= kNarrowTokens) {
+    plan_tile<TileNarrow<T>>(&p, kTileNarrow, rows, n, k);
+  } else {
+    plan_tile<TilePrompt<T>>(&p, kTilePrompt, rows, n, k);
+  }
   return p;
 }
 
@@ -467,7 +850,38 @@ template <typename T, typename S>
 static void launch_tile_shape(const MxLinearArgs &a, hipStream_t s) {
   static_assert(S::kLds <= 160 * 1024, "LDS");
   const unsigned groups = static_cast<unsigned>(a.n_tiles * a.splits + 7) / 8 * 8;
-  mx_tile_kernel<T, S><<<groups * a.m_tiles, S::kThreads, 0, s>>>(a);
+  if (a.vec) mx_tile_kernel<T, S, true><<<groups * a.m_tiles, S::kThreads, 0, s>>>(a);
+  else mx_tile_kernel<T, S, false><<<groups * a.m_tiles, S::kThreads, 0, s>>>(a);
+}
+
+template <typename T, int TOKENS, int LOADS, int ROWS>
+static void launch_rows(const MxLinearArgs &a, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>((a.n + 4 * ROWS - 1) / (4 * ROWS));
+  if (a.vec) mx_rows_kernel<T, TOKENS, LOADS, ROWS, true><<<grid, kMxlThreads, 0, s>>>(a);
+  else mx_rows_kernel<T, TOKENS, LOADS, ROWS, false><<<grid, kMxlThreads, 0, s>>>(a);
+}
+
+// Matrix rows a wave takes: as many as the registers hold beside the tokens
+// (1 x 4096 x 4096 4.1 us with 4 and with 2, 1 x 8192 x 8192 8.4 with 4, 9.5 with 2).
+template <typename T, int TOKENS>
+static void launch_rows(const MxLinearArgs &a, int loads, hipStream_t s) {
+  constexpr bool wide = sizeof(T) == 4;
+  if (loads == 1) return launch_rows<T, TOKENS, 1, 4>(a, s);
+  if (loads == 2) return launch_rows<T, TOKENS, 2, wide && TOKENS == 2 ? 2 : 4>(a, s);
+  if constexpr (!wide || TOKENS == 1)
+    if (loads == 4) return launch_rows<T, TOKENS, 4, wide || TOKENS == 2 ? 2 : 4>(a, s);
+  if constexpr (!wide && TOKENS == 1)
+    if (loads == 6) return launch_rows<T, TOKENS, 6, 2>(a, s);
+}
+
+// One workgroup of eight waves a CU, shared out among the splits.
+template <typename T, int MT, int BL, int RING>
+static void launch_few(const MxLinearArgs &a, hipStream_t s) {
+  const int groups = a.splits * a.m_tiles;
+  const dim3 grid(static_cast<unsigned>(std::min((a.n + 15) / 16, std::max(1, (256 + groups - 1) / groups))),
+                  static_cast<unsigned>(groups));
+  if (a.vec) mx_few_kernel<T, MT, BL, RING, true><<<grid, 512, 0, s>>>(a);
+  else mx_few_kernel<T, MT, BL, RING, false><<<grid, 512, 0, s>>>(a);
 }
 
 template <typename T>
@@ -477,9 +891,33 @@ static void mx_linear_launch(MxLinearArgs a, const MxPlan &p, hipStream_t s) {
   a.splits = p.splits;
   a.split_k = p.split_k;
   switch (p.kind) {
-    case 0: return mx_few_kernel<T><<<(a.n + 15) / 16, kMxlThreads, 0, s>>>(a);
-    case 1: launch_tile_shape<T, TileDecode32<T>>(a, s); break;
-    case 2: launch_tile_shape<T, TileDecode64<T>>(a, s); break;
+    case kRows:
+      if (a.rows == 1) launch_rows<T, 1>(a, p.blocks, s);
+      else launch_rows<T, 2>(a, p.blocks, s);
+      break;
+    // more than one block a lane only where k > 512 times it: a row then has
+    // more than 16 times as many
+    case kFew16:
+      if (p.blocks == 1) launch_few<T, 1, 1, 4>(a, s);
+      else if (p.blocks == 2) launch_few<T, 1, 2, 2>(a, s);
+      else if constexpr (sizeof(T) == 2) launch_few<T, 1, 4, 1>(a, s);
+      break;
+    case kFew32:
+      if constexpr (sizeof(T) == 2) {
+        if (p.blocks == 1) launch_few<T, 2, 1, 4>(a, s);
+        else if (p.blocks == 2) launch_few<T, 2, 2, 2>(a, s);
+        else launch_few<T, 2, 4, 1>(a, s);
+      }
+      break;
+    case kFew64:
+      if constexpr (sizeof(T) == 2) {
+        if (p.blocks == 1) launch_few<T, 4, 1, 4>(a, s);
+        else launch_few<T, 4, 2, 1>(a, s);
+      }
+      break;
+    case kTile32: launch_tile_shape<T, Tile32<T>>(a, s); break;
+    case kTile64: launch_tile_shape<T, Tile64<T>>(a, s); break;
+    case kTileNarrow: launch_tile_shape<T, TileNarrow<T>>(a, s); break;
     default: launch_tile_shape<T, TilePrompt<T>>(a, s);
   }
   if (a.splits > 1) {
@@ -493,6 +931,7 @@ static int mx_linear_check(int rows, int n, int k, int dtype, const char *what) 
     return fail(HEXKV_EINVAL, "%s: unknown dtype %d", what, dtype);
   if (rows < 0 || n < 0 || k < 0) return fail(HEXKV_EINVAL, "%s: negative size", what);
   if (k == 0 || k % kMxBlock) return fail(HEXKV_EINVAL, "%s: k %d is not a positive multiple of %d", what, k, kMxBlock);
+  if (k > (1 << 22)) return fail(HEXKV_ERANGE, "%s: k above 2^22", what);
   if (rows > (1 << 20) || (static_cast<int64_t>(rows) + 63) / 64 * ((n + 15) / 16) >= INT64_C(1) << 24)
     return fail(HEXKV_ERANGE, "%s: over 2^20 tokens, or 2^24 workgroups or more; split the call", what);
   return HEXKV_OK;
@@ -520,6 +959,9 @@ extern "C" int hexkv_mx_linear(const void *x, int64_t x_stride, const void *code
   const int elem = dtype == HEXKV_F32 ? 4 : 2;
   if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & (elem - 1)) || !aligned16(codes))
     return fail(HEXKV_EINVAL, "%s: x/out misaligned, or codes not 16-byte aligned", what);
+  // a tile's tokens are addressed with 32-bit offsets from its first
+  if (rows > 1 && (x_stride < 0 || x_stride > (1 << 22)))
+    return fail(HEXKV_ERANGE, "%s: x_stride %lld outside [0, 2^22]", what, static_cast<long long>(x_stride));
   const MxPlan plan = mx_plan_of(rows, n, k, dtype);
   const size_t need = mx_partial_bytes(plan, rows, n);
   if (need && (!workspace || workspace_bytes < need))

@@ -357,7 +357,13 @@ def linear_tolerance(x, w, want, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,n,k", [(1, 1, 32), (1, 16, 128), (2, 17, 96), (3, 250, 544), (16, 64, 2048), (17, 33, 160),
-                                      (33, 50, 1056), (64, 128, 512), (65, 15, 64), (130, 129, 256), (300, 260, 320)])
+                                      (33, 50, 1056), (64, 128, 512), (65, 15, 64), (130, 129, 256), (300, 260, 320),
+                                      # every kernel, tile and split: whole and ragged shares of the inner dimension
+                                      (1, 41, 2080), (1, 33, 4128), (1, 30, 8224), (1, 18, 12288), (1, 17, 12320),
+                                      (2, 19, 2048), (2, 35, 4064), (2, 21, 8192), (2, 18, 8224), (3, 18, 1056),
+                                      (9, 40, 4128), (16, 33, 9216), (20, 8200, 96), (32, 8192, 1088), (17, 8193, 4160),
+                                      (40, 8192, 160), (64, 8195, 1056), (50, 8192, 4128), (20, 100, 3200),
+                                      (60, 70, 5152), (128, 200, 4096), (193, 140, 2080), (257, 300, 1056)])
 def test_linear(device, dtype, rows, n, k):
     x = randn((rows, k), rows + n, dtype, device)
     w = fp4.quantize(randn((n, k), n + k, torch.float32, device, k ** -0.5))
