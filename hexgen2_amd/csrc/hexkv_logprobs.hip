@@ -3,19 +3,27 @@
 //
 // With m the row's largest logit, S = sum e^(x - m) and U = sum (x - m) e^(x - m):
 //   log p(token) = x_token - m - log S,   entropy = log S - U / S.
-// What bounds it: memory, every logit read once.  A workgroup walks a row (or,
-// where rows are few, a part of one) 8192 logits at a time, 32 of them in each
-// lane's registers; every lane keeps its own (m, S, U), rescaled when its
-// maximum moves, and the lanes' are joined once at the end.
+// What bounds it: memory, every logit read once; beside that about 11 vector
+// instructions a logit, one of them an exponential.  A workgroup walks a row
+// (or, where rows are few, a part of one) 4096 logits at a time, 16 of them in each lane's
+// registers and the next 16 in flight; every lane keeps its own (m, S, U),
+// rescaled when its maximum moves, and the lanes' are joined once at the end.
 //
 // The top alternatives are the largest keys, a key being the logit's order
 // above the complement of its id, so that ties go to the lowest id and no
-// two keys are equal.  The list of the best `top` so far sets the bar; logits above
-// it are collected in LDS and the list is re-ranked by counting, which
-// happens for few of them once a list is full.  Where too many pass the bar
-// (a row's first logits, rising rows), it is raised to the top-th largest of
-// 64 groups' maxima, below which no key can be among the best; where that
-// does not suffice, the largest is taken out `top` times over.
+// two keys are equal.  Every lane keeps the maximum of its logits too; the
+// top-th largest of the lanes' is a bar that at least `top` logits reach, and,
+// logits being spread over the lanes, little more do (21 of 32000 for the top 20).  The
+// lanes whose maximum reaches it, as few, have their logits read again (from
+// the caches) and what reaches the bar is ranked by counting.  Collecting during the walk
+// instead, above the worst of the best so far, doubled a row's time (186 us
+// against 97 without alternatives, 8191 x 32000 bf16): barriers and counting in
+// every step.  Where too many reach the bar (equal logits), those above it are
+// ranked and the lowest ids equal to it follow; where too many are above it, the
+// largest is taken out `top` times over.
+//
+// Measured on MI355X, bf16: 8191 x 32000 without alternatives 97 us (5.4 TB/s),
+// with the top 20 125 us (4.2); one row of 32000 fp16, top 5, 9.0 us (8 parts and their join).
 #include "hexkv_common.h"
 
 #include <algorithm>
@@ -24,9 +32,9 @@ namespace hexkv {
 
 constexpr int kLpThreads = 256;
 constexpr int kLpWaves = kLpThreads / 64;
-constexpr int kLpEach = 32;  // logits a lane holds at a time
+constexpr int kLpEach = 16;  // logits a lane holds at a time
 constexpr int kLpChunk = kLpThreads * kLpEach;
-constexpr int kLpRoom = 512;  // keys collected at a time, beside the list
+constexpr int kLpRoom = 256;  // keys that can be ranked
 constexpr int kLpMaxParts = 32;
 
 struct LogprobArgs {
@@ -74,38 +82,54 @@ struct LpStats {
     if (w == 0.f && s == s) s = u = 0.f;
     m = to;
   }
+  // Neither a probability nor a logarithm to give: minus infinities alone.
+  __device__ __forceinline__ bool none() const { return m == -INFINITY && s == 0.f; }
 };
 
 // What a row answers with, from its joined statistics.
-__device__ __forceinline__ void lp_finish(const LogprobArgs &a, int64_t row, const LpStats &st, float token_logit,
-                                          bool token_in) {
+template <typename T>
+__device__ __forceinline__ void lp_finish(const LogprobArgs &a, int64_t row, const LpStats &st) {
   const float log_s = logf(st.s);
-  // a row of minus infinities has no probability to give
-  const bool none = st.m == -INFINITY && st.s == 0.f;
-  if (a.entropy) a.entropy[row] = none ? 0.f : log_s - st.u / st.s;
+  if (a.entropy) a.entropy[row] = st.none() ? 0.f : log_s - st.u / st.s;
   if (a.tokens) {
     const int64_t t = a.tokens[row];
-    float lp = none ? -INFINITY : token_logit - st.m - log_s;
-    if (!token_in) lp = t < 0 ? 0.f : NAN;
+    float lp = t < 0 ? 0.f : NAN;
+    if (t >= 0 && t < a.vocab) {
+      const float x = static_cast<float>(static_cast<const T *>(a.logits)[row * a.stride + t]);
+      lp = st.none() ? -INFINITY : x - st.m - log_s;
+    }
     a.logprob[row] = lp;
   }
 }
 
 __device__ __forceinline__ void lp_write_top(const LogprobArgs &a, int64_t row, int rank, lp_key key, const LpStats &st) {
-  const bool none = st.m == -INFINITY && st.s == 0.f;
   const float v = lp_key_value(key);
   a.top_ids[row * a.top + rank] = lp_key_id(key);
-  a.top_logprobs[row * a.top + rank] = none ? -INFINITY : v - st.m - logf(st.s);
+  a.top_logprobs[row * a.top + rank] = st.none() ? -INFINITY : v - st.m - logf(st.s);
+}
+
+// One wave: the lowest ids in [first, last) of row x whose logit equals `value`,
+// as keys at ranks from `held` to `top`; returns how many ranks are held then.
+template <typename T>
+__device__ __forceinline__ int lp_equal(const T *x, int64_t first, int64_t last, float value, int held, int top, lp_key *list) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t base = first; base < last && held < top; base += 64) {
+    const int64_t id = base + lane;
+    const bool out = id < last && static_cast<float>(x[min(id, last - 1)]) == value;
+    const uint64_t mask = __ballot(out);
+    const int rank = held + __popcll(mask & ((uint64_t{1} << lane) - 1));
+    if (out && rank < top) list[rank] = lp_make_key(value, static_cast<unsigned int>(id));
+    held = min(top, held + __popcll(mask));
+  }
+  return held;
 }
 
 template <typename T>
 __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a) {
   constexpr int VEC = 16 / sizeof(T), NV = kLpEach / VEC;
-  __shared__ lp_key s_list[64 + kLpRoom];  // the best so far, then what was collected
-  __shared__ lp_key s_best[64];
-  __shared__ lp_key s_wave[kLpWaves];
-  __shared__ int s_count;
-  __shared__ lp_key s_bar;
+  __shared__ lp_key s_list[kLpRoom], s_best[64], s_wave[kLpWaves];
+  __shared__ float s_lane[kLpThreads], s_bar;
+  __shared__ int s_active[kLpThreads], s_active_count, s_count[2], s_held;
   __shared__ float s_stats[kLpWaves][3];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / static_cast<unsigned>(a.parts);
@@ -117,146 +141,92 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
   const int64_t last = min(first + a.span, static_cast<int64_t>(a.vocab) + skew);
   const int top = a.top;
   LpStats st = {-INFINITY, 0.f, 0.f};
-  int held = 0;  // keys in the list
-  if (top) {
-    if (tid < 64) s_list[tid] = 0;
-    if (tid == 0) s_count = 0;
-    __syncthreads();
-  }
+  float best = -INFINITY;  // NaN where there is one
 
+  u32x4 raw[NV];
+  // Whether every place of a chunk is a logit of this part: then it is loaded ahead.
+  const auto whole = [&](int64_t base) { return base >= skew && base + kLpChunk <= last; };
+  const auto fetch = [&](int64_t base) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      raw[i] = *reinterpret_cast<const u32x4 *>(x + (base - skew) + (i * kLpThreads + tid) * VEC);
+  };
+  // The vector at place `at` of the row; a place outside the part counts as
+  // minus infinity, which adds nothing and is never collected.
+  const auto vector_at = [&](int64_t at, float *v) {
+    if (at >= 0 && at + skew >= first && at + skew + VEC <= last) {
+      Elem<T>::to_float(*reinterpret_cast<const u32x4 *>(x + at), v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int64_t id = at + e;
+        v[e] = id >= 0 && id + skew < last ? static_cast<float>(x[id]) : -INFINITY;
+      }
+    }
+  };
+  if (whole(first)) fetch(first);
   for (int64_t base = first; base < last; base += kLpChunk) {
     float v[kLpEach];
+    if (whole(base)) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int64_t at = base + (i * kLpThreads + tid) * VEC - skew;
-      if (at >= 0 && at + VEC <= a.vocab && at + skew + VEC <= last) {
-        if constexpr (sizeof(T) == 2) Elem<T>::to_float(*reinterpret_cast<const u32x4 *>(x + at), v + i * VEC);
-        else Elem<T>::to_float(*reinterpret_cast<const u32x4 *>(x + at), v + i * VEC);
-      } else {
+      for (int i = 0; i < NV; ++i) Elem<T>::to_float(raw[i], v + i * VEC);
+    } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const int64_t id = at + e;
-          v[i * VEC + e] = id >= 0 && id < a.vocab && id + skew < last ? static_cast<float>(x[id]) : -INFINITY;
-        }
-      }
+      for (int i = 0; i < NV; ++i) vector_at(base + (i * kLpThreads + tid) * VEC - skew, v + i * VEC);
     }
-    // (A place outside the row counts as minus infinity, which adds nothing; it
-    // is kept from the keys below.)
-    float m = st.m;
+    if (base + kLpChunk < last && whole(base + kLpChunk)) fetch(base + kLpChunk);
+    float most = v[0];
 #pragma unroll
-    for (int i = 0; i < kLpEach; ++i) m = fmaxf(m, v[i]);
-    st.shift(m);
+    for (int i = 1; i < kLpEach; ++i) most = __builtin_elementwise_maximum(most, v[i]);
+    best = __builtin_elementwise_maximum(best, most);
+    st.shift(fmaxf(st.m, most));
+    // Below -200 an exponential is 0 in any case; kept finite, it adds 0 to U too.
+    const float m = st.m == -INFINITY ? 0.f : st.m;
 #pragma unroll
     for (int i = 0; i < kLpEach; ++i) {
-      const float d = v[i] - st.m, w = lp_exp(d);
-      if (v[i] == -INFINITY) continue;
+      const float d = __builtin_elementwise_maximum(v[i] - m, -200.f), w = lp_exp(d);
       st.s += w;
-      st.u += w == 0.f ? 0.f : d * w;
-    }
-    if (!top) continue;
-
-    const auto id_of = [&](int i) { return base + ((i / VEC) * kLpThreads + tid) * VEC + i % VEC - skew; };
-    const auto key_of = [&](int i) -> lp_key {
-      const int64_t id = id_of(i);
-      return id >= 0 && id < a.vocab && id + skew < last ? lp_make_key(v[i], static_cast<unsigned int>(id)) : 0;
-    };
-    lp_key bar = held == top ? s_list[top - 1] : 0;  // keys have to exceed it
-    bool raised = false;
-    for (;;) {
-      // collect what exceeds the bar
-      bool over = false;
-#pragma unroll
-      for (int i = 0; i < kLpEach; ++i) {
-        const lp_key k = key_of(i);
-        if (k > bar && !over) {
-          const int at = atomicAdd(&s_count, 1);
-          if (at < kLpRoom) s_list[64 + at] = k;
-          else over = true;
-        }
-      }
-      __syncthreads();
-      const int count = s_count;
-      __syncthreads();  // read by all before anyone counts again
-      if (count == 0) break;
-      if (count <= kLpRoom) {
-        // rank the list and what was collected by counting
-        const int total = 64 + count;
-        for (int i = tid; i < total; i += kLpThreads) {
-          const lp_key k = s_list[i];
-          int rank = 0;
-          for (int j = 0; j < total; ++j) rank += s_list[j] > k;
-          if (k && rank < 64) s_best[rank] = k;
-        }
-        __syncthreads();
-        const int known = min(top, held + count);
-        if (tid < 64) s_list[tid] = tid < known ? s_best[tid] : 0;
-        if (tid == 0) s_count = 0;
-        held = known;
-        __syncthreads();
-        break;
-      }
-      if (tid == 0) s_count = 0;
-      if (!raised) {
-        // the top-th largest of 64 groups' maxima
-        raised = true;
-        lp_key best = 0;
-#pragma unroll
-        for (int i = 0; i < kLpEach; ++i) best = max(best, key_of(i));
-        best = max(best, lp_shfl_xor(best, 1));
-        best = max(best, lp_shfl_xor(best, 2));
-        if (lane % 4 == 0) s_best[wave * 16 + lane / 4] = best;
-        __syncthreads();
-        if (tid < 64) {
-          const lp_key k = s_best[tid];
-          int rank = 0;
-          for (int j = 0; j < 64; ++j) rank += s_best[j] > k;
-          const int groups = __popcll(__ballot(k != 0));  // (a group without a logit has key 0)
-          if (groups < top ? tid == 0 : k && rank == top - 1) s_bar = groups < top ? 1 : k;
-        }
-        __syncthreads();
-        bar = max(bar, s_bar - 1);
-        __syncthreads();
-        continue;
-      }
-      // take the largest out `top` times over, from the list and the lanes
-      __syncthreads();
-      lp_key below = ~static_cast<lp_key>(0);
-      const lp_key mine = tid < 64 ? s_list[tid] : 0;
-      int found = 0;
-      for (; found < top; ++found) {
-        lp_key best = mine < below ? mine : 0;
-#pragma unroll
-        for (int i = 0; i < kLpEach; ++i) {
-          const lp_key k = key_of(i);
-          if (k < below) best = max(best, k);
-        }
-        for (int off = 1; off < 64; off <<= 1) best = max(best, lp_shfl_xor(best, off));
-        if (lane == 0) s_wave[wave] = best;
-        __syncthreads();
-        best = max(max(s_wave[0], s_wave[1]), max(s_wave[2], s_wave[3]));
-        if (tid == 0) s_best[found] = best;
-        __syncthreads();
-        if (!best) break;
-        below = best;
-      }
-      if (tid < 64) s_list[tid] = tid < found ? s_best[tid] : 0;
-      held = found;
-      __syncthreads();
-      break;
+      st.u = fmaf(d, w, st.u);
     }
   }
 
   // join the lanes
   float m = wave_max(st.m);
   if (lane == 0) s_stats[wave][0] = m;
+  if (best != best) best = INFINITY;  // a NaN is the largest there is
+  s_lane[tid] = best;
+  if (tid < 2) s_count[tid] = 0;
+  if (tid == 0) s_active_count = 0;
   __syncthreads();
   m = fmaxf(fmaxf(s_stats[0][0], s_stats[1][0]), fmaxf(s_stats[2][0], s_stats[3][0]));
-  __syncthreads();
   st.shift(m);
   const float s_sum = sum_from<1>(st.s), u_sum = sum_from<1>(st.u);
   if (lane == 0) {
     s_stats[wave][1] = s_sum;
     s_stats[wave][2] = u_sum;
+  }
+  // The bar: the top-th largest of the lanes' maxima (equal ones in the lanes'
+  // order), of 64 groups of four while those are several times as many as `top`.
+  if (top && top <= 24) {
+    if (wave == 0) {
+      const f32x4 four = *reinterpret_cast<const f32x4 *>(s_lane + 4 * lane);
+      const float mine = fmaxf(fmaxf(four[0], four[1]), fmaxf(four[2], four[3]));
+      int rank = 0;
+#pragma unroll
+      for (int j = 0; j < 64; ++j) {
+        const float other = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), j));
+        rank += other > mine || (other == mine && j < lane);
+      }
+      if (rank == top - 1) s_bar = mine;
+    }
+  } else if (top) {
+    int rank = 0;
+    for (int j = 0; j < kLpThreads; j += 4) {
+      const f32x4 four = *reinterpret_cast<const f32x4 *>(s_lane + j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) rank += four[e] > best || (four[e] == best && j + e < tid);
+    }
+    if (rank == top - 1) s_bar = best;
   }
   __syncthreads();
   LpStats all = {m, 0.f, 0.f};
@@ -265,66 +235,161 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
     all.s += s_stats[w][1];
     all.u += s_stats[w][2];
   }
+
+  int held = 0;  // ranked keys in s_best
+  if (top) {
+    const float bar = s_bar;
+    if (!(best < bar) && best > -INFINITY) s_active[atomicAdd(&s_active_count, 1)] = tid;
+    __syncthreads();
+    const int vectors = static_cast<int>((last - first + kLpChunk - 1) / kLpChunk) * NV, total = s_active_count * vectors;
+    // the active lanes' vectors, shared out over all lanes (in any order: the ranks do not depend on it)
+    const auto collect = [&](bool equal, int *counter) {
+      for (int item = tid; item < total; item += kLpThreads) {
+        const int of = item / vectors, j = item - of * vectors;
+        const int64_t at = first + static_cast<int64_t>(j / NV) * kLpChunk + (j % NV * kLpThreads + s_active[of]) * VEC - skew;
+        float v[VEC];
+        vector_at(at, v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if ((equal ? !(v[e] < bar) : !(v[e] <= bar)) && v[e] != -INFINITY) {
+            const int place = atomicAdd(counter, 1);
+            if (place < kLpRoom) s_list[place] = lp_make_key(v[e], static_cast<unsigned int>(at + e));
+          }
+      }
+    };
+    // Ranks by counting the larger keys: one wave by lane reads where a key
+    // fits a lane each, as it nearly always does, else every lane over all in LDS.
+    const auto rank_list = [&](int count) {
+      if (count <= 64) {
+        if (wave == 0) {
+          const lp_key k = lane < count ? s_list[lane] : 0;
+          const int lo = static_cast<int>(k), hi = static_cast<int>(k >> 32);
+          int rank = 0;
+          for (int j = 0; j < count; ++j) {
+            const lp_key other = static_cast<lp_key>(static_cast<unsigned int>(__builtin_amdgcn_readlane(hi, j))) << 32 |
+                                 static_cast<unsigned int>(__builtin_amdgcn_readlane(lo, j));
+            rank += other > k;
+          }
+          if (lane < count && rank < top) s_best[rank] = k;
+        }
+      } else {
+        for (int i = tid; i < count; i += kLpThreads) {
+          const lp_key k = s_list[i];
+          int rank = 0;
+          for (int j = 0; j < count; ++j) rank += s_list[j] > k;
+          if (rank < top) s_best[rank] = k;
+        }
+      }
+      held = min(top, count);
+      __syncthreads();
+    };
+    collect(true, &s_count[0]);
+    __syncthreads();
+    int count = s_count[0];
+    if (count <= kLpRoom) {
+      rank_list(count);
+    } else {
+      collect(false, &s_count[1]);
+      __syncthreads();
+      count = s_count[1];
+      if (count <= kLpRoom) {
+        rank_list(count);
+        if (wave == 0 && held < top) {
+          const int64_t from = max(first - skew, INT64_C(0));
+          const int now = bar == -INFINITY ? held : lp_equal(x, from, last - skew, bar, held, top, s_best);
+          if (lane == 0) s_held = now;
+        } else if (tid == 0) {
+          s_held = held;
+        }
+        __syncthreads();
+        held = s_held;
+      } else {
+        lp_key below = ~static_cast<lp_key>(0);
+        for (; held < top; ++held) {
+          lp_key k = 0;
+#pragma unroll 1
+          for (int64_t id = max(first - skew, INT64_C(0)) + tid; id + skew < last; id += kLpThreads) {
+            const float v = static_cast<float>(x[id]);
+            const lp_key other = v == -INFINITY ? 0 : lp_make_key(v, static_cast<unsigned int>(id));
+            if (other < below) k = max(k, other);
+          }
+          for (int off = 1; off < 64; off <<= 1) k = max(k, lp_shfl_xor(k, off));
+          if (lane == 0) s_wave[wave] = k;
+          __syncthreads();
+          k = max(max(s_wave[0], s_wave[1]), max(s_wave[2], s_wave[3]));
+          if (tid == 0) s_best[held] = k;
+          __syncthreads();
+          if (!k) break;
+          below = k;
+        }
+      }
+    }
+  }
   if (a.parts > 1) {
     if (tid == 0) *reinterpret_cast<f32x4 *>(a.ws_stats + (row * a.parts + part) * 4) = f32x4{all.m, all.s, all.u, 0.f};
-    if (tid < top) a.ws_keys[(row * a.parts + part) * top + tid] = s_list[tid];
+    if (tid < top) a.ws_keys[(row * a.parts + part) * top + tid] = tid < held ? s_best[tid] : 0;
     return;
   }
-  if (tid == 0) {
-    float logit = 0.f;
-    bool in = false;
-    if (a.tokens) {
-      const int64_t t = a.tokens[row];
-      in = t >= 0 && t < a.vocab;
-      if (in) logit = static_cast<float>(x[t]);
-    }
-    lp_finish(a, row, all, logit, in);
+  if (tid == 0) lp_finish<T>(a, row, all);
+  // a list that ends short is filled with minus infinities, none of which was collected
+  if (wave == 0) {
+    if (held < top) lp_equal(x, 0, a.vocab, -INFINITY, held, top, s_best);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (lane < top) lp_write_top(a, row, lane, s_best[lane], all);
   }
-  if (tid < top) lp_write_top(a, row, tid, s_list[tid], all);
 }
 
 // Joins a row's parts.
 template <typename T>
 __global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(const LogprobArgs a) {
-  __shared__ lp_key s_keys[kLpMaxParts * 64];
+  __shared__ lp_key s_keys[kLpMaxParts * 64], s_best[64];
+  __shared__ int s_keyed;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
-  const float *stats = a.ws_stats + row * a.parts * 4;
+  const int lane = tid & 63;
+  // a part a lane (every wave for itself)
   LpStats all = {-INFINITY, 0.f, 0.f};
-  for (int p = 0; p < a.parts; ++p) all.m = fmaxf(all.m, stats[4 * p]);
-  for (int p = 0; p < a.parts; ++p) {
-    LpStats st = {stats[4 * p], stats[4 * p + 1], stats[4 * p + 2]};
-    st.shift(all.m);
-    all.s += st.s;
-    all.u += st.u;
+  if (lane < a.parts) {
+    const f32x4 v = *reinterpret_cast<const f32x4 *>(a.ws_stats + (row * a.parts + lane) * 4);
+    all = LpStats{v[0], v[1], v[2]};
   }
-  if (tid == 0) {
-    float logit = 0.f;
-    bool in = false;
-    if (a.tokens) {
-      const int64_t t = a.tokens[row];
-      in = t >= 0 && t < a.vocab;
-      if (in) logit = static_cast<float>(static_cast<const T *>(a.logits)[row * a.stride + t]);
-    }
-    lp_finish(a, row, all, logit, in);
-  }
+  all.shift(wave_max(all.m));
+  all = LpStats{wave_max(all.m), sum_from<1>(all.s), sum_from<1>(all.u)};
+  if (tid == 0) lp_finish<T>(a, row, all);
   if (!a.top) return;
   const int n = a.parts * a.top;
+  if (tid == 0) s_keyed = 0;
   for (int i = tid; i < n; i += kLpThreads) s_keys[i] = a.ws_keys[row * n + i];
   __syncthreads();
   for (int i = tid; i < n; i += kLpThreads) {
     const lp_key k = s_keys[i];
+    if (!k) continue;
     int rank = 0;
     for (int j = 0; j < n; ++j) rank += s_keys[j] > k;
-    if (k && rank < a.top) lp_write_top(a, row, rank, k, all);
+    if (rank < a.top) {
+      s_best[rank] = k;
+      atomicAdd(&s_keyed, 1);
+    }
+  }
+  __syncthreads();
+  if (tid < 64) {
+    if (s_keyed < a.top)
+      lp_equal(static_cast<const T *>(a.logits) + row * a.stride, 0, a.vocab, -INFINITY, s_keyed, a.top, s_best);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (tid < a.top) lp_write_top(a, row, tid, s_best[tid], all);
   }
 }
 
-// Parts a row is cut into: one where the rows alone give every CU several
-// workgroups.
+// Parts a row is cut into: enough for a workgroup a CU, and for few rows of long
+// vocabularies about twelve chunks each.
 static int lp_parts(int64_t rows, int vocab, int64_t *span) {
   const int64_t chunks = (static_cast<int64_t>(vocab) + 7 + kLpChunk - 1) / kLpChunk;
-  const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>({chunks, kLpMaxParts, 1024 / std::max<int64_t>(rows, 1)}));
+  // (64 x 128000, top 20: 17 us at one workgroup a CU, 25.6 at four; 300 x 128000:
+  // 31.5 us in one part, 25.9 in three)
+  const int64_t fill = 256 / std::max<int64_t>(rows, 1), long_rows = rows < 1024 ? chunks / 12 : 1;
+  const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>({chunks, kLpMaxParts, std::max(fill, long_rows)}));
   const int64_t each = (chunks + wanted - 1) / wanted;
   *span = each * kLpChunk;
   return static_cast<int>((chunks + each - 1) / each);
