@@ -13,6 +13,11 @@ same validation errors.  What changes is where the bytes go:
   layers into a single preallocated decode cache (model.py:104-108 allocated
   and copied per layer);
 * each decode step appends and attends through hexkv (mha.py:286, 568-569).
+
+Additions: ``kv_bits`` 4 keeps and hands over the caches in four bits (uint8 rows,
+``{layer: [1, L, row_bytes]}``; a prompt attends its own keys unrounded),
+``weight_bits`` 4 the layers' matrices, and ``decode(on_logprobs=...)`` and
+``score`` report what the logits say of the tokens.
 """
 from __future__ import annotations
 
@@ -22,9 +27,10 @@ from pathlib import Path
 
 import torch
 
-from . import ops
+from . import fp4, ops
 from .generation import CacheState
 from .llama import LlamaHost, LlamaShape, read_config
+from .logprobs import TokenLogprobs, token_logprobs
 from .mha import check_kv_status
 
 
@@ -46,7 +52,9 @@ def model_identity(model_dir) -> dict:
 
 class Engine:
     def __init__(self, model_dir, engine="native", device="cuda", dtype="float16",
-                 fused_append: bool = False):
+                 fused_append: bool = False, *, kv_bits: int = 16, weight_bits: int = 16):
+        if kv_bits not in (16, 4) or weight_bits not in (16, 4):
+            raise ValueError(f"caches and weights hold 16 bits (their dtype) or 4, got {kv_bits} and {weight_bits}")
         self.device, self.dtype = torch.device(device), getattr(torch, dtype)
         self.shape = LlamaShape.from_config(read_config(model_dir))
         self.identity = model_identity(model_dir)
@@ -56,7 +64,9 @@ class Engine:
                              "hf-reference engine is the reference's CPU validator")
         if self.device.type != "cuda" or not torch.cuda.is_available():
             raise ValueError("The hexkv engine requires a HIP GPU (torch.cuda on ROCm)")
-        self.model = LlamaHost.load(model_dir, self.device, self.dtype)
+        self.kv_bits = kv_bits
+        self._cache_row()  # (refuses heads that a 4-bit cache cannot hold)
+        self.model = LlamaHost.load(model_dir, self.device, self.dtype, weight_bits)
         self.fused_append = fused_append
         self.config = self.shape
 
@@ -64,10 +74,17 @@ class Engine:
         s = self.shape
         return s.num_hidden_layers, s.num_key_value_heads, s.head_dim
 
+    def _cache_row(self):
+        """Shape and type of one position's cache row."""
+        _, kv_heads, head_dim = self._cache_geometry()
+        if self.kv_bits == 4:
+            return (fp4.row_bytes(kv_heads, head_dim),), torch.uint8
+        return (2, kv_heads, head_dim), self.dtype
+
     @torch.inference_mode()
     def prefill(self, input_ids, max_new_tokens):
         ids = torch.tensor([input_ids], dtype=torch.long, device=self.device)
-        state = CacheState(len(input_ids) + max_new_tokens)
+        state = CacheState(len(input_ids) + max_new_tokens, kv_bits=self.kv_bits)
         logits = self.model.forward(ids, inference_params=state, last_token_only=True)
         n_layers = len(state.key_value_memory_dict)
         layers = [state.key_value_memory_dict[i] for i in range(n_layers)]
@@ -77,7 +94,7 @@ class Engine:
         row_shape = layers[0].shape[2:]
         nbytes = n_layers * len(input_ids) * layers[0][0, 0].numel() * layers[0].element_size()
         if nbytes >= PER_LAYER_HANDOFF_BYTES:
-            out = [torch.empty((len(input_ids), *row_shape), dtype=self.dtype, device=self.device)
+            out = [torch.empty((len(input_ids), *row_shape), dtype=layers[0].dtype, device=self.device)
                    for _ in range(n_layers)]
             packed = ops.pack_live(layers, [len(input_ids)], out=out)
         else:
@@ -86,27 +103,31 @@ class Engine:
         return logits.argmax(-1), cache, logits
 
     @torch.inference_mode()
-    def decode(self, first_token, cache, prompt_length, max_new_tokens, on_token=None, *, on_logits=None):
+    def decode(self, first_token, cache, prompt_length, max_new_tokens, on_token=None, *, on_logits=None,
+               on_logprobs=None, top_logprobs=0):
         """Greedy decode from the handed-off cache (model.py:86-120).
         ``on_logits`` (an addition) receives each decode step's logits
-        ``[1, vocab]``, for logit-level checks."""
+        ``[1, vocab]``, for logit-level checks; ``on_logprobs`` (another) each
+        decode step's ``TokenLogprobs`` of the token taken, with the
+        ``top_logprobs`` likeliest ones.  (The first token's are
+        ``token_logprobs`` of the logits ``prefill`` returns.)"""
         token = first_token.to(self.device).reshape(1)
         generated = [int(token.item())]
         if on_token:
             on_token(generated[-1])
-        n_layers, kv_heads, head_dim = self._cache_geometry()
+        n_layers = self._cache_geometry()[0]
+        row_shape, row_dtype = self._cache_row()
         if set(cache) != set(range(n_layers)):
             raise ValueError("KV cache does not match the configured layer count")
-        expected = (1, prompt_length, 2, kv_heads, head_dim)
+        expected = (1, prompt_length, *row_shape)
         for value in cache.values():
-            if tuple(value.shape) != expected or value.dtype != self.dtype:
+            if tuple(value.shape) != expected or value.dtype != row_dtype:
                 raise ValueError("KV cache shape/dtype does not match checkpoint and prompt")
-        state = CacheState(prompt_length + max_new_tokens)
+        state = CacheState(prompt_length + max_new_tokens, kv_bits=self.kv_bits)
         state.sequence_len_offset = prompt_length
         # One decode cache for all layers; rows >= prompt_length stay
         # uninitialised as in model.py:105.
-        full = torch.empty((n_layers, 1, state.max_sequence_len, 2, kv_heads, head_dim),
-                           device=self.device, dtype=self.dtype)
+        full = torch.empty((n_layers, 1, state.max_sequence_len, *row_shape), device=self.device, dtype=row_dtype)
         live = [cache[i].to(self.device) for i in range(n_layers)]
         live = [t if t.is_contiguous() else t.contiguous() for t in live]
         ops.unpack_live(live, full, [prompt_length])
@@ -120,6 +141,8 @@ class Engine:
             if on_logits:
                 on_logits(logits)
             token = logits.argmax(-1)
+            if on_logprobs:
+                on_logprobs(token_logprobs(logits, token, top_logprobs))
             generated.append(int(token.item()))
             # the token read synchronised: report any out-of-contract device
             # position the step's kernels met (mha.py:281-282's assert)
@@ -127,6 +150,17 @@ class Engine:
             if on_token:
                 on_token(generated[-1])
         return generated
+
+    @torch.inference_mode()
+    def score(self, input_ids, top_logprobs=0) -> TokenLogprobs:
+        """What the model says of a sequence's tokens: entry t of each result
+        belongs to ``input_ids[t + 1]`` after the t + 1 tokens before it."""
+        if not len(input_ids):
+            raise ValueError("score needs a token")
+        ids = torch.tensor([input_ids], dtype=torch.long, device=self.device)
+        state = CacheState(len(input_ids), kv_bits=self.kv_bits)
+        logits = self.model.forward(ids, inference_params=state, last_token_only=False)
+        return token_logprobs(logits[0, :-1], ids[0, 1:], top_logprobs)
 
     def synchronize(self):
         if self.device.type == "cuda":

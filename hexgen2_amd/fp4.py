@@ -212,7 +212,7 @@ def decode_attention(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, *, max
                 break
     p, needs = _lib.MxAttendParams.from_buffer_copy(form[0]), form[1]
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     p.q, p.cache, p.out, p.capacity = q.data_ptr(), cache.data_ptr(), out.data_ptr(), shape[1]
     if kv_new is not None:
         p.kv_new = kv_new.data_ptr()

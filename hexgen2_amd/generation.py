@@ -1,6 +1,6 @@
 """Cache-state type of the decode path.
 
-Same fields and defaults as hexgen_core's ``InferenceParams``
+Fields and defaults of hexgen_core's ``InferenceParams``
 (hexgen/hexgen_core/generation.py:20-30) and the pilot's ``CacheState``
 (hexgen2/model.py:11-19), so callers written against either keep working.
 """
@@ -24,7 +24,8 @@ class InferenceParams:
     ``lengths_per_sample`` (int32, device), when set, gives each sequence's
     own position (its cached length) in a ragged decode batch, on the FT path
     and on the standard layout alike; ``sequence_len_offset`` then bounds
-    every sample's position.
+    every sample's position.  ``kv_bits`` (an addition) 4 keeps the caches in
+    four bits, ``[max_batch_size, max_sequence_len, row_bytes]`` (``fp4``).
     """
     max_sequence_len: int
     max_batch_size: int = 1
@@ -33,6 +34,7 @@ class InferenceParams:
     key_value_memory_dict: dict = field(default_factory=dict)
     fused_ft_kernel: bool = False
     lengths_per_sample: Optional[torch.Tensor] = None
+    kv_bits: int = 16
 
 
 # hexgen2/model.py:11-19 names the same record CacheState.

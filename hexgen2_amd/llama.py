@@ -15,7 +15,9 @@ long for it); the steps between them are one hexkv launch each (residual sum
 and RMSNorm, head split and rotary, SwiGLU).  For one or two tokens the
 products are hexkv's too (``ops.norm_linear``, ``ops.norm_rope_linear``), with
 the norm before and the rotary or SwiGLU after them in the same launch.  Every
-KV byte moves through hexkv.
+KV byte moves through hexkv.  With ``weight_bits`` 4 the layers' matrices are
+rounded to four bits when the host is built and multiplied by ``fp4.linear``
+(the embedding, the norms and the LM head stay as they are).
 """
 from __future__ import annotations
 
@@ -26,7 +28,7 @@ from pathlib import Path
 import torch
 import torch.nn.functional as F
 
-from . import ops
+from . import fp4, ops
 from .mha import FlashCrossAttention, _apply_rotary_single_query_attention, _update_kv_cache, update_and_attend
 
 
@@ -79,7 +81,9 @@ class LlamaHost:
     """Greedy-decode host; ``forward`` mirrors GPTLMHeadModel.forward's
     ``(input_ids, inference_params, last_token_only)`` contract."""
 
-    def __init__(self, shape: LlamaShape, weights: dict, device, dtype):
+    def __init__(self, shape: LlamaShape, weights: dict, device, dtype, weight_bits: int = 16):
+        if weight_bits not in (16, 4):
+            raise ValueError(f"weights hold 16 bits (their dtype) or 4, not {weight_bits}")
         self.shape = shape
         self.device, self.dtype = torch.device(device), dtype
         w = {k: v.to(device=self.device, dtype=dtype) for k, v in weights.items()}
@@ -98,6 +102,11 @@ class LlamaHost:
                 "gate_up": torch.cat([w.pop(p + f"mlp.{n}_proj.weight") for n in ("gate", "up")]),
                 "down": w[p + "mlp.down_proj.weight"],
             })
+        if weight_bits == 4:
+            for layer in self.layers:
+                for name in ("wqkv", "wo", "gate_up", "down"):
+                    layer[name] = fp4.quantize(layer[name])
+            del w
         d = shape.head_dim
         self.inv_freq = 1.0 / (shape.rope_theta ** (torch.arange(0, d, 2, device=self.device,
                                                                   dtype=torch.float32) / d))
@@ -105,7 +114,7 @@ class LlamaHost:
         self.attn = FlashCrossAttention(causal=True, softmax_scale=self.scale)
 
     @classmethod
-    def load(cls, model_dir, device, dtype) -> "LlamaHost":
+    def load(cls, model_dir, device, dtype, weight_bits: int = 16) -> "LlamaHost":
         from safetensors.torch import load_file
         shape = LlamaShape.from_config(read_config(model_dir))
         shards = sorted(Path(model_dir).glob("*.safetensors"))
@@ -117,19 +126,26 @@ class LlamaHost:
             if set(state).intersection(values):
                 raise ValueError("Duplicate checkpoint keys")
             state.update(values)
-        return cls(shape, state, device, dtype)
+        return cls(shape, state, device, dtype, weight_bits)
 
     def _norm_linear(self, h, y, norm, weight, glu=False, keep_sum=True):
         """``(product, h + y)`` of RMSNorm(h + y) and ``weight``, with ``glu``
         SwiGLU of its two halves: one launch for a few tokens, else the norm's,
         the library product and the SwiGLU's."""
-        if ops.linear_fits(h, norm, weight):
+        if self._fits(weight, h, norm):
             return ops.norm_linear(h, y, norm, self.shape.rms_norm_eps, weight, glu, keep_sum)
-        x = F.linear(ops.add_rms_norm(h, y, norm, self.shape.rms_norm_eps, keep_sum), weight)
+        x = self._linear(ops.add_rms_norm(h, y, norm, self.shape.rms_norm_eps, keep_sum), weight, False)
         return (ops.silu_mul(x) if glu else x), h
 
-    def _linear(self, x, weight):
-        if ops.linear_fits(x, weight):
+    @staticmethod
+    def _fits(weight, *others):
+        """Whether ``ops.norm_linear`` takes this product (16-bit weights, few tokens)."""
+        return not isinstance(weight, fp4.Fp4Tensor) and ops.linear_fits(*others, weight)
+
+    def _linear(self, x, weight, few=True):
+        if isinstance(weight, fp4.Fp4Tensor):
+            return fp4.linear(x, weight)
+        if few and ops.linear_fits(x, weight):
             return ops.norm_linear(x, None, None, 0.0, weight)[0]
         return F.linear(x, weight)
 
@@ -157,7 +173,7 @@ class LlamaHost:
                 kv = qkv[..., heads * d:].view(batch, seqlen, 2, kv_heads, d)
                 context = _apply_rotary_single_query_attention(q, inference_params, i, d, s.rope_theta, kv=kv)
             else:
-                if ops.linear_fits(h, layer["ln1"], layer["wqkv"]):
+                if self._fits(layer["wqkv"], h, layer["ln1"]):
                     q, kv, h = ops.norm_rope_linear(h, y, layer["ln1"], s.rms_norm_eps, layer["wqkv"], heads, kv_heads, d,
                                                     self.inv_freq, offset, positions)
                 else:

@@ -7,6 +7,7 @@ The reference's engines read no more of the logits than their argmax
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -24,6 +25,11 @@ class TokenLogprobs(NamedTuple):
     entropy: torch.Tensor
     top_logprobs: Optional[torch.Tensor]
     top_ids: Optional[torch.Tensor]
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(rows: int, vocab: int, top: int) -> int:
+    return int(_lib.load().hexkv_token_logprobs_workspace_bytes(rows, vocab, top))
 
 
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
@@ -53,12 +59,12 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     rows = logits.numel() // vocab
     device = logits.device
     entropy = torch.empty(shape, dtype=torch.float32, device=device)
-    logprob = None if tokens is None else torch.empty(shape, dtype=torch.float32, device=device)
+    logprob = None if tokens is None else torch.empty_like(entropy)
     values = ids = None
     if top:
         values = torch.empty((*shape, top), dtype=torch.float32, device=device)
         ids = torch.empty((*shape, top), dtype=torch.int64, device=device)
-    need = int(_lib.load().hexkv_token_logprobs_workspace_bytes(rows, vocab, top))
+    need = _workspace(rows, vocab, top)
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _call("hexkv_token_logprobs", logits, logits.data_ptr(), stride, rows, vocab, _DTYPES[logits.dtype],
           None if tokens is None else tokens.data_ptr(), top, None if tokens is None else logprob.data_ptr(),

@@ -23,11 +23,11 @@ from typing import Optional
 import torch
 from torch import nn
 
-from . import ops
+from . import fp4, ops
 
 
 def inference_cache(batch_size: int, max_seqlen: int, num_heads_kv: int, head_dim: int,
-                    dtype: torch.dtype, device, fused_ft_kernel: bool = False):
+                    dtype: torch.dtype, device, fused_ft_kernel: bool = False, kv_bits: int = 16):
     """One layer's cache in the shapes ``MHA.allocate_inference_cache``
     gives it: ``torch.empty(batch, max_seqlen, 2, kv_heads, head_dim)``
     (mha.py:418-420), or with ``fused_ft_kernel`` the FT pair ``(K [batch,
@@ -35,7 +35,12 @@ def inference_cache(batch_size: int, max_seqlen: int, num_heads_kv: int, head_di
     max_seqlen, head_dim])``, pack = 4 for float32 and 8 for 16-bit data
     (mha.py:421-428).  The head geometry, dtype and device are arguments here
     (the reference method reads them from the module); the reference method
-    itself needs no replacement, since it only calls ``torch.empty``."""
+    itself needs no replacement, since it only calls ``torch.empty``.
+    ``kv_bits`` 4: the 4-bit cache of ``fp4`` instead, whatever ``dtype`` is."""
+    if kv_bits != 16:
+        if kv_bits != 4 or fused_ft_kernel:
+            raise ValueError(f"caches hold 16 bits (their dtype) or 4, the FT caches 16 only (got {kv_bits})")
+        return fp4.kv_cache(batch_size, max_seqlen, num_heads_kv, head_dim, device)
     if not fused_ft_kernel:
         return torch.empty(batch_size, max_seqlen, 2, num_heads_kv, head_dim, dtype=dtype, device=device)
     assert dtype in (torch.float16, torch.bfloat16, torch.float32)
@@ -46,6 +51,8 @@ def inference_cache(batch_size: int, max_seqlen: int, num_heads_kv: int, head_di
 # Attribute of the cache view _update_kv_cache returns for a ragged decode
 # step: (seqlens, bias) with sequence b attending seqlens[b] + bias keys.
 _SEQLENS_ATTR = "_hexkv_seqlens"
+# Attribute of a 4-bit cache view: its KV heads, which its shape does not tell.
+_HEADS_ATTR = "_hexkv_kv_heads"
 
 
 def _sample_positions(inference_params, batch_start: int, batch_end: int) -> Optional[torch.Tensor]:
@@ -92,14 +99,20 @@ def _update_kv_cache(kv: torch.Tensor, inference_params, layer_idx: int) -> torc
     so the reference's capacity assert (mha.py:281-282) becomes a device
     check: a position past the cache is not written, a row past the view is
     cut to it, and ``check_kv_status`` raises ValueError for either at the
-    caller's next synchronisation."""
-    if inference_params.fused_ft_kernel:
+    caller's next synchronisation.
+
+    With ``kv_bits`` 4 the rows are rounded to four bits as they are written, and
+    the view is the 4-bit cache's, which ``FlashCrossAttention`` attends as
+    it attends the other; the prompt (``sequence_len_offset`` 0) gets ``kv``
+    back, as on the FT path: it attends its own keys as they were computed."""
+    if inference_params.fused_ft_kernel and inference_params.kv_bits == 16:
         return _update_ft_cache(kv, inference_params, layer_idx)
     num_heads, head_dim = kv.shape[-2:]
     cache = inference_params.key_value_memory_dict.get(layer_idx)
     if cache is None:
         cache = inference_cache(inference_params.max_batch_size, inference_params.max_sequence_len,
-                                num_heads, head_dim, kv.dtype, kv.device)
+                                num_heads, head_dim, kv.dtype, kv.device, inference_params.fused_ft_kernel,
+                                inference_params.kv_bits)
         inference_params.key_value_memory_dict[layer_idx] = cache
     batch_start = inference_params.batch_size_offset
     batch_end = batch_start + kv.shape[0]
@@ -109,7 +122,11 @@ def _update_kv_cache(kv: torch.Tensor, inference_params, layer_idx: int) -> torc
     assert sequence_end <= cache.shape[1]
     kv = kv.contiguous()
     positions = _sample_positions(inference_params, batch_start, batch_end) if kv.shape[1] == 1 else None
-    if positions is not None:
+    if inference_params.kv_bits == 4:
+        fp4.store_kv(_batch_rows(cache, batch_start, batch_end), kv, positions, 0 if positions is not None else sequence_start)
+        if sequence_start == 0:
+            return kv
+    elif positions is not None:
         ops.append_kv(_batch_rows(cache, batch_start, batch_end), kv, positions)
     elif kv.shape[1] == 1:
         ops.append_kv(_batch_rows(cache, batch_start, batch_end), kv, position_bias=sequence_start)
@@ -118,6 +135,8 @@ def _update_kv_cache(kv: torch.Tensor, inference_params, layer_idx: int) -> torc
     view = cache[batch_start:batch_end, :sequence_end]
     if positions is not None:
         setattr(view, _SEQLENS_ATTR, (positions, 1))
+    if inference_params.kv_bits == 4:
+        setattr(view, _HEADS_ATTR, num_heads)
     return view
 
 
@@ -214,7 +233,8 @@ class FlashCrossAttention(nn.Module):
         causal = self.causal if causal is None else causal
         batch_size = q.shape[0]
         seqlen_k = kv.shape[1]
-        assert kv.shape[0] == batch_size and kv.shape[4] == q.shape[3]
+        heads_k = getattr(kv, _HEADS_ATTR, None)  # (set: a 4-bit cache)
+        assert kv.shape[0] == batch_size and (heads_k is not None or kv.shape[4] == q.shape[3])
         bias = seqlen_k
         if seqlens_k is None and getattr(kv, _SEQLENS_ATTR, None) is not None:
             seqlens_k, bias = getattr(kv, _SEQLENS_ATTR)
@@ -225,6 +245,9 @@ class FlashCrossAttention(nn.Module):
             assert seqlens_k.dtype == torch.int32 and seqlens_k.is_cuda and seqlens_k.numel() == batch_size
             seqlens_k = seqlens_k.contiguous()
         q = q if q.stride(-1) == 1 and q.stride(-2) == q.shape[-1] else q.contiguous()
+        if heads_k is not None:
+            return fp4.decode_attention(q, kv, heads_k, max_seqlen=seqlen_k, seqlens=seqlens_k, seqlen_bias=bias,
+                                        causal=bool(causal) and q.shape[1] > 1, softmax_scale=self.softmax_scale)
         if kv.stride(-1) != 1 or kv.stride(-2) != kv.shape[-1] or kv.stride(1) != kv.shape[2:].numel():
             kv = kv.contiguous()
         return ops.decode_attention(q, kv, max_seqlen=seqlen_k, seqlens=seqlens_k, seqlen_bias=bias,
@@ -258,6 +281,10 @@ def update_and_attend(q: torch.Tensor, kv: torch.Tensor, inference_params, layer
     assert batch_end <= cache.shape[0] and offset + 1 <= cache.shape[1]
     target = _batch_rows(cache, batch_start, batch_end)
     positions = _sample_positions(inference_params, batch_start, batch_end)
+    if inference_params.kv_bits == 4:
+        return fp4.decode_attention(q.contiguous(), target, kv.shape[3], max_seqlen=offset + 1, seqlens=positions,
+                                    seqlen_bias=0 if positions is not None else offset,
+                                    kv_new=kv.contiguous(), softmax_scale=softmax_scale)
     return ops.decode_attention(q.contiguous(), target, max_seqlen=offset + 1, seqlens=positions,
                                 seqlen_bias=0 if positions is not None else offset,
                                 kv_new=kv.contiguous(), softmax_scale=softmax_scale)

@@ -165,7 +165,8 @@ class Pilot:
         self.args, self.rank, self.log = args, rank, log
         self.handoff = "host wire" if args.wire else "device memory (IPC)"
         self.channel = None if args.wire else IpcChannel()
-        self.engine = Engine(args.model_dir, args.engine, "cuda", args.dtype, fused_append=args.fused_append)
+        self.engine = Engine(args.model_dir, args.engine, "cuda", args.dtype, fused_append=args.fused_append,
+                             kv_bits=args.kv_bits, weight_bits=args.weight_bits)
         cfg = self.engine.config
         self.requests = read_trace(args.trace, args.model_dir, cfg.max_position_embeddings, cfg.vocab_size)
 
@@ -173,7 +174,7 @@ class Pilot:
         """What both ranks must agree on before the first request."""
         trace = json.dumps([asdict(r) for r in self.requests], sort_keys=True)
         settings = {k: getattr(self.args, k) for k in ("engine", "dtype", "seed", "warmup", "profile_first",
-                                                        "fused_append", "wire")}
+                                                        "fused_append", "kv_bits", "weight_bits", "logprobs", "wire")}
         settings["trace_sha256"] = hashlib.sha256(trace.encode()).hexdigest()
         settings["model"] = self.engine.identity["sha256"]
         return hashlib.sha256(json.dumps(settings, sort_keys=True).encode()).hexdigest()
@@ -236,13 +237,18 @@ class Pilot:
 
         first = tensors.pop("first")
         layers = {int(name): kv for name, kv in tensors.items()}
-        tokens = self.engine.decode(first, layers, len(req.input_ids), req.max_new_tokens, on_token)
+        scores = [] if self.args.logprobs else None
+        tokens = self.engine.decode(first, layers, len(req.input_ids), req.max_new_tokens, on_token,
+                                    on_logprobs=None if scores is None else scores.append)
         t1 = now()
         # The received views alias the prefill rank's memory: release (unmap)
         # them before answering, so it may free its packet.
         del tensors, layers, first
         reply = {"id": req.id, "receive_end": t0, "decode_end": t1, "token_events": marks,
                  "decode_ms": elapsed_ms(t0, t1)}
+        if scores is not None:  # of the tokens after the first
+            reply["logprobs"] = [s.logprob.item() for s in scores]
+            reply["entropies"] = [s.entropy.item() for s in scores]
         self.log.event("decode_complete", **reply)
         send_packet({"tokens": torch.tensor(tokens, dtype=torch.long, device="cuda")}, reply,
                     dst=PREFILL_RANK, channel=self.channel)
@@ -285,6 +291,12 @@ def parse_args(argv=None):
     ap.add_argument("--warmup", type=int, default=1)
     ap.add_argument("--timeout", type=int, default=180)
     ap.add_argument("--fused-append", action="store_true", help="decode with the fused append+attend launch")
+    ap.add_argument("--kv-bits", type=int, choices=[16, 4], default=16,
+                    help="keep and hand over the caches in the data type or in four bits")
+    ap.add_argument("--weight-bits", type=int, choices=[16, 4], default=16,
+                    help="hold the layers' matrices in the data type or in four bits")
+    ap.add_argument("--logprobs", action="store_true",
+                    help="record the decoded tokens' log-probabilities and entropies")
     ap.add_argument("--wire", action="store_true",
                     help="send KV payloads through host memory over the process group (reference path)")
     ap.add_argument("--check-colocated", action="store_true",

@@ -222,6 +222,29 @@ def test_attention(device, dtype, case, causal):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,hq,h,d,longest,q_len,partition", [
+    (2, 4, 2, 64, 700, 1, 32),     # 22 partitions: eight waves join a row
+    (9, 2, 1, 32, 260, 2, 128),    # joined by one wave; a sequence of one key beside them
+    (70, 8, 4, 64, 300, 1, 0),     # more workgroups than CUs: four waves each
+    (1, 2, 1, 128, 1100, 1, 0),    # split by the rule
+    (3, 24, 1, 32, 90, 6, 0),      # fewer (sequence, partition) pairs than XCDs, more with the row tiles
+    (257, 1, 1, 32, 40, 1, 0),
+])
+def test_attention_of_many_workgroups(device, dtype, batch, hq, h, d, longest, q_len, partition):
+    lens = [1 + (i * 977 + longest - 1) % longest for i in range(batch)]  # the first one longest
+    kv = randn((batch, longest, 2, h, d), batch, dtype, device)
+    q = randn((batch, q_len, hq, d), 9, dtype, device, 2.0)
+    cache = make_cache(kv, longest, device)
+    for b, n in enumerate(lens):
+        cache[b, n:] = 0xFF
+    got = fp4.decode_attention(q, cache, h, max_seqlen=longest, causal=True, partition=partition,
+                               seqlens=torch.tensor(lens, dtype=torch.int32, device=device))
+    stored = oracle.rounded(wide(kv))
+    want = oracle.attend(wide(q), stored, lens, q_len > 1)
+    assert (np.abs(wide(got) - want) <= attend_tolerance(wide(q), stored, want, dtype)).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("geometry", [(32, 8, 128), (8, 1, 128), (32, 4, 64), (4, 2, 32), (4, 2, 256), (40, 2, 64)])
 @pytest.mark.parametrize("partition", [0, 32])
 def test_fused_append(device, dtype, geometry, partition):

@@ -7,9 +7,15 @@ import numpy as np
 import pytest
 import torch
 
-from hexgen2_amd import _lib, fp4, logprobs
+from hexgen2_amd import _lib, fp4, logprobs, mha
+from hexgen2_amd.engine import Engine
+from hexgen2_amd.generation import InferenceParams
+from hexgen2_amd.llama import LlamaHost, LlamaShape, read_config
+from hexgen2_amd.run import parse_args
 from oracle import mx_oracle as oracle
 from tests.test_abi import ROOT
+
+GOLDEN = ROOT / "tests" / "golden"
 
 
 def test_oracle_rounds_to_the_nearest_even_code():
@@ -185,3 +191,37 @@ def test_row_bytes():
     for bad in ((0, 64), (2, 48), (2, 0)):
         with pytest.raises(ValueError):
             fp4.row_bytes(*bad)
+
+
+def test_four_bit_caches_through_the_module_calls():
+    assert mha.inference_cache(2, 9, 2, 64, torch.float16, "cpu", kv_bits=4).shape == (2, 9, 144)
+    assert mha.inference_cache(2, 9, 2, 64, torch.float16, "cpu").shape == (2, 9, 2, 2, 64)
+    for bits, ft, d in ((8, False, 64), (4, True, 64), (4, False, 48)):
+        with pytest.raises(ValueError):
+            mha.inference_cache(2, 9, 2, d, torch.float16, "cpu", ft, bits)
+    params = InferenceParams(9, kv_bits=4)
+    with pytest.raises(ValueError, match="HIP device"):
+        mha._update_kv_cache(torch.zeros(1, 2, 2, 2, 64), params, 0)
+    assert InferenceParams(9).kv_bits == 16
+
+
+@pytest.mark.parametrize("bits", [{"kv_bits": 8}, {"weight_bits": 2}, {"kv_bits": 0}])
+def test_engine_refuses_other_widths(bits):
+    with pytest.raises(ValueError, match="16 bits"):
+        Engine(GOLDEN / "fixture_seed17", "native", "cpu", "float16", **bits)
+
+
+def test_host_refuses_other_widths():
+    shape = LlamaShape.from_config(read_config(GOLDEN / "fixture_seed17"))
+    with pytest.raises(ValueError, match="16 bits"):
+        LlamaHost(shape, {}, "cpu", torch.float16, weight_bits=8)
+
+
+def test_pilot_arguments(capsys):
+    base = ["--model-dir", "m", "--trace", "t", "--output", "o"]
+    args = parse_args(base)
+    assert (args.kv_bits, args.weight_bits, args.logprobs) == (16, 16, False)
+    args = parse_args(base + ["--kv-bits", "4", "--weight-bits", "4", "--logprobs"])
+    assert (args.kv_bits, args.weight_bits, args.logprobs) == (4, 4, True)
+    with pytest.raises(SystemExit):
+        parse_args(base + ["--kv-bits", "8"])
