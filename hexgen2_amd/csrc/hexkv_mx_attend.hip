@@ -559,6 +559,8 @@ static int mx_validate(const hexkv_mx_attend_params *p, const char *what) {
   if (p->head_dim != 32 && p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
     return fail(HEXKV_EUNSUPPORTED, "%s: head_dim %d (compiled: 32, 64, 128, 256)", what, p->head_dim);
   if (p->kv_new && p->q_len != 1) return fail(HEXKV_EINVAL, "%s: fused append needs q_len 1", what);
+  if (p->max_seqlen > INT32_MAX - (1 << 17))  // (steps are counted past the end, in 32 bits)
+    return fail(HEXKV_ERANGE, "%s: max_seqlen %d too long", what, p->max_seqlen);
   if (p->max_seqlen < 0 || p->max_seqlen > p->capacity)
     return fail(HEXKV_ERANGE, "%s: max_seqlen %d outside [0, capacity %lld]", what, p->max_seqlen,
                 static_cast<long long>(p->capacity));

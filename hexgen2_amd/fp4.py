@@ -78,6 +78,14 @@ def _counts(t: Optional[torch.Tensor], batch: int, device, name: str) -> Optiona
     return t.data_ptr()
 
 
+def _int32(value: int, name: str) -> int:
+    """``value`` as the library's 32-bit argument (ctypes would wrap it)."""
+    value = int(value)
+    if not -(1 << 31) <= value < 1 << 31:
+        raise ValueError(f"{name} {value} does not fit 32 bits")
+    return value
+
+
 def _call(name: str, tensor: torch.Tensor, *args) -> None:
     """One library call on the current stream of ``tensor``'s device."""
     fn = getattr(_lib.load(), name)
@@ -116,7 +124,7 @@ def store_kv(cache: torch.Tensor, kv: torch.Tensor, positions: Optional[torch.Te
         raise ValueError(f"cache of {cache.shape[0]} sequences on {cache.device} for kv of {b} on {kv.device}")
     at = _counts(positions, b, kv.device, "positions")
     _call("hexkv_mx_store", kv, kv.data_ptr(), st[0], st[1], st[2], cache.data_ptr(), batch_bytes, row, cache.shape[1],
-          b, s, heads, d, _DTYPES[kv.dtype], at, int(position_bias))
+          b, s, heads, d, _DTYPES[kv.dtype], at, _int32(position_bias, "position_bias"))
 
 
 def load_kv(cache: torch.Tensor, length: int, kv_heads: int, head_dim: int, dtype: torch.dtype,
@@ -128,7 +136,7 @@ def load_kv(cache: torch.Tensor, length: int, kv_heads: int, head_dim: int, dtyp
     cache come back as zeros and are flagged."""
     _require_device(cache)
     batch_bytes, row = _check_cache(cache, kv_heads, head_dim)
-    b, length = cache.shape[0], int(length)
+    b, length = cache.shape[0], _int32(length, "length")
     if dtype not in _DTYPES or length < 0:
         raise ValueError("load_kv gives float16, bfloat16 or float32 rows, none or more of them")
     if out is None:
@@ -136,9 +144,11 @@ def load_kv(cache: torch.Tensor, length: int, kv_heads: int, head_dim: int, dtyp
     elif out.shape != (b, length, 2, kv_heads, head_dim) or out.dtype != dtype or out.device != cache.device:
         raise ValueError(f"out must be {dtype} [{b}, {length}, 2, {kv_heads}, {head_dim}] on {cache.device}")
     st = _check_rows(out)
+    if 0 in st[:3] and any(s == 0 and n > 1 for s, n in zip(st, out.shape)):
+        raise ValueError("out's rows must not overlap")
     at = _counts(positions, b, cache.device, "positions")
     _call("hexkv_mx_load", cache, cache.data_ptr(), batch_bytes, row, cache.shape[1], out.data_ptr(), st[0], st[1], st[2],
-          b, length, kv_heads, head_dim, _DTYPES[dtype], at, int(position_bias))
+          b, length, kv_heads, head_dim, _DTYPES[dtype], at, _int32(position_bias, "position_bias"))
     return out
 
 
@@ -168,7 +178,7 @@ def _attend_form(q, cache, kv_heads, out, kv_new, causal, softmax_scale, partiti
     p.cache_batch_bytes, p.cache_row_bytes = batch_bytes, row
     # (a fresh output is contiguous)
     p.out_batch_stride, p.out_row_stride = (q_len * q_heads * d, q_heads * d) if out is None else out.stride()[:2]
-    p.partition = int(partition)
+    p.partition = _int32(partition, "partition")
     return p
 
 
@@ -217,7 +227,7 @@ def decode_attention(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, *, max
     if kv_new is not None:
         p.kv_new = kv_new.data_ptr()
     p.seqlens_dev = _counts(seqlens, p.batch, q.device, "seqlens")
-    p.seqlen_bias, p.max_seqlen = int(seqlen_bias), int(max_seqlen)
+    p.seqlen_bias, p.max_seqlen = _int32(seqlen_bias, "seqlen_bias"), _int32(max_seqlen, "max_seqlen")
     if not 0 <= p.max_seqlen <= p.capacity:
         raise ValueError(f"max_seqlen {max_seqlen} outside [0, capacity {p.capacity}]")
     need = needs.get((p.max_seqlen, p.q % 16))
@@ -241,14 +251,14 @@ def attend_workspace_bytes(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, 
                            partition: int = 0, causal: bool = False) -> int:
     """Workspace bytes ``decode_attention`` needs for this geometry and bound."""
     p = _attend_form(q, cache, int(kv_heads), None, None, causal, None, partition)
-    p.q, p.capacity, p.max_seqlen = q.data_ptr(), cache.shape[1], int(max_seqlen)
+    p.q, p.capacity, p.max_seqlen = q.data_ptr(), cache.shape[1], _int32(max_seqlen, "max_seqlen")
     return int(_lib.load().hexkv_mx_attend_workspace_bytes(ctypes.byref(p)))
 
 
 def _matrix_rows(t: torch.Tensor, name: str) -> int:
     """Elements between consecutive rows (last dim) of ``t``, whose outer dims
     fold into one."""
-    if t.is_contiguous() or t.dim() == 1:
+    if t.is_contiguous():
         return t.shape[-1]
     if t.dim() != 2 or t.stride(1) != 1:
         raise ValueError(f"{name} rows must be contiguous and lie at one stride")
@@ -309,9 +319,11 @@ def linear(x: torch.Tensor, weight: Fp4Tensor) -> torch.Tensor:
         raise ValueError(f"x {x.dtype} {tuple(x.shape)} on {x.device} does not fit a matrix [{codes.shape[0]}, "
                          f"{codes.shape[-1] * 2}] on {codes.device}")
     n, k = codes.shape[0], x.shape[-1]
+    if not k:
+        raise ValueError("a product needs a block of elements")
     stride = _matrix_rows(x, "x")
     out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-    rows, dtype = x.numel() // max(k, 1), _DTYPES[x.dtype]
+    rows, n, dtype = _int32(x.numel() // k, "tokens"), _int32(n, "rows"), _DTYPES[x.dtype]
     need = _linear_workspace(rows, n, k, dtype)
     workspace = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _call("hexkv_mx_linear", x, x.data_ptr(), stride, codes.data_ptr(), powers.data_ptr(), out.data_ptr(), rows, n, k, dtype,

@@ -76,6 +76,11 @@ def _sample_positions(inference_params, batch_start: int, batch_end: int) -> Opt
     return positions
 
 
+def _kv_bits(inference_params) -> int:
+    """Bits of the caches (the reference's own ``InferenceParams`` has no such field)."""
+    return getattr(inference_params, "kv_bits", 16)
+
+
 def _batch_rows(cache: torch.Tensor, start: int, end: int) -> torch.Tensor:
     """``cache[start:end]``, without building a view of the whole cache."""
     return cache if start == 0 and end == cache.shape[0] else cache[start:end]
@@ -105,14 +110,14 @@ def _update_kv_cache(kv: torch.Tensor, inference_params, layer_idx: int) -> torc
     the view is the 4-bit cache's, which ``FlashCrossAttention`` attends as
     it attends the other; the prompt (``sequence_len_offset`` 0) gets ``kv``
     back, as on the FT path: it attends its own keys as they were computed."""
-    if inference_params.fused_ft_kernel and inference_params.kv_bits == 16:
+    kv_bits = _kv_bits(inference_params)
+    if inference_params.fused_ft_kernel and kv_bits == 16:
         return _update_ft_cache(kv, inference_params, layer_idx)
     num_heads, head_dim = kv.shape[-2:]
     cache = inference_params.key_value_memory_dict.get(layer_idx)
     if cache is None:
         cache = inference_cache(inference_params.max_batch_size, inference_params.max_sequence_len,
-                                num_heads, head_dim, kv.dtype, kv.device, inference_params.fused_ft_kernel,
-                                inference_params.kv_bits)
+                                num_heads, head_dim, kv.dtype, kv.device, inference_params.fused_ft_kernel, kv_bits)
         inference_params.key_value_memory_dict[layer_idx] = cache
     batch_start = inference_params.batch_size_offset
     batch_end = batch_start + kv.shape[0]
@@ -122,7 +127,7 @@ def _update_kv_cache(kv: torch.Tensor, inference_params, layer_idx: int) -> torc
     assert sequence_end <= cache.shape[1]
     kv = kv.contiguous()
     positions = _sample_positions(inference_params, batch_start, batch_end) if kv.shape[1] == 1 else None
-    if inference_params.kv_bits == 4:
+    if kv_bits == 4:
         fp4.store_kv(_batch_rows(cache, batch_start, batch_end), kv, positions, 0 if positions is not None else sequence_start)
         if sequence_start == 0:
             return kv
@@ -135,7 +140,7 @@ def _update_kv_cache(kv: torch.Tensor, inference_params, layer_idx: int) -> torc
     view = cache[batch_start:batch_end, :sequence_end]
     if positions is not None:
         setattr(view, _SEQLENS_ATTR, (positions, 1))
-    if inference_params.kv_bits == 4:
+    if kv_bits == 4:
         setattr(view, _HEADS_ATTR, num_heads)
     return view
 
@@ -281,7 +286,7 @@ def update_and_attend(q: torch.Tensor, kv: torch.Tensor, inference_params, layer
     assert batch_end <= cache.shape[0] and offset + 1 <= cache.shape[1]
     target = _batch_rows(cache, batch_start, batch_end)
     positions = _sample_positions(inference_params, batch_start, batch_end)
-    if inference_params.kv_bits == 4:
+    if _kv_bits(inference_params) == 4:
         return fp4.decode_attention(q.contiguous(), target, kv.shape[3], max_seqlen=offset + 1, seqlens=positions,
                                     seqlen_bias=0 if positions is not None else offset,
                                     kv_new=kv.contiguous(), softmax_scale=softmax_scale)

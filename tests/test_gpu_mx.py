@@ -550,3 +550,62 @@ def test_a_step_on_another_stream_and_in_a_graph(device):
         assert all(torch.equal(a, b) for a, b in zip(want, result))
         assert torch.equal(captured, cache)
         step(fresh())  # eager work between
+
+
+# --------------------------------------------------- refusals on the device ---
+
+
+def test_calls_refuse_what_they_would_misread(device):
+    x = randn((4, 64), 1, torch.float16, device)
+    w = fp4.quantize(x)
+    cache = fp4.kv_cache(2, 8, 2, 64, device)
+    q = randn((2, 1, 4, 64), 1, torch.float16, device)
+    empty = fp4.Fp4Tensor(w.codes[:, :0].contiguous(), w.powers[:, :0].contiguous())
+    for call in (lambda: fp4.quantize(torch.zeros(128, device=device)[::2]),
+                 lambda: fp4.linear(torch.zeros(128, device=device, dtype=torch.float16)[::2], w),
+                 lambda: fp4.linear(x[:, :0], empty),
+                 lambda: fp4.store_kv(cache, torch.zeros(2, 1, 2, 2, 64, device=device), None, 1 << 32),
+                 lambda: fp4.load_kv(cache, (1 << 32) + 1, 2, 64, torch.float16),
+                 lambda: fp4.load_kv(cache, 4, 2, 64, torch.float16,
+                                     out=torch.empty(2, 1, 2, 2, 64, device=device, dtype=torch.float16).expand(2, 4, 2, 2, 64)),
+                 lambda: fp4.decode_attention(q, cache, 2, max_seqlen=(1 << 32) + 4),
+                 lambda: fp4.decode_attention(q, cache, 2, max_seqlen=4, seqlen_bias=1 << 32),
+                 lambda: fp4.decode_attention(q, cache, 2, max_seqlen=4, partition=1 << 32)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_products_and_scores_of_nothing(device):
+    w = fp4.quantize(randn((6, 64), 1, torch.float16, device))
+    assert fp4.linear(torch.zeros(0, 64, device=device, dtype=torch.float16), w).shape == (0, 6)
+    none = fp4.Fp4Tensor(w.codes[:0], w.powers[:0])
+    assert fp4.linear(torch.zeros(3, 64, device=device, dtype=torch.float16), none).shape == (3, 0)
+    got = logprobs.token_logprobs(torch.zeros(0, 9, device=device), torch.zeros(0, dtype=torch.int64, device=device), 2)
+    assert got.logprob.shape == got.entropy.shape == (0,) and got.top_ids.shape == (0, 2)
+    assert fp4.quantize(torch.zeros(3, 0, device=device)).codes.shape == (3, 0)
+
+
+def test_calls_of_two_streams_side_by_side(device):
+    """The same calls at once on two streams, their workspaces their own."""
+    kv = randn((2, 1500, 2, 2, 64), 1, torch.bfloat16, device)
+    cache = make_cache(kv, 1500, device)
+    qs = [randn((2, 1, 8, 64), 5 + i, torch.bfloat16, device) for i in range(2)]
+    xs = [randn((5, 512), 8 + i, torch.bfloat16, device) for i in range(2)]
+    logits = [randn((2, 40000), 3 + i, torch.bfloat16, device) for i in range(2)]
+    w = fp4.quantize(randn((512, 512), 2, torch.bfloat16, device))
+
+    def calls(i):
+        return [fp4.decode_attention(qs[i], cache, 2, max_seqlen=1500, seqlen_bias=1500), fp4.linear(xs[i], w),
+                *logprobs.token_logprobs(logits[i], None, 7)[1:]]
+
+    want = [calls(0), calls(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(calls(i))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))

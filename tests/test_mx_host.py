@@ -225,3 +225,30 @@ def test_pilot_arguments(capsys):
     assert (args.kv_bits, args.weight_bits, args.logprobs) == (4, 4, True)
     with pytest.raises(SystemExit):
         parse_args(base + ["--kv-bits", "8"])
+
+
+def test_a_row_of_strided_elements_is_refused():
+    assert fp4._matrix_rows(torch.zeros(64), "x") == 64
+    assert fp4._matrix_rows(torch.zeros(3, 128)[:, :64], "x") == 128
+    for t in (torch.zeros(128)[::2], torch.zeros(64, 3).t(), torch.zeros(2, 3, 128)[..., :64]):
+        with pytest.raises(ValueError, match="contiguous"):
+            fp4._matrix_rows(t, "x")
+
+
+def test_sizes_past_32_bits_are_refused():
+    assert [fp4._int32(v, "x") for v in (-(1 << 31), (1 << 31) - 1)] == [-(1 << 31), (1 << 31) - 1]
+    for value in (1 << 31, 1 << 32, -(1 << 31) - 1):
+        with pytest.raises(ValueError, match="32 bits"):
+            fp4._int32(value, "x")
+    p = attend_params(max_seqlen=(1 << 31) - 1, capacity=1 << 31, batch=1)
+    assert _lib.load().hexkv_mx_attend(ctypes.byref(p), None, 0, None) == R
+
+
+def test_parameters_without_the_field_keep_16_bits():
+    class Plain:  # the reference's own fields
+        max_sequence_len, max_batch_size, sequence_len_offset, batch_size_offset = 9, 1, 0, 0
+        fused_ft_kernel, lengths_per_sample, key_value_memory_dict = False, None, {}
+    assert mha._kv_bits(Plain()) == 16 and mha._kv_bits(InferenceParams(9, kv_bits=4)) == 4
+    with pytest.raises(ValueError, match="HIP device"):
+        mha._update_kv_cache(torch.zeros(1, 2, 2, 2, 64), Plain(), 0)
+    assert Plain.key_value_memory_dict[0].shape == (1, 9, 2, 2, 64)
