@@ -98,15 +98,17 @@ def _call(name: str, tensor: torch.Tensor, *args) -> None:
         _lib.check(rc, name)
 
 
-def _check_rows(kv: torch.Tensor):
-    if kv.dim() != 5 or kv.shape[2] != 2:
-        raise ValueError(f"kv must be [batch, positions, 2, kv_heads, head_dim], got {tuple(kv.shape)}")
-    if kv.dtype not in _DTYPES:
+@functools.lru_cache(maxsize=256)
+def _rows_form(shape, stride, dtype):
+    """``shape, stride`` and type code of checked rows (by what they depend on:
+    most of a small call's time is the host's)."""
+    if len(shape) != 5 or shape[2] != 2:
+        raise ValueError(f"kv must be [batch, positions, 2, kv_heads, head_dim], got {tuple(shape)}")
+    if dtype not in _DTYPES:
         raise ValueError("kv must be one of float16, bfloat16, float32")
-    st = kv.stride()
-    if st[4] != 1 or (kv.shape[3] > 1 and st[3] != kv.shape[4]):
+    if stride[4] != 1 or (shape[3] > 1 and stride[3] != shape[4]):
         raise ValueError("kv heads must be contiguous [.., heads, head_dim]")
-    return st
+    return (*shape, *stride[:3], _DTYPES[dtype])
 
 
 def store_kv(cache: torch.Tensor, kv: torch.Tensor, positions: Optional[torch.Tensor] = None,
@@ -117,14 +119,13 @@ def store_kv(cache: torch.Tensor, kv: torch.Tensor, positions: Optional[torch.Te
     A row whose position, read from device memory, lies outside the cache is
     not written and flagged (``ops.check_device_status``)."""
     _require_device(cache, kv)
-    st = _check_rows(kv)
-    b, s, _, heads, d = kv.shape
+    b, s, _, heads, d, *strides, dtype = _rows_form(kv.shape, kv.stride(), kv.dtype)
     batch_bytes, row = _check_cache(cache, heads, d)
     if cache.device != kv.device or cache.shape[0] < b:
         raise ValueError(f"cache of {cache.shape[0]} sequences on {cache.device} for kv of {b} on {kv.device}")
     at = _counts(positions, b, kv.device, "positions")
-    _call("hexkv_mx_store", kv, kv.data_ptr(), st[0], st[1], st[2], cache.data_ptr(), batch_bytes, row, cache.shape[1],
-          b, s, heads, d, _DTYPES[kv.dtype], at, _int32(position_bias, "position_bias"))
+    _call("hexkv_mx_store", kv, kv.data_ptr(), *strides, cache.data_ptr(), batch_bytes, row, cache.shape[1], b, s, heads, d,
+          dtype, at, _int32(position_bias, "position_bias"))
 
 
 def load_kv(cache: torch.Tensor, length: int, kv_heads: int, head_dim: int, dtype: torch.dtype,
@@ -140,15 +141,15 @@ def load_kv(cache: torch.Tensor, length: int, kv_heads: int, head_dim: int, dtyp
     if dtype not in _DTYPES or length < 0:
         raise ValueError("load_kv gives float16, bfloat16 or float32 rows, none or more of them")
     if out is None:
-        out = torch.empty((b, length, 2, kv_heads, head_dim), dtype=dtype, device=cache.device)
+        out = cache.new_empty((b, length, 2, kv_heads, head_dim), dtype=dtype)
     elif out.shape != (b, length, 2, kv_heads, head_dim) or out.dtype != dtype or out.device != cache.device:
         raise ValueError(f"out must be {dtype} [{b}, {length}, 2, {kv_heads}, {head_dim}] on {cache.device}")
-    st = _check_rows(out)
-    if 0 in st[:3] and any(s == 0 and n > 1 for s, n in zip(st, out.shape)):
+    *_, s0, s1, s2, code = _rows_form(out.shape, out.stride(), dtype)
+    if 0 in (s0, s1, s2) and any(s == 0 and n > 1 for s, n in zip((s0, s1, s2), out.shape)):
         raise ValueError("out's rows must not overlap")
     at = _counts(positions, b, cache.device, "positions")
-    _call("hexkv_mx_load", cache, cache.data_ptr(), batch_bytes, row, cache.shape[1], out.data_ptr(), st[0], st[1], st[2],
-          b, length, kv_heads, head_dim, _DTYPES[dtype], at, _int32(position_bias, "position_bias"))
+    _call("hexkv_mx_load", cache, cache.data_ptr(), batch_bytes, row, cache.shape[1], out.data_ptr(), s0, s1, s2,
+          b, length, kv_heads, head_dim, code, at, _int32(position_bias, "position_bias"))
     return out
 
 
@@ -239,7 +240,7 @@ def decode_attention(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, *, max
     at, size = None, 0
     if need:
         if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            workspace = cache.new_empty(need)
         elif workspace.device != q.device or not workspace.is_contiguous():
             raise ValueError(f"workspace must be contiguous on {q.device}")
         at, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
@@ -255,14 +256,21 @@ def attend_workspace_bytes(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, 
     return int(_lib.load().hexkv_mx_attend_workspace_bytes(ctypes.byref(p)))
 
 
-def _matrix_rows(t: torch.Tensor, name: str) -> int:
-    """Elements between consecutive rows (last dim) of ``t``, whose outer dims
+def _row_stride(shape, stride, name: str) -> int:
+    """Elements between consecutive rows (last dim) of a tensor whose outer dims
     fold into one."""
-    if t.is_contiguous():
-        return t.shape[-1]
-    if t.dim() != 2 or t.stride(1) != 1:
-        raise ValueError(f"{name} rows must be contiguous and lie at one stride")
-    return t.stride(0)
+    if len(shape) == 2 and stride[1] == 1 and shape[0] > 1:
+        return stride[0]
+    step = 1
+    for n, at in zip(reversed(shape), reversed(stride)):
+        if n != 1 and at != step and 0 not in shape:
+            raise ValueError(f"{name} rows must be contiguous and lie at one stride")
+        step *= n
+    return shape[-1]
+
+
+def _matrix_rows(t: torch.Tensor, name: str) -> int:
+    return _row_stride(t.shape, t.stride(), name)
 
 
 def quantize(x: torch.Tensor) -> Fp4Tensor:
@@ -281,11 +289,16 @@ def quantize(x: torch.Tensor) -> Fp4Tensor:
     return Fp4Tensor(codes, powers)
 
 
+@functools.lru_cache(maxsize=1024)
+def _is_matrix(codes_shape, powers_shape) -> bool:
+    return (len(codes_shape) >= 1 and codes_shape[:-1] == powers_shape[:-1]
+            and codes_shape[-1] == powers_shape[-1] * (BLOCK // 2))
+
+
 def _check_matrix(weight: Fp4Tensor):
     codes, powers = weight
-    if codes.dtype != torch.uint8 or powers.dtype != torch.uint8 or codes.device != powers.device \
-            or codes.dim() < 1 or codes.shape[:-1] != powers.shape[:-1] or codes.shape[-1] != powers.shape[-1] * (BLOCK // 2) \
-            or not codes.is_contiguous() or not powers.is_contiguous():
+    if codes.dtype != torch.uint8 or powers.dtype != torch.uint8 or codes.get_device() != powers.get_device() \
+            or not _is_matrix(codes.shape, powers.shape) or not codes.is_contiguous() or not powers.is_contiguous():
         raise ValueError(f"a 4-bit tensor is contiguous uint8 codes [..., k / 2] and powers [..., k / {BLOCK}] on one "
                          f"device, got {tuple(codes.shape)} and {tuple(powers.shape)}")
     return codes, powers
@@ -305,8 +318,17 @@ def dequantize(weight: Fp4Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=1024)
-def _linear_workspace(rows: int, n: int, k: int, dtype: int) -> int:
-    return int(_lib.load().hexkv_mx_linear_workspace_bytes(rows, n, k, dtype))
+def _linear_form(shape, stride, dtype, codes_shape, powers_shape):
+    """A product's tokens, rows, inner dimension, token stride, type code,
+    output shape and workspace bytes."""
+    if len(codes_shape) != 2 or dtype not in _DTYPES or not shape or shape[-1] != codes_shape[1] * 2:
+        raise ValueError(f"x {dtype} {tuple(shape)} does not fit a matrix [{codes_shape[0]}, {codes_shape[-1] * 2}]")
+    n, k = codes_shape[0], shape[-1]
+    if not k:
+        raise ValueError("a product needs a block of elements")
+    rows, n, code = _int32(shape.numel() // k, "tokens"), _int32(n, "rows"), _DTYPES[dtype]
+    return (rows, n, k, _row_stride(shape, stride, "x"), code, torch.Size((*shape[:-1], n)),
+            int(_lib.load().hexkv_mx_linear_workspace_bytes(rows, n, k, code)))
 
 
 def linear(x: torch.Tensor, weight: Fp4Tensor) -> torch.Tensor:
@@ -314,18 +336,11 @@ def linear(x: torch.Tensor, weight: Fp4Tensor) -> torch.Tensor:
     fp32 over the weights' exact values, rounded once to ``x``'s type."""
     codes, powers = _check_matrix(weight)
     _require_device(x, codes)
-    if codes.dim() != 2 or x.dtype not in _DTYPES or x.device != codes.device or x.dim() < 1 \
-            or x.shape[-1] != codes.shape[1] * 2:
-        raise ValueError(f"x {x.dtype} {tuple(x.shape)} on {x.device} does not fit a matrix [{codes.shape[0]}, "
-                         f"{codes.shape[-1] * 2}] on {codes.device}")
-    n, k = codes.shape[0], x.shape[-1]
-    if not k:
-        raise ValueError("a product needs a block of elements")
-    stride = _matrix_rows(x, "x")
-    out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-    rows, n, dtype = _int32(x.numel() // k, "tokens"), _int32(n, "rows"), _DTYPES[x.dtype]
-    need = _linear_workspace(rows, n, k, dtype)
-    workspace = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    if x.device != codes.device:
+        raise ValueError(f"x on {x.device} for a matrix on {codes.device}")
+    rows, n, k, stride, dtype, shape, need = _linear_form(x.shape, x.stride(), x.dtype, codes.shape, powers.shape)
+    out = x.new_empty(shape)
+    workspace = codes.new_empty(need) if need else None
     _call("hexkv_mx_linear", x, x.data_ptr(), stride, codes.data_ptr(), powers.data_ptr(), out.data_ptr(), rows, n, k, dtype,
           workspace.data_ptr() if need else None, need)
     return out

@@ -57,15 +57,14 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
                                or not tokens.is_contiguous()):
         raise ValueError(f"tokens must be contiguous int64 {tuple(shape)} on {logits.device}")
     rows = logits.numel() // vocab
-    device = logits.device
-    entropy = torch.empty(shape, dtype=torch.float32, device=device)
+    entropy = logits.new_empty(shape, dtype=torch.float32)
     logprob = None if tokens is None else torch.empty_like(entropy)
     values = ids = None
     if top:
-        values = torch.empty((*shape, top), dtype=torch.float32, device=device)
-        ids = torch.empty((*shape, top), dtype=torch.int64, device=device)
+        values = entropy.new_empty((*shape, top))
+        ids = logits.new_empty((*shape, top), dtype=torch.int64)
     need = _workspace(rows, vocab, top)
-    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    workspace = logits.new_empty(need, dtype=torch.uint8) if need else None
     _call("hexkv_token_logprobs", logits, logits.data_ptr(), stride, rows, vocab, _DTYPES[logits.dtype],
           None if tokens is None else tokens.data_ptr(), top, None if tokens is None else logprob.data_ptr(),
           entropy.data_ptr(), None if values is None else values.data_ptr(), None if ids is None else ids.data_ptr(),
