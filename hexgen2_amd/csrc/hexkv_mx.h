@@ -6,7 +6,7 @@
 // A block's power is the smallest that leaves no element above 6 (a smaller
 // one would clip the largest elements, by up to a quarter), and within
 // [-125, 126], so that every non-zero value is a normal bf16 number: over
-// normally distributed data the error is 0.105 of their deviation.  Since the
+// normally distributed data the error is 0.116 of their deviation.  Since the
 // power is exact, x / power is, and the only rounding is the element's own
 // (nearest, halfway to the even code).
 //
