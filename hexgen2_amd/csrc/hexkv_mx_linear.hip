@@ -5,11 +5,12 @@
 // Everywhere a lane loads whole blocks of a row (16 bytes, 32 elements, one
 // power) and converts them in registers; the matrix instructions' inner dimension is laid
 // out to fit what a lane holds, the tokens' operand in the same order, so a
-// converted block is an operand as it stands.  Three kernels, see mx_plan:
+// converted block is an operand as it stands.  Four kernels, see mx_plan:
 //   mx_rows_kernel  one or two tokens: a wave reads rows from end to end;
 //   mx_few_kernel   up to 64: a wave holds the tokens' operands of its share of
 //                   the inner dimension in registers and walks the matrix;
-//   mx_tile_kernel  more: tiles, with the tokens in LDS.
+//   mx_tile_kernel  as many in small matrices, and fp32: tiles, with the tokens in LDS;
+//   mx_prompt_kernel  more: tiles, with the tokens and the matrix's four bits in LDS.
 //
 // bf16 activations meet the matrix as bf16, exact for every power.  fp16 ones
 // meet it as fp16, exact for powers from 2^-23 to 2^13; blocks with another
@@ -473,6 +474,66 @@ __device__ __forceinline__ f32x16 mma32_f16(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// The blocks whose power fp16 does not hold, in bf16.
+template <typename T, typename S>
+__device__ __forceinline__ void tile_far(const MxLinearArgs &a, int m0, int n0, int k_first, int k_last, int wm, int wn, int wk,
+                                         int c, int h, f32x16 (&acc)[S::MT][S::NT]) {
+  constexpr int MT = S::MT, NT = S::NT;
+#pragma unroll 1
+  for (int k0 = k_first; k0 < k_last; k0 += S::kStep)
+#pragma unroll 1
+    for (int s = 0; s < S::STEPS; ++s) {
+      const int k = k0 + (wk * S::STEPS + s) * 64 + h * kMxBlock;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        FarBlock block;
+        block.read(a, min(n0 + (wn * NT + t) * 32 + c, a.n - 1), k / kMxBlock, k < k_last);
+        if (!__ballot(block.any)) continue;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const int token = min(m0 + (wm * MT + m) * 32 + c, a.rows - 1);
+          const _Float16 *p = static_cast<const _Float16 *>(a.x) + static_cast<int64_t>(token) * a.x_stride + k;
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j) {
+            u32x4 terms[2];
+            far_terms(p + 8 * j, k < k_last, terms);
+            const u32x4 w = block.operand(j);
+            acc[m][t] = mma32_bf16(w, terms[1], mma32_bf16(w, terms[0], acc[m][t]));
+          }
+        }
+      }
+    }
+}
+
+template <typename T, typename S>
+__device__ __forceinline__ void tile_store(const MxLinearArgs &a, int m0, int n0, int split, int wm, int wn, int c, int h,
+                                           const f32x16 (&acc)[S::MT][S::NT]) {
+  constexpr int MT = S::MT, NT = S::NT;
+  // acc: column c is the token, rows 8 i + 4 h + e the matrix's
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int token = m0 + (wm * MT + m) * 32 + c;
+    if (token >= a.rows) continue;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = n0 + (wn * NT + t) * 32 + 8 * i + 4 * h;
+        const f32x4 v = {acc[m][t][4 * i], acc[m][t][4 * i + 1], acc[m][t][4 * i + 2], acc[m][t][4 * i + 3]};
+        if (n >= a.n) continue;
+        if (a.splits > 1) {
+          float *o = a.partial + (static_cast<int64_t>(split) * a.rows + token) * a.n + n;
+          if (n + 4 <= a.n) store4(o, v);
+          else for (int e = 0; e < a.n - n; ++e) o[e] = v[e];
+        } else {
+          T *o = static_cast<T *>(a.out) + static_cast<int64_t>(token) * a.n + n;
+          if (n + 4 <= a.n) store4(o, v);
+          else for (int e = 0; e < a.n - n; ++e) o[e] = Elem<T>::from_float(v[e]);
+        }
+      }
+  }
+}
+
 template <typename T, typename S, bool VEC>
 __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs a) {
   constexpr int MT = S::MT, NT = S::NT, CH = S::kChunks, PL = S::kPlanes;
@@ -661,32 +722,7 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs
     }
   }
 
-  if (Elem<T>::kDtype == HEXKV_F16 && __ballot(far)) {
-#pragma unroll 1
-    for (int k0 = k_first; k0 < k_last; k0 += S::kStep)
-#pragma unroll 1
-      for (int s = 0; s < S::STEPS; ++s) {
-        const int k = k0 + (wk * S::STEPS + s) * 64 + h * kMxBlock;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          FarBlock block;
-          block.read(a, min(n0 + (wn * NT + t) * 32 + c, a.n - 1), k / kMxBlock, k < k_last);
-          if (!__ballot(block.any)) continue;
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            const int token = min(m0 + (wm * MT + m) * 32 + c, a.rows - 1);
-            const _Float16 *p = static_cast<const _Float16 *>(a.x) + static_cast<int64_t>(token) * a.x_stride + k;
-#pragma unroll 1
-            for (int j = 0; j < 4; ++j) {
-              u32x4 terms[2];
-              far_terms(p + 8 * j, k < k_last, terms);
-              const u32x4 w = block.operand(j);
-              acc[m][t] = mma32_bf16(w, terms[1], mma32_bf16(w, terms[0], acc[m][t]));
-            }
-          }
-        }
-      }
-  }
+  if (Elem<T>::kDtype == HEXKV_F16 && __ballot(far)) tile_far<T, S>(a, m0, n0, k_first, k_last, wm, wn, wk, c, h, acc);
 
   // the waves that share the inner dimension join, half of them at a time
   if constexpr (S::WK > 1) {
@@ -717,29 +753,171 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs
     }
     if (wk > 0) return;
   }
-  // acc: column c is the token, rows 8 i + 4 h + e the matrix's
+  tile_store<T, S>(a, m0, n0, split, wm, wn, c, h, acc);
+}
+
+// A prompt's tile (16-bit data): as mx_tile_kernel, but the matrix reaches its
+// waves through LDS as well, in four bits, so that a load's four lanes read one
+// row (lanes of different rows each cost a line: the address units were
+// the bound at 27% of the matrix cores), and each element is loaded once a workgroup.  A step is 128 of
+// the inner dimension in one buffer, the next one's in registers; several
+// workgroups a CU fill the barriers.
+template <typename T, int MT_, int NT_, int WM_, int WN_>
+struct MxPromptShape {
+  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, WK = 1, STEPS = 2;
+  static constexpr int kThreads = 64 * WM * WN;
+  static constexpr int kTokens = 32 * MT * WM, kRows = 32 * NT * WN, kStep = 128;
+  static constexpr int kChunks = kStep / 8;
+  static constexpr int kLoads = kTokens * kChunks / kThreads;     // chunks of the tokens a thread stages
+  static constexpr int kLoadsW = kRows * 4 / kThreads;            // blocks of the matrix
+  static constexpr size_t kLds = size_t{16} * (kTokens * kChunks + kRows * 4) + size_t{4} * kRows;
+  static_assert(kTokens * kChunks % kThreads == 0 && kRows * 4 % kThreads == 0, "every thread stages as much");
+  static_assert(kThreads % kRows == 0 || kRows % kThreads == 0, "powers");
+};
+
+template <typename T, typename S, bool VEC>
+__global__ __launch_bounds__(S::kThreads, 2) void mx_prompt_kernel(const MxLinearArgs a) {
+  constexpr int MT = S::MT, NT = S::NT, CH = S::kChunks;
+  constexpr int PR = S::kRows > S::kThreads ? S::kRows / S::kThreads : 1;  // rows' powers a thread stages
+  __shared__ __attribute__((aligned(16))) char s_mem[S::kLds];
+  u32x4 *s_x = reinterpret_cast<u32x4 *>(s_mem);           // [tokens][chunks], chunk c of token t at c ^ t % 16
+  u32x4 *s_w = s_x + S::kTokens * CH;                       // [rows][4], block b of row r at b ^ r / 4 % 4
+  unsigned int *s_p = reinterpret_cast<unsigned int *>(s_w + S::kRows * 4);  // [rows] the four blocks' powers
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, h = lane >> 5, wn = wave % S::WN, wm = wave / S::WN;
+
+  // (XCDs and pieces as in mx_tile_kernel)
+  const int local = static_cast<int>(blockIdx.x >> 3);
+  const int group = local / a.m_tiles * 8 + static_cast<int>(blockIdx.x & 7);
+  const int m0 = (local % a.m_tiles) * S::kTokens;
+  if (group >= a.n_tiles * a.splits) return;
+  const int n0 = group / a.splits * S::kRows, split = group % a.splits;
+  const int k_first = split * a.split_k, k_last = min(a.k, k_first + a.split_k);
+  const int blocks = a.k / kMxBlock;  // at least 4
+
+  const char *x_base = static_cast<const char *>(a.x) + static_cast<int64_t>(m0) * a.x_stride * sizeof(T);
+  const unsigned char *w_base = a.codes + static_cast<int64_t>(n0) * (a.k / 2);
+  const unsigned char *p_base = a.powers + static_cast<int64_t>(n0) * blocks;
+  unsigned int x_off[S::kLoads], w_off[S::kLoadsW], p_off[PR];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int token = m0 + (wm * MT + m) * 32 + c;
-    if (token >= a.rows) continue;
+  for (int i = 0; i < S::kLoads; ++i) {
+    const int at = i * S::kThreads + tid, token = min(at / CH, a.rows - 1 - m0);
+    x_off[i] = (static_cast<unsigned int>(token) * static_cast<unsigned int>(a.x_stride) + at % CH * 8) * sizeof(T);
+  }
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+  for (int i = 0; i < S::kLoadsW; ++i) {
+    const int at = i * S::kThreads + tid;
+    w_off[i] = static_cast<unsigned int>(min(at / 4, a.n - 1 - n0)) * (a.k / 2) + at % 4 * 16;
+  }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int n = n0 + (wn * NT + t) * 32 + 8 * i + 4 * h;
-        const f32x4 v = {acc[m][t][4 * i], acc[m][t][4 * i + 1], acc[m][t][4 * i + 2], acc[m][t][4 * i + 3]};
-        if (n >= a.n) continue;
-        if (a.splits > 1) {
-          float *o = a.partial + (static_cast<int64_t>(split) * a.rows + token) * a.n + n;
-          if (n + 4 <= a.n) store4(o, v);
-          else for (int e = 0; e < a.n - n; ++e) o[e] = v[e];
-        } else {
-          T *o = static_cast<T *>(a.out) + static_cast<int64_t>(token) * a.n + n;
-          if (n + 4 <= a.n) store4(o, v);
-          else for (int e = 0; e < a.n - n; ++e) o[e] = Elem<T>::from_float(v[e]);
+  for (int i = 0; i < PR; ++i)
+    p_off[i] = static_cast<unsigned int>(min((i * S::kThreads + tid) % S::kRows, a.n - 1 - n0)) * blocks;
+
+  // In the last step what lies past the end is loaded from the last piece (the
+  // powers from the row's last four) and counts as zero.
+  u32x4 x[S::kLoads], w[S::kLoadsW];
+  unsigned int pw[PR];
+  const auto fetch = [&](int k0) {
+    const bool whole = k0 + S::kStep <= k_last;
+    const char *xp = x_base + static_cast<int64_t>(k0) * sizeof(T);
+    const unsigned char *wp = w_base + k0 / 2, *pp = p_base + min(k0 / kMxBlock, blocks - 4);
+#pragma unroll
+    for (int i = 0; i < S::kLoadsW; ++i) {
+      unsigned int off = w_off[i];
+      if (!whole) off -= max(0, k0 / kMxBlock + tid % 4 - (k_last / kMxBlock - 1)) * 16;
+      w[i] = *reinterpret_cast<const u32x4 *>(wp + off);
+    }
+#pragma unroll
+    for (int i = 0; i < PR; ++i) __builtin_memcpy(&pw[i], pp + p_off[i], 4);
+#pragma unroll
+    for (int i = 0; i < S::kLoads; ++i) {
+      unsigned int off = x_off[i];
+      if (!whole) off -= max(0, k0 + (i * S::kThreads + tid) % CH * 8 - (k_last - 8)) * sizeof(T);
+      x[i] = raw8(reinterpret_cast<const T *>(xp + off), VEC);
+    }
+  };
+  const auto store = [&](int k0) {
+    if (k0 + S::kStep > k_last) {
+      const int past = k0 / kMxBlock + 4 - k_last / kMxBlock;  // blocks of this step past the end, 1 to 3
+#pragma unroll
+      for (int i = 0; i < S::kLoads; ++i)
+        if (k0 + (i * S::kThreads + tid) % CH * 8 >= k_last) x[i] = u32x4{};
+#pragma unroll
+      for (int i = 0; i < S::kLoadsW; ++i)
+        if (tid % 4 >= 4 - past) w[i] = u32x4{};
+#pragma unroll
+      for (int i = 0; i < PR; ++i) pw[i] = pw[i] >> (8 * past) | 0x7f7f7f7fu << (32 - 8 * past);
+    }
+#pragma unroll
+    for (int i = 0; i < S::kLoads; ++i) {
+      const int at = i * S::kThreads + tid, token = at / CH;
+      s_x[token * CH + (at % CH ^ (token & 15))] = x[i];
+    }
+#pragma unroll
+    for (int i = 0; i < S::kLoadsW; ++i) {
+      const int at = i * S::kThreads + tid, row = at / 4;
+      s_w[row * 4 + (at % 4 ^ (row >> 2 & 3))] = w[i];
+    }
+#pragma unroll
+    for (int i = 0; i < PR; ++i)
+      if (PR > 1 || tid < S::kRows) s_p[i * S::kThreads + tid] = pw[i];
+  };
+
+  f32x16 acc[MT][NT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[m][t] = f32x16{};
+  bool far = false;
+  const auto compute = [&]() {
+    unsigned int bytes[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) bytes[t] = s_p[(wn * NT + t) * 32 + c] >> (8 * h);
+#pragma unroll
+    for (int s = 0; s < S::STEPS; ++s) {
+      float scale[NT];
+      u32x4 block[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const unsigned int byte = bytes[t] >> (16 * s) & 255;
+        scale[t] = Elem<T>::kDtype == HEXKV_F16 ? near_scale(byte, &far) : mx_scale(byte);
+        const int row = (wn * NT + t) * 32 + c;
+        block[t] = s_w[row * 4 + ((s * 2 + h) ^ (row >> 2 & 3))];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u32x4 b[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const int token = (wm * MT + m) * 32 + c;
+          b[m] = s_x[token * CH + ((s * 8 + h * 4 + j) ^ (token & 15))];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (Elem<T>::kDtype == HEXKV_F16) {
+            const u32x4 e = mx_f16(block[t][j], scale[t]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[m][t] = mma32_f16(e, b[m], acc[m][t]);
+          } else {
+            const u32x4 e = mx_bf16(block[t][j], scale[t]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[m][t] = mma32_bf16(e, b[m], acc[m][t]);
+          }
         }
       }
+    }
+  };
+
+  fetch(k_first);
+  for (int k0 = k_first; k0 < k_last; k0 += S::kStep) {
+    store(k0);
+    __syncthreads();
+    fetch(min(k0 + S::kStep, k_last - kMxBlock));  // (after the last step: loaded, never used)
+    compute();
+    __syncthreads();
   }
+  if (Elem<T>::kDtype == HEXKV_F16 && __ballot(far)) tile_far<T, S>(a, m0, n0, k_first, k_last, wm, wn, 0, c, h, acc);
+  tile_store<T, S>(a, m0, n0, split, wm, wn, c, h, acc);
 }
 
 // out = the sum of the splits' products, in their order.
@@ -769,11 +947,15 @@ __global__ __launch_bounds__(kMxlThreads) void mx_sum_kernel(const MxLinearArgs 
 //           tokens 30.8 against 37): each workgroup reads every token once,
 //           which many matrix tiles share.  Below that a tile: 64 x 4096 x
 //           11264 23.7 us against 37.
-//   65-     tiles of 64 tokens up to kNarrowTokens (128 x 22528 x 4096 54 us against
-//           62), of 128 above (611 x 4096 x 11264 fp16 96 us against 107, 590
-//           TFLOP/s).
-enum MxKind { kRows, kFew16, kFew32, kFew64, kTile32, kTile64, kTileNarrow, kTilePrompt };
-constexpr int kFewRows = 8192, kNarrowTokens = 192;
+//   65-     16-bit: mx_prompt_kernel, by tiles of 64 tokens x 128 rows up to
+//           kNarrowTokens (128 x 22528 x 4096 45 us, x 256 rows 49; 300 x 6144 x
+//           4096 30.2 / 32.3), then 64 x 256 (611 x 4096 x 11264 74 us, fp16 84; x 128
+//           rows over 82), and 128 x 256 where those make kLargeTiles (2048 x
+//           22528 x 4096 341 us, 1.1 PFLOP/s; 64 x 256 over 369; 611 x 4096 x 11264 78 / 74).
+//           Below 128 of the inner dimension, tiles of 64.  fp32: mx_tile_kernel,
+//           64 tokens up to kWideTokens, 128 above.
+enum MxKind { kRows, kFew16, kFew32, kFew64, kTile32, kTile64, kNarrow, kPrompt, kLarge, kWide32, kWider32 };
+constexpr int kFewRows = 8192, kNarrowTokens = 320, kLargeTiles = 512, kWideTokens = 192;
 
 struct MxPlan {
   int kind;
@@ -786,8 +968,11 @@ struct MxPlan {
 constexpr int inner_waves(size_t elem) { return elem == 4 ? 2 : 4; }
 template <typename T> using Tile32 = MxTileShape<T, 1, 1, 1, 2, inner_waves(sizeof(T)), 1, 4, 4>;
 template <typename T> using Tile64 = MxTileShape<T, 2, 1, 1, 2, inner_waves(sizeof(T)), 1, 4, 2>;
-template <typename T> using TileNarrow = MxTileShape<T, 2, 2, 1, 2, 2, 1, 2, 2>;
-template <typename T> using TilePrompt = MxTileShape<T, 2, 2, 2, 2, 1, 1, 2, 1>;
+template <typename T> using Narrow = MxPromptShape<T, 1, 2, 2, 2>;
+template <typename T> using Prompt = MxPromptShape<T, 2, 2, 1, 4>;
+template <typename T> using Large = MxPromptShape<T, 2, 4, 2, 2>;
+using Wide32 = MxTileShape<float, 2, 2, 1, 2, 2, 1, 2, 2>;
+using Wider32 = MxTileShape<float, 2, 2, 2, 2, 1, 1, 2, 1>;
 
 // Splits of the inner dimension: two workgroups a CU, at least four steps each.
 template <typename S>
@@ -828,12 +1013,16 @@ static MxPlan mx_plan(int rows, int n, int k) {
     else plan_few(&p, kFew64, 2, rows, k);
   } else if (rows <= 32) {
     plan_tile<Tile32<T>>(&p, kTile32, rows, n, k);
-  } else if (rows <= 64) {
+  } else if (rows <= 64 || (sizeof(T) == 2 && k < 128)) {
     plan_tile<Tile64<T>>(&p, kTile64, rows, n, k);
+  } else if constexpr (sizeof(T) == 4) {
+    if (rows <= kWideTokens) plan_tile<Wide32>(&p, kWide32, rows, n, k);
+    else plan_tile<Wider32>(&p, kWider32, rows, n, k);
   } else if (rows <= kNarrowTokens) {
-    plan_tile<TileNarrow<T>>(&p, kTileNarrow, rows, n, k);
+    plan_tile<Narrow<T>>(&p, kNarrow, rows, n, k);
   } else {
-    plan_tile<TilePrompt<T>>(&p, kTilePrompt, rows, n, k);
+    plan_tile<Large<T>>(&p, kLarge, rows, n, k);
+    if (p.m_tiles * p.n_tiles < kLargeTiles) plan_tile<Prompt<T>>(&p, kPrompt, rows, n, k);
   }
   return p;
 }
@@ -852,6 +1041,14 @@ static void launch_tile_shape(const MxLinearArgs &a, hipStream_t s) {
   const unsigned groups = static_cast<unsigned>(a.n_tiles * a.splits + 7) / 8 * 8;
   if (a.vec) mx_tile_kernel<T, S, true><<<groups * a.m_tiles, S::kThreads, 0, s>>>(a);
   else mx_tile_kernel<T, S, false><<<groups * a.m_tiles, S::kThreads, 0, s>>>(a);
+}
+
+template <typename T, typename S>
+static void launch_prompt(const MxLinearArgs &a, hipStream_t s) {
+  static_assert(S::kLds <= 64 * 1024, "LDS");
+  const unsigned groups = static_cast<unsigned>(a.n_tiles * a.splits + 7) / 8 * 8;
+  if (a.vec) mx_prompt_kernel<T, S, true><<<groups * a.m_tiles, S::kThreads, 0, s>>>(a);
+  else mx_prompt_kernel<T, S, false><<<groups * a.m_tiles, S::kThreads, 0, s>>>(a);
 }
 
 template <typename T, int TOKENS, int LOADS, int ROWS>
@@ -917,8 +1114,15 @@ static void mx_linear_launch(MxLinearArgs a, const MxPlan &p, hipStream_t s) {
       break;
     case kTile32: launch_tile_shape<T, Tile32<T>>(a, s); break;
     case kTile64: launch_tile_shape<T, Tile64<T>>(a, s); break;
-    case kTileNarrow: launch_tile_shape<T, TileNarrow<T>>(a, s); break;
-    default: launch_tile_shape<T, TilePrompt<T>>(a, s);
+    default:
+      if constexpr (sizeof(T) == 4) {
+        if (p.kind == kWide32) launch_tile_shape<T, Wide32>(a, s);
+        else launch_tile_shape<T, Wider32>(a, s);
+      } else {
+        if (p.kind == kNarrow) launch_prompt<T, Narrow<T>>(a, s);
+        else if (p.kind == kPrompt) launch_prompt<T, Prompt<T>>(a, s);
+        else launch_prompt<T, Large<T>>(a, s);
+      }
   }
   if (a.splits > 1) {
     const int64_t total = static_cast<int64_t>(a.rows) * a.n;

@@ -401,6 +401,30 @@ def test_linear(device, dtype, rows, n, k):
         assert torch.equal(fp4.linear(skewed, w), got)
 
 
+# rows, n and k on either side of a prompt's tiles, of a step of 128 and of the
+# splits; the largest tiles; inner dimensions below a step
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,n,k", [(65, 127, 128), (64 + 63, 129, 160), (128, 1, 224), (129, 257, 192), (320, 128, 1056),
+                                      (321, 256, 416), (383, 257, 128), (330, 15, 2080), (70, 33, 96), (200, 40, 32),
+                                      (4000, 4090, 160)])
+def test_linear_of_a_prompt(device, dtype, rows, n, k):
+    test_linear(device, dtype, rows, n, k)
+
+
+@pytest.mark.parametrize("rows", [70, 400])
+def test_a_prompt_with_a_far_power_in_the_last_step(device, rows):
+    k, n = 416, 300
+    x = randn((rows, k), 1, torch.float16, device)
+    w = fp4.quantize(randn((n, k), 2, torch.float32, device))
+    w.powers[7, 12], w.powers[299, 9], w.powers[260, 0] = 95, 100, 103
+    values = wide(fp4.dequantize(w, torch.float32))
+    want = wide(x) @ values.T
+    assert (np.abs(wide(fp4.linear(x, w)) - want) <= linear_tolerance(wide(x), values, want, torch.float16)).all()
+    w.powers[5, 12] = 255
+    got = fp4.linear(x, w)
+    assert torch.isnan(got[:, 5]).all() and torch.isfinite(got).sum() == rows * (n - 1)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [1, 40, 150])
 def test_linear_with_far_powers_and_nan(device, dtype, rows):
