@@ -344,6 +344,16 @@ def test_attention_of_strided_rows(device):
     assert not out[..., :3].any()
 
 
+@pytest.mark.parametrize("q_len,partition", [(1, 0), (1, 32), (5, 0), (5, 64), (130, 0)])
+def test_attention_in_place(device, q_len, partition):
+    kv = randn((2, 200, 2, 2, 64), 1, torch.bfloat16, device)
+    q = randn((2, q_len, 8, 64), 2, torch.bfloat16, device)
+    cache = make_cache(kv, 200, device)
+    want = fp4.decode_attention(q, cache, 2, max_seqlen=200, seqlen_bias=200, causal=True, partition=partition)
+    assert fp4.decode_attention(q, cache, 2, max_seqlen=200, seqlen_bias=200, causal=True, partition=partition, out=q) is q
+    assert torch.equal(q, want)
+
+
 def test_a_long_row_at_far_offsets(device):
     """A sequence whose rows lie beyond 4 GiB of the cache's start."""
     heads, d, n = 8, 128, 300
