@@ -949,7 +949,7 @@ __global__ __launch_bounds__(kMxlThreads) void mx_sum_kernel(const MxLinearArgs 
 //           11264 23.7 us against 37.
 //   65-     16-bit: mx_prompt_kernel, by tiles of 64 tokens x 128 rows up to
 //           kNarrowTokens (128 x 22528 x 4096 45 us, x 256 rows 49; 300 x 6144 x
-//           4096 30.2 / 32.3), then 64 x 256 (611 x 4096 x 11264 74 us, fp16 84; x 128
+//           4096 30.2 / 32.3), then 64 x 256 (611 x 4096 x 11264 74 us, fp16 79; x 128
 //           rows over 82), and 128 x 256 where those make kLargeTiles (2048 x
 //           22528 x 4096 341 us, 1.1 PFLOP/s; 64 x 256 over 369; 611 x 4096 x 11264 78 / 74).
 //           Below 128 of the inner dimension, tiles of 64.  fp32: mx_tile_kernel,
