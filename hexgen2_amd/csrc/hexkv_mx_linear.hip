@@ -9,8 +9,8 @@
 //   mx_rows_kernel  one or two tokens: a wave reads rows from end to end;
 //   mx_few_kernel   up to 64: a wave holds the tokens' operands of its share of
 //                   the inner dimension in registers and walks the matrix;
-//   mx_tile_kernel  as many in small matrices, and fp32: tiles, with the tokens in LDS;
-//   mx_prompt_kernel  more: tiles, with the tokens and the matrix's four bits in LDS.
+//   mx_prompt_kernel  more: tiles, with the tokens and the matrix's four bits in LDS;
+//   mx_tile_kernel  fp32 above 16 tokens: tiles, with the tokens' three terms in LDS.
 //
 // bf16 activations meet the matrix as bf16, exact for every power.  fp16 ones
 // meet it as fp16, exact for powers from 2^-23 to 2^13; blocks with another
@@ -268,14 +268,26 @@ struct PowerBytes {
   __device__ __forceinline__ unsigned int operator[](int i) const { return v[i / 4] >> 8 * (i % 4) & 255; }
 };
 
+__device__ __forceinline__ void lds_fence() {  // orders this wave's LDS accesses
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Up to 16 MT tokens over one split of the inner dimension (1024 BL of it): each
 // of eight waves takes an eighth, its tokens' operands in registers (16 MT BL of
-// them), and walks the matrix 16 rows at a time; the waves join through LDS.  BL: consecutive blocks of a row that a lane holds; RING: matrix tiles a
-// wave has loaded or in flight; VEC: the activations' rows are 16-byte aligned.
+// them), and walks the matrix 16 rows at a time; the waves join through LDS.
+// What bounded it were the address units, where a load's lanes read different
+// rows: the matrix's words now change lanes after the load, the tokens go through
+// LDS once (64 x 22528 x 4096 30.5 -> 24.0 us, 16 x 4096 x 4096 8.0 -> 5.9).  BL: consecutive
+// blocks of a row that a lane holds; RING: matrix tiles a wave has loaded or in
+// flight (one more cost 1 to 5%); VEC: the activations' rows are 16-byte aligned.
 template <typename T, int MT, int BL, int RING, bool VEC>
 __global__ __launch_bounds__(512) void mx_few_kernel(const MxLinearArgs a) {
   constexpr int XW = kOperandWords<T>, WAVES = 8;
-  __shared__ f32x4 s_part[2][WAVES][MT][64];
+  // the join's, and before it the tokens on their way to the lanes
+  constexpr int kJoin = 2 * WAVES * MT * 64, kStage = sizeof(T) == 2 ? WAVES * 256 * BL : 0;
+  __shared__ f32x4 s_mem[kJoin > kStage ? kJoin : kStage];
+  auto *s_part = reinterpret_cast<f32x4(*)[WAVES][MT][64]>(s_mem);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int row_blocks = a.k / kMxBlock, n_tiles = (a.n + 15) / 16;
@@ -288,19 +300,26 @@ __global__ __launch_bounds__(512) void mx_few_kernel(const MxLinearArgs a) {
   // No load is conditional (the launch has rows of at least BL blocks): a lane
   // whose blocks do not all exist reads BL before the end, and those
   // that are not its own count as zero.
-  const int from = max(0, min(first, blocks - BL));
+  const auto nearest = [&](int block) { return max(0, min(block, blocks - BL)); };
+  const int from = nearest(first);
   const auto foreign = [&](int s) { return from + s < first || from + s >= blocks; };
   struct Tile {
     u32x4 w[BL];
     PowerBytes<BL> power;
   };
   Tile ring[RING];
+  // Loaded, lane 4 c + g has what lane (c, g) needs: four lanes read one row, and
+  // a load touches 16 to 32 lines instead of 64.
+  const int loads_from = nearest(block0 + (wave * 4 + (lane & 3)) * BL);
   const auto fetch = [&](int tile, Tile &t) {
-    const int64_t row = min(tile * 16 + c, a.n - 1);
-    const unsigned char *p = a.codes + (row * row_blocks + from) * 16;
+    const int64_t row = min(tile * 16 + (lane >> 2), a.n - 1);
+    const unsigned char *p = a.codes + (row * row_blocks + loads_from) * 16;
 #pragma unroll
     for (int i = 0; i < BL; ++i) t.w[i] = *reinterpret_cast<const u32x4 *>(p + i * 16);
-    t.power.read(a.powers + row * row_blocks + from);
+    t.power.read(a.powers + row * row_blocks + loads_from);
+  };
+  const auto exchange = [&](unsigned int v) {
+    return static_cast<unsigned int>(__builtin_amdgcn_ds_bpermute(16 * c + 4 * g, static_cast<int>(v)));
   };
   const int stride = static_cast<int>(gridDim.x);
   const int tile0 = static_cast<int>(blockIdx.x);
@@ -314,15 +333,44 @@ __global__ __launch_bounds__(512) void mx_few_kernel(const MxLinearArgs a) {
 #pragma unroll
   for (int m = 0; m < MT; ++m)
     tokens[m] = static_cast<const T *>(a.x) + static_cast<int64_t>(min(m0 + 16 * m + c, a.rows - 1)) * a.x_stride + from * kMxBlock;
+  if constexpr (sizeof(T) == 2) {
+    // (through LDS: lanes that load their own token's 16 bytes touch 64 lines a
+    // load, 7 of the 25 us of 64 x 22528 x 4096)
+    constexpr int CH = 16 * BL;  // chunks of 8 elements of a token's share
+    u32x4 *stage = reinterpret_cast<u32x4 *>(s_mem) + wave * 256 * BL;
+    const int share = block0 + wave * 4 * BL;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      u32x4 v[4 * BL];
+#pragma unroll
+      for (int i = 0; i < 4 * BL; ++i) {
+        const int at = i * 64 + lane;
+        const T *row = static_cast<const T *>(a.x) + static_cast<int64_t>(min(m0 + 16 * m + at / CH, a.rows - 1)) * a.x_stride;
+        v[i] = raw8(row + min(share * kMxBlock + at % CH * 8, a.k - 8), VEC);
+      }
+#pragma unroll
+      for (int i = 0; i < 4 * BL; ++i) {
+        const int at = i * 64 + lane, token = at / CH;
+        stage[token * CH + (at % CH ^ (token & 7))] = v[i];
+      }
+      lds_fence();
+#pragma unroll
+      for (int s = 0; s < BL; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int chunk = max(0, from + s - share) * 4 + j;  // (a foreign block: any)
+          x[m][s][j] = stage[c * CH + (chunk ^ (c & 7))];
+        }
+      lds_fence();
+    }
+    __syncthreads();
+  }
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int s = 0; s < BL; ++s) {
       const T *p = tokens[m] + s * kMxBlock;
-      if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[m][s][j] = raw8(p + 8 * j, VEC);
-      } else {
+      if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float f[8];
@@ -343,7 +391,7 @@ __global__ __launch_bounds__(512) void mx_few_kernel(const MxLinearArgs a) {
   }
 #pragma unroll
   for (int r = 1; r < RING; ++r)
-    if (!idle && tile0 + r * stride < n_tiles) fetch(tile0 + r * stride, ring[r]);
+    if (!idle) fetch(tile0 + r * stride, ring[r]);
 
   for (int base = tile0, turn = 0; base < n_tiles; base += RING * stride) {
 #pragma unroll
@@ -357,6 +405,13 @@ __global__ __launch_bounds__(512) void mx_few_kernel(const MxLinearArgs a) {
       if (!idle) {
         Tile &t = ring[r];
         unsigned int byte[BL];
+#pragma unroll
+        for (int s = 0; s < BL; ++s) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) t.w[s][j] = exchange(t.w[s][j]);
+        }
+#pragma unroll
+        for (int i = 0; i < (BL + 3) / 4; ++i) t.power.v[i] = exchange(t.power.v[i]);
 #pragma unroll
         for (int s = 0; s < BL; ++s) byte[s] = t.power[s];
         if (ragged) {
@@ -389,7 +444,7 @@ __global__ __launch_bounds__(512) void mx_few_kernel(const MxLinearArgs a) {
             }
           }
         }
-        if (tile + RING * stride < n_tiles) fetch(tile + RING * stride, t);
+        fetch(tile + RING * stride, t);  // (past the end the last row again)
       }
       if (Elem<T>::kDtype == HEXKV_F16 && __ballot(far)) {
         const int64_t row = min(tile * 16 + c, a.n - 1);
@@ -440,7 +495,7 @@ __global__ __launch_bounds__(512) void mx_few_kernel(const MxLinearArgs a) {
   }
 }
 
-// More tokens: a workgroup takes 32 MT WM tokens by 32 NT WN rows of the matrix;
+// fp32 above 16 tokens: a workgroup takes 32 MT WM tokens by 32 NT WN rows of the matrix;
 // its waves are WM x WN pieces of that, times WK that share the inner
 // dimension.  A step is STEPS times 64 of the inner dimension for each of the
 // WK: the tokens' piece of it lies in LDS (two of them, loaded through
@@ -451,14 +506,14 @@ __global__ __launch_bounds__(512) void mx_few_kernel(const MxLinearArgs a) {
 // and the tokens' operand the same elements.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-template <typename T, int MT_, int NT_, int WM_, int WN_, int WK_, int STEPS_, int RING_, int XR_>
+template <int MT_, int NT_, int WM_, int WN_, int WK_, int STEPS_, int RING_, int XR_>
 struct MxTileShape {
   static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, WK = WK_, STEPS = STEPS_, RING = RING_, XR = XR_;
   static_assert(RING % XR == 0 && RING % 2 == 0, "the loop is unrolled by the ring");
   static constexpr int kWaves = WM * WN * WK, kThreads = 64 * kWaves;
   static constexpr int kTokens = 32 * MT * WM, kRows = 32 * NT * WN;
   static constexpr int kStep = 64 * WK * STEPS;            // inner dimension of one step
-  static constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;   // 16-bit terms of an activation in LDS
+  static constexpr int kPlanes = 3;                        // 16-bit terms of an activation in LDS
   static constexpr int kChunks = kStep / 8;                // 16-byte chunks of a token's row in LDS
   static constexpr int kPlane = kTokens * kChunks;         // chunks of a plane
   static constexpr int kLoads = kPlane / kThreads;         // chunks a thread stages
@@ -476,14 +531,14 @@ __device__ __forceinline__ f32x16 mma32_f16(u32x4 a, u32x4 b, f32x16 c) {
 
 // The blocks whose power fp16 does not hold, in bf16.
 template <typename T, typename S>
-__device__ __forceinline__ void tile_far(const MxLinearArgs &a, int m0, int n0, int k_first, int k_last, int wm, int wn, int wk,
+__device__ __forceinline__ void tile_far(const MxLinearArgs &a, int m0, int n0, int k_first, int k_last, int wm, int wn,
                                          int c, int h, f32x16 (&acc)[S::MT][S::NT]) {
   constexpr int MT = S::MT, NT = S::NT;
 #pragma unroll 1
   for (int k0 = k_first; k0 < k_last; k0 += S::kStep)
 #pragma unroll 1
     for (int s = 0; s < S::STEPS; ++s) {
-      const int k = k0 + (wk * S::STEPS + s) * 64 + h * kMxBlock;
+      const int k = k0 + s * 64 + h * kMxBlock;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         FarBlock block;
@@ -534,8 +589,9 @@ __device__ __forceinline__ void tile_store(const MxLinearArgs &a, int m0, int n0
   }
 }
 
-template <typename T, typename S, bool VEC>
+template <typename S, bool VEC>
 __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs a) {
+  using T = float;
   constexpr int MT = S::MT, NT = S::NT, CH = S::kChunks, PL = S::kPlanes;
   constexpr int kSpread = CH >= 16 ? 1 : 16 / CH;  // rows whose chunks fill the banks once
   constexpr int kMask = CH >= 16 ? 15 : CH - 1;
@@ -574,7 +630,7 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs
   }
 
   struct Tokens {
-    u32x4 v[PL == 1 ? 1 : 2][S::kLoads];
+    u32x4 v[2][S::kLoads];
   };
   const auto fetch_x = [&](int k0, Tokens &stage) {
     const char *base = x_base + static_cast<int64_t>(k0) * sizeof(T);
@@ -584,22 +640,18 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs
       unsigned int off = x_off[i];
       if (!whole) off -= max(0, k0 + (i * S::kThreads + tid) % CH * 8 - (k_last - 8)) * sizeof(T);
       const T *p = reinterpret_cast<const T *>(base + off);
-      if constexpr (PL == 1) {
-        stage.v[0][i] = raw8(p, VEC);
+      u32x4 f[2];
+      if constexpr (VEC) {
+        f[0] = *reinterpret_cast<const u32x4 *>(p);
+        f[1] = *reinterpret_cast<const u32x4 *>(p + 4);
       } else {
-        u32x4 f[2];
-        if constexpr (VEC) {
-          f[0] = *reinterpret_cast<const u32x4 *>(p);
-          f[1] = *reinterpret_cast<const u32x4 *>(p + 4);
-        } else {
-          float e[8];
+        float e[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) e[j] = p[j];
-          __builtin_memcpy(f, e, sizeof(e));
-        }
-        stage.v[0][i] = f[0];
-        stage.v[1][i] = f[1];
+        for (int j = 0; j < 8; ++j) e[j] = p[j];
+        __builtin_memcpy(f, e, sizeof(e));
       }
+      stage.v[0][i] = f[0];
+      stage.v[1][i] = f[1];
     }
   };
   // (Tokens past the last repeat it and are not stored.)
@@ -609,14 +661,10 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs
     for (int i = 0; i < S::kLoads; ++i) {
       const int at = i * S::kThreads + tid, token = at / CH, chunk = at % CH;
       u32x4 terms[PL];
-      if constexpr (PL == 1) {
-        terms[0] = stage.v[0][i];
-      } else {
-        float f[8];
-        Elem<float>::to_float(stage.v[0][i], f);
-        Elem<float>::to_float(stage.v[1][i], f + 4);
-        terms8<3>(f, terms);
-      }
+      float f[8];
+      Elem<float>::to_float(stage.v[0][i], f);
+      Elem<float>::to_float(stage.v[1][i], f + 4);
+      terms8<3>(f, terms);
       if (!whole && k0 + chunk * 8 >= k_last) {
 #pragma unroll
         for (int n = 0; n < PL; ++n) terms[n] = u32x4{};
@@ -651,7 +699,6 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[m][t] = f32x16{};
 
-  bool far = false;
   const auto compute = [&](int buf, int k0, Weights &x) {
     if (k0 + S::kStep > k_last) {  // what lies past the end counts as zero
 #pragma unroll
@@ -669,7 +716,7 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs
       float scale[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
-        scale[t] = Elem<T>::kDtype == HEXKV_F16 ? near_scale(x.byte[s][t], &far) : mx_scale(x.byte[s][t]);
+        scale[t] = mx_scale(x.byte[s][t]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         u32x4 b[PL][MT];
@@ -682,17 +729,11 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs
           }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          if constexpr (Elem<T>::kDtype == HEXKV_F16) {
-            const u32x4 w = mx_f16(x.w[s][t][j], scale[t]);
+          const u32x4 w = mx_bf16(x.w[s][t][j], scale[t]);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) acc[m][t] = mma32_f16(w, b[0][m], acc[m][t]);
-          } else {
-            const u32x4 w = mx_bf16(x.w[s][t][j], scale[t]);
+          for (int n = 0; n < PL; ++n)
 #pragma unroll
-            for (int n = 0; n < PL; ++n)
-#pragma unroll
-              for (int m = 0; m < MT; ++m) acc[m][t] = mma32_bf16(w, b[n][m], acc[m][t]);
-          }
+            for (int m = 0; m < MT; ++m) acc[m][t] = mma32_bf16(w, b[n][m], acc[m][t]);
         }
       }
     }
@@ -721,8 +762,6 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs
       __syncthreads();
     }
   }
-
-  if (Elem<T>::kDtype == HEXKV_F16 && __ballot(far)) tile_far<T, S>(a, m0, n0, k_first, k_last, wm, wn, wk, c, h, acc);
 
   // the waves that share the inner dimension join, half of them at a time
   if constexpr (S::WK > 1) {
@@ -764,7 +803,7 @@ __global__ __launch_bounds__(S::kThreads) void mx_tile_kernel(const MxLinearArgs
 // workgroups a CU fill the barriers.
 template <typename T, int MT_, int NT_, int WM_, int WN_>
 struct MxPromptShape {
-  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, WK = 1, STEPS = 2;
+  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, STEPS = 2;
   static constexpr int kThreads = 64 * WM * WN;
   static constexpr int kTokens = 32 * MT * WM, kRows = 32 * NT * WN, kStep = 128;
   static constexpr int kChunks = kStep / 8;
@@ -916,7 +955,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void mx_prompt_kernel(const MxLinea
     compute();
     __syncthreads();
   }
-  if (Elem<T>::kDtype == HEXKV_F16 && __ballot(far)) tile_far<T, S>(a, m0, n0, k_first, k_last, wm, wn, 0, c, h, acc);
+  if (Elem<T>::kDtype == HEXKV_F16 && __ballot(far)) tile_far<T, S>(a, m0, n0, k_first, k_last, wm, wn, c, h, acc);
   tile_store<T, S>(a, m0, n0, split, wm, wn, c, h, acc);
 }
 
@@ -941,21 +980,20 @@ __global__ __launch_bounds__(kMxlThreads) void mx_sum_kernel(const MxLinearArgs 
 
 // The kernels and tiles a call may run, by tokens (GPU time of a call on MI355X,
 // weights from memory, bf16 unless said):
-//   1, 2    kRows: 1 x 22528 x 4096 10.9 us (4.5 TB/s); kFew 12.7.
-//   3-16    kFew, 16 tokens a wave: 16 x 22528 x 4096 16.8 us; a tile 29.
-//   17-64   kFew where the matrix has kFewRows rows or more (32 tokens 21.0 us, a tile 29.6; 64
-//           tokens 30.8 against 37): each workgroup reads every token once,
-//           which many matrix tiles share.  Below that a tile: 64 x 4096 x
-//           11264 23.7 us against 37.
+//   1, 2    kRows: 1 x 22528 x 4096 10.9 us (4.5 TB/s); kFew 14.2.
+//   3-64    kFew, 16, 32 or 64 tokens a wave (16 x 22528 x 4096 14.7 us, 32 x 16.8, 64 x
+//           25.8; 64 x 4096 x 4096 11.2, where a tile of the tokens in LDS took
+//           14.8; 32 x 2560 x 2048 4.6 and 9.0; 32 x 4096 x 11264 18.2 and 17.8).
+//           fp32: to 16, then tiles (three registers a token of each).
 //   65-     16-bit: mx_prompt_kernel, by tiles of 64 tokens x 128 rows up to
 //           kNarrowTokens (128 x 22528 x 4096 45 us, x 256 rows 49; 300 x 6144 x
 //           4096 30.2 / 32.3), then 64 x 256 (611 x 4096 x 11264 74 us, fp16 79; x 128
 //           rows over 82), and 128 x 256 where those make kLargeTiles (2048 x
 //           22528 x 4096 341 us, 1.1 PFLOP/s; 64 x 256 over 369; 611 x 4096 x 11264 78 / 74).
-//           Below 128 of the inner dimension, tiles of 64.  fp32: mx_tile_kernel,
-//           64 tokens up to kWideTokens, 128 above.
+//           Below 128 of the inner dimension, kFew 64 at a time.  fp32:
+//           mx_tile_kernel, 64 tokens up to kWideTokens, 128 above.
 enum MxKind { kRows, kFew16, kFew32, kFew64, kTile32, kTile64, kNarrow, kPrompt, kLarge, kWide32, kWider32 };
-constexpr int kFewRows = 8192, kNarrowTokens = 320, kLargeTiles = 512, kWideTokens = 192;
+constexpr int kNarrowTokens = 320, kLargeTiles = 512, kWideTokens = 192;
 
 struct MxPlan {
   int kind;
@@ -963,16 +1001,13 @@ struct MxPlan {
   int m_tiles, n_tiles, splits, split_k;
 };
 
-// fp32 tokens are three terms each: shorter steps and fewer waves on the inner dimension, so
-// that they fit LDS.
-constexpr int inner_waves(size_t elem) { return elem == 4 ? 2 : 4; }
-template <typename T> using Tile32 = MxTileShape<T, 1, 1, 1, 2, inner_waves(sizeof(T)), 1, 4, 4>;
-template <typename T> using Tile64 = MxTileShape<T, 2, 1, 1, 2, inner_waves(sizeof(T)), 1, 4, 2>;
+using Tile32 = MxTileShape<1, 1, 1, 2, 2, 1, 4, 4>;
+using Tile64 = MxTileShape<2, 1, 1, 2, 2, 1, 4, 2>;
 template <typename T> using Narrow = MxPromptShape<T, 1, 2, 2, 2>;
 template <typename T> using Prompt = MxPromptShape<T, 2, 2, 1, 4>;
 template <typename T> using Large = MxPromptShape<T, 2, 4, 2, 2>;
-using Wide32 = MxTileShape<float, 2, 2, 1, 2, 2, 1, 2, 2>;
-using Wider32 = MxTileShape<float, 2, 2, 2, 2, 1, 1, 2, 1>;
+using Wide32 = MxTileShape<2, 2, 1, 2, 2, 1, 2, 2>;
+using Wider32 = MxTileShape<2, 2, 2, 2, 1, 1, 2, 1>;
 
 // Splits of the inner dimension: two workgroups a CU, at least four steps each.
 template <typename S>
@@ -1008,16 +1043,15 @@ static MxPlan mx_plan(int rows, int n, int k) {
     p.blocks = loads <= 2 ? loads : loads <= 4 ? 4 : 6;
   } else if (rows <= 16) {
     plan_few(&p, kFew16, sizeof(T) == 4 ? 2 : 4, rows, k);
-  } else if (rows <= 64 && n >= kFewRows && sizeof(T) == 2) {
-    if (rows <= 32) plan_few(&p, kFew32, 4, rows, k);
-    else plan_few(&p, kFew64, 2, rows, k);
-  } else if (rows <= 32) {
-    plan_tile<Tile32<T>>(&p, kTile32, rows, n, k);
-  } else if (rows <= 64 || (sizeof(T) == 2 && k < 128)) {
-    plan_tile<Tile64<T>>(&p, kTile64, rows, n, k);
   } else if constexpr (sizeof(T) == 4) {
-    if (rows <= kWideTokens) plan_tile<Wide32>(&p, kWide32, rows, n, k);
+    if (rows <= 32) plan_tile<Tile32>(&p, kTile32, rows, n, k);
+    else if (rows <= 64) plan_tile<Tile64>(&p, kTile64, rows, n, k);
+    else if (rows <= kWideTokens) plan_tile<Wide32>(&p, kWide32, rows, n, k);
     else plan_tile<Wider32>(&p, kWider32, rows, n, k);
+  } else if (rows <= 32) {
+    plan_few(&p, kFew32, 4, rows, k);
+  } else if (rows <= 64 || k < 128) {
+    plan_few(&p, kFew64, 2, rows, k);
   } else if (rows <= kNarrowTokens) {
     plan_tile<Narrow<T>>(&p, kNarrow, rows, n, k);
   } else {
@@ -1035,12 +1069,12 @@ static size_t mx_partial_bytes(const MxPlan &p, int rows, int n) {
   return p.splits > 1 ? static_cast<size_t>(p.splits) * rows * n * sizeof(float) : 0;
 }
 
-template <typename T, typename S>
-static void launch_tile_shape(const MxLinearArgs &a, hipStream_t s) {
+template <typename S>
+static void launch_tile(const MxLinearArgs &a, hipStream_t s) {
   static_assert(S::kLds <= 160 * 1024, "LDS");
   const unsigned groups = static_cast<unsigned>(a.n_tiles * a.splits + 7) / 8 * 8;
-  if (a.vec) mx_tile_kernel<T, S, true><<<groups * a.m_tiles, S::kThreads, 0, s>>>(a);
-  else mx_tile_kernel<T, S, false><<<groups * a.m_tiles, S::kThreads, 0, s>>>(a);
+  if (a.vec) mx_tile_kernel<S, true><<<groups * a.m_tiles, S::kThreads, 0, s>>>(a);
+  else mx_tile_kernel<S, false><<<groups * a.m_tiles, S::kThreads, 0, s>>>(a);
 }
 
 template <typename T, typename S>
@@ -1095,29 +1129,29 @@ static void mx_linear_launch(MxLinearArgs a, const MxPlan &p, hipStream_t s) {
     // more than one block a lane only where k > 512 times it: a row then has
     // more than 16 times as many
     case kFew16:
-      if (p.blocks == 1) launch_few<T, 1, 1, 4>(a, s);
-      else if (p.blocks == 2) launch_few<T, 1, 2, 2>(a, s);
+      if (p.blocks == 1) launch_few<T, 1, 1, 2>(a, s);
+      else if (p.blocks == 2) launch_few<T, 1, 2, 1>(a, s);
       else if constexpr (sizeof(T) == 2) launch_few<T, 1, 4, 1>(a, s);
       break;
     case kFew32:
       if constexpr (sizeof(T) == 2) {
-        if (p.blocks == 1) launch_few<T, 2, 1, 4>(a, s);
-        else if (p.blocks == 2) launch_few<T, 2, 2, 2>(a, s);
+        if (p.blocks == 1) launch_few<T, 2, 1, 2>(a, s);
+        else if (p.blocks == 2) launch_few<T, 2, 2, 1>(a, s);
         else launch_few<T, 2, 4, 1>(a, s);
       }
       break;
     case kFew64:
       if constexpr (sizeof(T) == 2) {
-        if (p.blocks == 1) launch_few<T, 4, 1, 4>(a, s);
+        if (p.blocks == 1) launch_few<T, 4, 1, 2>(a, s);
         else launch_few<T, 4, 2, 1>(a, s);
       }
       break;
-    case kTile32: launch_tile_shape<T, Tile32<T>>(a, s); break;
-    case kTile64: launch_tile_shape<T, Tile64<T>>(a, s); break;
     default:
       if constexpr (sizeof(T) == 4) {
-        if (p.kind == kWide32) launch_tile_shape<T, Wide32>(a, s);
-        else launch_tile_shape<T, Wider32>(a, s);
+        if (p.kind == kTile32) launch_tile<Tile32>(a, s);
+        else if (p.kind == kTile64) launch_tile<Tile64>(a, s);
+        else if (p.kind == kWide32) launch_tile<Wide32>(a, s);
+        else launch_tile<Wider32>(a, s);
       } else {
         if (p.kind == kNarrow) launch_prompt<T, Narrow<T>>(a, s);
         else if (p.kind == kPrompt) launch_prompt<T, Prompt<T>>(a, s);
