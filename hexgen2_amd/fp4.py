@@ -210,7 +210,7 @@ def decode_attention(q: torch.Tensor, cache: torch.Tensor, kv_heads: int, *, max
     kv_heads = int(kv_heads)
     softmax_scale = None if softmax_scale is None else float(softmax_scale)
     shape = cache.shape
-    key = (_layout(q), shape[0], shape[2:], cache.stride(), cache.dtype, cache.get_device(), kv_heads, _layout(out),
+    key = (_layout(q), shape[0], shape[1] == 1, shape[2:], cache.stride(), cache.dtype, cache.get_device(), kv_heads, _layout(out),
            _layout(kv_new), bool(causal), softmax_scale, int(partition))
     form = _FORMS.get(key)
     if form is None:

@@ -344,6 +344,19 @@ def test_attention_of_strided_rows(device):
     assert not out[..., :3].any()
 
 
+def test_attention_of_padded_rows_after_a_single_position(device):
+    """Two views of a cache whose rows lie further apart than they are long, the
+    first of one position (whose stride says nothing)."""
+    kv = randn((1, 8, 2, 2, 64), 1, torch.float16, device)
+    q = randn((1, 1, 4, 64), 2, torch.float16, device)
+    packed = make_cache(kv, 8, device)
+    padded = torch.full((1, 8, 192), 0xFF, dtype=torch.uint8, device=device)[..., :144]
+    padded.copy_(packed)
+    for n in (1, 8, 5):
+        got = fp4.decode_attention(q, padded[:, :n], 2, max_seqlen=n, seqlen_bias=n)
+        assert torch.equal(got, fp4.decode_attention(q, packed[:, :n], 2, max_seqlen=n, seqlen_bias=n)), n
+
+
 @pytest.mark.parametrize("q_len,partition", [(1, 0), (1, 32), (5, 0), (5, 64), (130, 0)])
 def test_attention_in_place(device, q_len, partition):
     kv = randn((2, 200, 2, 2, 64), 1, torch.bfloat16, device)
