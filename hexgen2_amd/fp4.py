@@ -26,9 +26,12 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _require_device, _stream
+from .ops import _DTYPES, _raw_stream, _require_device, _stream
 
 BLOCK = 32
+
+# (torch's own accessor, as ``_raw_stream``: 0.1 us a call less)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 class Fp4Tensor(NamedTuple):
@@ -89,8 +92,9 @@ def _int32(value: int, name: str) -> int:
 def _call(name: str, tensor: torch.Tensor, *args) -> None:
     """One library call on the current stream of ``tensor``'s device."""
     fn = getattr(_lib.load(), name)
-    if tensor.device.index == torch.cuda.current_device():
-        rc = fn(*args, _stream(tensor))
+    index = tensor.get_device()
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index) if _raw_stream is not None else _stream(tensor))
     else:
         with torch.cuda.device(tensor.device):
             rc = fn(*args, _stream(tensor))
