@@ -23,7 +23,7 @@
 // largest is taken out `top` times over.
 //
 // Measured on MI355X, bf16: 8191 x 32000 without alternatives 97 us (5.4 TB/s),
-// with the top 20 125 us (4.2); one row of 32000 fp16, top 5, 9.0 us (8 parts and their join).
+// with the top 20 125 us (4.2); one row of 32000 fp16, top 5, 9.8 us.
 #include "hexkv_common.h"
 
 #include <algorithm>
@@ -382,14 +382,19 @@ __global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(const LogprobA
   }
 }
 
-// Parts a row is cut into: enough for a workgroup a CU, and for few rows of long
-// vocabularies about twelve chunks each.
-static int lp_parts(int64_t rows, int vocab, int64_t *span) {
+// Parts a row is cut into: one to kLpShort chunks (the join's launch and the
+// workspace cost more: a call for 1 x 32000, top 5, 11.0 us and 15.2 in 8 parts,
+// host included); beyond, enough for a workgroup a CU, and for few rows of long
+// vocabularies about twelve chunks each, but no more keys than a join ranks in
+// passing, since it compares all of them (us in 1 / 4 / 8 / 32 parts: 1 x 128000, top 20
+// 25.6 / 15.5 / 13 / 36, top 64 51 / 33 / 38 / 234, top 5 21 / 12.6 / 10.8 / 11.1;
+// 64 x 128000, top 20, 27.6 / 16.7 / 16.6 / 25.6; 300 x 128000 37.4 / 32.8 / 32.3).
+constexpr int kLpShort = 12, kLpKeys = 160;
+static int lp_parts(int64_t rows, int vocab, int top, int64_t *span) {
   const int64_t chunks = (static_cast<int64_t>(vocab) + 7 + kLpChunk - 1) / kLpChunk;
-  // (64 x 128000, top 20: 17 us at one workgroup a CU, 25.6 at four; 300 x 128000:
-  // 31.5 us in one part, 25.9 in three)
   const int64_t fill = 256 / std::max<int64_t>(rows, 1), long_rows = rows < 1024 ? chunks / 12 : 1;
-  const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>({chunks, kLpMaxParts, std::max(fill, long_rows)}));
+  const int64_t most = top ? std::min(kLpMaxParts, std::max(4, kLpKeys / top)) : kLpMaxParts;
+  const int64_t wanted = chunks <= kLpShort ? 1 : std::max<int64_t>(1, std::min<int64_t>({chunks, most, std::max(fill, long_rows)}));
   const int64_t each = (chunks + wanted - 1) / wanted;
   *span = each * kLpChunk;
   return static_cast<int>((chunks + each - 1) / each);
@@ -397,7 +402,7 @@ static int lp_parts(int64_t rows, int vocab, int64_t *span) {
 
 static size_t lp_workspace(int64_t rows, int vocab, int top) {
   int64_t span;
-  const int parts = lp_parts(rows, vocab, &span);
+  const int parts = lp_parts(rows, vocab, top, &span);
   return parts == 1 ? 0 : static_cast<size_t>(rows) * parts * (16 + 8 * static_cast<size_t>(top));
 }
 
@@ -452,7 +457,7 @@ extern "C" int hexkv_token_logprobs(const void *logits, int64_t row_stride, int6
   a.top = top;
   a.rows = rows;
   int64_t span;
-  a.parts = lp_parts(rows, vocab, &span);
+  a.parts = lp_parts(rows, vocab, top, &span);
   a.span = static_cast<int32_t>(std::min<int64_t>(span, INT32_MAX));
   if (a.parts > 1) {
     a.ws_stats = static_cast<float *>(workspace);

@@ -536,6 +536,20 @@ def test_logprobs_of_rows_that_strain_it(device, dtype, vocab):
     check_logprobs(logits, tokens, 20)
 
 
+# rows in one part and in several, on either side of the border between them, and
+# of the most parts that each `top` allows
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,top", [(2, 49137, 5), (2, 49152, 5), (3, 60001, 20), (1, 131100, 5), (2, 131072, 64),
+                                            (2, 70000, 0), (1, 140000, 1), (40, 50001, 9), (1100, 49200, 2)])
+def test_logprobs_of_long_vocabularies(device, dtype, rows, vocab, top):
+    test_logprobs(device, dtype, rows, vocab, top)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_logprobs_of_long_rows_that_strain_it(device, dtype):
+    test_logprobs_of_rows_that_strain_it(device, dtype, 60001)
+
+
 def test_logprobs_of_strided_rows(device):
     base = randn((7, 12000), 3, torch.bfloat16, device)
     tokens = torch.tensor([5, 0, 7, 11, 2, 9, 4], device=device)

@@ -168,7 +168,7 @@ def logprob_call(**change):
     (dict(dtype=4), E), (dict(rows=-1), E), (dict(vocab=0), E), (dict(vocab=(1 << 30) + 1), E), (dict(top=-1), E),
     (dict(top=65), E), (dict(top=9, vocab=8), E), (dict(rows=1 << 19), R), (dict(logits=None), E), (dict(lp=None), E),
     (dict(ids=None), E), (dict(values=None), E), (dict(logits=ADDRESS + 1), E), (dict(tokens=ADDRESS + 4), E),
-    (dict(vocab=32000), W), (dict(vocab=32000, ws=ADDRESS, size=8), W), (dict(rows=0), 0)])
+    (dict(vocab=64000), W), (dict(vocab=64000, ws=ADDRESS, size=8), W), (dict(rows=0), 0)])
 def test_logprobs_refuse(change, code):
     assert logprob_call(**change) == code
 
