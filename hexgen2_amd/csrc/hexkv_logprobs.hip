@@ -164,10 +164,23 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
       }
     }
   };
-  if (whole(first)) fetch(first);
+  // A row of one chunk goes to the lanes logit by logit, so that every lane and
+  // group has some however short the row or whatever a mask rules out: with
+  // vectors, groups without any left no bar (709 x 825, part of it masked, top 20:
+  // 36 us).
+  const bool single = a.vocab + skew <= kLpChunk;
+  const auto strided = [&](int i, int of) {
+    const int id = i * kLpThreads + of;
+    const float v = static_cast<float>(x[min(id, a.vocab - 1)]);
+    return id < a.vocab ? v : -INFINITY;
+  };
+  if (!single && whole(first)) fetch(first);
   for (int64_t base = first; base < last; base += kLpChunk) {
     float v[kLpEach];
-    if (whole(base)) {
+    if (single) {
+#pragma unroll
+      for (int i = 0; i < kLpEach; ++i) v[i] = strided(i, tid);
+    } else if (whole(base)) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) Elem<T>::to_float(raw[i], v + i * VEC);
     } else {
@@ -243,18 +256,28 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
     __syncthreads();
     const int vectors = static_cast<int>((last - first + kLpChunk - 1) / kLpChunk) * NV, total = s_active_count * vectors;
     // the active lanes' vectors, shared out over all lanes (in any order: the ranks do not depend on it)
+    const auto take = [&](bool equal, int *counter, float v, int64_t id) {
+      if ((equal ? !(v < bar) : !(v <= bar)) && v != -INFINITY) {
+        const int place = atomicAdd(counter, 1);
+        if (place < kLpRoom) s_list[place] = lp_make_key(v, static_cast<unsigned int>(id));
+      }
+    };
     const auto collect = [&](bool equal, int *counter) {
+      if (single) {
+        const int each = (a.vocab + kLpThreads - 1) / kLpThreads;
+        for (int item = tid; item < s_active_count * each; item += kLpThreads) {
+          const int of = item / each, i = item - of * each;
+          take(equal, counter, strided(i, s_active[of]), static_cast<int64_t>(i) * kLpThreads + s_active[of]);
+        }
+        return;
+      }
       for (int item = tid; item < total; item += kLpThreads) {
         const int of = item / vectors, j = item - of * vectors;
         const int64_t at = first + static_cast<int64_t>(j / NV) * kLpChunk + (j % NV * kLpThreads + s_active[of]) * VEC - skew;
         float v[VEC];
         vector_at(at, v);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if ((equal ? !(v[e] < bar) : !(v[e] <= bar)) && v[e] != -INFINITY) {
-            const int place = atomicAdd(counter, 1);
-            if (place < kLpRoom) s_list[place] = lp_make_key(v[e], static_cast<unsigned int>(at + e));
-          }
+        for (int e = 0; e < VEC; ++e) take(equal, counter, v[e], at + e);
       }
     };
     // Ranks by counting the larger keys: one wave by lane reads where a key
