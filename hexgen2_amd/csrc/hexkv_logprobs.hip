@@ -23,7 +23,7 @@
 // largest is taken out `top` times over.
 //
 // Measured on MI355X, bf16: 8191 x 32000 without alternatives 97 us (5.4 TB/s),
-// with the top 20 125 us (4.2); one row of 32000 fp16, top 5, 9.8 us.
+// with the top 20 125 us (4.2); one row of 32000 fp16, top 5, 10.0 us.
 #include "hexkv_common.h"
 
 #include <algorithm>
@@ -218,8 +218,9 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
     s_stats[wave][1] = s_sum;
     s_stats[wave][2] = u_sum;
   }
-  // The bar: the top-th largest of the lanes' maxima (equal ones in the lanes'
-  // order), of 64 groups of four while those are several times as many as `top`.
+  // The bar: the top-th largest of the lanes' maxima, of 64 groups of four while
+  // those are several times as many as `top` (ranked by lane reads; 1 x 305, top 24, 6.3
+  // us, by bits of all 256 7.4; top 32 by bits 7.6, ranking all 256 17).
   if (top && top <= 24) {
     if (wave == 0) {
       const f32x4 four = *reinterpret_cast<const f32x4 *>(s_lane + 4 * lane);
@@ -232,14 +233,21 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
       }
       if (rank == top - 1) s_bar = mine;
     }
-  } else if (top) {
-    int rank = 0;
-    for (int j = 0; j < kLpThreads; j += 4) {
-      const f32x4 four = *reinterpret_cast<const f32x4 *>(s_lane + j);
+  } else if (top && wave == 0) {
+    // all 256, bit by bit from the top: the largest order that `top` of them reach
+    const f32x4 four = *reinterpret_cast<const f32x4 *>(s_lane + 4 * lane);
+    unsigned int order[4], found = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) rank += four[e] > best || (four[e] == best && j + e < tid);
+    for (int e = 0; e < 4; ++e) order[e] = static_cast<unsigned int>(lp_make_key(four[e], 0) >> 32);
+#pragma unroll 4
+    for (int bit = 31; bit >= 0; --bit) {
+      const unsigned int next = found | 1u << bit;
+      int reach = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) reach += __popcll(__ballot(order[e] >= next));
+      if (reach >= top) found = next;
     }
-    if (rank == top - 1) s_bar = best;
+    if (lane == 0) s_bar = lp_key_value(static_cast<lp_key>(found) << 32);
   }
   __syncthreads();
   LpStats all = {m, 0.f, 0.f};
@@ -410,7 +418,8 @@ __global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(const LogprobA
 // host included); beyond, enough for a workgroup a CU, and for few rows of long
 // vocabularies about twelve chunks each, but no more keys than a join ranks in
 // passing, since it compares all of them (us in 1 / 4 / 8 / 32 parts: 1 x 128000, top 20
-// 25.6 / 15.5 / 13 / 36, top 64 51 / 33 / 38 / 234, top 5 21 / 12.6 / 10.8 / 11.1;
+// 25.6 / 15.5 / 13 / 36, top 5 21 / 12.6 / 10.8 / 11.1; top 64 in 4 parts 23.5, in 32
+// over 200;
 // 64 x 128000, top 20, 27.6 / 16.7 / 16.6 / 25.6; 300 x 128000 37.4 / 32.8 / 32.3).
 constexpr int kLpShort = 12, kLpKeys = 160;
 static int lp_parts(int64_t rows, int vocab, int top, int64_t *span) {
