@@ -18,8 +18,11 @@
 //   O^T += V^T P^T the scores' layout is the operand as it stands; V^T comes
 //                  from row-major LDS (bf16, written by the lanes that
 //                  converted it) by transposing reads.  Probabilities enter as two
-//                  bf16 terms (2^-16 of the largest; three for fp32), both
-//                  products in fp32.
+//                  bf16 terms, each rounded (off by 2^-16 of the probability at
+//                  most; three for fp32: exact), both products in fp32.
+//                  Truncated terms (2^-14, all to one side) turned 3.4 in 1000 bf16 outputs to their other
+//                  neighbour, rounded ones 0.7, three terms 0.3 at 3% more time
+//                  (64 sequences of 128 to 8192).
 // A lane's accumulators belong to its own row, so rescaling and the final
 // division need no exchange.  The waves' sums meet in LDS; rows split over
 // partitions leave (sum, maximum, unscaled output) in the workspace and a
@@ -73,7 +76,7 @@ struct MxAttendArgs {
   bool q_vec;
 };
 
-// Terms whose sum is an element of T (query), and of a probability.
+// Terms whose sum is an element of T (query), and that hold a probability.
 template <typename T>
 struct MxTerms;
 template <>
@@ -89,7 +92,7 @@ __device__ __forceinline__ f32x4 mx_mma(u32x4 a, u32x4 b, f32x4 c) {
 
 // The bf16 terms of (x0, x1), each the truncated rest of those before: 8 bits
 // of the significand a term, and never past the largest bf16.
-template <int N, bool kFinite = false>
+template <int N>
 __device__ __forceinline__ void mx_split(float x0, float x1, unsigned int *terms) {
 #pragma unroll
   for (int n = 0; n < N; ++n) {
@@ -97,9 +100,22 @@ __device__ __forceinline__ void mx_split(float x0, float x1, unsigned int *terms
     terms[n] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);  // the upper halves
     if (n + 1 < N) {
       const float r0 = x0 - __uint_as_float(u0 & 0xffff0000u), r1 = x1 - __uint_as_float(u1 & 0xffff0000u);
-      x0 = kFinite || r0 == r0 ? r0 : 0.f;  // an infinity is its first term alone
-      x1 = kFinite || r1 == r1 ? r1 : 0.f;
+      x0 = r0 == r0 ? r0 : 0.f;  // an infinity is its first term alone
+      x1 = r1 == r1 ? r1 : 0.f;
     }
+  }
+}
+
+// The same of two probabilities (at most 2^kMxaSlack), each term the rounded
+// rest of those before: N terms are off by 2^-8N of the probability at most.
+template <int N>
+__device__ __forceinline__ void mx_split_rounded(float x0, float x1, unsigned int *terms) {
+  typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    terms[n] = __builtin_bit_cast(unsigned int, v2{static_cast<__bf16>(x0), static_cast<__bf16>(x1)});
+    x0 -= __uint_as_float(terms[n] << 16);
+    x1 -= __uint_as_float(terms[n] & 0xffff0000u);
   }
 }
 
@@ -380,7 +396,7 @@ __global__ __launch_bounds__(64 * kMxaMaxWaves, 2) void mx_attend_kernel(const M
         const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[s][i + 1], a.scale_log2, -m));
         l += e0 + e1;
         unsigned int terms[NP];
-        mx_split<NP, true>(e0, e1, terms);  // (at most 2^kSlack)
+        mx_split_rounded<NP>(e0, e1, terms);
 #pragma unroll
         for (int n = 0; n < NP; ++n) p[n][s * 2 + i / 2] = terms[n];
       }

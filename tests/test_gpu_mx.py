@@ -367,6 +367,28 @@ def test_attention_in_place(device, q_len, partition):
     assert torch.equal(q, want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("partition", [0, 32])
+def test_the_rounding_of_probabilities(device, dtype, partition):
+    """Two keys of one step whose values cancel but for the difference of their probabilities,
+    1 and exp(-gap): both terms of the second, below 1, are rounded, 2^-9 and then 2^-18 off at
+    most; half of that times the value 6 is left in the output, beside
+    fp32's errors (2^-22 for the exponential, the sum and the quotient) and the
+    output's own rounding."""
+    d, rows = 64, 32
+    kv = np.zeros((1, 64, 2, 1, d))
+    kv[0, 0, 0, 0, 0] = 1
+    kv[0, 1:, 0, 0, 2], kv[0, 20, 0, 0, 2] = 6, 0  # the others score -600
+    kv[0, 0, 1], kv[0, 20, 1] = 6, -6
+    q = torch.zeros((1, 1, rows, d), dtype=dtype, device=device)
+    q[0, 0, :, 0] = torch.from_numpy(np.random.default_rng(1).uniform(2.0 ** -14, 2.0 ** -13, rows)).to(dtype).to(device)
+    q[0, 0, :, 2] = -100
+    cache = make_cache(torch.from_numpy(kv).to(dtype).to(device), 64, device)
+    got = fp4.decode_attention(q, cache, 1, max_seqlen=64, seqlen_bias=64, softmax_scale=1.0, partition=partition)
+    want = oracle.attend(wide(q), oracle.rounded(kv), [64], scale=1.0)
+    assert (np.abs(wide(got) - want) <= torch.finfo(dtype).eps / 2 * np.abs(want) + 6 * (2.0 ** -19 + 2.0 ** -22)).all()
+
+
 def test_a_long_row_at_far_offsets(device):
     """A sequence whose rows lie beyond 4 GiB of the cache's start."""
     heads, d, n = 8, 128, 300
