@@ -20,9 +20,9 @@
 //                  converted it) by transposing reads.  Probabilities enter as two
 //                  bf16 terms, each rounded (off by 2^-16 of the probability at
 //                  most; three for fp32: exact), both products in fp32.
-//                  Truncated terms (2^-14, all to one side) turned 3.4 in 1000 bf16 outputs to their other
-//                  neighbour, rounded ones 0.7, three terms 0.3 at 3% more time
-//                  (64 sequences of 128 to 8192).
+//                  Truncated terms (2^-14, all to one side) turned 3.4 in
+//                  1000 bf16 outputs to a neighbour, rounded ones 0.5, three
+//                  terms 0.3 at 3% more time (64 sequences of 128 to 8192).
 // A lane's accumulators belong to its own row, so rescaling and the final
 // division need no exchange.  The waves' sums meet in LDS; rows split over
 // partitions leave (sum, maximum, unscaled output) in the workspace and a
@@ -605,20 +605,23 @@ static int64_t mx_units(const hexkv_mx_attend_params *p) {
 }
 
 // Positions per partition.  One partition where the join would cost more than
-// it saves: to 1024 keys, and to 2048 where there is a unit for each of the 256
-// CUs.  Beyond, two workgroups a CU, of 256 to 1024 keys each (the upper end
-// for ragged lengths).  us, one partition / 256 / 512 / 1024 keys each, bf16,
-// head_dim 128, 32 query heads:
+// it saves: to 1024 keys; where there is a unit for each of the 256 CUs to 2048;
+// and for more than kFewTiles row tiles there whatever the length (their rows'
+// lengths differ little).  Beyond, two workgroups a CU, of 256 to 1024 keys
+// each (the upper end for ragged lengths).  us, one partition / 256 / 512 /
+// 1024 keys each, bf16, head_dim 128, 32 query heads:
 //   8 KV heads, B 1 of 1024     11.3 /  9.8 / 10.7 /  -     of 2048  14.4 / 11.2 / 11.1 / 14
 //               B 1 of 8192     38.2 / 11.8 / 12.4 / 18.9
 //               B 32 of 1024    13.0 / 21.2 / 17   /  -     of 2048  24.2 / 39   / 30   / 27.8
 //               B 64 of 128..8192  86 / 99 / 83.2 / 80.7
 //   32 KV heads, B 8 of 256..2048 (fp16)  17.8 / 38 / 23 / 19.9
-constexpr int64_t kCus = 256;
+//   400 rows, B 2 of 4096, 8 heads on 1 (fp16)  45 / - / - / 51;  1600 rows, 32 on 8  385 / - / - / 571;
+//   60 rows, B 16 of 1..8192, 8 on 1  71 / - / - / 62
+constexpr int64_t kCus = 256, kFewTiles = 24;
 static int mx_partition(const hexkv_mx_attend_params *p) {
   const int64_t units = std::max<int64_t>(1, mx_units(p)), n = std::max<int64_t>(1, p->max_seqlen);
   int64_t part = p->partition;
-  if (!part && n <= (units >= kCus ? 2560 : 1024)) part = n;
+  if (!part && (n <= (units >= kCus ? 2560 : 1024) || (units >= kCus && row_tiles(p) > kFewTiles))) part = n;
   if (!part) {
     const int64_t parts = std::max<int64_t>(1, 2 * kCus / units);
     part = std::min<int64_t>(1024, std::max<int64_t>(256, n / parts / 128 * 128));
@@ -639,18 +642,20 @@ static size_t mx_join_bytes(const hexkv_mx_attend_params *p) {
   return static_cast<size_t>(p->batch) * p->q_len * p->q_heads * parts * (p->head_dim + 2) * sizeof(float);
 }
 
-// Many query rows (a prompt's chunk): the rows' keys and values are taken out
-// of the cache once and attended by hexkv_attend's query tiles, where those
-// are compiled.  To kFewTiles row tiles the keys are read in four bits (four
-// bits / taken out, us, 4 query heads a KV head: 2 x 2048 keys, 5 tiles 16 / 28,
-// 24 tiles 29 / 45; 16 x 2048 keys, 5 tiles 42 / 82, 24 tiles 120 / 129; one query
-// head a KV head, 32 of them, fp16, 4096 keys, 24 tiles 96 / 79).
-constexpr int64_t kFewTiles = 24;
+// Many bf16 query rows (a prompt's chunk): the rows' keys and values are taken
+// out of the cache once, exactly, and attended by hexkv_attend's query tiles,
+// where those are compiled.  To kFewTiles row tiles the keys are read in four
+// bits (four bits / taken out, us, 4 query heads a KV head: 2 x 2048 keys, 5 tiles
+// 16 / 28, 24 tiles 29 / 45; 16 x 2048 keys, 5 tiles 42 / 82, 24 tiles 120 / 129).
+// fp16 queries always read them in four bits: fp16 holds neither a power
+// above 2^13 (an fp16 value from 57344 up is stored as 2^16) nor all below
+// 2^-23, so rows taken out as fp16 would not be the stored ones.  What that
+// costs (four bits / taken out, 2 x 4096 keys, 32 heads on 8 of 128): 400 rows
+// 133 / 134, 800 228 / 170, 1600 385 / 263; on 4 of 64: 84 / 101, 142 / 113, 240 / 160.
 static bool mx_unpacks(const hexkv_mx_attend_params *p) {
-  const int vec = 16 / elem_bytes(p->dtype);
-  return p->dtype != HEXKV_F32 && (p->head_dim == 64 || p->head_dim == 128) && p->q_len > 1 && p->partition == 0 &&
+  return p->dtype == HEXKV_BF16 && (p->head_dim == 64 || p->head_dim == 128) && p->q_len > 1 && p->partition == 0 &&
          row_tiles(p) > kFewTiles && static_cast<int64_t>(p->batch) * p->q_len <= 65535 && p->max_seqlen > 0 &&
-         aligned16(p->q) && p->q_batch_stride % vec == 0 && p->q_row_stride % vec == 0 &&
+         aligned16(p->q) && p->q_batch_stride % 8 == 0 && p->q_row_stride % 8 == 0 &&
          static_cast<int64_t>(p->max_seqlen) * 2 * p->kv_heads * p->head_dim * 2 < INT64_C(0xffff0000);
 }
 
@@ -683,7 +688,7 @@ static hexkv_attend_params mx_unpacked(const hexkv_mx_attend_params *p, void *kv
 }
 
 static size_t mx_unpacked_bytes(const hexkv_mx_attend_params *p) {
-  const size_t n = static_cast<size_t>(p->batch) * p->max_seqlen * 2 * p->kv_heads * p->head_dim * elem_bytes(p->dtype);
+  const size_t n = static_cast<size_t>(p->batch) * p->max_seqlen * 2 * p->kv_heads * p->head_dim * 2;
   return (n + 255) / 256 * 256;
 }
 

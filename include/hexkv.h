@@ -703,8 +703,8 @@ int hexkv_mx_dequantize(const void *codes, const void *powers, void *out, int64_
 /* hexkv_attend over a 4-bit cache: the same rows, lengths, causal rule and
  * fused append (kv_new is stored as hexkv_mx_store does and attended as
  * stored).  q and out as there, at any element strides with heads contiguous.
- * A call of many query rows first takes the cache's [0, max_seqlen) positions
- * out into the workspace. */
+ * A bf16 call of many query rows first takes the cache's [0, max_seqlen)
+ * positions out into the workspace, which changes no stored value. */
 typedef struct hexkv_mx_attend_params {
   int dtype;      /* enum hexkv_dtype of q, kv_new and out */
   int batch;

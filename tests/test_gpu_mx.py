@@ -389,6 +389,82 @@ def test_the_rounding_of_probabilities(device, dtype, partition):
     assert (np.abs(wide(got) - want) <= torch.finfo(dtype).eps / 2 * np.abs(want) + 6 * (2.0 ** -19 + 2.0 ** -22)).all()
 
 
+def takes_out(q, cache, kv_heads, longest, causal):
+    """Whether this call attends a copy of the cache in 16 bits: its workspace is
+    another than the same call's at an odd address, which reads four bits."""
+    b, t, hq, d = q.shape
+    odd = torch.empty((b, t, hq * d + 1), dtype=q.dtype, device=q.device)[..., 1:].unflatten(-1, (hq, d))
+    return (fp4.attend_workspace_bytes(q, cache, kv_heads, longest, causal=causal)
+            != fp4.attend_workspace_bytes(odd, cache, kv_heads, longest, causal=causal))
+
+
+CHUNKS = [
+    # q_heads, kv_heads, head_dim, lens, q_len: 25 and more tiles of 16 rows per KV head
+    (4, 1, 128, [130, 0, 257], 100), (8, 2, 64, [300, 97], 128), (2, 1, 64, [90], 200), (4, 1, 128, [2900], 110),
+    (8, 1, 64, [701, 40], 70),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("case,causal", itertools.product(range(len(CHUNKS)), (False, True)))
+def test_attention_of_a_chunk(device, dtype, case, causal):
+    hq, h, d, lens, t = CHUNKS[case]
+    b = len(lens)
+    kv = randn((b, max(lens), 2, h, d), case, dtype, device)
+    q = randn((b, t, hq, d), 100 + case, dtype, device, 2.0)
+    cache = make_cache(kv, max(lens) + 5, device)
+    for i, n in enumerate(lens):
+        cache[i, n:] = 0xFF  # NaN behind every sequence's own length
+    seqlens = torch.tensor(lens, dtype=torch.int32, device=device)
+    stored = oracle.rounded(wide(kv))
+    want = oracle.attend(wide(q), stored, lens, causal)
+    tol = attend_tolerance(wide(q), stored, want, dtype)
+    rows = torch.zeros((b, t, hq * d + 3), dtype=dtype, device=device)
+    odd_out = rows[..., 3:].unflatten(-1, (hq, d))
+    odd_q = torch.zeros((b, t, hq * d + 1), dtype=dtype, device=device)[..., 1:].unflatten(-1, (hq, d)).copy_(q)
+    for query, out in ((q, None), (q, odd_out), (odd_q, None), (odd_q, odd_out)):
+        assert takes_out(query, cache, h, max(lens), causal) == (dtype == torch.bfloat16 and query is q)
+        got = fp4.decode_attention(query, cache, h, max_seqlen=max(lens), seqlens=seqlens, causal=causal, out=out)
+        assert (np.abs(wide(got) - want) <= tol).all()
+        for i, n in enumerate(lens):
+            assert not got[i, :max(0, t - n) if causal else (t if n == 0 else 0)].any()
+    assert not rows[..., :3].any()
+
+
+def test_nan_reaches_the_rows_of_a_chunk_that_attend_it(device):
+    cache = fp4.kv_cache(2, 80, 2, 64, device)
+    assert takes_out(torch.empty((2, 200, 4, 64), dtype=torch.bfloat16, device=device), cache, 2, 70, True)
+    test_nan_reaches_the_rows_that_attend_it(device, 200)
+
+
+@pytest.mark.parametrize("source", [torch.float16, torch.float32])
+@pytest.mark.parametrize("q_len", [40, 130])
+def test_chunks_over_values_that_fp16_does_not_hold(device, source, q_len):
+    """fp16 queries on either side of the tiles that bf16 ones are taken out at:
+    fp16 values from 57344 up, stored as 65536; keys of powers far from fp16's."""
+    kv = randn((2, 150, 2, 2, 64), 3, torch.float32, device)
+    kv[:, :, 1, :, :32] *= 2.0 ** 13
+    kv[0, ::7, 1, 0, 5], kv[0, 1::7, 1, 0, 5] = 60000, -60000  # their means stay within fp16
+    kv[:, :, 1].clamp_(-60000, 60000)
+    kv[:, :, 0, 1] *= 2.0 ** (14 if source == torch.float16 else 20)
+    if source == torch.float16:
+        kv[:, :, 0].clamp_(-65000, 65000)
+    kv = kv.to(source)
+    q = randn((2, q_len, 8, 64), 4, torch.float16, device, 2.0)
+    q[:, :, 4:] *= 2.0 ** (-14 if source == torch.float16 else -20)
+    lens = [150, 61]
+    got = fp4.decode_attention(q, make_cache(kv, 160, device), 2, max_seqlen=150, causal=True,
+                               seqlens=torch.tensor(lens, dtype=torch.int32, device=device))
+    stored = oracle.rounded(wide(kv))
+    assert (np.abs(stored[..., 1, :, :]) == 65536).any()
+    want = oracle.attend(wide(q), stored, lens, True)
+    for h in range(2):
+        own = slice(4 * h, 4 * h + 4)
+        tol = attend_tolerance(wide(q)[:, :, own], stored[:, :, :, h:h + 1], want[:, :, own], torch.float16)
+        # (two sums of values that nearly cancel, in halves of fp16's smallest step too)
+        assert (np.abs(wide(got)[:, :, own] - want[:, :, own]) <= tol + 2.0 ** -25).all()
+
+
 def test_a_long_row_at_far_offsets(device):
     """A sequence whose rows lie beyond 4 GiB of the cache's start."""
     heads, d, n = 8, 128, 300
