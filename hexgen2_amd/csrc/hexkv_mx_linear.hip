@@ -15,8 +15,10 @@
 // bf16 activations meet the matrix as bf16, exact for every power.  fp16 ones
 // meet it as fp16, exact for powers from 2^-23 to 2^13; blocks with another
 // power are left out there and added afterwards in bf16, with each activation as two
-// terms (fp32 in mx_rows_kernel).  fp32 activations are three bf16 terms.  All
-// sums are fp32.
+// terms (fp32 in mx_rows_kernel).  Left out they are zeros, whose product with an
+// infinite activation is a NaN: where the sum without them is not finite, all
+// blocks are added up that way instead.  fp32 activations are three bf16 terms.  All sums
+// are fp32.
 #include "hexkv_mx.h"
 
 #include <algorithm>
@@ -81,14 +83,14 @@ __device__ __forceinline__ float near_scale(unsigned int byte, bool *far) {
   return out ? 0.f : mx_scale(byte);
 }
 
-// Such a block alone, as bf16; any other is zero.
+// Such a block alone (with `all` any block), as bf16; the others are zero.
 struct FarBlock {
   u32x4 w;
   float scale;
   bool any;
-  __device__ __forceinline__ void read(const MxLinearArgs &a, int64_t row, int block, bool live) {
+  __device__ __forceinline__ void read(const MxLinearArgs &a, int64_t row, int block, bool live, bool all) {
     const unsigned int byte = live ? a.powers[row * (a.k / kMxBlock) + block] : 127u;
-    any = byte - kMxF16Low > kMxF16High - kMxF16Low;
+    any = (all && live) || byte - kMxF16Low > kMxF16High - kMxF16Low;
     w = u32x4{};
     if (any) w = *reinterpret_cast<const u32x4 *>(a.codes + row * (a.k / 2) + block * 16);
     scale = any ? mx_scale(byte) : 1.f;
@@ -212,12 +214,24 @@ __global__ __launch_bounds__(kMxlThreads) void mx_rows_kernel(const MxLinearArgs
         sum[t][r] = c >> 2 == lane >> 4 ? d : 0.f;
       }
     if (Elem<T>::kDtype == HEXKV_F16 && __ballot(far)) {
+      float check = 0.f;
+#pragma unroll
+      for (int t = 0; t < TOKENS; ++t)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) check = fmaf(sum[t][r], 0.f, check);
+      const bool all = __ballot(!(check == 0.f)) != 0;
+      if (all) {
+#pragma unroll
+        for (int t = 0; t < TOKENS; ++t)
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) sum[t][r] = 0.f;
+      }
 #pragma unroll 1
       for (int b = lane; b < blocks; b += 64)
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
           FarBlock block;
-          block.read(a, min(n0 + r, a.n - 1), b, true);
+          block.read(a, min(n0 + r, a.n - 1), b, true, all);
           if (!block.any) continue;
 #pragma unroll 1
           for (int j = 0; j < 4; ++j) {
@@ -448,10 +462,20 @@ __global__ __launch_bounds__(512) void mx_few_kernel(const MxLinearArgs a) {
       }
       if (Elem<T>::kDtype == HEXKV_F16 && __ballot(far)) {
         const int64_t row = min(tile * 16 + c, a.n - 1);
+        float check = 0.f;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) check = fmaf(acc[m][i], 0.f, check);
+        const bool all = __ballot(!(check == 0.f)) != 0;
+        if (all) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[m] = f32x4{};
+        }
 #pragma unroll 1
         for (int s = 0; s < BL; ++s) {
           FarBlock block;
-          block.read(a, row, from + s, !foreign(s));
+          block.read(a, row, from + s, !foreign(s), all);
           if (!__ballot(block.any)) continue;
 #pragma unroll 1
           for (int j = 0; j < 4; ++j) {
@@ -529,11 +553,26 @@ __device__ __forceinline__ f32x16 mma32_f16(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// The blocks whose power fp16 does not hold, in bf16.
+// The blocks whose power fp16 does not hold, in bf16; all blocks, from zero,
+// where the sum is not finite.
 template <typename T, typename S>
 __device__ __forceinline__ void tile_far(const MxLinearArgs &a, int m0, int n0, int k_first, int k_last, int wm, int wn,
                                          int c, int h, f32x16 (&acc)[S::MT][S::NT]) {
   constexpr int MT = S::MT, NT = S::NT;
+  float check = 0.f;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) check = fmaf(acc[m][t][i], 0.f, check);
+  const bool all = __ballot(!(check == 0.f)) != 0;
+  if (all) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[m][t] = f32x16{};
+  }
 #pragma unroll 1
   for (int k0 = k_first; k0 < k_last; k0 += S::kStep)
 #pragma unroll 1
@@ -542,7 +581,7 @@ __device__ __forceinline__ void tile_far(const MxLinearArgs &a, int m0, int n0, 
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         FarBlock block;
-        block.read(a, min(n0 + (wn * NT + t) * 32 + c, a.n - 1), k / kMxBlock, k < k_last);
+        block.read(a, min(n0 + (wn * NT + t) * 32 + c, a.n - 1), k / kMxBlock, k < k_last, all);
         if (!__ballot(block.any)) continue;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {

@@ -579,6 +579,30 @@ def test_linear_of_a_token_that_is_not_finite(device):
     assert bad[3] and bad[4] and bad.sum() == 2
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,n", [(1, 300), (2, 300), (3, 300), (20, 300), (40, 300), (100, 300), (400, 300), (4000, 4090)])
+def test_an_infinite_activation_against_far_powers(device, dtype, rows, n):
+    """Its product with a block that fp16 does not hold is an infinity, and no
+    other block's zeros turn that, or an infinity beside them, into NaN."""
+    k = 416
+    x = randn((rows, k), 1, dtype, device)
+    x[rows // 2, 70], x[rows - 1, 130] = float("inf"), -float("inf")
+    w = fp4.quantize(randn((n, k), 2, torch.float32, device))
+    w.codes.bitwise_or_(0x22)  # no element is zero
+    w.powers[7, 2], w.powers[8, 4], w.powers[299, 2], w.powers[33, 12] = 95, 150, 100, 90
+    values = wide(fp4.dequantize(w, torch.float32))
+    finite = np.where(np.isfinite(wide(x)), wide(x), 0)
+    want = finite @ values.T
+    with np.errstate(invalid="ignore"):
+        want += np.where(wide(x)[:, 70:71] == np.inf, np.inf * values[:, 70], 0)
+        want += np.where(wide(x)[:, 130:131] == -np.inf, -np.inf * values[:, 130], 0)
+    got, fine = wide(fp4.linear(x, w)), np.isfinite(want)
+    assert np.array_equal(got[~fine], want[~fine], equal_nan=True)
+    fine &= np.abs(want) < 60000  # (within fp16, rounded)
+    tol = linear_tolerance(finite, values, np.where(fine, want, 0), dtype)
+    assert (np.abs(got[fine] - want[fine]) <= tol[fine]).all()
+
+
 # ----------------------------------------------------------- log-probabilities ---
 
 
