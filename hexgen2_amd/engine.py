@@ -154,11 +154,13 @@ class Engine:
     @torch.inference_mode()
     def score(self, input_ids, top_logprobs=0) -> TokenLogprobs:
         """What the model says of a sequence's tokens: entry t of each result
-        belongs to ``input_ids[t + 1]`` after the t + 1 tokens before it."""
+        belongs to ``input_ids[t + 1]`` after the t + 1 tokens before it.  With
+        ``kv_bits`` 4 every token attends its rows as the cache holds them, as
+        a decode step does (``prefill`` attends them unrounded)."""
         if not len(input_ids):
             raise ValueError("score needs a token")
         ids = torch.tensor([input_ids], dtype=torch.long, device=self.device)
-        state = CacheState(len(input_ids), kv_bits=self.kv_bits)
+        state = CacheState(len(input_ids), kv_bits=self.kv_bits, attend_stored=True)
         logits = self.model.forward(ids, inference_params=state, last_token_only=False)
         return token_logprobs(logits[0, :-1], ids[0, 1:], top_logprobs)
 

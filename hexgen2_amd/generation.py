@@ -25,7 +25,8 @@ class InferenceParams:
     own position (its cached length) in a ragged decode batch, on the FT path
     and on the standard layout alike; ``sequence_len_offset`` then bounds
     every sample's position.  ``kv_bits`` (an addition) 4 keeps the caches in
-    four bits, ``[max_batch_size, max_sequence_len, row_bytes]`` (``fp4``).
+    four bits, ``[max_batch_size, max_sequence_len, row_bytes]`` (``fp4``); with
+    ``attend_stored`` a prompt, too, attends its rows as they are stored there.
     """
     max_sequence_len: int
     max_batch_size: int = 1
@@ -35,6 +36,7 @@ class InferenceParams:
     fused_ft_kernel: bool = False
     lengths_per_sample: Optional[torch.Tensor] = None
     kv_bits: int = 16
+    attend_stored: bool = False
 
 
 # hexgen2/model.py:11-19 names the same record CacheState.

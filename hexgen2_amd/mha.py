@@ -109,7 +109,8 @@ def _update_kv_cache(kv: torch.Tensor, inference_params, layer_idx: int) -> torc
     With ``kv_bits`` 4 the rows are rounded to four bits as they are written, and
     the view is the 4-bit cache's, which ``FlashCrossAttention`` attends as
     it attends the other; the prompt (``sequence_len_offset`` 0) gets ``kv``
-    back, as on the FT path: it attends its own keys as they were computed."""
+    back, as on the FT path: it attends its own keys as they were computed
+    (with ``attend_stored``: the view, as they were stored)."""
     kv_bits = _kv_bits(inference_params)
     if inference_params.fused_ft_kernel and kv_bits == 16:
         return _update_ft_cache(kv, inference_params, layer_idx)
@@ -129,7 +130,7 @@ def _update_kv_cache(kv: torch.Tensor, inference_params, layer_idx: int) -> torc
     positions = _sample_positions(inference_params, batch_start, batch_end) if kv.shape[1] == 1 else None
     if kv_bits == 4:
         fp4.store_kv(_batch_rows(cache, batch_start, batch_end), kv, positions, 0 if positions is not None else sequence_start)
-        if sequence_start == 0:
+        if sequence_start == 0 and not getattr(inference_params, "attend_stored", False):
             return kv
     elif positions is not None:
         ops.append_kv(_batch_rows(cache, batch_start, batch_end), kv, positions)

@@ -201,6 +201,27 @@ def test_score_matches_the_steps(device):
         engine.score([])
 
 
+@pytest.mark.parametrize("weight_bits", [16, 4])
+def test_scores_over_a_four_bit_cache_are_the_steps(device, weight_bits):
+    """Scoring with ``kv_bits`` 4 gives what steps over the 4-bit cache say of
+    the same tokens, and not what the 16-bit cache does."""
+    ids = [(37 * i * i + 11 * i + 5) % 128 for i in range(40)]
+    engine = Engine(MODEL, "native", "cuda", "float32", kv_bits=4, weight_bits=weight_bits)
+    got = engine.score(ids, top_logprobs=2)
+    plain = Engine(MODEL, "native", "cuda", "float32", weight_bits=weight_bits).score(ids, top_logprobs=2)
+    state, steps, largest = InferenceParams(40, kv_bits=4, attend_stored=True), [], 0.0
+    for t in range(39):
+        state.sequence_len_offset = t
+        logits = engine.model.forward(torch.tensor([[ids[t]]], device=device), state, fused_append=t % 3 == 2)
+        steps.append(token_logprobs(logits, torch.tensor([ids[t + 1]], device=device), 2))
+        largest = max(largest, float(logits.abs().max()))
+    scale = LOGITS * 2 * largest  # of two logits
+    for at, step in enumerate(steps):
+        for a, b in zip(got, step):
+            assert a.dtype == torch.int64 or float((a[at] - b[0]).abs().max()) <= scale * 8  # entropy: times -log p < 8
+    assert float((got.logprob - plain.logprob).abs().max()) > scale, "the rounding must show"
+
+
 def test_engine_refuses_heads_without_whole_blocks(device):
     with pytest.raises(ValueError, match="head_dim"):
         Engine(GOLDEN / "tiny_llama", "native", "cuda", "float16", kv_bits=4)  # head_dim 16
