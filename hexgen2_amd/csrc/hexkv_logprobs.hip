@@ -18,9 +18,12 @@
 // the caches) and what reaches the bar is ranked by counting.  Collecting during the walk
 // instead, above the worst of the best so far, doubled a row's time (186 us
 // against 97 without alternatives, 8191 x 32000 bf16): barriers and counting in
-// every step.  Where too many reach the bar (equal logits), those above it are
-// ranked and the lowest ids equal to it follow; where too many are above it, the
-// largest is taken out `top` times over.
+// every step.  A mask that leaves a few hundred neighbours makes all of them reach the bar
+// (one lane in eight has any): up to 1024 are ranked (1 x 32000, 300 left, top 20: 21 us).
+// Where more reach the bar (equal logits), those above it are ranked and the lowest ids
+// equal to it follow; where more are above it (sorted logits), the top-th key is
+// found by counting, eight bits at a time (1 x 32000 41 us; taking out the largest
+// `top` times over took 474, and 370 for the mask).
 //
 // Measured on MI355X, bf16: 8191 x 32000 without alternatives 97 us (5.4 TB/s),
 // with the top 20 125 us (4.2); one row of 32000 fp16, top 5, 10.0 us.
@@ -34,7 +37,7 @@ constexpr int kLpThreads = 256;
 constexpr int kLpWaves = kLpThreads / 64;
 constexpr int kLpEach = 16;  // logits a lane holds at a time
 constexpr int kLpChunk = kLpThreads * kLpEach;
-constexpr int kLpRoom = 256;  // keys that can be ranked
+constexpr int kLpRoom = 1024;  // keys that can be ranked
 constexpr int kLpMaxParts = 32;
 
 struct LogprobArgs {
@@ -63,11 +66,6 @@ __device__ __forceinline__ float lp_key_value(lp_key k) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 __device__ __forceinline__ int64_t lp_key_id(lp_key k) { return 0xffffffffu - static_cast<unsigned int>(k); }
-
-__device__ __forceinline__ lp_key lp_shfl_xor(lp_key k, int off) {
-  const unsigned int lo = __shfl_xor(static_cast<unsigned int>(k), off), hi = __shfl_xor(static_cast<unsigned int>(k >> 32), off);
-  return static_cast<lp_key>(hi) << 32 | lo;
-}
 
 __device__ __forceinline__ float lp_exp(float u) { return __builtin_amdgcn_exp2f(u * 1.4426950408889634f); }
 
@@ -112,14 +110,21 @@ __device__ __forceinline__ void lp_write_top(const LogprobArgs &a, int64_t row, 
 // as keys at ranks from `held` to `top`; returns how many ranks are held then.
 template <typename T>
 __device__ __forceinline__ int lp_equal(const T *x, int64_t first, int64_t last, float value, int held, int top, lp_key *list) {
+  constexpr int U = 8;  // loads in flight
   const int lane = threadIdx.x & 63;
-  for (int64_t base = first; base < last && held < top; base += 64) {
-    const int64_t id = base + lane;
-    const bool out = id < last && static_cast<float>(x[min(id, last - 1)]) == value;
-    const uint64_t mask = __ballot(out);
-    const int rank = held + __popcll(mask & ((uint64_t{1} << lane) - 1));
-    if (out && rank < top) list[rank] = lp_make_key(value, static_cast<unsigned int>(id));
-    held = min(top, held + __popcll(mask));
+  for (int64_t base = first; base < last && held < top; base += 64 * U) {
+    float v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = static_cast<float>(x[min(base + u * 64 + lane, last - 1)]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t id = base + u * 64 + lane;
+      const bool out = id < last && v[u] == value;
+      const uint64_t mask = __ballot(out);
+      const int rank = held + __popcll(mask & ((uint64_t{1} << lane) - 1));
+      if (out && rank < top) list[rank] = lp_make_key(value, static_cast<unsigned int>(id));
+      held = min(top, held + __popcll(mask));
+    }
   }
   return held;
 }
@@ -127,9 +132,9 @@ __device__ __forceinline__ int lp_equal(const T *x, int64_t first, int64_t last,
 template <typename T>
 __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a) {
   constexpr int VEC = 16 / sizeof(T), NV = kLpEach / VEC;
-  __shared__ lp_key s_list[kLpRoom], s_best[64], s_wave[kLpWaves];
+  __shared__ lp_key s_list[kLpRoom], s_best[64];
   __shared__ float s_lane[kLpThreads], s_bar;
-  __shared__ int s_active[kLpThreads], s_active_count, s_count[2], s_held;
+  __shared__ int s_active[kLpThreads], s_active_count, s_count[2], s_held, s_hist[256], s_pick[3];
   __shared__ float s_stats[kLpWaves][3];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / static_cast<unsigned>(a.parts);
@@ -264,18 +269,12 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
     __syncthreads();
     const int vectors = static_cast<int>((last - first + kLpChunk - 1) / kLpChunk) * NV, total = s_active_count * vectors;
     // the active lanes' vectors, shared out over all lanes (in any order: the ranks do not depend on it)
-    const auto take = [&](bool equal, int *counter, float v, int64_t id) {
-      if ((equal ? !(v < bar) : !(v <= bar)) && v != -INFINITY) {
-        const int place = atomicAdd(counter, 1);
-        if (place < kLpRoom) s_list[place] = lp_make_key(v, static_cast<unsigned int>(id));
-      }
-    };
-    const auto collect = [&](bool equal, int *counter) {
+    const auto visit = [&](auto &&f) {
       if (single) {
         const int each = (a.vocab + kLpThreads - 1) / kLpThreads;
         for (int item = tid; item < s_active_count * each; item += kLpThreads) {
           const int of = item / each, i = item - of * each;
-          take(equal, counter, strided(i, s_active[of]), static_cast<int64_t>(i) * kLpThreads + s_active[of]);
+          f(strided(i, s_active[of]), static_cast<int64_t>(i) * kLpThreads + s_active[of]);
         }
         return;
       }
@@ -285,8 +284,16 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
         float v[VEC];
         vector_at(at, v);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) take(equal, counter, v[e], at + e);
+        for (int e = 0; e < VEC; ++e) f(v[e], at + e);
       }
+    };
+    const auto collect = [&](bool equal, int *counter) {
+      visit([&](float v, int64_t id) {
+        if ((equal ? !(v < bar) : !(v <= bar)) && v != -INFINITY) {
+          const int place = atomicAdd(counter, 1);
+          if (place < kLpRoom) s_list[place] = lp_make_key(v, static_cast<unsigned int>(id));
+        }
+      });
     };
     // Ranks by counting the larger keys: one wave by lane reads where a key
     // fits a lane each, as it nearly always does, else every lane over all in LDS.
@@ -335,24 +342,59 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(const LogprobArgs a
         __syncthreads();
         held = s_held;
       } else {
-        lp_key below = ~static_cast<lp_key>(0);
-        for (; held < top; ++held) {
-          lp_key k = 0;
-#pragma unroll 1
-          for (int64_t id = max(first - skew, INT64_C(0)) + tid; id + skew < last; id += kLpThreads) {
-            const float v = static_cast<float>(x[id]);
-            const lp_key other = v == -INFINITY ? 0 : lp_make_key(v, static_cast<unsigned int>(id));
-            if (other < below) k = max(k, other);
+        // The top-th largest key, eight bits at a time from the top: the keys
+        // at or above the bar that agree with it so far are counted by their next
+        // eight, until all of a count are among the top.
+        lp_key found = 0;
+        int want = top;  // of the keys that agree with `found`
+        for (int shift = 56;; shift -= 8) {
+          s_hist[tid] = 0;
+          __syncthreads();
+          visit([&](float v, int64_t id) {
+            if (v < bar || v == -INFINITY) return;
+            const lp_key k = lp_make_key(v, static_cast<unsigned int>(id));
+            if ((k ^ found) >> shift >> 8) return;
+            const int bin = static_cast<int>(k >> shift) & 255, one = __builtin_amdgcn_readfirstlane(bin);
+            const uint64_t same = __ballot(bin == one);  // mostly all of them: one addition
+            if (bin != one) atomicAdd(&s_hist[bin], 1);
+            else if (lane == __builtin_ctzll(same)) atomicAdd(&s_hist[one], __popcll(same));
+          });
+          __syncthreads();
+          if (wave == 0) {  // four bins a lane, from the top down
+            int n[4], own = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) own += n[e] = s_hist[255 - 4 * lane - e];
+            int above = own;
+            for (int off = 1; off < 64; off <<= 1) {
+              const int other = __shfl_up(above, off);
+              if (lane >= off) above += other;
+            }
+            above -= own;
+            if (above < want && want <= above + own)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (above < want && want <= above + n[e]) {
+                  s_pick[0] = 255 - 4 * lane - e;
+                  s_pick[1] = want - above;
+                  s_pick[2] = n[e];
+                }
+                above += n[e];
+              }
           }
-          for (int off = 1; off < 64; off <<= 1) k = max(k, lp_shfl_xor(k, off));
-          if (lane == 0) s_wave[wave] = k;
+          if (tid == 0) s_count[0] = 0;
           __syncthreads();
-          k = max(max(s_wave[0], s_wave[1]), max(s_wave[2], s_wave[3]));
-          if (tid == 0) s_best[held] = k;
-          __syncthreads();
-          if (!k) break;
-          below = k;
+          found |= static_cast<lp_key>(s_pick[0]) << shift;
+          want = s_pick[1];
+          if (want == s_pick[2] || shift == 0) break;
         }
+        visit([&](float v, int64_t id) {
+          const lp_key k = lp_make_key(v, static_cast<unsigned int>(id));
+          if (v < bar || v == -INFINITY || k < found) return;
+          const int place = atomicAdd(&s_count[0], 1);
+          if (place < kLpRoom) s_list[place] = k;
+        });
+        __syncthreads();
+        rank_list(min(s_count[0], kLpRoom));  // (`top` of them)
       }
     }
   }
