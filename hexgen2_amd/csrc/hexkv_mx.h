@@ -5,8 +5,9 @@
 //
 // A block's power is the smallest that leaves no element above 6 (a smaller
 // one would clip the largest elements, by up to a quarter), and within
-// [-125, 126], so that every non-zero value is a normal bf16 number: over
-// normally distributed data the error is 0.116 of their deviation.  Since the
+// [-125, 126], so that every non-zero value is a normal bf16 number (or, from
+// 3.5 times 2^126 up, rounded to 2^128, past bf16's and fp32's range: an infinity to
+// every reader): over normally distributed data the error is 0.116 of their deviation.  Since the
 // power is exact, x / power is, and the only rounding is the element's own
 // (nearest, halfway to the even code).
 //
@@ -30,6 +31,13 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 // vectors are aligned.
 __host__ __device__ constexpr int64_t mx_row_bytes(int64_t heads, int64_t head_dim) {
   return (2 * heads * (head_dim / 2 + head_dim / kMxBlock) + 15) / 16 * 16;
+}
+
+// Whether one of 8 elements reads as an infinity or a NaN: byte 255, 4 and 6
+// times 2^126 (kMxLastPower), 2, 3, 4 and 6 times 2^127.
+constexpr unsigned int kMxLastPower = 253;
+__device__ __forceinline__ bool mx_past(unsigned int w, unsigned int byte) {
+  return byte == 255 || (byte == 254 && (w & 0x44444444u)) || (byte == 253 && (w & w << 1 & 0x44444444u));
 }
 
 // The float whose exponent field a conversion takes the power from.

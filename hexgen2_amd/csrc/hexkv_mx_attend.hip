@@ -36,8 +36,9 @@
 // or three steps ahead instead of one cost 3 to 10% (registers), steps of one
 // wave a partition 12% at 64 sequences and 20 to 60% at one to four.
 //
-// A NaN block of V is taken out of the product (0 times NaN would reach rows
-// that do not attend it) and put into the outputs of the rows that do.
+// A NaN block of V, or one with an element that fp32 does not hold (2^128 and
+// above), is taken out of the product (0 times either is a NaN, which would reach
+// rows that do not attend it); the rows that do get NaN there.
 #include "hexkv_mx.h"
 
 #include <algorithm>
@@ -317,19 +318,23 @@ __global__ __launch_bounds__(64 * kMxaMaxWaves, 2) void mx_attend_kernel(const M
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int n = 0; n < NB; ++n) bad |= x.vp[s][n] == 255;
+      for (int n = 0; n < NB; ++n) bad |= x.vp[s][n] >= kMxLastPower;
     if (__ballot(bad)) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         unsigned int bits = 0;
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-          if (x.vp[s][n] == 255) {
+        for (int n = 0; n < NB; ++n) {
+          bool past = false;
+#pragma unroll
+          for (int i = 0; i < NW / NB; ++i) past |= mx_past(x.v[s][n * (NW / NB) + i], x.vp[s][n]);
+          if (past) {
             bits |= 1u << (blk + n);
             x.vp[s][n] = 127;
 #pragma unroll
             for (int i = 0; i < NW / NB; ++i) x.v[s][n * (NW / NB) + i] = 0;
           }
+        }
         uint64_t from = __ballot(bits != 0);
         while (from) {
           const int r = __builtin_ctzll(from);

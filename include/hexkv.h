@@ -704,7 +704,9 @@ int hexkv_mx_dequantize(const void *codes, const void *powers, void *out, int64_
  * fused append (kv_new is stored as hexkv_mx_store does and attended as
  * stored).  q and out as there, at any element strides with heads contiguous.
  * A bf16 call of many query rows first takes the cache's [0, max_seqlen)
- * positions out into the workspace, which changes no stored value. */
+ * positions out into the workspace, which changes no stored value.  A NaN
+ * block, or an element that fp32 does not hold (2^128 and above, which reads as an
+ * infinity), reaches the rows that attend it and no others. */
 typedef struct hexkv_mx_attend_params {
   int dtype;      /* enum hexkv_dtype of q, kv_new and out */
   int batch;

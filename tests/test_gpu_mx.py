@@ -306,6 +306,28 @@ def test_nan_reaches_the_rows_that_attend_it(device, q_len):
     assert not nan[1].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("q_len", [3, 20, 200])
+@pytest.mark.parametrize("d", [32, 64, 256])
+def test_values_past_the_largest_float_reach_the_rows_that_attend_them(device, dtype, q_len, d):
+    """A value rounded to 2^128, and such codes of the two largest powers."""
+    kv = randn((1, 70, 2, 2, d), 7, dtype, device)
+    kv[0, 69, 1, 0, d - 3] = 3.3e38
+    q = torch.zeros((1, q_len, 4, d), dtype=dtype, device=device)  # every key counts alike
+    cache = make_cache(kv, 70, device)
+    power = 2 * d + 2 * (d // 32)  # the first of the values' powers, behind 2 d bytes of elements and the keys' powers
+    assert cache[0, 69, power + d // 32 - 1] == 253
+    for byte, code, finite in ((253, None, False), (254, 4, False), (254, 0xC, False), (254, 3, True), (253, 5, True), (253, 0xF, False)):
+        cache[0, 69, power + d // 32 - 1] = byte
+        if code is not None:
+            start = d + d // 2 - 16  # head 0's last block of values
+            cache[0, 69, start:start + 16] = 0
+            cache[0, 69, start + 14] = code << 4
+        got = wide(fp4.decode_attention(q, cache, 2, max_seqlen=70, seqlen_bias=70, causal=True))
+        assert np.isfinite(got[0, :-1]).all() and np.isfinite(got[0, -1, 2:]).all() and np.isfinite(got[0, -1, :2, :d - 32]).all()
+        assert np.isfinite(got[0, -1, :2, d - 3]).all() == finite, (byte, code)
+
+
 def test_an_infinite_query(device):
     kv = randn((1, 9, 2, 1, 64), 7, torch.float16, device)
     q = randn((1, 1, 2, 64), 8, torch.float16, device)
