@@ -49,7 +49,7 @@ constexpr int kMxaMaxWaves = 8;
 constexpr int kXcds = 8;
 constexpr int kMxaRows = 16;  // query rows of a wave
 constexpr int kMxaKeys = 32;  // keys of one step
-constexpr float kMxaLowest = -1e30f;  // finite "minus infinity" of the running maximum
+constexpr float kMxaLowest = -3.4028234e38f;  // the running maximum's start: the lowest float, finite in differences
 constexpr float kMxaSlack = 8.f;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));

@@ -328,6 +328,20 @@ def test_values_past_the_largest_float_reach_the_rows_that_attend_them(device, d
         assert np.isfinite(got[0, -1, :2, d - 3]).all() == finite, (byte, code)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("partition", [0, 32])
+@pytest.mark.parametrize("q_len", [1, 9])
+def test_scores_far_below_zero(device, dtype, partition, q_len):
+    """Equal scores of -2^114 and below: the mean of the values."""
+    kv = randn((1, 70, 2, 1, 64), 3, dtype, device)
+    kv[:, :, 0] = -2.0 ** 60
+    q = torch.full((1, q_len, 2, 64), 2.0 ** 50, dtype=dtype, device=device)
+    got = fp4.decode_attention(q, make_cache(kv, 70, device), 1, max_seqlen=70, seqlen_bias=70, partition=partition)
+    values = oracle.rounded(wide(kv))[0, :, 1, 0]
+    tol = torch.finfo(dtype).eps / 2 * np.abs(values.mean(0)) + 70 * 2.0 ** -24 * np.abs(values).max() + 2.0 ** -16 * np.abs(values).max()
+    assert (np.abs(wide(got) - values.mean(0)) <= tol).all()
+
+
 def test_an_infinite_query(device):
     kv = randn((1, 9, 2, 1, 64), 7, torch.float16, device)
     q = randn((1, 1, 2, 64), 8, torch.float16, device)
