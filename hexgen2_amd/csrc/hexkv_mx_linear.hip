@@ -50,6 +50,13 @@ __device__ __forceinline__ u32x4 raw8(const T *p, bool vec) {
   return r;
 }
 
+// x less its upper half; of an infinity nothing is left, of a NaN (whose payload
+// may lie in the lower half alone, which leaves an infinity's upper half) a NaN.
+__device__ __forceinline__ float first_rest(float x) {
+  const float rest = x - __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+  return __builtin_amdgcn_classf(x, 0x204) ? 0.f : rest;  // minus and plus infinity
+}
+
 // The first N bf16 terms of 8 floats (each the truncated rest of those before).
 template <int N>
 __device__ __forceinline__ void terms8(const float *f, u32x4 *t) {
@@ -60,9 +67,8 @@ __device__ __forceinline__ void terms8(const float *f, u32x4 *t) {
     for (int n = 0; n < N; ++n) {
       const unsigned int u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
       t[n][i] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
-      const float r0 = x0 - __uint_as_float(u0 & 0xffff0000u), r1 = x1 - __uint_as_float(u1 & 0xffff0000u);
-      x0 = r0 == r0 ? r0 : 0.f;  // an infinity is its first term alone
-      x1 = r1 == r1 ? r1 : 0.f;
+      x0 = n == 0 ? first_rest(x0) : x0 - __uint_as_float(u0 & 0xffff0000u);
+      x1 = n == 0 ? first_rest(x1) : x1 - __uint_as_float(u1 & 0xffff0000u);
     }
   }
 }

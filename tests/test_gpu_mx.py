@@ -639,6 +639,15 @@ def test_an_infinite_activation_against_far_powers(device, dtype, rows, n):
     assert (np.abs(got[fine] - want[fine]) <= tol[fine]).all()
 
 
+@pytest.mark.parametrize("rows", [1, 3, 20, 50, 100, 200])
+def test_linear_of_a_nan_with_a_small_payload(device, rows):
+    """Its upper half alone would read as an infinity."""
+    x = randn((rows, 64), 1, torch.float32, device)
+    x.view(torch.int32)[rows - 1, 5] = 0x7F800001
+    got = fp4.linear(x, fp4.quantize(randn((40, 64), 2, torch.float32, device)))
+    assert torch.isnan(got[rows - 1]).all() and torch.isfinite(got[:rows - 1]).all()
+
+
 # ----------------------------------------------------------- log-probabilities ---
 
 
