@@ -112,6 +112,8 @@ def _rows_form(shape, stride, dtype):
         raise ValueError("kv must be one of float16, bfloat16, float32")
     if stride[4] != 1 or (shape[3] > 1 and stride[3] != shape[4]):
         raise ValueError("kv heads must be contiguous [.., heads, head_dim]")
+    for n in shape:
+        _int32(n, "kv's size")
     return (*shape, *stride[:3], _DTYPES[dtype])
 
 
@@ -161,7 +163,7 @@ def _attend_form(q, cache, kv_heads, out, kv_new, causal, softmax_scale, partiti
     """The checked parameter block of a call, without addresses and lengths."""
     if q.dim() != 4 or q.dtype not in _DTYPES:
         raise ValueError("q must be [batch, q_len, q_heads, head_dim] in float16, bfloat16 or float32")
-    batch, q_len, q_heads, d = q.shape
+    batch, q_len, q_heads, d = (_int32(n, "q's size") for n in q.shape)
     if kv_heads < 1 or q_heads % kv_heads:
         raise ValueError("q_heads must be a multiple of kv_heads")
     batch_bytes, row = _check_cache(cache, kv_heads, d)
@@ -277,6 +279,11 @@ def _matrix_rows(t: torch.Tensor, name: str) -> int:
     return _row_stride(t.shape, t.stride(), name)
 
 
+def _matrix_size(shape) -> int:
+    """Elements of a matrix's row."""
+    return _int32(shape[-1], "a row of elements")
+
+
 def quantize(x: torch.Tensor) -> Fp4Tensor:
     """``x [..., k]`` (k a multiple of 32) in four bits: ``codes [..., k / 2]``
     and ``powers [..., k / 32]``."""
@@ -284,7 +291,7 @@ def quantize(x: torch.Tensor) -> Fp4Tensor:
     if x.dtype not in _DTYPES or x.dim() < 1 or x.shape[-1] % BLOCK:
         raise ValueError(f"x must be float16, bfloat16 or float32 with rows of whole blocks of {BLOCK}, "
                          f"got {x.dtype} {tuple(x.shape)}")
-    k = x.shape[-1]
+    k = _matrix_size(x.shape)
     stride = _matrix_rows(x, "x")
     codes = torch.empty((*x.shape[:-1], k // 2), dtype=torch.uint8, device=x.device)
     powers = torch.empty((*x.shape[:-1], k // BLOCK), dtype=torch.uint8, device=x.device)
@@ -314,7 +321,7 @@ def dequantize(weight: Fp4Tensor, dtype: torch.dtype) -> torch.Tensor:
     _require_device(codes)
     if dtype not in _DTYPES:
         raise ValueError("dequantize gives float16, bfloat16 or float32")
-    k = powers.shape[-1] * BLOCK
+    k = _matrix_size((*powers.shape[:-1], powers.shape[-1] * BLOCK))
     out = torch.empty((*codes.shape[:-1], k), dtype=dtype, device=codes.device)
     _call("hexkv_mx_dequantize", codes, codes.data_ptr(), powers.data_ptr(), out.data_ptr(), k,
           out.numel() // max(k, 1), k, _DTYPES[dtype])
@@ -330,7 +337,7 @@ def _linear_form(shape, stride, dtype, codes_shape, powers_shape):
     n, k = codes_shape[0], shape[-1]
     if not k:
         raise ValueError("a product needs a block of elements")
-    rows, n, code = _int32(shape.numel() // k, "tokens"), _int32(n, "rows"), _DTYPES[dtype]
+    k, rows, n, code = _int32(k, "k"), _int32(shape.numel() // k, "tokens"), _int32(n, "rows"), _DTYPES[dtype]
     return (rows, n, k, _row_stride(shape, stride, "x"), code, torch.Size((*shape[:-1], n)),
             int(_lib.load().hexkv_mx_linear_workspace_bytes(rows, n, k, code)))
 

@@ -244,6 +244,23 @@ def test_sizes_past_32_bits_are_refused():
     assert _lib.load().hexkv_mx_attend(ctypes.byref(p), None, 0, None) == R
 
 
+def test_shapes_past_32_bits_are_refused():
+    """Sizes that ctypes would wrap to a smaller call (views of one element: nothing is allocated)."""
+    long, bits = (1 << 32) + 64, torch.float16
+    one = torch.zeros(1, dtype=bits)
+    with pytest.raises(ValueError, match="32 bits"):
+        logprobs._form(torch.Size((1, long)), (long, 1), bits, 2)
+    with pytest.raises(ValueError, match="32 bits"):
+        fp4._linear_form(torch.Size((1, long)), (long, 1), bits, torch.Size((4, long // 2)), torch.Size((4, long // 32)))
+    with pytest.raises(ValueError, match="32 bits"):
+        fp4._rows_form(one.expand(1, long, 2, 1, 32).shape, (0, 0, 0, 32, 1), bits)
+    with pytest.raises(ValueError, match="32 bits"):
+        fp4._attend_form(one.expand(1, long, 1, 32), torch.zeros(1, 4, 48, dtype=torch.uint8), 1, None, None, False, None, 0)
+    with pytest.raises(ValueError, match="32 bits"):
+        fp4._matrix_size((1, long))
+    assert logprobs._form(torch.Size((2, 9)), (16, 1), bits, 2)[:3] == (2, 9, 16)
+
+
 def test_parameters_without_the_field_keep_16_bits():
     class Plain:  # the reference's own fields
         max_sequence_len, max_batch_size, sequence_len_offset, batch_size_offset = 9, 1, 0, 0
