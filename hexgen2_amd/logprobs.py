@@ -13,7 +13,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .fp4 import _call, _int32, _row_stride
+from .fp4 import _call, _int32
 from .ops import _DTYPES, _require_device
 
 
@@ -36,11 +36,17 @@ def _form(shape, stride, dtype, top: int):
     vocab = _int32(shape[-1], "vocab")
     if not 0 <= top <= min(_lib.MAX_TOP, vocab):
         raise ValueError(f"top {top} outside [0, {min(_lib.MAX_TOP, vocab)}]")
-    rows = shape.numel() // vocab
-    if len(shape) == 2 and rows > 1 and stride[1] == 1:
-        step = stride[0]
-    else:
-        step = _row_stride(shape, stride, "logits")
+    if vocab > 1 and stride[-1] != 1:
+        raise ValueError("logits rows must be contiguous")
+    rows, step, span = shape.numel() // vocab, vocab, None
+    for n, at in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+        if n == 1 or not rows:
+            continue
+        if span is None:
+            step, span = at, at
+        if at != span:
+            raise ValueError("logits rows must lie at one stride")
+        span *= n
     return rows, vocab, step, _DTYPES[dtype], int(_lib.load().hexkv_token_logprobs_workspace_bytes(rows, vocab, top))
 
 

@@ -775,6 +775,14 @@ def test_narrow_masks_take_the_time_of_others(device, dtype, rows, vocab, live, 
     assert time(narrow(rows, vocab, live, dtype, device, step)) <= 8 * time(whole)
 
 
+def test_logprobs_of_a_padded_vocabulary(device):
+    base = randn((2, 3, 9100), 3, torch.bfloat16, device)
+    tokens = torch.tensor([[5, 0, 7], [11, 2, 9]], device=device)
+    got = logprobs.token_logprobs(base[..., :9001], tokens, 4)
+    want = logprobs.token_logprobs(base[..., :9001].contiguous(), tokens, 4)
+    assert got.top_ids.shape == (2, 3, 4) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ------------------------------------------------------ streams and graphs ---
 
 

@@ -261,6 +261,17 @@ def test_shapes_past_32_bits_are_refused():
     assert logprobs._form(torch.Size((2, 9)), (16, 1), bits, 2)[:3] == (2, 9, 16)
 
 
+def test_logits_of_any_dims_whose_rows_lie_at_one_stride():
+    x = torch.zeros(4, 3, 5, 20)
+    for t, want in ((x, (60, 20, 20)), (x[..., :17], (60, 17, 20)), (x[1, 2, 3], (1, 20, 20)), (x[:, :, 2:3, :9], (12, 9, 100)),
+                    (x[:, 1, 2, :1], (4, 1, 300)), (x[:0, ..., :9], (0, 9, 9)), (x[:1, :1, :, 3:], (5, 17, 20)),
+                    (x[0, 0, 0].expand(6, 20), (6, 20, 0)), (torch.zeros(20, 7).t()[:, :1], (7, 1, 1))):
+        assert logprobs._form(t.shape, t.stride(), t.dtype, 0)[:3] == want
+    for t in (x[:, :2], x[..., ::2], x.transpose(0, 1), x[:, :, :2, :9], x[:, :1].expand(4, 3, 5, 20)):
+        with pytest.raises(ValueError, match="logits rows"):
+            logprobs._form(t.shape, t.stride(), t.dtype, 0)
+
+
 def test_parameters_without_the_field_keep_16_bits():
     class Plain:  # the reference's own fields
         max_sequence_len, max_batch_size, sequence_len_offset, batch_size_offset = 9, 1, 0, 0
