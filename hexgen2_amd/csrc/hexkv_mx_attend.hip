@@ -706,15 +706,17 @@ static size_t mx_workspace(const hexkv_mx_attend_params *p) {
 // To kJoinAlone partitions a wave joins a row by itself: 17 of them 28 us
 // instead of 20 in a call of 4 sequences, two 22.4 instead of 24.5 in one of 64.
 constexpr int kJoinAlone = 16;
+static int64_t mx_slots(const MxAttendArgs &a) { return (a.groups + kXcds - 1) / kXcds * kXcds * a.members; }
+static int64_t mx_join_groups(const MxAttendArgs &a) {
+  return a.max_parts > kJoinAlone ? a.rows : a.max_parts > 1 ? (a.rows + kJoinWaves - 1) / kJoinWaves : 0;
+}
+
 template <typename T, int D>
 static void mx_launch(const MxAttendArgs &a, hipStream_t s) {
-  const int64_t slots = (a.groups + kXcds - 1) / kXcds * kXcds * a.members;
-  mx_attend_kernel<T, D><<<static_cast<unsigned>(slots), 64 * a.waves, a.waves * MxLds<D>::kWave, s>>>(a);
-  if (a.max_parts > kJoinAlone)
-    mx_join_kernel<T, D, kJoinWaves><<<static_cast<unsigned>(a.rows), 64 * kJoinWaves, 0, s>>>(a);
-  else if (a.max_parts > 1)
-    mx_join_kernel<T, D, 1>
-        <<<static_cast<unsigned>((a.rows + kJoinWaves - 1) / kJoinWaves), 64 * kJoinWaves, 0, s>>>(a);
+  mx_attend_kernel<T, D><<<static_cast<unsigned>(mx_slots(a)), 64 * a.waves, a.waves * MxLds<D>::kWave, s>>>(a);
+  const unsigned join = static_cast<unsigned>(mx_join_groups(a));
+  if (a.max_parts > kJoinAlone) mx_join_kernel<T, D, kJoinWaves><<<join, 64 * kJoinWaves, 0, s>>>(a);
+  else if (join) mx_join_kernel<T, D, 1><<<join, 64 * kJoinWaves, 0, s>>>(a);
 }
 
 template <typename T>
@@ -788,7 +790,7 @@ extern "C" int hexkv_mx_attend(const hexkv_mx_attend_params *p, void *workspace,
   a.part = mx_partition(p);
   a.max_parts = static_cast<int32_t>(mx_parts(p, a.part));
   const int64_t workgroups = mx_units(p) * a.max_parts;
-  if (workgroups + kXcds * p->kv_heads >= INT64_C(1) << 24)
+  if (workgroups >= INT64_C(1) << 24)
     return fail(HEXKV_ERANGE, "%s: 2^24 workgroups or more; split the call", what);
   // (a call too small to give every XCD a group parts its tiles, then its heads)
   const int64_t pairs = static_cast<int64_t>(p->batch) * a.max_parts;
@@ -798,9 +800,11 @@ extern "C" int hexkv_mx_attend(const hexkv_mx_attend_params *p, void *workspace,
   // (8 / 4 waves: 577 keys of 4 KV heads 6.6 / 7.5 us, 17.8 / 19.4 for the 8 x
   // 32 heads above), four else (B 64 of 1024 keys, 32 KV heads: 86.6 / 85.7).
   a.waves = workgroups <= kCus ? kMxaMaxWaves : kMxaMaxWaves / 2;
+  a.rows = static_cast<int64_t>(p->batch) * p->q_len * p->q_heads;
+  if (mx_slots(a) * 64 * a.waves >= INT64_C(1) << 32 || mx_join_groups(a) * 64 * kJoinWaves >= INT64_C(1) << 32)
+    return fail(HEXKV_ERANGE, "%s: 2^32 lanes or more in a launch; split the call", what);
   a.kv_new = p->kv_new;
   a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
-  a.rows = static_cast<int64_t>(p->batch) * p->q_len * p->q_heads;
   if (a.max_parts > 1) {
     a.ws_o = static_cast<float *>(workspace);
     a.ws_ml = a.ws_o + a.rows * a.max_parts * p->head_dim;

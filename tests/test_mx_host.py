@@ -136,6 +136,19 @@ def test_attention_refuses(change, code):
     assert _lib.load().hexkv_last_error()
 
 
+@pytest.mark.parametrize("change", [
+    # nine pairs take the places of sixteen: 9/16 of 2^24 workgroups and a few more
+    dict(batch=9, q_len=(1 << 24) + 16, q_heads=1, kv_heads=1, head_dim=32, max_seqlen=32),
+    # a workgroup per row in the join of 17 partitions, eight rows a workgroup in that of two
+    dict(batch=1, q_len=1 << 23, q_heads=1, kv_heads=1, head_dim=32, max_seqlen=17 * 32, partition=32),
+    dict(batch=1, q_len=1 << 26, q_heads=1, kv_heads=1, head_dim=32, max_seqlen=64, partition=32)])
+def test_attention_refuses_launches_of_too_many_lanes(change):
+    """(With room enough said to be at an address that is never read: the refusal comes first.)"""
+    p = attend_params(dtype=0, capacity=1 << 10, cache_row_bytes=48, cache_batch_bytes=48 << 10, **change)
+    assert _lib.load().hexkv_mx_attend(ctypes.byref(p), ADDRESS, 1 << 62, None) == R
+    assert b"2^32 lanes" in _lib.load().hexkv_last_error()
+
+
 def test_attention_refuses_a_small_workspace_and_null_params():
     lib, p = _lib.load(), attend_params(partition=32)
     need = lib.hexkv_mx_attend_workspace_bytes(ctypes.byref(p))
