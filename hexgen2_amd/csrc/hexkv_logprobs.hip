@@ -26,7 +26,7 @@
 // `top` times over took 474, and 370 for the mask).
 //
 // Measured on MI355X, bf16: 8191 x 32000 without alternatives 97 us (5.4 TB/s),
-// with the top 20 125 us (4.2); one row of 32000 fp16, top 5, 10.0 us.
+// with the top 20 126 us (4.2); one row of 32000 fp16, top 5, 10.2 us.
 #include "hexkv_common.h"
 
 #include <algorithm>
@@ -455,13 +455,15 @@ __global__ __launch_bounds__(kLpThreads) void logprob_join_kernel(const LogprobA
   }
 }
 
-// Parts a row is cut into: one to kLpShort chunks (the join's launch and the
-// workspace cost more: a call for 1 x 32000, top 5, 11.0 us and 15.2 in 8 parts,
-// host included); beyond, enough for a workgroup a CU, and for few rows of long
-// vocabularies about twelve chunks each, but no more keys than a join ranks in
-// passing, since it compares all of them (us in 1 / 4 / 8 / 32 parts: 1 x 128000, top 20
-// 25.6 / 15.5 / 13 / 36, top 5 21 / 12.6 / 10.8 / 11.1; top 64 in 4 parts 23.5, in 32
-// over 200;
+// Parts a row is cut into: one to kLpShort chunks, where the join's launch and
+// the workspace cost more than the shorter walk saves (us a call, host included, one
+// part / split, top 5 and 20: 1 x 32000 10.0 / 13.4 and 11.8 / 13.4; 40960 10.4 / 13.4
+// and 12.1 / 13.3; 49145, the longest of 12 chunks, 12.0 / 13.3 and 14.2 / 13.2; 65536 13.4
+// / 13.4 and 16.0 / 13.3; 16 x 49145 12.7 / 13.4 and 15.2 / 13.4); beyond, enough for a
+// workgroup a CU, and for few rows of long vocabularies about twelve chunks
+// each, but no more keys than a join ranks in passing, since it compares all of them (us
+// in 1 / 4 / 8 / 32 parts: 1 x 128000, top 20 25.6 / 15.5 / 13 / 36, top 5 21 / 12.6 /
+// 10.8 / 11.1; top 64 in 4 parts 23.5, in 32 over 200;
 // 64 x 128000, top 20, 27.6 / 16.7 / 16.6 / 25.6; 300 x 128000 37.4 / 32.8 / 32.3).
 constexpr int kLpShort = 12, kLpKeys = 160;
 static int lp_parts(int64_t rows, int vocab, int top, int64_t *span) {

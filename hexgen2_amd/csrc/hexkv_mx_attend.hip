@@ -29,12 +29,15 @@
 // second kernel joins them.
 //
 // Measured (append included, bf16, head_dim 128, 32 query heads on 8 KV heads):
-// 64 sequences of 128 to 8192 81 us, 3.6 TB/s of the cache, and 4.4 TB/s from
-// one length to the next (a copy reaches 4.85): what is above that is the launch,
-// the prologue's chain of loads and the last round.  Few keys a wave are bound
-// by a step's own latency, about 1 us from LDS to the last product; loading two
-// or three steps ahead instead of one cost 3 to 10% (registers), steps of one
-// wave a partition 12% at 64 sequences and 20 to 60% at one to four.
+// 64 sequences of 128 to 8192 81 us, 3.2 TB/s; reading alone could reach 7.1 (36
+// us).  What bounds it is a step's own instructions: VALU 41% and LDS 37% of the
+// cycles (a third of the latter bank conflicts of V's stores), matrix cores
+// 15%, at 2.6 waves per SIMD that wait for memory 30% of their time.  Few keys a
+// wave are bound by a step's latency, about 1 us from LDS to the last product;
+// loading two or three steps ahead instead of one cost 3 to 10%
+// (registers), steps of one wave a partition 12% at 64 sequences and 20 to 60%
+// at one to four.  16 x 90 rows over 2048 keys: 122 us, VALU 64% and LDS 58% busy
+// (a tile of 16 rows converts every key for itself).
 //
 // A NaN block of V, or one with an element that fp32 does not hold (2^128 and
 // above), is taken out of the product (0 times either is a NaN, which would reach
@@ -610,7 +613,7 @@ static int64_t mx_units(const hexkv_mx_attend_params *p) {
 }
 
 // Positions per partition.  One partition where the join would cost more than
-// it saves: to 1024 keys; where there is a unit for each of the 256 CUs to 2048;
+// it saves: to 1024 keys; where there is a unit for each of the 256 CUs to 2560;
 // and for more than kFewTiles row tiles there whatever the length (their rows'
 // lengths differ little).  Beyond, two workgroups a CU, of 256 to 1024 keys
 // each (the upper end for ragged lengths).  us, one partition / 256 / 512 /
@@ -619,6 +622,10 @@ static int64_t mx_units(const hexkv_mx_attend_params *p) {
 //               B 1 of 8192     38.2 / 11.8 / 12.4 / 18.9
 //               B 32 of 1024    13.0 / 21.2 / 17   /  -     of 2048  24.2 / 39   / 30   / 27.8
 //               B 64 of 128..8192  86 / 99 / 83.2 / 80.7
+//   (one / 1024 keys each)
+//               B 32 of 2304  25.7 / 29.4, of 2816  29.7 / 34.4, of 4096  41 / 44
+//               B 32 of n / 32..n, n 2560  23.9 / 24.0, 3000  24.6 / 28.2, 4096  33.6 / 31.9
+//               B 64 of n / 32..n, n 2560  36.6 / 37.1, 3000  45.8 / 45.9, 4096  63.4 / 59.7
 //   32 KV heads, B 8 of 256..2048 (fp16)  17.8 / 38 / 23 / 19.9
 //   400 rows, B 2 of 4096, 8 heads on 1 (fp16)  45 / - / - / 51;  1600 rows, 32 on 8  385 / - / - / 571;
 //   60 rows, B 16 of 1..8192, 8 on 1  71 / - / - / 62

@@ -1,7 +1,7 @@
 // Products with 4-bit matrices: hexkv_mx_linear.
 //
 // What bounds it: reading the matrix while tokens are few, 17/32 byte an element
-// (at the rate of a large copy, 4.85 TB/s), the matrix cores for a prompt.
+// (read-only streams reach 7.1 TB/s here), the matrix cores for a prompt.
 // Everywhere a lane loads whole blocks of a row (16 bytes, 32 elements, one
 // power) and converts them in registers; the matrix instructions' inner dimension is laid
 // out to fit what a lane holds, the tokens' operand in the same order, so a
@@ -128,7 +128,7 @@ __device__ __forceinline__ float mx_dot(u32x4 w, unsigned int byte, const u32x4 
 // One or two tokens: a wave takes ROWS rows of the matrix, its lanes the
 // blocks of a row in turn (LOADS of them each), and the activations of those
 // blocks stay in registers.  No load is conditional: loads inside branches
-// waited for one another's latency (15.5 us where this takes 10.9, 1 x 22528 x 4096).
+// waited for one another's latency (15.5 us where this takes 11, 1 x 22528 x 4096).
 template <typename T, int TOKENS, int LOADS, int ROWS, bool VEC>
 __global__ __launch_bounds__(kMxlThreads) void mx_rows_kernel(const MxLinearArgs a) {
   constexpr int XW = sizeof(T) * 2;
@@ -298,7 +298,7 @@ __device__ __forceinline__ void lds_fence() {  // orders this wave's LDS accesse
 // them), and walks the matrix 16 rows at a time; the waves join through LDS.
 // What bounded it were the address units, where a load's lanes read different
 // rows: the matrix's words now change lanes after the load, the tokens go through
-// LDS once (64 x 22528 x 4096 30.5 -> 24.0 us, 16 x 4096 x 4096 8.0 -> 5.9).  BL: consecutive
+// LDS once (64 x 22528 x 4096 31 -> 25 us, 16 x 4096 x 4096 8 -> 6).  BL: consecutive
 // blocks of a row that a lane holds; RING: matrix tiles a wave has loaded or in
 // flight (one more cost 1 to 5%); VEC: the activations' rows are 16-byte aligned.
 template <typename T, int MT, int BL, int RING, bool VEC>
@@ -1025,16 +1025,17 @@ __global__ __launch_bounds__(kMxlThreads) void mx_sum_kernel(const MxLinearArgs 
 
 // The kernels and tiles a call may run, by tokens (GPU time of a call on MI355X,
 // weights from memory, bf16 unless said):
-//   1, 2    kRows: 1 x 22528 x 4096 10.9 us (4.5 TB/s); kFew 14.2.
-//   3-64    kFew, 16, 32 or 64 tokens a wave (16 x 22528 x 4096 14.7 us, 32 x 16.8, 64 x
-//           25.8; 64 x 4096 x 4096 11.2, where a tile of the tokens in LDS took
-//           14.8; 32 x 2560 x 2048 4.6 and 9.0; 32 x 4096 x 11264 18.2 and 17.8).
+//   1, 2    kRows: 1 x 22528 x 4096 11 us (4.4 TB/s); kFew 14.
+//   3-64    kFew, 16, 32 or 64 tokens a wave (16 x 22528 x 4096 15 us, 32 x 17, 64 x 25;
+//           64 x 4096 x 4096 11.2, where a tile of the tokens in LDS took 14.8; 32 x
+//           2560 x 2048 4.6 and 9.0; 32 x 4096 x 11264 18.7 and 17.8).
 //           fp32: to 16, then tiles (three registers a token of each).
 //   65-     16-bit: mx_prompt_kernel, by tiles of 64 tokens x 128 rows up to
 //           kNarrowTokens (128 x 22528 x 4096 45 us, x 256 rows 49; 300 x 6144 x
-//           4096 30.2 / 32.3), then 64 x 256 (611 x 4096 x 11264 74 us, fp16 79; x 128
+//           4096 30.5 / 32.3), then 64 x 256 (611 x 4096 x 11264 76 us, x 128
 //           rows over 82), and 128 x 256 where those make kLargeTiles (2048 x
-//           22528 x 4096 341 us, 1.1 PFLOP/s; 64 x 256 over 369; 611 x 4096 x 11264 78 / 74).
+//           22528 x 4096 355 us, 1.06 PFLOP/s; 64 x 256 over 369; 611 x 4096 x
+//           11264 80 / 76).
 //           Below 128 of the inner dimension, kFew 64 at a time.  fp32:
 //           mx_tile_kernel, 64 tokens up to kWideTokens, 128 above.
 enum MxKind { kRows, kFew16, kFew32, kFew64, kTile32, kTile64, kNarrow, kPrompt, kLarge, kWide32, kWider32 };

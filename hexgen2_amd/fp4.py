@@ -1,8 +1,10 @@
 """Caches and weights in four bits: the OCP microscaling format MXFP4, blocks of
 32 consecutive elements that share a power of two (4.25 bits an element).
 
-The reference holds both in the data type; a decode step is bound by reading
-them, so a quarter of the bytes is close to a quarter of the time.  A 4-bit
+The reference holds both in the data type, 3.76 times the bytes.  How much of
+the time that saves depends on the call (MI355X, us, four bits against 16): attention of
+a Llama-3-8B layer, 64 sequences of 128 to 8192, 81 against 156; of one sequence
+of 577, 6.8 against 6.0; a product of one token, 22528 x 4096, 11 against 30.  A 4-bit
 cache is one layer's uint8 ``[batch, capacity, row_bytes(kv_heads, head_dim)]``,
 a row one position's K and V of every KV head like the 16-bit cache's, so
 ``ops.pack_live`` and ``ops.unpack_live`` hand it over unchanged.  A 4-bit matrix
