@@ -763,13 +763,16 @@ def test_narrow_masks_take_the_time_of_others(device, dtype, rows, vocab, live, 
     largest was taken out ``top`` times over)."""
     def time(x):
         logprobs.token_logprobs(x, None, 20)
-        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-        start.record()
-        for _ in range(30):
-            logprobs.token_logprobs(x, None, 20)
-        end.record()
-        end.synchronize()
-        return start.elapsed_time(end) / 30
+        rounds = []
+        for _ in range(7):  # the least of them: what else the machine does is not timed
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            for _ in range(10):
+                logprobs.token_logprobs(x, None, 20)
+            end.record()
+            end.synchronize()
+            rounds.append(start.elapsed_time(end))
+        return min(rounds)
 
     whole = randn((rows, vocab), 3, dtype, device, 3.0)
     assert time(narrow(rows, vocab, live, dtype, device, step)) <= 8 * time(whole)
@@ -831,6 +834,44 @@ def test_a_step_on_another_stream_and_in_a_graph(device):
         assert all(torch.equal(a, b) for a, b in zip(want, result))
         assert torch.equal(captured, cache)
         step(fresh())  # eager work between
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_every_path_in_a_graph(device, dtype):
+    """Chunks taken out and read in four bits (their keys split, so that both
+    join), products with blocks fp16 does not hold and prompts, and rows of logits that are
+    ranked, filled and counted: three replays, with the same calls made eagerly between them."""
+    heads, hq, d, t, n = 1, 4, 128, 110, 2900
+    kv = randn((1, n, 2, heads, d), 1, dtype, device)
+    cache = make_cache(kv, n + 9, device)
+    q = randn((1, t, hq, d), 2, dtype, device, 2.0)
+    lens = torch.tensor([n - 3], dtype=torch.int32, device=device)
+    w = fp4.quantize(randn((300, 4512), 3, dtype, device, 0.02))
+    w.powers[7, 2], w.powers[290, 140] = 95, 150
+    xs = [randn((rows, 4512), rows, dtype, device) for rows in (1, 9, 40, 200)]
+    xs[1][3, 70] = float("inf")
+    logits = torch.cat((narrow(2, 32000, 300, dtype, device), narrow(2, 32000, 0, dtype, device),
+                        narrow(2, 32000, 9, dtype, device), torch.zeros((2, 32000), dtype=dtype, device=device)))
+
+    def calls():
+        return [fp4.decode_attention(q, cache, heads, max_seqlen=n, seqlens=lens, causal=True),
+                fp4.decode_attention(q[:, :5], cache, heads, max_seqlen=n, seqlens=lens, causal=True),
+                *(fp4.linear(x, w) for x in xs), *logprobs.token_logprobs(logits, None, 20)[1:],
+                *logprobs.token_logprobs(logits[:, :9000], None, 20)[1:]]
+
+    want = calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        result = calls()
+    for _ in range(3):
+        for r in result:
+            r.fill_(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(torch.nan_to_num(a.double(), 7.5, 8.5, 9.5), torch.nan_to_num(b.double(), 7.5, 8.5, 9.5))
+                   for a, b in zip(want, result))
+        calls()  # eager work between
 
 
 # --------------------------------------------------- refusals on the device ---
