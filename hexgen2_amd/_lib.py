@@ -29,15 +29,17 @@ EXPORTS = ("hexkv_version", "hexkv_last_error", "hexkv_pack", "hexkv_unpack", "h
            "hexkv_attend_plan_layers", "hexkv_mx_store", "hexkv_mx_load", "hexkv_mx_quantize", "hexkv_mx_dequantize",
            "hexkv_mx_attend", "hexkv_mx_attend_workspace_bytes", "hexkv_mx_linear",
            "hexkv_mx_linear_workspace_bytes", "hexkv_token_logprobs",
-           "hexkv_token_logprobs_workspace_bytes")
+           "hexkv_token_logprobs_workspace_bytes", "hexkv_paged_append", "hexkv_paged_attend",
+           "hexkv_paged_attend_workspace_bytes", "hexkv_paged_pack", "hexkv_paged_unpack")
 NOALLOC_SCRATCH_BYTES = 32 << 20
 # Arrival counters at the front of every attention workspace (zero them once).
 ATTEND_COUNTER_BYTES = 256 << 10
 ATTEND_COUNTER_WORDS = ATTEND_COUNTER_BYTES // 8  # one 64-bit counter per (row, head group)
 # Device status flags (hexkv_device_status).
 STATUS_APPEND_SKIPPED, STATUS_LENGTH_CLAMPED, STATUS_PLACEMENT, STATUS_DISPATCH, STATUS_LIST = 1, 2, 4, 8, 16
-STATUS_LOAD_SKIPPED = 32
-STATUS_ERRORS = STATUS_APPEND_SKIPPED | STATUS_LENGTH_CLAMPED | STATUS_PLACEMENT | STATUS_LIST | STATUS_LOAD_SKIPPED
+STATUS_LOAD_SKIPPED, STATUS_PAGE = 32, 64
+STATUS_ERRORS = (STATUS_APPEND_SKIPPED | STATUS_LENGTH_CLAMPED | STATUS_PLACEMENT | STATUS_LIST | STATUS_LOAD_SKIPPED
+                 | STATUS_PAGE)
 MAX_TOP = 64  # most alternatives of hexkv_token_logprobs
 
 
@@ -101,6 +103,39 @@ class MxAttendParams(ctypes.Structure):
         ("seqlens_dev", ctypes.c_void_p), ("seqlen_bias", ctypes.c_int32), ("max_seqlen", ctypes.c_int32),
         ("kv_new", ctypes.c_void_p), ("partition", ctypes.c_int),
     ]
+
+
+class Pool(ctypes.Structure):
+    """Mirror of ``hexkv_pool``."""
+    _fields_ = [("dtype", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("n_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("page_stride", ctypes.c_int64), ("pos_stride", ctypes.c_int64), ("kv_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+class PagedBatch(ctypes.Structure):
+    """Mirror of ``hexkv_paged_batch``."""
+    _fields_ = [("tables", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int32),
+                ("batch", ctypes.c_int32), ("starts", ctypes.c_void_p), ("cu_tokens", ctypes.c_void_p),
+                ("tokens", ctypes.c_int32)]
+
+
+class PagedAppendParams(ctypes.Structure):
+    """Mirror of ``hexkv_paged_append_params``."""
+    _fields_ = [("pool", Pool), ("seqs", PagedBatch), ("q_heads", ctypes.c_int),
+                ("qkv", ctypes.c_void_p), ("qkv_stride", ctypes.c_int64),
+                ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64),
+                ("pages", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
+                ("rotary_dim", ctypes.c_int), ("interleaved", ctypes.c_int), ("rotary_scale", ctypes.c_float)]
+
+
+class PagedAttendParams(ctypes.Structure):
+    """Mirror of ``hexkv_paged_attend_params``."""
+    _fields_ = [("pool", Pool), ("seqs", PagedBatch), ("q_heads", ctypes.c_int), ("causal", ctypes.c_int),
+                ("softmax_scale", ctypes.c_float), ("max_tokens", ctypes.c_int32), ("max_seqlen", ctypes.c_int32),
+                ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64),
+                ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64),
+                ("pages", ctypes.c_void_p), ("partition", ctypes.c_int32)]
 
 
 class Block(ctypes.Structure):
@@ -225,6 +260,16 @@ def load() -> ctypes.CDLL:
     lib.hexkv_token_logprobs_workspace_bytes.argtypes = [i64, ci, ci]
     lib.hexkv_token_logprobs.restype = ci
     lib.hexkv_token_logprobs.argtypes = [vp, i64, i64, ci, ci, vp, ci, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
+    lib.hexkv_paged_append.restype = ci
+    lib.hexkv_paged_append.argtypes = [ctypes.POINTER(PagedAppendParams), vp]
+    lib.hexkv_paged_attend.restype = ci
+    lib.hexkv_paged_attend.argtypes = [ctypes.POINTER(PagedAttendParams), vp, ctypes.c_size_t, vp]
+    lib.hexkv_paged_attend_workspace_bytes.restype = ctypes.c_size_t
+    lib.hexkv_paged_attend_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttendParams)]
+    for name in ("hexkv_paged_pack", "hexkv_paged_unpack"):
+        fn = getattr(lib, name)
+        fn.restype = ci
+        fn.argtypes = [ctypes.POINTER(Pool), ptrs, ptrs, ci, vp, i64, ci, ci, ctypes.POINTER(i64), vp]
     _lib = lib
     return lib
 

@@ -28,7 +28,7 @@ COMMON = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", f"-I{INCLUDE}"
           "-Wall", "-Wno-unused-function"]
 SOURCES = ["hexkv_status.cpp", "hexkv_copy.hip", "hexkv_attend.hip", "hexkv_prefill.hip", "hexkv_blocks.hip",
            "hexkv_layer.hip", "hexkv_ipc.cpp", "hexkv_mx.hip", "hexkv_mx_attend.hip", "hexkv_mx_linear.hip",
-           "hexkv_logprobs.hip"]
+           "hexkv_logprobs.hip", "hexkv_paged.hip", "hexkv_paged_attend.hip"]
 # Register, LDS and occupancy figures of the attention kernels, from the
 # compiler's resource remarks: the work-list planner sizes row-block lists
 # for the workgroups a CU holds at once (tests/test_kernel_resources.py).

@@ -68,6 +68,8 @@ _STATUS_TEXT = {
                       "launched, and its items were skipped",
     _lib.STATUS_LOAD_SKIPPED: "a position read from device memory to load from a 4-bit cache fell outside it, so "
                               "that row came back as zeros",
+    _lib.STATUS_PAGE: "a page table named a page outside the pool: what it stood for was not written, came back as "
+                      "zeros or was not attended",
 }
 
 

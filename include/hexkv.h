@@ -104,6 +104,8 @@ const char *hexkv_last_error(void);
 #define HEXKV_STATUS_LIST 16u          /* hexkv_attend: a work item planned for another head-group size (another
                                           kernel) was skipped, so its outputs were not written */
 #define HEXKV_STATUS_LOAD_SKIPPED 32u  /* hexkv_mx_load: a position outside [0, capacity); that row came back as zeros */
+#define HEXKV_STATUS_PAGE 64u          /* hexkv_paged_*: a page table's entry outside the pool; its rows were not written
+                                          (append, unpack), came back as zeros (pack) or were not attended */
 
 /*
  * Waits for `stream`, then reads the status word of the stream's device into
@@ -765,6 +767,108 @@ size_t hexkv_token_logprobs_workspace_bytes(int64_t rows, int vocab, int top);
 int hexkv_token_logprobs(const void *logits, int64_t row_stride, int64_t rows, int vocab, int dtype,
                          const int64_t *tokens_dev, int top, float *logprob, float *entropy, float *top_logprobs,
                          int64_t *top_ids, void *workspace, size_t workspace_bytes, hexkv_stream_t stream);
+
+/* ------------------------------------------------------- paged caches --- */
+
+/*
+ * A layer's cache as a pool of pages (no counterpart in the reference, whose
+ * caches are [batch][capacity][row], mha.py:260-265): a page holds page_size
+ * positions of one sequence, and position p of sequence b is row p % page_size
+ * of page tables[b][p / page_size].  A row is one position's K and V of every
+ * KV head as in the other caches; where its parts lie is given by strides, so
+ * that a page may be [page_size][2][kv_heads][head_dim] or, what the kernels
+ * read best, [kv_heads][2][page_size][head_dim].
+ */
+typedef struct hexkv_pool {
+  int dtype;              /* enum hexkv_dtype */
+  int kv_heads, head_dim; /* head_dim 16, 32, 64, 128 or 256 */
+  int32_t n_pages;        /* at least 1 */
+  int32_t page_size;      /* a power of two from 16 to 2^20 */
+  /* Elements from page to page, position to position, K to V, head to head;
+   * whole numbers of 16 bytes, as the base address is. */
+  int64_t page_stride, pos_stride, kv_stride, head_stride;
+} hexkv_pool;
+
+/*
+ * The sequences of a call and their new tokens.  Tokens lie sequence after
+ * sequence: sequence b's are [cu_tokens[b], cu_tokens[b + 1]) of `tokens`, or,
+ * without cu_tokens, an equal share of them each; the first of them has position
+ * starts[b] (so many rows are cached before).  A sequence with a negative start
+ * is not in use: none of its tokens is looked at, and its attention is zero.
+ * Tokens that belong to no sequence, as those behind the last, are left alone.
+ */
+typedef struct hexkv_paged_batch {
+  const int32_t *tables;   /* device, [batch] rows of table_width entries */
+  int64_t table_stride;    /* entries from row to row */
+  int32_t table_width, batch;
+  const int32_t *starts;   /* device, [batch] */
+  const int32_t *cu_tokens; /* device, [batch + 1], or NULL */
+  int32_t tokens;          /* rows of the token tensors */
+} hexkv_paged_batch;
+
+typedef struct hexkv_paged_append_params {
+  hexkv_pool pool;
+  hexkv_paged_batch seqs;
+  int q_heads;
+  const void *qkv;        /* [tokens] rows of (q_heads + 2 kv_heads) heads: q, k, v */
+  int64_t qkv_stride;     /* elements from row to row */
+  void *q;                /* [tokens][q_heads][head_dim], rotated; may be the q heads of qkv themselves */
+  int64_t q_stride;       /* elements from row to row */
+  void *pages;
+  const float *inv_freq;  /* device, [rotary_dim / 2] */
+  int rotary_dim;         /* leading dims of a head that turn: even, 0 to head_dim */
+  int interleaved;        /* 0: pairs (j, j + rotary_dim / 2); 1: pairs (2 j, 2 j + 1) */
+  float rotary_scale;     /* what sines and cosines are multiplied by */
+} hexkv_paged_append_params;
+
+/*
+ * Rotates the new tokens' q and k heads to their positions and writes k and v
+ * into the pages.  Pair j of a token at position p turns by p * inv_freq[j]:
+ * (x, y) -> (x cos - y sin, y cos + x sin), the angle reduced in 64 bits, sines,
+ * cosines and products in fp32, rounded once.  A token past the table, or whose page lies outside
+ * the pool, is not written and flagged (its q is).  No two tokens may share a row.
+ */
+int hexkv_paged_append(const hexkv_paged_append_params *params, hexkv_stream_t stream);
+
+typedef struct hexkv_paged_attend_params {
+  hexkv_pool pool;
+  hexkv_paged_batch seqs;
+  int q_heads;            /* a multiple of kv_heads */
+  int causal;             /* 1: token i of a sequence sees its first starts + i + 1 rows; 0: all of starts + count */
+  float softmax_scale;    /* above 0 */
+  int32_t max_tokens;     /* bound on a sequence's new tokens (with cu_tokens) */
+  int32_t max_seqlen;     /* bound on a sequence's rows, its new ones included */
+  const void *q;          /* [tokens][q_heads][head_dim], rows 16-byte aligned */
+  int64_t q_stride;       /* elements from row to row */
+  void *out;              /* like q, and may be q */
+  int64_t out_stride;
+  const void *pages;
+  int32_t partition;      /* rows per partition of a split row, a multiple of 64; 0: the library's choice */
+} hexkv_paged_attend_params;
+
+/*
+ * Attention of the new tokens over their sequences' rows in the pages, their
+ * own (already appended) included: decode rows, chunks of prompts and both in
+ * one call.  A sequence with more than max_tokens tokens or max_seqlen rows is
+ * cut to them and flagged HEXKV_STATUS_LENGTH_CLAMPED.  A row that attends
+ * nothing is zero.
+ */
+int hexkv_paged_attend(const hexkv_paged_attend_params *params, void *workspace, size_t workspace_bytes,
+                       hexkv_stream_t stream);
+size_t hexkv_paged_attend_workspace_bytes(const hexkv_paged_attend_params *params);
+
+/*
+ * hexkv_pack / hexkv_unpack for pools: rows [0, lens[b]) of every sequence of
+ * every layer between the pages and [sum(lens)][2][kv_heads][head_dim] per
+ * layer, one launch for up to HEXKV_MAX_LAYERS_PER_LAUNCH layers that share
+ * the tables.  `pages` and `packed` are host arrays of device addresses.
+ */
+int hexkv_paged_pack(const hexkv_pool *pool, const void *const *pages, void *const *packed, int n_layers,
+                     const int32_t *tables_dev, int64_t table_stride, int table_width, int batch, const int64_t *lens,
+                     hexkv_stream_t stream);
+int hexkv_paged_unpack(const hexkv_pool *pool, const void *const *packed, void *const *pages, int n_layers,
+                       const int32_t *tables_dev, int64_t table_stride, int table_width, int batch, const int64_t *lens,
+                       hexkv_stream_t stream);
 
 #ifdef __cplusplus
 }
