@@ -38,6 +38,17 @@ __device__ __forceinline__ Sequence sequence_of(const PageTables &p, int b) {
   return s;
 }
 
+// The sequence that token t belongs to, or -1: a wave looks at 64 at a time.
+__device__ __forceinline__ int token_sequence(const PageTables &p, int t) {
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < p.batch; b0 += 64) {
+    const int b = min(b0 + lane, p.batch - 1), lo = p.cu[b], hi = p.cu[b + 1];
+    const uint64_t in = __ballot(lo >= 0 && lo <= t && t < hi && hi <= p.tokens);
+    if (in) return min(b0 + __builtin_ctzll(in), p.batch - 1);
+  }
+  return -1;
+}
+
 // Checks a pool and a call's sequences and fills `p`; the library's status.
 int check_pool(const hexkv_pool &pool, const char *what);
 int fill_tables(const hexkv_pool &pool, const hexkv_paged_batch &seqs, PageTables *p, const char *what);

@@ -87,17 +87,6 @@ struct alignas(sizeof(T) * VEC) Vec {
   T e[VEC];
 };
 
-// The sequence that token t belongs to, or -1: a wave looks at 64 at a time.
-__device__ __forceinline__ int token_sequence(const PageTables &p, int t) {
-  const int lane = threadIdx.x & 63;
-  for (int b0 = 0; b0 < p.batch; b0 += 64) {
-    const int b = min(b0 + lane, p.batch - 1), lo = p.cu[b], hi = p.cu[b + 1];
-    const uint64_t in = __ballot(lo >= 0 && lo <= t && t < hi && hi <= p.tokens);
-    if (in) return min(b0 + __builtin_ctzll(in), p.batch - 1);
-  }
-  return -1;
-}
-
 // One token a workgroup.  Its sines and cosines are made once, by one lane a pair,
 // and shared by all heads through LDS.  The angle p f / 2 pi (in turns) is a
 // product in 64 bits less its whole turns: 32 bits leave 2^-8 of a radian at

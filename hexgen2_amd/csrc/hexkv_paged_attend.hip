@@ -3,7 +3,7 @@
 // A row is one query head of one new token; the rows of a sequence that share
 // a KV head (tokens x group of them, in (token, head) order) read the same keys.
 //
-// Row kernel: 16 rows a workgroup, its waves taking steps of the keys in turn.
+// Row path: 16 rows a workgroup, its waves taking steps of the keys in turn.
 //   S^T = K Q^T    16 keys x 16 rows a matrix instruction; K's operand is
 //                  loaded as it lies: lane (r, g) holds key r, dims of chunk g
 //   softmax        a lane's scores are all its own row's; the other 3 lanes
@@ -14,6 +14,13 @@
 //                  transposed out, fp32 V is loaded in place
 // What bounds it: a decode row's K and V are read once, 4 D flops a key, so
 // memory.  Steps are loaded one ahead into registers, page numbers two ahead.
+//
+// Tile path (16-bit, head_dim 64 or 128, sequences of more than kFewRows rows):
+// 128 rows a workgroup, 32 a wave, which share tiles of 64 keys in LDS; the same
+// products on 32 x 32 x 16 matrix instructions.  What bounds it: the matrix cores, and
+// the softmax on the VALU beside them.  A probability enters P V as one 16-bit
+// term, rounded to nearest: an error of the order of the output's own rounding (that
+// of p averages over the keys), for two thirds of the matrix work.
 #include "hexkv_paged.h"
 
 #include <algorithm>
@@ -22,6 +29,7 @@
 namespace hexkv {
 
 typedef short h4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) h4 lds_h4;
 
 struct PagedAttendArgs {
@@ -32,13 +40,23 @@ struct PagedAttendArgs {
   int32_t q_heads, kv_heads, group, causal;
   int32_t max_tokens, max_seqlen;
   float scale_log2;
-  int32_t row_tiles;        // 16-row tiles of a sequence and KV head
-  int32_t part, max_parts;  // rows per partition, partitions of the longest row
-  float *ws_o, *ws_ml;      // split rows: [pair][row][max_parts][D] sums, [..][2] maximum and sum
+  int32_t few_rows;         // a sequence's rows per KV head up to which it takes the row path
+  // row path: 16-row tiles of a sequence and KV head, keys per partition,
+  // partitions of the longest row
+  int32_t row_tiles, part, max_parts;
+  // tile path: the same for tiles of 128 rows, and its workgroups
+  int32_t tiles, tile_part, tile_parts, tile_blocks;
+  // split rows: [pair][row][max_parts] and [token][head][tile_parts] of D sums, and of
+  // (maximum, sum)
+  float *ws_o, *ws_ml, *ws_tile_o, *ws_tile_ml;
   unsigned int *status;
 };
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// What a row's sums are multiplied by: its softmax's reciprocal sum, 0 where
+// nothing was attended.
+__device__ __forceinline__ float weight_of(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
 
 // Tokens of sequence b as this call sees them, and the keys they attend.
 struct Rows {
@@ -82,6 +100,12 @@ struct Mma<__bf16> {
   __device__ __forceinline__ static f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
   }
+  __device__ __forceinline__ static f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+  __device__ __forceinline__ static unsigned int pair(float p0, float p1) {
+    return __builtin_bit_cast(unsigned int, v2{static_cast<__bf16>(p0), static_cast<__bf16>(p1)});
+  }
   __device__ __forceinline__ static void split(float p0, float p1, unsigned int *hi, unsigned int *lo) {
     const v2 h = {static_cast<__bf16>(p0), static_cast<__bf16>(p1)};
     const v2 r = {static_cast<__bf16>(p0 - static_cast<float>(h[0])), static_cast<__bf16>(p1 - static_cast<float>(h[1]))};
@@ -97,6 +121,12 @@ struct Mma<_Float16> {
   static constexpr float kShift = 11.f, kSlack = 4.f;
   __device__ __forceinline__ static f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+  __device__ __forceinline__ static f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+  __device__ __forceinline__ static unsigned int pair(float p0, float p1) {
+    return __builtin_bit_cast(unsigned int, v2{static_cast<_Float16>(p0), static_cast<_Float16>(p1)});
   }
   __device__ __forceinline__ static void split(float p0, float p1, unsigned int *hi, unsigned int *lo) {
     const v2 h = {static_cast<_Float16>(p0), static_cast<_Float16>(p1)};
@@ -168,8 +198,15 @@ __device__ void exact_row(const PagedAttendArgs &a, const T *q, int b, int hk, i
   *l_out = sum_from<1>(l);
 }
 
+// LDS bytes of the row path: V as its waves turn it, then their sums.
 template <typename T, int D, int W>
-__global__ __launch_bounds__(W * 64) void paged_rows_kernel(const PagedAttendArgs a) {
+constexpr int rows_lds() {
+  const int v = std::is_same<T, float>::value ? 0 : W * 32 * (2 * D + 32), o = W * 16 * (D + 4) * 4;
+  return (v > o ? v : o) + 2 * W * 16 * 4 + 16;
+}
+
+template <typename T, int D, int W>
+__device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, char *s_mem) {
   constexpr bool F32 = std::is_same<T, float>::value;
   using M = Mma<T>;
   constexpr int KEYS = F32 ? 16 : 32;       // keys of a step
@@ -182,23 +219,21 @@ __global__ __launch_bounds__(W * 64) void paged_rows_kernel(const PagedAttendArg
   constexpr int CH = D / 8;                 // 16-bit: 16-byte chunks of a V row
   constexpr int VP = 2 * D + 32;            // 16-bit: LDS bytes of a V row
   constexpr int OP = D + 4;                 // floats of a row in the join
-  constexpr int kVBytes = F32 ? 0 : W * KEYS * VP, kOBytes = W * 16 * OP * 4;
-  __shared__ __attribute__((aligned(16))) char s_mem[kVBytes > kOBytes ? kVBytes : kOBytes];
-  __shared__ float s_m[W][16], s_l[W][16];
-  __shared__ int s_bad;
+  constexpr int kMl = rows_lds<T, D, W>() - 2 * W * 16 * 4 - 16;
+  float(*s_m)[16] = reinterpret_cast<float(*)[16]>(s_mem + kMl), (*s_l)[16] = s_m + W;
+  int &s_bad = *reinterpret_cast<int *>(s_mem + kMl + 2 * W * 16 * 4);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
   const int pairs = a.p.batch * a.kv_heads;
-  int block = blockIdx.x;
   const int pair = block % pairs;
   block /= pairs;
   const int part = block % a.max_parts, tile = block / a.max_parts;
   const int b = pair / a.kv_heads, hk = pair - b * a.kv_heads;
   const Rows seq = rows_of(a, b);
   const int rows = seq.count * a.group, row0 = tile * 16;
+  if (row0 >= rows || rows > a.few_rows) return;
   if (seq.cut && threadIdx.x == 0 && part == 0 && tile == 0) raise_status(a.status, HEXKV_STATUS_LENGTH_CLAMPED);
-  if (row0 >= rows) return;
   const int p0 = part * a.part;
   const int live = min(16, rows - row0);
   const int t_first = row0 / a.group, t_last = (row0 + live - 1) / a.group;
@@ -466,8 +501,7 @@ __global__ __launch_bounds__(W * 64) void paged_rows_kernel(const PagedAttendArg
     const int rlen = seq.keys(a, tt);
     if (part > 0 && rlen <= p0) continue;
     if (rlen <= a.part) {
-      if (rlen <= 0) o[n] = f32x4{};
-      else o[n] *= 1.f / sum[n];
+      o[n] *= weight_of(sum[n]);
       store4(static_cast<T *>(a.out) + (seq.first + tt) * a.o_stride + static_cast<int64_t>(hh) * D + 4 * c, o[n]);
     } else {
       const int64_t slot = ((static_cast<int64_t>(pair) * a.row_tiles + tile) * 16 + rr) * a.max_parts + part;
@@ -491,10 +525,292 @@ __global__ __launch_bounds__(W * 64) void paged_rows_kernel(const PagedAttendArg
 #pragma unroll
     for (int e = 0; e < DPL; ++e) {
       if (split) a.ws_o[slot * D + lane * DPL + e] = eo[e];
-      else out[e] = Elem<T>::from_float(rlen <= 0 ? 0.f : eo[e] / el);
+      else out[e] = Elem<T>::from_float(eo[e] * weight_of(el));
     }
     if (split && lane == 0) *reinterpret_cast<float2 *>(a.ws_ml + slot * 2) = float2{em, el};
   }
+}
+
+// ------------------------------------------------------------ tile path ---
+
+constexpr int kTileRows = 128, kTileKeys = 64;
+// A sequence of so many rows per KV head, or fewer, takes the row path.
+constexpr int kFewRows = 32;
+
+template <int D>
+struct TileLds {
+  static constexpr int KP = 2 * D + 16;  // bytes per K row: 16 rows' chunks over all banks
+  static constexpr int VP = 2 * D + 64;  // per V row: the 4 rows of a transposed read over all banks
+  static constexpr int kBytes = 2 * kTileKeys * (KP + VP) + 16;
+};
+
+// A wave, 32 rows, one per lane and half h:
+//   S^T = K Q^T: K (A) from LDS, Q (B) in registers; lane (c, h) gets row c's
+//   scores of keys 8 i + 4 h + e.
+//   O^T += V^T P^T: that layout is the B operand as it stands (the contraction
+//   index of a 16-key step is key 4 h + e, then 8 + 4 h + e), V^T (A) comes from
+//   row-major LDS by transposing reads in the same order.
+// All of a lane's accumulators belong to its own row.
+template <typename T, int D>
+__device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, char *s_mem) {
+  using M = Mma<T>;
+  using L = TileLds<D>;
+  constexpr int KT = kTileKeys, NKB = KT / 32;
+  constexpr int NJ = D / 16;   // score steps
+  constexpr int ND = D / 32;   // output blocks
+  constexpr int CH = D / 8;    // 16-byte chunks of a head's row
+  constexpr int CPT = KT * CH / 256, RPP = 256 / CH;  // chunks per thread; rows the workgroup loads at a time
+  constexpr int KP = L::KP, VP = L::VP;
+  char *s_k = s_mem, *s_v = s_mem + 2 * KT * KP;
+  int &s_bad = *reinterpret_cast<int *>(s_mem + 2 * KT * (KP + VP));
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, h = lane >> 5;
+  const int pairs = a.p.batch * a.kv_heads;
+  const int pair = block % pairs, rest = block / pairs;
+  const int part = rest % a.tile_parts, tile = a.tiles - 1 - rest / a.tile_parts;
+  const int b = pair / a.kv_heads, hk = pair - b * a.kv_heads;
+  const Rows seq = rows_of(a, b);
+  const int total = seq.count * a.group, row0 = tile * kTileRows;
+  if (total <= a.few_rows || row0 >= total) return;
+  const int p0 = part * a.tile_part;
+  const int t_last = (min(row0 + kTileRows, total) - 1) / a.group;
+  if (seq.cut && tid == 0 && part == 0 && tile == 0) raise_status(a.status, HEXKV_STATUS_LENGTH_CLAMPED);
+  const int end = min(seq.keys(a, t_last), p0 + a.tile_part);
+  if (part > 0 && end <= p0) return;
+
+  // This wave's rows and this lane's; rows past the last repeat it.  A wave
+  // without rows only stages.
+  const int wrow0 = row0 + wave * 32;
+  const bool idle = wrow0 >= total, live = wrow0 + c < total;
+  const int row = min(wrow0 + c, total - 1), t = row / a.group, qh = hk * a.group + row - t * a.group;
+  const int len = seq.keys(a, t), lim = min(len, p0 + a.tile_part);
+  const int w_end = idle ? p0 : min(seq.keys(a, (min(wrow0 + 32, total) - 1) / a.group), p0 + a.tile_part);
+  const int w_full = idle ? p0 : min(seq.keys(a, wrow0 / a.group), p0 + a.tile_part);
+  const T *q_row = static_cast<const T *>(a.q) + (seq.first + t) * a.q_stride + static_cast<int64_t>(qh) * D;
+  u32x4 qf[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) qf[j] = *reinterpret_cast<const u32x4 *>(q_row + h * 8 + j * 16);
+
+  const T *head = static_cast<const T *>(a.pages) + hk * a.p.head_stride;
+  const int32_t *table = a.p.tables + b * a.p.table_stride;
+  const int last = (max(end, 1) - 1) & ~15;
+  int bad_pages = 0;
+  // Thread tid moves chunk tid % CH of rows tid / CH + i * RPP; those of one
+  // wave lie in one block of 16 positions, and that in one page.
+  const int s_row = tid / CH, s_ch = tid % CH;
+  const int s_block = __builtin_amdgcn_readfirstlane(s_row >> 4);
+  auto place = [&](int k) {
+    const int at = min(k, last);
+    const int page = __builtin_amdgcn_readfirstlane(table[at >> a.p.shift]);
+    const bool in_pool = static_cast<unsigned>(page) < static_cast<unsigned>(a.p.n_pages);
+    bad_pages |= !in_pool;
+    return (in_pool ? page : 0) * a.p.page_stride + (at & ((1 << a.p.shift) - 1)) * a.p.pos_stride;
+  };
+  const int64_t lane_at = (s_row & 15) * a.p.pos_stride + 8 * s_ch;
+  u32x4 kr[CPT], vr[CPT];
+  int64_t at[CPT];
+  auto places = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) at[i] = place(k0 + i * RPP + 16 * s_block);
+  };
+  auto fetch = [&]() {
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      const T *x = head + at[i] + lane_at;
+      kr[i] = *reinterpret_cast<const u32x4 *>(x);
+      vr[i] = *reinterpret_cast<const u32x4 *>(x + a.p.kv_stride);
+    }
+  };
+  auto stage = [&](int buf, int k0) {
+    if (k0 + KT > end) {  // rows of the page not yet written give zeros
+#pragma unroll
+      for (int i = 0; i < CPT; ++i)
+        if (k0 + s_row + i * RPP >= end) vr[i] = u32x4{};
+    }
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      const int r = s_row + i * RPP;
+      *reinterpret_cast<u32x4 *>(s_k + (buf * KT + r) * KP + s_ch * 16) = kr[i];
+      *reinterpret_cast<u32x4 *>(s_v + (buf * KT + r) * VP + s_ch * 16) = vr[i];
+    }
+  };
+
+  float m = -INFINITY, l = 0.f;  // m: the running maximum less kShift
+  f32x16 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
+  const uint32_t k_read = static_cast<uint32_t>(c * KP + h * 16);
+  const int s16 = lane & 15;
+  const uint32_t v_read = static_cast<uint32_t>((4 * h + s16 / 4) * VP + ((lane >> 4) & 1) * 32 + (s16 % 4) * 8);
+  auto *shared_v = (__attribute__((address_space(3))) char *)s_v;
+
+  auto compute = [&](int buf, int k0, auto masked) {
+    constexpr bool MASK = decltype(masked)::value;
+    f32x16 s[NKB];
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) {
+      s[kb] = f32x16{};
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        s[kb] = M::mma32(*reinterpret_cast<const u32x4 *>(s_k + (buf * KT + kb * 32) * KP + k_read + j * 32), qf[j], s[kb]);
+    }
+    if constexpr (MASK) {
+      const int left = lim - k0 - 4 * h;
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = kb * 32 + 8 * (i / 4) + i % 4 < left ? s[kb][i] : -INFINITY;
+    }
+    float mt = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[kb][i]);
+    mt = xor_step<32>(mt, MaxOp{}) * a.scale_log2;
+    const bool up = mt > m + (M::kShift + M::kSlack);
+    if (__any(up)) {
+      const float mnew = up ? mt - M::kShift : m;
+      const float f = up ? exp2_of(m - mnew) : 1.f;
+      m = mnew;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+    }
+    const float base = m == -INFINITY ? 0.f : -m;
+    float l0 = 0.f, l1 = 0.f;
+    u32x4 p[2 * NKB];
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float e0 = exp2_of(fmaf(s[kb][i], a.scale_log2, base)), e1 = exp2_of(fmaf(s[kb][i + 1], a.scale_log2, base));
+        l0 += e0;
+        l1 += e1;
+        p[2 * kb + i / 8][i % 8 / 2] = M::pair(e0, e1);
+      }
+    l += l0 + l1;
+#pragma unroll
+    for (int ks = 0; ks < 2 * NKB; ++ks)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const uint32_t from = static_cast<uint32_t>((buf * KT + ks * 16) * VP + d * 64) + v_read;
+        const h4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_h4 *)(shared_v + from));
+        const h4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_h4 *)(shared_v + from + 8 * VP));
+        acc[d] = M::mma32(__builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7)), p[ks], acc[d]);
+      }
+  };
+
+  if (tid == 0) s_bad = 0;
+  if (end > p0) {
+    places(p0);
+    fetch();
+    places(p0 + KT);
+    stage(0, p0);
+    __syncthreads();
+    int buf = 0;
+    for (int k0 = p0; k0 < end; k0 += KT) {
+      const bool more = k0 + KT < end;
+      if (more) {
+        fetch();
+        places(k0 + 2 * KT);
+      }
+      if (k0 + KT <= w_full) compute(buf, k0, std::false_type{});
+      else if (k0 < w_end) compute(buf, k0, std::true_type{});
+      if (more) stage(buf ^ 1, k0 + KT);
+      buf ^= 1;
+      __syncthreads();
+    }
+  }
+  if (bad_pages && lane == 0) {
+    s_bad = 1;
+    raise_status(a.status, HEXKV_STATUS_PAGE);
+  }
+  __syncthreads();
+  if (idle) return;
+
+  l = xor_step<32>(l, AddOp{});
+  const bool holds = live && (part == 0 || lim > p0);  // this lane's row has something to write
+  float check = l * 0.f;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) check = fmaf(acc[d][i], 0.f, check);
+  // Decided for the row, over both lanes that hold its outputs, before either
+  // stores: out may be q, and exact_row reads the row's query again.
+  uint64_t redo = __ballot(holds && lim > p0 && (s_bad || !(check == 0.f)));
+  redo = (redo | redo >> 32) & 0xffffffffu;
+  const bool split = len > a.tile_part;
+  T *out = static_cast<T *>(a.out) + (seq.first + t) * a.o_stride + static_cast<int64_t>(qh) * D;
+  const int64_t slot = (static_cast<int64_t>(seq.first + t) * a.q_heads + qh) * a.tile_parts + part;
+  if (holds && !(redo >> c & 1)) {
+    if (!split) {
+      const float inv = weight_of(l);
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 o = {acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+          store4(out + d * 32 + i * 8 + 4 * h, len > 0 ? o * inv : f32x4{});
+        }
+    } else {
+      float *o = a.ws_tile_o + slot * D + 4 * h;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<f32x4 *>(o + d * 32 + i * 8) =
+              f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+      if (h == 0) *reinterpret_cast<float2 *>(a.ws_tile_ml + slot * 2) = float2{m, l};
+    }
+  }
+  while (redo) {
+    const int r = __builtin_ctzll(redo);
+    redo &= redo - 1;
+    constexpr int DPL = D / 64;
+    const int tr = __shfl(t, r), hr = __shfl(qh, r);
+    const bool row_split = __shfl(static_cast<int>(split), r);
+    float em, el, eo[DPL];
+    exact_row<T, D>(a, static_cast<const T *>(a.q) + (seq.first + tr) * a.q_stride + static_cast<int64_t>(hr) * D, b, hk, p0,
+                    __shfl(lim, r), &em, &el, eo);
+    const int64_t to = (static_cast<int64_t>(seq.first + tr) * a.q_heads + hr) * a.tile_parts + part;
+    T *row_out = static_cast<T *>(a.out) + (seq.first + tr) * a.o_stride + static_cast<int64_t>(hr) * D + lane * DPL;
+#pragma unroll
+    for (int e = 0; e < DPL; ++e) {
+      if (row_split) a.ws_tile_o[to * D + lane * DPL + e] = eo[e];
+      else row_out[e] = Elem<T>::from_float(eo[e] * weight_of(el));
+    }
+    if (row_split && lane == 0) *reinterpret_cast<float2 *>(a.ws_tile_ml + to * 2) = float2{em, el};
+  }
+}
+
+template <typename T, int D>
+constexpr bool has_tiles() {
+  return !std::is_same<T, float>::value && (D == 64 || D == 128);
+}
+
+template <typename T, int D, int W>
+__global__ __launch_bounds__(W * 64) void paged_rows_kernel(const PagedAttendArgs a) {
+  __shared__ __attribute__((aligned(16))) char s_mem[rows_lds<T, D, W>()];
+  rows_path<T, D, W>(a, blockIdx.x, s_mem);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedAttendArgs a) {
+  __shared__ __attribute__((aligned(16))) char s_mem[TileLds<D>::kBytes];
+  tile_path<T, D>(a, blockIdx.x, s_mem);
+}
+
+// A call that may hold sequences of either kind: tiles first (they take longest).
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void paged_mixed_kernel(const PagedAttendArgs a) {
+  constexpr int kRows = rows_lds<T, D, 4>(), kTiles = TileLds<D>::kBytes;
+  __shared__ __attribute__((aligned(16))) char s_mem[kRows > kTiles ? kRows : kTiles];
+  const int block = blockIdx.x;
+  if (block < a.tile_blocks) tile_path<T, D>(a, block, s_mem);
+  else rows_path<T, D, 4>(a, block - a.tile_blocks, s_mem);
 }
 
 // The partitions of a split row, joined: a wave a row.
@@ -502,38 +818,58 @@ constexpr int kJoinThreads = 256;
 constexpr int kMaxParts = 64;  // a lane each
 
 template <typename T, int D>
-__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAttendArgs a) {
+__device__ __forceinline__ void join_row(const float *o_parts, const float *ml_parts, int parts, T *out) {
   const int lane = threadIdx.x & 63;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / 64) + (threadIdx.x >> 6);
-  const int per = a.row_tiles * 16;
-  const int64_t pair = id / per;
-  if (pair >= static_cast<int64_t>(a.p.batch) * a.kv_heads) return;
-  const int row = static_cast<int>(id - pair * per);
-  const int b = static_cast<int>(pair / a.kv_heads), hk = static_cast<int>(pair - static_cast<int64_t>(b) * a.kv_heads);
-  const Rows seq = rows_of(a, b);
-  if (row >= seq.count * a.group) return;
-  const int t = row / a.group, qh = hk * a.group + row - t * a.group;
-  const int len = seq.keys(a, t);
-  if (len <= a.part) return;
-  const int parts = (len + a.part - 1) / a.part;
-  const int64_t slot = id * a.max_parts;
   float2 ml{-INFINITY, 0.f};
-  if (lane < parts) ml = *reinterpret_cast<const float2 *>(a.ws_ml + (slot + lane) * 2);
+  if (lane < parts) ml = *reinterpret_cast<const float2 *>(ml_parts + lane * 2);
   const float top = wave_max(ml.x);
   const float w = ml.x == -INFINITY ? 0.f : exp2_of(ml.x - top);
   const float sum = sum_from<1>(ml.y * w);
+  const float inv = weight_of(sum);
   constexpr int DPL = D >= 64 ? D / 64 : 1;
-  if (lane * DPL >= D) return;
   float o[DPL] = {};
-  const float *src = a.ws_o + slot * D + lane * DPL;
+  const float *src = o_parts + (D >= 64 ? lane * DPL : lane & (D - 1));
   for (int p = 0; p < parts; ++p) {
     const float wp = __shfl(w, p);
 #pragma unroll
-    for (int e = 0; e < DPL; ++e) o[e] = fmaf(src[static_cast<int64_t>(p) * D + e], wp, o[e]);
+    for (int e = 0; e < DPL; ++e) o[e] = fmaf(src[p * D + e], wp, o[e]);
   }
-  T *out = static_cast<T *>(a.out) + (seq.first + t) * a.o_stride + static_cast<int64_t>(qh) * D + lane * DPL;
+  if (lane * DPL >= D) return;
 #pragma unroll
-  for (int e = 0; e < DPL; ++e) out[e] = Elem<T>::from_float(o[e] / sum);
+  for (int e = 0; e < DPL; ++e) out[lane * DPL + e] = Elem<T>::from_float(o[e] * inv);
+}
+
+// Rows of the row path first, by pair and row, then those of the tile path,
+// by token and head.
+template <typename T, int D>
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAttendArgs a, int64_t few) {
+  int64_t id = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / 64) + (threadIdx.x >> 6);
+  if (id < few) {
+    const int per = a.row_tiles * 16, pair = static_cast<int>(id / per), row = static_cast<int>(id - static_cast<int64_t>(pair) * per);
+    const int b = pair / a.kv_heads, hk = pair - b * a.kv_heads;
+    const Rows seq = rows_of(a, b);
+    const int rows = seq.count * a.group;
+    if (row >= rows || rows > a.few_rows) return;
+    const int t = row / a.group, qh = hk * a.group + row - t * a.group, len = seq.keys(a, t);
+    if (len <= a.part) return;
+    const int64_t slot = id * a.max_parts;
+    join_row<T, D>(a.ws_o + slot * D, a.ws_ml + slot * 2, (len + a.part - 1) / a.part,
+                   static_cast<T *>(a.out) + (seq.first + t) * a.o_stride + static_cast<int64_t>(qh) * D);
+    return;
+  }
+  id -= few;
+  const int token = static_cast<int>(id / a.q_heads), qh = static_cast<int>(id - static_cast<int64_t>(token) * a.q_heads);
+  if (token >= a.p.tokens) return;
+  const int b = a.p.cu ? token_sequence(a.p, token) : token / a.p.each;
+  if (b < 0) return;
+  const Rows seq = rows_of(a, b);
+  const int t = token - seq.first;
+  if (t >= seq.count || seq.count * a.group <= a.few_rows) return;
+  const int len = seq.keys(a, t);
+  if (len <= a.tile_part) return;
+  const int64_t slot = id * a.tile_parts;
+  join_row<T, D>(a.ws_tile_o + slot * D, a.ws_tile_ml + slot * 2, (len + a.tile_part - 1) / a.tile_part,
+                 static_cast<T *>(a.out) + token * a.o_stride + static_cast<int64_t>(qh) * D);
 }
 
 // ------------------------------------------------------------------ host ---
@@ -572,43 +908,68 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   a->max_seqlen = p.max_seqlen;
   a->scale_log2 = p.softmax_scale * 1.44269504f;
   const int64_t rows = static_cast<int64_t>(a->max_tokens) * a->group, pairs = static_cast<int64_t>(p.seqs.batch) * a->kv_heads;
-  const int64_t tiles = (rows + 15) / 16;
-  if (rows > INT32_MAX || pairs * tiles >= INT64_C(1) << 24)
-    return fail(HEXKV_ERANGE, "%s: 2^24 tiles of rows or more", what);
-  a->row_tiles = static_cast<int32_t>(tiles);
-  int64_t part = p.partition;
-  if (!part) {
-    const int64_t want = pairs * tiles ? std::max<int64_t>(1, 768 / (pairs * tiles)) : 1;
-    part = std::max<int64_t>(256, round_up((p.max_seqlen + want - 1) / want, 64));
-  }
-  while ((p.max_seqlen + part - 1) / part > kMaxParts) part = round_up((p.max_seqlen + kMaxParts - 1) / kMaxParts, 64);
-  a->part = static_cast<int32_t>(part);
-  a->max_parts = static_cast<int32_t>(std::max<int64_t>(1, (p.max_seqlen + part - 1) / part));
-  if (pairs * tiles * a->max_parts >= INT64_C(1) << 24) return fail(HEXKV_ERANGE, "%s: 2^24 workgroups or more", what);
+  if (rows > INT32_MAX - kTileRows) return fail(HEXKV_ERANGE, "%s: 2^31 rows or more", what);
+  // Which paths can have work: without cu_tokens every sequence has as many rows.
+  const bool tiled = p.pool.dtype != HEXKV_F32 && (d == 64 || d == 128) && rows > kFewRows;
+  const bool few = !tiled || p.seqs.cu_tokens;
+  a->few_rows = tiled ? kFewRows : INT32_MAX;
+  a->row_tiles = few ? static_cast<int32_t>((std::min<int64_t>(rows, a->few_rows) + 15) / 16) : 0;
+  a->tiles = tiled ? static_cast<int32_t>((rows + kTileRows - 1) / kTileRows) : 0;
+  // Partitions, so that the workgroups of either path fill the CUs.
+  auto split = [&](int64_t blocks, int64_t want, int64_t least, int32_t *part, int32_t *parts) {
+    int64_t n = p.partition;
+    if (!n) {
+      const int64_t each = std::max<int64_t>(1, want / std::max<int64_t>(blocks, 1));
+      n = std::max(least, round_up((p.max_seqlen + each - 1) / each, 64));
+    }
+    if ((p.max_seqlen + n - 1) / n > kMaxParts) n = round_up((p.max_seqlen + kMaxParts - 1) / kMaxParts, 64);
+    *part = static_cast<int32_t>(std::min<int64_t>(n, 1 << 30));
+    *parts = static_cast<int32_t>(std::max<int64_t>(1, (p.max_seqlen + n - 1) / n));
+  };
+  split(pairs * a->row_tiles, 768, 256, &a->part, &a->max_parts);
+  const int64_t full = (tokens * a->group + kTileRows - 1) / kTileRows * a->kv_heads;  // tiles, if all were full
+  split(full, 512, 512, &a->tile_part, &a->tile_parts);
+  if (!few) a->max_parts = 1;
+  if (!tiled) a->tile_parts = 1;
+  const int64_t row_blocks = pairs * a->row_tiles * a->max_parts, tile_blocks = pairs * a->tiles * a->tile_parts;
+  if (row_blocks + tile_blocks >= INT64_C(1) << 24) return fail(HEXKV_ERANGE, "%s: 2^24 workgroups or more", what);
+  a->tile_blocks = static_cast<int32_t>(tile_blocks);
   return HEXKV_OK;
 }
 
+// Split rows of either path, each with its partitions' slots.
+static int64_t few_slots(const PagedAttendArgs &a) {
+  return a.max_parts > 1 ? static_cast<int64_t>(a.p.batch) * a.kv_heads * a.row_tiles * 16 * a.max_parts : 0;
+}
+static int64_t tile_slots(const PagedAttendArgs &a) {
+  return a.tile_parts > 1 ? static_cast<int64_t>(a.p.tokens) * a.q_heads * a.tile_parts : 0;
+}
+
 static size_t attend_workspace(const PagedAttendArgs &a, int head_dim) {
-  if (a.max_parts <= 1) return 0;
-  return static_cast<size_t>(a.p.batch) * a.kv_heads * a.row_tiles * 16 * a.max_parts * (head_dim + 2) * sizeof(float);
+  return static_cast<size_t>(few_slots(a) + tile_slots(a)) * (head_dim + 2) * sizeof(float);
 }
 
 template <typename T, int D>
-static void launch_rows(const PagedAttendArgs &a, hipStream_t s) {
-  const int64_t rows = static_cast<int64_t>(a.p.batch) * a.kv_heads * a.row_tiles;
-  constexpr int W = 4;
-  paged_rows_kernel<T, D, W><<<dim3(static_cast<unsigned>(rows * a.max_parts)), W * 64, 0, s>>>(a);
-  if (a.max_parts > 1) paged_join_kernel<T, D><<<dim3(static_cast<unsigned>(rows * 4)), kJoinThreads, 0, s>>>(a);
+static void launch_attend(const PagedAttendArgs &a, hipStream_t s) {
+  const unsigned rows = static_cast<unsigned>(static_cast<int64_t>(a.p.batch) * a.kv_heads * a.row_tiles * a.max_parts);
+  const unsigned tiles = static_cast<unsigned>(a.tile_blocks);
+  if constexpr (has_tiles<T, D>()) {
+    if (rows && tiles) paged_mixed_kernel<T, D><<<dim3(rows + tiles), 256, 0, s>>>(a);
+    else if (tiles) paged_tile_kernel<T, D><<<dim3(tiles), 256, 0, s>>>(a);
+  }
+  if (!tiles) paged_rows_kernel<T, D, 4><<<dim3(rows), 256, 0, s>>>(a);
+  const int64_t few = a.max_parts > 1 ? few_slots(a) / a.max_parts : 0, tile = a.tile_parts > 1 ? tile_slots(a) / a.tile_parts : 0;
+  if (few + tile) paged_join_kernel<T, D><<<dim3(static_cast<unsigned>((few + tile + 3) / 4)), kJoinThreads, 0, s>>>(a, few);
 }
 
 template <typename T>
 static void launch_dims(const PagedAttendArgs &a, int head_dim, hipStream_t s) {
   switch (head_dim) {
-    case 16: launch_rows<T, 16>(a, s); break;
-    case 32: launch_rows<T, 32>(a, s); break;
-    case 64: launch_rows<T, 64>(a, s); break;
-    case 128: launch_rows<T, 128>(a, s); break;
-    default: launch_rows<T, 256>(a, s); break;
+    case 16: launch_attend<T, 16>(a, s); break;
+    case 32: launch_attend<T, 32>(a, s); break;
+    case 64: launch_attend<T, 64>(a, s); break;
+    case 128: launch_attend<T, 128>(a, s); break;
+    default: launch_attend<T, 256>(a, s); break;
   }
 }
 
@@ -637,8 +998,15 @@ extern "C" int hexkv_paged_attend(const hexkv_paged_attend_params *params, void 
   const size_t need = attend_workspace(a, d);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(HEXKV_EWORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", what, need, workspace_bytes);
-  a.ws_o = static_cast<float *>(workspace);
-  a.ws_ml = need ? a.ws_o + static_cast<int64_t>(a.p.batch) * a.kv_heads * a.row_tiles * 16 * a.max_parts * d : nullptr;
+  if (need) {
+    const int64_t few = few_slots(a), tile = tile_slots(a);
+    a.ws_o = static_cast<float *>(workspace);
+    a.ws_tile_o = a.ws_o + few * d;
+    a.ws_ml = a.ws_tile_o + tile * d;
+    a.ws_tile_ml = a.ws_ml + few * 2;
+  } else {
+    a.ws_o = a.ws_ml = a.ws_tile_o = a.ws_tile_ml = nullptr;
+  }
   rc = status_word(stream, &a.status, what);
   if (rc != HEXKV_OK) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -851,7 +851,7 @@ typedef struct hexkv_paged_attend_params {
  * own (already appended) included: decode rows, chunks of prompts and both in
  * one call.  A sequence with more than max_tokens tokens or max_seqlen rows is
  * cut to them and flagged HEXKV_STATUS_LENGTH_CLAMPED.  A row that attends
- * nothing is zero.
+ * nothing, or only scores of -infinity, is zero.
  */
 int hexkv_paged_attend(const hexkv_paged_attend_params *params, void *workspace, size_t workspace_bytes,
                        hexkv_stream_t stream);
