@@ -41,10 +41,11 @@ struct PagedAttendArgs {
   int32_t max_tokens, max_seqlen;
   float scale_log2;
   int32_t few_rows;         // a sequence's rows per KV head up to which it takes the row path
-  // row path: 16-row tiles of a sequence and KV head, keys per partition,
-  // partitions of the longest row
-  int32_t row_tiles, part, max_parts;
-  // tile path: the same for tiles of 128 rows, and its workgroups
+  // row path: 16-row tiles of a sequence and KV head (at most), keys per partition,
+  // partitions of the longest row, workgroups
+  int32_t row_tiles, part, max_parts, row_blocks;
+  // tile path: a bound on the tiles of all sequences, keys per partition and
+  // partitions, and workgroups
   int32_t tiles, tile_part, tile_parts, tile_blocks;
   // split rows: [pair][row][max_parts] and [token][head][tile_parts] of D sums, and of
   // (maximum, sum)
@@ -81,6 +82,55 @@ __device__ __forceinline__ Rows rows_of(const PagedAttendArgs &a, int b) {
   r.total = static_cast<int>(min(all, static_cast<int64_t>(a.max_seqlen)));
   r.cut = s.count > a.max_tokens || all > a.max_seqlen;
   return r;
+}
+
+// Workgroups of either path are numbered by (tile, partition, KV head), the
+// head fastest; a tile is one of those of all sequences, which the host bounds by
+// the tokens' number: a launch over (sequence, most tiles) of 2 chunks beside 46 single tokens
+// was 17000 workgroups, 200 us of them leaving at once.
+struct Place {
+  int b, tile, part, hk;
+};
+
+// The sequence that has the index-th of all tiles, and which of its own that is
+// (b -1: none).  tiles(count): those of a sequence of so many tokens.
+template <typename F>
+__device__ __forceinline__ Place place_of(const PagedAttendArgs &a, int block, int parts, int reversed_from, F tiles) {
+  Place p;
+  const int rest = block / a.kv_heads;
+  p.hk = block - rest * a.kv_heads;
+  p.part = rest % parts;
+  int index = rest / parts;
+  if (reversed_from) index = reversed_from - 1 - index;
+  if (!a.p.cu) {
+    const int each = tiles(a.max_tokens);
+    p.b = each ? index / each : a.p.batch;
+    p.tile = index - p.b * each;
+    if (p.b >= a.p.batch) p.b = -1;
+    return p;
+  }
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < a.p.batch; b0 += 64) {
+    const int b = b0 + lane;
+    const int n = b < a.p.batch ? tiles(min(sequence_of(a.p, b).count, a.max_tokens)) : 0;
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int x = __shfl_up(upto, d);
+      if (lane >= d) upto += x;
+    }
+    const uint64_t past = __ballot(upto > index);
+    if (past) {
+      const int j = __builtin_ctzll(past);
+      p.b = __builtin_amdgcn_readfirstlane(b0 + j);
+      p.tile = __builtin_amdgcn_readfirstlane(index - __shfl(upto - n, j));
+      return p;
+    }
+    index -= __shfl(upto, 63);
+  }
+  p.b = -1;
+  p.tile = 0;
+  return p;
 }
 
 // The matrix products of one type.  A probability is held at 2^kShift of the
@@ -225,14 +275,14 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int pairs = a.p.batch * a.kv_heads;
-  const int pair = block % pairs;
-  block /= pairs;
-  const int part = block % a.max_parts, tile = block / a.max_parts;
-  const int b = pair / a.kv_heads, hk = pair - b * a.kv_heads;
+  const Place mine = place_of(a, block, a.max_parts, 0, [&](int count) {
+    return count * a.group <= a.few_rows ? (count * a.group + 15) / 16 : 0;
+  });
+  const int b = mine.b, hk = mine.hk, part = mine.part, tile = mine.tile;
+  if (b < 0) return;
+  const int pair = b * a.kv_heads + hk;
   const Rows seq = rows_of(a, b);
   const int rows = seq.count * a.group, row0 = tile * 16;
-  if (row0 >= rows || rows > a.few_rows) return;
   if (seq.cut && threadIdx.x == 0 && part == 0 && tile == 0) raise_status(a.status, HEXKV_STATUS_LENGTH_CLAMPED);
   const int p0 = part * a.part;
   const int live = min(16, rows - row0);
@@ -566,13 +616,14 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
-  const int pairs = a.p.batch * a.kv_heads;
-  const int pair = block % pairs, rest = block / pairs;
-  const int part = rest % a.tile_parts, tile = a.tiles - 1 - rest / a.tile_parts;
-  const int b = pair / a.kv_heads, hk = pair - b * a.kv_heads;
+  // (the last tiles first: theirs are the most keys)
+  const Place mine = place_of(a, block, a.tile_parts, a.tiles, [&](int count) {
+    return count * a.group > a.few_rows ? (count * a.group + kTileRows - 1) / kTileRows : 0;
+  });
+  const int b = mine.b, hk = mine.hk, part = mine.part, tile = mine.tile;
+  if (b < 0) return;
   const Rows seq = rows_of(a, b);
   const int total = seq.count * a.group, row0 = tile * kTileRows;
-  if (total <= a.few_rows || row0 >= total) return;
   const int p0 = part * a.tile_part;
   const int t_last = (min(row0 + kTileRows, total) - 1) / a.group;
   if (seq.cut && tid == 0 && part == 0 && tile == 0) raise_status(a.status, HEXKV_STATUS_LENGTH_CLAMPED);
@@ -907,14 +958,21 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   a->max_tokens = p.seqs.cu_tokens ? std::min(p.max_tokens, p.seqs.tokens) : a->p.each;
   a->max_seqlen = p.max_seqlen;
   a->scale_log2 = p.softmax_scale * 1.44269504f;
-  const int64_t rows = static_cast<int64_t>(a->max_tokens) * a->group, pairs = static_cast<int64_t>(p.seqs.batch) * a->kv_heads;
+  const int64_t rows = static_cast<int64_t>(a->max_tokens) * a->group;
   if (rows > INT32_MAX - kTileRows) return fail(HEXKV_ERANGE, "%s: 2^31 rows or more", what);
   // Which paths can have work: without cu_tokens every sequence has as many rows.
   const bool tiled = p.pool.dtype != HEXKV_F32 && (d == 64 || d == 128) && rows > kFewRows;
   const bool few = !tiled || p.seqs.cu_tokens;
   a->few_rows = tiled ? kFewRows : INT32_MAX;
   a->row_tiles = few ? static_cast<int32_t>((std::min<int64_t>(rows, a->few_rows) + 15) / 16) : 0;
-  a->tiles = tiled ? static_cast<int32_t>((rows + kTileRows - 1) / kTileRows) : 0;
+  // Tiles of all sequences: without cu_tokens as they are, else at most one a
+  // sequence more than full ones, of sequences with enough rows to have any.
+  const int64_t batch = p.seqs.batch, all_rows = tokens * a->group;
+  int64_t few_tiles = batch * a->row_tiles, tiles = tiled ? batch * ((rows + kTileRows - 1) / kTileRows) : 0;
+  if (p.seqs.cu_tokens) {
+    few_tiles = std::min(few_tiles, all_rows / 16 + std::min<int64_t>(batch, tokens));
+    tiles = std::min(tiles, all_rows / kTileRows + std::min<int64_t>(batch, all_rows / (kFewRows + 1)));
+  }
   // Partitions, so that the workgroups of either path fill the CUs.
   auto split = [&](int64_t blocks, int64_t want, int64_t least, int32_t *part, int32_t *parts) {
     int64_t n = p.partition;
@@ -926,13 +984,14 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
     *part = static_cast<int32_t>(std::min<int64_t>(n, 1 << 30));
     *parts = static_cast<int32_t>(std::max<int64_t>(1, (p.max_seqlen + n - 1) / n));
   };
-  split(pairs * a->row_tiles, 768, 256, &a->part, &a->max_parts);
-  const int64_t full = (tokens * a->group + kTileRows - 1) / kTileRows * a->kv_heads;  // tiles, if all were full
-  split(full, 512, 512, &a->tile_part, &a->tile_parts);
+  split(few_tiles * a->kv_heads, 768, 256, &a->part, &a->max_parts);
+  split((all_rows + kTileRows - 1) / kTileRows * a->kv_heads, 512, 512, &a->tile_part, &a->tile_parts);
   if (!few) a->max_parts = 1;
   if (!tiled) a->tile_parts = 1;
-  const int64_t row_blocks = pairs * a->row_tiles * a->max_parts, tile_blocks = pairs * a->tiles * a->tile_parts;
+  const int64_t row_blocks = few_tiles * a->kv_heads * a->max_parts, tile_blocks = tiles * a->kv_heads * a->tile_parts;
   if (row_blocks + tile_blocks >= INT64_C(1) << 24) return fail(HEXKV_ERANGE, "%s: 2^24 workgroups or more", what);
+  a->row_blocks = static_cast<int32_t>(row_blocks);
+  a->tiles = static_cast<int32_t>(tiles);
   a->tile_blocks = static_cast<int32_t>(tile_blocks);
   return HEXKV_OK;
 }
@@ -951,7 +1010,7 @@ static size_t attend_workspace(const PagedAttendArgs &a, int head_dim) {
 
 template <typename T, int D>
 static void launch_attend(const PagedAttendArgs &a, hipStream_t s) {
-  const unsigned rows = static_cast<unsigned>(static_cast<int64_t>(a.p.batch) * a.kv_heads * a.row_tiles * a.max_parts);
+  const unsigned rows = static_cast<unsigned>(a.row_blocks);
   const unsigned tiles = static_cast<unsigned>(a.tile_blocks);
   if constexpr (has_tiles<T, D>()) {
     if (rows && tiles) paged_mixed_kernel<T, D><<<dim3(rows + tiles), 256, 0, s>>>(a);
