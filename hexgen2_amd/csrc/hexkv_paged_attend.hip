@@ -4,14 +4,17 @@
 // a KV head (tokens x group of them, in (token, head) order) read the same keys.
 //
 // Row path: 16 rows a workgroup, its waves taking steps of the keys in turn.
-//   S^T = K Q^T    16 keys x 16 rows a matrix instruction; K's operand is
-//                  loaded as it lies: lane (r, g) holds key r, dims of chunk g
+//   S^T = K Q^T    16 keys x 16 rows a matrix instruction: lane (r, g) holds key
+//                  r, dims of chunk g
 //   softmax        a lane's scores are all its own row's; the other 3 lanes
 //                  of a row are two exchanges away
 //   O^T += V^T P^T the scores' layout is P's operand as it stands, with the contraction
 //                  index of a step being key 4 g + i (16-bit: then 16 + 4 g + i);
-//                  16-bit V goes through the wave's own LDS, row-major in and
-//                  transposed out, fp32 V is loaded in place
+//                  V^T is read transposed from LDS, fp32 V loaded in place
+// 16-bit rows are loaded whole, 16 lanes a row, and pass through the wave's own
+// LDS (K, then V in the same place): loaded as K's operand takes it, in 64 bytes of
+// each of 16 rows, a line was asked for twice, and the loads could not be
+// nontemporal (Llama-3-8B decode batch 211 us, 224 nontemporal, against XXX).
 // What bounds it: a decode row's K and V are read once, 4 D flops a key, so
 // memory.  Steps are loaded one ahead into registers, page numbers two ahead.
 //
@@ -131,6 +134,30 @@ __device__ __forceinline__ Place place_of(const PagedAttendArgs &a, int block, i
   p.b = -1;
   p.tile = 0;
   return p;
+}
+
+// A sequence's table, read by scalar loads: a wave's lanes need the same page,
+// and a vector load's number would be waited for behind the rows loaded before it
+// (Llama-3-8B decode batch 217 us instead of XXX).
+typedef const __attribute__((address_space(4))) int32_t *ScalarTable;
+
+__device__ __forceinline__ ScalarTable scalar_table(const PagedAttendArgs &a, int b) {
+  return (ScalarTable)(a.p.tables + __builtin_amdgcn_readfirstlane(b) * a.p.table_stride);
+}
+
+// 16 rows of one head in a page, as a buffer that ends behind the last row that
+// holds a key: rows past it (those of the page not yet written) and every row of
+// a page outside the pool read as zeros, and blocks past the end, which the
+// loads made ahead ask for, cost nothing.  (Addressed as memory the last block
+// was loaded again in their place: 512 keys of a partition moved 25% more.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t block_of(const char *at, int rows, uint32_t pos_bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(at), 0,
+                                           __builtin_amdgcn_readfirstlane(max(0, min(rows, 16)) * pos_bytes), 0x00027000);
+}
+constexpr int kNontemporal = 2;  // a buffer load's cache policy
+template <int POLICY>
+__device__ __forceinline__ u32x4 load_16(__amdgpu_buffer_rsrc_t block, uint32_t offset) {
+  return __builtin_amdgcn_raw_buffer_load_b128(block, offset, 0, POLICY);
 }
 
 // The matrix products of one type.  A probability is held at 2^kShift of the
@@ -262,12 +289,13 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
   constexpr int KEYS = F32 ? 16 : 32;       // keys of a step
   constexpr int NT = KEYS / 16;             // 16-key blocks of a step
   constexpr int NK = F32 ? D / 16 : (D >= 32 ? D / 32 : 1);  // K vectors of a lane and block
-  constexpr int NV = D / 16;                // 16-bit: V vectors of a lane and step
+  constexpr int NV = D >= 32 ? D / 16 : 2;  // 16-bit: vectors of a lane, of a step's K or V
   constexpr int VW = D >= 64 ? 4 : D / 16;  // fp32: V elements of a load
   constexpr int NB = D / (16 * VW);         // fp32: loads of a V row
   constexpr int ND = D / 16;                // output blocks
   constexpr int CH = D / 8;                 // 16-bit: 16-byte chunks of a V row
-  constexpr int VP = 2 * D + 32;            // 16-bit: LDS bytes of a V row
+  constexpr int KP = 2 * D + 16;            // 16-bit: LDS bytes of a K row: 16 rows' chunks over all banks
+  constexpr int VP = 2 * D + 32;            // of a V row: the 16 rows of a transposed read in two passes
   constexpr int OP = D + 4;                 // floats of a row in the join
   constexpr int kMl = rows_lds<T, D, W>() - 2 * W * 16 * 4 - 16;
   float(*s_m)[16] = reinterpret_cast<float(*)[16]>(s_mem + kMl), (*s_l)[16] = s_m + W;
@@ -303,45 +331,63 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
     else qf[j] = g < 2 ? *reinterpret_cast<const u32x4 *>(q_row + 8 * g) : u32x4{};
   }
 
-  const T *head = static_cast<const T *>(a.pages) + hk * a.p.head_stride;
-  const int32_t *table = a.p.tables + b * a.p.table_stride;
+  // (addresses: a uniform base and a lane's 32-bit offset inside a block)
+  constexpr int ES = static_cast<int>(sizeof(T));
+  const char *head = static_cast<const char *>(a.pages) + hk * a.p.head_stride * ES;
+  const ScalarTable table = scalar_table(a, b);
   const int last = (max(end, 1) - 1) & ~15;
+  const uint32_t pos_bytes = static_cast<uint32_t>(a.p.pos_stride * ES);
+  const int64_t kv_bytes = a.p.kv_stride * ES;
   unsigned bad_pages = 0;
 
-  // Where the 16-key block at position k lies (blocks past the end: the last one's place).
-  auto place = [&](int k, bool *in_pool) {
-    const int at = min(k, last);
-    const int page = __builtin_amdgcn_readfirstlane(table[at >> a.p.shift]);
-    *in_pool = static_cast<unsigned>(page) < static_cast<unsigned>(a.p.n_pages);
-    return (*in_pool ? page : 0) * a.p.page_stride + (at & ((1 << a.p.shift) - 1)) * a.p.pos_stride;
+  // The page of the 16-key block at position k, and the block.
+  struct Block {
+    __amdgpu_buffer_rsrc_t k, v;
+    bool in_pool;
   };
-  const int64_t k_lane = F32 ? r * a.p.pos_stride + 4 * g : r * a.p.pos_stride + (D >= 32 ? 8 * g : 8 * (g & 1));
-  auto load_k = [&](u32x4 (&k)[NT][NK], const int64_t *at) {
-#pragma unroll
-    for (int kt = 0; kt < NT; ++kt)
-#pragma unroll
-      for (int j = 0; j < NK; ++j)
-        k[kt][j] = *reinterpret_cast<const u32x4 *>(head + at[kt] + k_lane + (F32 ? 16 : 32) * j);
+  auto page_of = [&](int k) { return table[min(k, last) >> a.p.shift]; };
+  auto block_at = [&](int k, int page) {
+    Block x;
+    x.in_pool = static_cast<unsigned>(page) < static_cast<unsigned>(a.p.n_pages);
+    const char *at = head + ((x.in_pool ? page : 0) * a.p.page_stride + (min(k, last) & ((1 << a.p.shift) - 1)) * a.p.pos_stride) * ES;
+    x.k = block_of(at, x.in_pool ? end - k : 0, pos_bytes);
+    x.v = block_of(at + kv_bytes, x.in_pool ? end - k : 0, pos_bytes);
+    return x;
   };
-  // 16-bit: lane l loads chunk l % CH of row l / CH + i * 64 / CH.
+  // 16-bit: lane l loads chunk l % CH of row l / CH + i * RPL, so that a load takes
+  // whole rows, which nothing else reads (head_dim 16: by half of the lanes).
+  constexpr int RPL = D >= 32 ? 64 / CH : 16;  // rows of a load
   const int v_row = lane / CH, v_ch = lane % CH;
-  auto load_v16 = [&](u32x4 (&v)[NV], const int64_t *at) {
+  const bool loads = v_row < RPL;
+  auto load16 = [&](u32x4 (&v)[NV], const Block *at, bool values) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int kk = v_row + i * (64 / CH);
-      const int64_t base = D == 16 ? (kk < 16 ? at[0] : at[NT - 1]) : at[(i * (64 / CH)) / 16];
-      v[i] = *reinterpret_cast<const u32x4 *>(head + base + a.p.kv_stride + (kk & 15) * a.p.pos_stride + 8 * v_ch);
+      const uint32_t off = ((v_row + i * RPL) & 15) * pos_bytes + 16 * v_ch;
+      v[i] = load_16<kNontemporal>(values ? at[i * RPL / 16].v : at[i * RPL / 16].k, loads ? off : ~0u);
     }
+  };
+  auto store16 = [&](const u32x4 (&v)[NV], char *to, int pitch) {
+    if (!loads) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) *reinterpret_cast<u32x4 *>(to + (v_row + i * RPL) * pitch + v_ch * 16) = v[i];
+  };
+  const uint32_t k_lane = r * pos_bytes + 16 * g;
+  auto load_k32 = [&](u32x4 (&k)[NK], const Block &at) {
+#pragma unroll
+    for (int j = 0; j < NK; ++j) k[j] = load_16<0>(at.k, k_lane + 64 * j);
   };
   // fp32: lane (r, g) loads dims VW r of key 4 g + i.
   typedef float vw __attribute__((ext_vector_type(VW)));
-  auto load_v32 = [&](vw (&v)[4][NB], const int64_t *at) {
+  auto load_v32 = [&](vw (&v)[4][NB], const Block &at) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
-        v[i][n] = *reinterpret_cast<const vw *>(reinterpret_cast<const float *>(head) + at[0] + a.p.kv_stride +
-                                                (4 * g + i) * a.p.pos_stride + n * 16 * VW + VW * r);
+      for (int n = 0; n < NB; ++n) {
+        const uint32_t off = (4 * g + i) * pos_bytes + 4 * (n * 16 * VW + VW * r);
+        if constexpr (VW == 4) v[i][n] = __builtin_bit_cast(vw, load_16<0>(at.v, off));
+        else if constexpr (VW == 2) v[i][n] = __builtin_bit_cast(vw, __builtin_amdgcn_raw_buffer_load_b64(at.v, off, 0, 0));
+        else v[i][n] = vw{__uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(at.v, off, 0, 0))};
+      }
   };
 
   float m = -INFINITY, l = 0.f;  // m: the running maximum less kShift
@@ -352,48 +398,56 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
   constexpr int STRIDE = W * KEYS;
   int k0 = p0 + wave * KEYS;
   if (k0 < end) {
-    u32x4 kf[NT][NK];
-    u32x4 v16[F32 ? 1 : NV];
+    u32x4 k32[F32 ? NK : 1];
+    u32x4 k16[F32 ? 1 : NV], v16[F32 ? 1 : NV];
     vw v32[F32 ? 4 : 1][F32 ? NB : 1];
-    int64_t at[NT], at_next[NT];
-    bool in[NT], in_next[NT];
+    Block at[NT];
+    bool in[NT];
+    int page[NT];
 #pragma unroll
-    for (int kt = 0; kt < NT; ++kt) at[kt] = place(k0 + 16 * kt, &in[kt]);
-    load_k(kf, at);
-    if constexpr (F32) load_v32(v32, at);
-    else load_v16(v16, at);
+    for (int kt = 0; kt < NT; ++kt) {
+      at[kt] = block_at(k0 + 16 * kt, page_of(k0 + 16 * kt));
+      in[kt] = at[kt].in_pool;
+    }
+    if constexpr (F32) load_k32(k32, at[0]);
+    else load16(k16, at, false);
+    __builtin_amdgcn_sched_barrier(0);  // (in this order here, too: the loop waits for K alone)
+    if constexpr (F32) load_v32(v32, at[0]);
+    else load16(v16, at, true);
 #pragma unroll
-    for (int kt = 0; kt < NT; ++kt) at_next[kt] = place(k0 + STRIDE + 16 * kt, &in_next[kt]);
+    for (int kt = 0; kt < NT; ++kt) page[kt] = page_of(k0 + STRIDE + 16 * kt);
     char *s_v = s_mem + wave * KEYS * VP;
     for (; k0 < end; k0 += STRIDE) {
-      f32x4 s[NT];
 #pragma unroll
       for (int kt = 0; kt < NT; ++kt) {
-        s[kt] = f32x4{};
-#pragma unroll
-        for (int j = 0; j < NK; ++j) {
-          if constexpr (F32) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              s[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[kt][j][e]), __uint_as_float(qf[j][e]), s[kt], 0, 0, 0);
-          } else {
-            u32x4 kv = kf[kt][j];
-            if constexpr (D == 16) kv = g < 2 ? kv : u32x4{};
-            s[kt] = M::mma(kv, qf[j], s[kt]);
-          }
-        }
+        at[kt] = block_at(k0 + STRIDE + 16 * kt, page[kt]);
+        page[kt] = page_of(k0 + 2 * STRIDE + 16 * kt);
       }
-      load_k(kf, at_next);
+      f32x4 s[NT];
+#pragma unroll
+      for (int kt = 0; kt < NT; ++kt) s[kt] = f32x4{};
+      if constexpr (F32) {
+#pragma unroll
+        for (int j = 0; j < NK; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k32[j][e]), __uint_as_float(qf[j][e]), s[0], 0, 0, 0);
+        load_k32(k32, at[0]);
+      } else {
+        store16(k16, s_v, KP);
+        load16(k16, at, false);
+#pragma unroll
+        for (int j = 0; j < NK; ++j)
+#pragma unroll
+          for (int kt = 0; kt < NT; ++kt) {
+            u32x4 k = *reinterpret_cast<const u32x4 *>(s_v + (16 * kt + r) * KP + (D >= 32 ? 64 * j + 16 * g : 16 * (g & 1)));
+            if constexpr (D == 16) k = g < 2 ? k : u32x4{};
+            s[kt] = M::mma(k, qf[j], s[kt]);
+          }
+      }
       bool masked = k0 + KEYS > full;
 #pragma unroll
       for (int kt = 0; kt < NT; ++kt) masked |= !in[kt];
-      vw vf[F32 ? 4 : 1][F32 ? NB : 1];
-      if constexpr (F32) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int n = 0; n < NB; ++n) vf[i][n] = v32[i][n];
-      }
       if (masked) {
         const int left = lim - k0;
 #pragma unroll
@@ -402,35 +456,20 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[kt][i] = in[kt] && 16 * kt + 4 * g + i < left ? s[kt][i] : -INFINITY;
         }
-        // keys that no row of the tile attends (rows of the page not yet
-        // written, pages outside the pool) give zeros
-        if constexpr (F32) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-              if (!in[0] || k0 + 4 * g + i >= end) vf[i][n] = vw{};
-        } else {
-#pragma unroll
-          for (int i = 0; i < NV; ++i) {
-            const int kk = v_row + i * (64 / CH);
-            if (k0 + kk >= end || !(kk < 16 ? in[0] : in[NT - 1])) v16[i] = u32x4{};
-          }
-        }
       }
+      vw vf[F32 ? 4 : 1][F32 ? NB : 1];
       if constexpr (F32) {
-        load_v32(v32, at_next);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int n = 0; n < NB; ++n) vf[i][n] = v32[i][n];
+        load_v32(v32, at[0]);
       } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          *reinterpret_cast<u32x4 *>(s_v + (v_row + i * (64 / CH)) * VP + v_ch * 16) = v16[i];
-        load_v16(v16, at_next);
+        store16(v16, s_v, VP);
+        load16(v16, at, true);
       }
 #pragma unroll
-      for (int kt = 0; kt < NT; ++kt) {
-        in[kt] = in_next[kt];
-        at_next[kt] = place(k0 + 2 * STRIDE + 16 * kt, &in_next[kt]);
-      }
+      for (int kt = 0; kt < NT; ++kt) in[kt] = at[kt].in_pool;
 
       float mt = s[0][0];
 #pragma unroll
@@ -643,42 +682,35 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
 #pragma unroll
   for (int j = 0; j < NJ; ++j) qf[j] = *reinterpret_cast<const u32x4 *>(q_row + h * 8 + j * 16);
 
-  const T *head = static_cast<const T *>(a.pages) + hk * a.p.head_stride;
-  const int32_t *table = a.p.tables + b * a.p.table_stride;
+  constexpr int ES = static_cast<int>(sizeof(T));
+  const char *head = static_cast<const char *>(a.pages) + hk * a.p.head_stride * ES;
+  const int64_t kv_bytes = a.p.kv_stride * ES;
+  const ScalarTable table = scalar_table(a, b);
   const int last = (max(end, 1) - 1) & ~15;
   int bad_pages = 0;
   // Thread tid moves chunk tid % CH of rows tid / CH + i * RPP; those of one
   // wave lie in one block of 16 positions, and that in one page.
   const int s_row = tid / CH, s_ch = tid % CH;
   const int s_block = __builtin_amdgcn_readfirstlane(s_row >> 4);
-  auto place = [&](int k) {
-    const int at = min(k, last);
-    const int page = __builtin_amdgcn_readfirstlane(table[at >> a.p.shift]);
-    const bool in_pool = static_cast<unsigned>(page) < static_cast<unsigned>(a.p.n_pages);
-    bad_pages |= !in_pool;
-    return (in_pool ? page : 0) * a.p.page_stride + (at & ((1 << a.p.shift) - 1)) * a.p.pos_stride;
-  };
-  const int64_t lane_at = (s_row & 15) * a.p.pos_stride + 8 * s_ch;
+  const uint32_t pos_bytes = static_cast<uint32_t>(a.p.pos_stride * ES), lane_at = (s_row & 15) * pos_bytes + 16 * s_ch;
   u32x4 kr[CPT], vr[CPT];
-  int64_t at[CPT];
-  auto places = [&](int k0) {
+  int page[CPT];
+  auto find = [&](int k0) {
 #pragma unroll
-    for (int i = 0; i < CPT; ++i) at[i] = place(k0 + i * RPP + 16 * s_block);
+    for (int i = 0; i < CPT; ++i) page[i] = table[min(k0 + i * RPP + 16 * s_block, last) >> a.p.shift];
   };
-  auto fetch = [&]() {
+  auto fetch = [&](int k0) {
 #pragma unroll
     for (int i = 0; i < CPT; ++i) {
-      const T *x = head + at[i] + lane_at;
-      kr[i] = *reinterpret_cast<const u32x4 *>(x);
-      vr[i] = *reinterpret_cast<const u32x4 *>(x + a.p.kv_stride);
+      const bool in_pool = static_cast<unsigned>(page[i]) < static_cast<unsigned>(a.p.n_pages);
+      const int k = k0 + i * RPP + 16 * s_block;
+      bad_pages |= !in_pool && k < end;
+      const char *at = head + ((in_pool ? page[i] : 0) * a.p.page_stride + (k & ((1 << a.p.shift) - 1)) * a.p.pos_stride) * ES;
+      kr[i] = load_16<0>(block_of(at, end - k, pos_bytes), lane_at);
+      vr[i] = load_16<0>(block_of(at + kv_bytes, end - k, pos_bytes), lane_at);
     }
   };
-  auto stage = [&](int buf, int k0) {
-    if (k0 + KT > end) {  // rows of the page not yet written give zeros
-#pragma unroll
-      for (int i = 0; i < CPT; ++i)
-        if (k0 + s_row + i * RPP >= end) vr[i] = u32x4{};
-    }
+  auto stage = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < CPT; ++i) {
       const int r = s_row + i * RPP;
@@ -696,17 +728,16 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
   const uint32_t v_read = static_cast<uint32_t>((4 * h + s16 / 4) * VP + ((lane >> 4) & 1) * 32 + (s16 % 4) * 8);
   auto *shared_v = (__attribute__((address_space(3))) char *)s_v;
 
-  auto compute = [&](int buf, int k0, auto masked) {
-    constexpr bool MASK = decltype(masked)::value;
+  auto compute = [&](int buf, int k0) {
     f32x16 s[NKB];
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) {
-      s[kb] = f32x16{};
+    for (int kb = 0; kb < NKB; ++kb) s[kb] = f32x16{};
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb)
         s[kb] = M::mma32(*reinterpret_cast<const u32x4 *>(s_k + (buf * KT + kb * 32) * KP + k_read + j * 32), qf[j], s[kb]);
-    }
-    if constexpr (MASK) {
+    if (k0 + KT > w_full) {
       const int left = lim - k0 - 4 * h;
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb)
@@ -756,21 +787,20 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
 
   if (tid == 0) s_bad = 0;
   if (end > p0) {
-    places(p0);
-    fetch();
-    places(p0 + KT);
-    stage(0, p0);
+    find(p0);
+    fetch(p0);
+    find(p0 + KT);
+    stage(0);
     __syncthreads();
     int buf = 0;
     for (int k0 = p0; k0 < end; k0 += KT) {
       const bool more = k0 + KT < end;
       if (more) {
-        fetch();
-        places(k0 + 2 * KT);
+        fetch(k0 + KT);
+        find(k0 + 2 * KT);
       }
-      if (k0 + KT <= w_full) compute(buf, k0, std::false_type{});
-      else if (k0 < w_end) compute(buf, k0, std::true_type{});
-      if (more) stage(buf ^ 1, k0 + KT);
+      if (k0 < w_end) compute(buf, k0);
+      if (more) stage(buf ^ 1);
       buf ^= 1;
       __syncthreads();
     }
@@ -843,7 +873,7 @@ constexpr bool has_tiles() {
 }
 
 template <typename T, int D, int W>
-__global__ __launch_bounds__(W * 64) void paged_rows_kernel(const PagedAttendArgs a) {
+__global__ __launch_bounds__(W * 64, D <= 128 ? 12 / W : 1) void paged_rows_kernel(const PagedAttendArgs a) {
   __shared__ __attribute__((aligned(16))) char s_mem[rows_lds<T, D, W>()];
   rows_path<T, D, W>(a, blockIdx.x, s_mem);
 }
@@ -878,32 +908,36 @@ __device__ __forceinline__ void join_row(const float *o_parts, const float *ml_p
   const float sum = sum_from<1>(ml.y * w);
   const float inv = weight_of(sum);
   constexpr int DPL = D >= 64 ? D / 64 : 1;
-  float o[DPL] = {};
-  const float *src = o_parts + (D >= 64 ? lane * DPL : lane & (D - 1));
-  for (int p = 0; p < parts; ++p) {
-    const float wp = __shfl(w, p);
+  typedef float vd __attribute__((ext_vector_type(DPL)));
+  const int at = D >= 64 ? lane * DPL : lane & (D - 1);
+  vd o = {};
+  constexpr int kDepth = 8;  // parts in flight
+  for (int p0 = 0; p0 < parts; p0 += kDepth) {
+    vd v[kDepth];
 #pragma unroll
-    for (int e = 0; e < DPL; ++e) o[e] = fmaf(src[p * D + e], wp, o[e]);
+    for (int k = 0; k < kDepth; ++k) v[k] = *reinterpret_cast<const vd *>(o_parts + min(p0 + k, parts - 1) * D + at);
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k) o += v[k] * (p0 + k < parts ? __shfl(w, (p0 + k) & 63) : 0.f);
   }
   if (lane * DPL >= D) return;
 #pragma unroll
-  for (int e = 0; e < DPL; ++e) out[lane * DPL + e] = Elem<T>::from_float(o[e] * inv);
+  for (int e = 0; e < DPL; ++e) out[at + e] = Elem<T>::from_float(o[e] * inv);
 }
 
-// Rows of the row path first, by pair and row, then those of the tile path,
-// by token and head.
+// Rows of the row path first, `each` a sequence and KV head, then those of the tile
+// path, by token and head.
 template <typename T, int D>
-__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAttendArgs a, int64_t few) {
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAttendArgs a, int64_t few, int each) {
   int64_t id = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / 64) + (threadIdx.x >> 6);
   if (id < few) {
-    const int per = a.row_tiles * 16, pair = static_cast<int>(id / per), row = static_cast<int>(id - static_cast<int64_t>(pair) * per);
+    const int pair = static_cast<int>(id / each), row = static_cast<int>(id - static_cast<int64_t>(pair) * each);
     const int b = pair / a.kv_heads, hk = pair - b * a.kv_heads;
     const Rows seq = rows_of(a, b);
     const int rows = seq.count * a.group;
     if (row >= rows || rows > a.few_rows) return;
     const int t = row / a.group, qh = hk * a.group + row - t * a.group, len = seq.keys(a, t);
     if (len <= a.part) return;
-    const int64_t slot = id * a.max_parts;
+    const int64_t slot = (static_cast<int64_t>(pair) * a.row_tiles * 16 + row) * a.max_parts;
     join_row<T, D>(a.ws_o + slot * D, a.ws_ml + slot * 2, (len + a.part - 1) / a.part,
                    static_cast<T *>(a.out) + (seq.first + t) * a.o_stride + static_cast<int64_t>(qh) * D);
     return;
@@ -1017,8 +1051,10 @@ static void launch_attend(const PagedAttendArgs &a, hipStream_t s) {
     else if (tiles) paged_tile_kernel<T, D><<<dim3(tiles), 256, 0, s>>>(a);
   }
   if (!tiles) paged_rows_kernel<T, D, 4><<<dim3(rows), 256, 0, s>>>(a);
-  const int64_t few = a.max_parts > 1 ? few_slots(a) / a.max_parts : 0, tile = a.tile_parts > 1 ? tile_slots(a) / a.tile_parts : 0;
-  if (few + tile) paged_join_kernel<T, D><<<dim3(static_cast<unsigned>((few + tile + 3) / 4)), kJoinThreads, 0, s>>>(a, few);
+  const int each = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(a.max_tokens) * a.group, a.row_tiles * 16));
+  const int64_t few = a.max_parts > 1 ? static_cast<int64_t>(a.p.batch) * a.kv_heads * each : 0;
+  const int64_t tile = a.tile_parts > 1 ? static_cast<int64_t>(a.p.tokens) * a.q_heads : 0;
+  if (few + tile) paged_join_kernel<T, D><<<dim3(static_cast<unsigned>((few + tile + 3) / 4)), kJoinThreads, 0, s>>>(a, few, each);
 }
 
 template <typename T>

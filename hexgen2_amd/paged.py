@@ -230,7 +230,7 @@ def attention(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, starts
     ``max_tokens`` its new tokens: both are host values that size the launch.
     Softmax sums are fp32.  ``out`` may be ``q``; tokens of no sequence are left as they
     were in it, those of a sequence not in use become zero.  ``partition``: rows
-    per partition of a split row, a multiple of 64 (0: the library's choice); ``workspace``:
+    per partition of a split row, a multiple of 128 (0: the library's choice); ``workspace``:
     scratch that no overlapping call shares (default: one of this call's own)."""
     _require_device(q, pages, tables, starts)
     softmax_scale = None if softmax_scale is None else float(softmax_scale)

@@ -843,7 +843,7 @@ typedef struct hexkv_paged_attend_params {
   void *out;              /* like q, and may be q */
   int64_t out_stride;
   const void *pages;
-  int32_t partition;      /* rows per partition of a split row, a multiple of 64; 0: the library's choice */
+  int32_t partition;      /* rows per partition of a split row, a multiple of 128; 0: the library's choice */
 } hexkv_paged_attend_params;
 
 /*
