@@ -24,6 +24,7 @@ int check_pool(const hexkv_pool &pool, const char *what) {
   for (const int64_t s : {pool.page_stride, pool.pos_stride, pool.kv_stride, pool.head_stride})
     if (s < 0 || s % vec || s > INT64_C(1) << 40)
       return fail(HEXKV_EINVAL, "%s: pool stride %lld is not a whole number of 16 bytes", what, static_cast<long long>(s));
+  if (pool.page_stride >= 1 << 30) return fail(HEXKV_ERANGE, "%s: pages are 2^30 elements apart or more", what);
   if (pool.pos_stride < d || pool.pos_stride > 1 << 26)
     return fail(HEXKV_EINVAL, "%s: positions of a page are %lld elements apart, not %d to 2^26", what,
                 static_cast<long long>(pool.pos_stride), d);

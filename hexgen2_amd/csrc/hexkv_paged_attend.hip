@@ -42,6 +42,7 @@ struct PagedAttendArgs {
   int64_t q_stride, o_stride;
   int32_t q_heads, kv_heads, group, causal;
   int32_t max_tokens, max_seqlen;
+  uint32_t page_bytes, pos_bytes;  // of the pool
   float scale_log2;
   int32_t few_rows;         // a sequence's rows per KV head up to which it takes the row path
   // row path: 16-row tiles of a sequence and KV head (at most), keys per partition,
@@ -145,14 +146,20 @@ __device__ __forceinline__ ScalarTable scalar_table(const PagedAttendArgs &a, in
   return (ScalarTable)(a.p.tables + __builtin_amdgcn_readfirstlane(b) * a.p.table_stride);
 }
 
+// Bytes from the pool's base to position k's row in a page.
+__device__ __forceinline__ uint64_t block_offset(const PagedAttendArgs &a, int page, int k) {
+  return static_cast<uint64_t>(static_cast<uint32_t>(page)) * a.page_bytes +
+         static_cast<uint32_t>(k & ((1 << a.p.shift) - 1)) * a.pos_bytes;
+}
+
 // 16 rows of one head in a page, as a buffer that ends behind the last row that
 // holds a key: rows past it (those of the page not yet written) and every row of
 // a page outside the pool read as zeros, and blocks past the end, which the
 // loads made ahead ask for, cost nothing.  (Addressed as memory the last block
 // was loaded again in their place: 512 keys of a partition moved 25% more.)
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t block_of(const char *at, int rows, uint32_t pos_bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(at), 0,
-                                           __builtin_amdgcn_readfirstlane(max(0, min(rows, 16)) * pos_bytes), 0x00027000);
+  const uint32_t bytes = rows >= 16 ? 16 * pos_bytes : rows > 0 ? rows * pos_bytes : 0;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(at), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00027000);
 }
 constexpr int kNontemporal = 2;  // a buffer load's cache policy
 template <int POLICY>
@@ -336,7 +343,7 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
   const char *head = static_cast<const char *>(a.pages) + hk * a.p.head_stride * ES;
   const ScalarTable table = scalar_table(a, b);
   const int last = (max(end, 1) - 1) & ~15;
-  const uint32_t pos_bytes = static_cast<uint32_t>(a.p.pos_stride * ES);
+  const uint32_t pos_bytes = a.pos_bytes;
   const int64_t kv_bytes = a.p.kv_stride * ES;
   unsigned bad_pages = 0;
 
@@ -349,7 +356,7 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
   auto block_at = [&](int k, int page) {
     Block x;
     x.in_pool = static_cast<unsigned>(page) < static_cast<unsigned>(a.p.n_pages);
-    const char *at = head + ((x.in_pool ? page : 0) * a.p.page_stride + (min(k, last) & ((1 << a.p.shift) - 1)) * a.p.pos_stride) * ES;
+    const char *at = head + block_offset(a, x.in_pool ? page : 0, k);
     x.k = block_of(at, x.in_pool ? end - k : 0, pos_bytes);
     x.v = block_of(at + kv_bytes, x.in_pool ? end - k : 0, pos_bytes);
     return x;
@@ -648,7 +655,7 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
   constexpr int NJ = D / 16;   // score steps
   constexpr int ND = D / 32;   // output blocks
   constexpr int CH = D / 8;    // 16-byte chunks of a head's row
-  constexpr int CPT = KT * CH / 256, RPP = 256 / CH;  // chunks per thread; rows the workgroup loads at a time
+  static_assert(KT == 4 * 16, "a block of 16 rows a wave");
   constexpr int KP = L::KP, VP = L::VP;
   char *s_k = s_mem, *s_v = s_mem + 2 * KT * KP;
   int &s_bad = *reinterpret_cast<int *>(s_mem + 2 * KT * (KP + VP));
@@ -688,35 +695,33 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
   const ScalarTable table = scalar_table(a, b);
   const int last = (max(end, 1) - 1) & ~15;
   int bad_pages = 0;
-  // Thread tid moves chunk tid % CH of rows tid / CH + i * RPP; those of one
-  // wave lie in one block of 16 positions, and that in one page.
-  const int s_row = tid / CH, s_ch = tid % CH;
-  const int s_block = __builtin_amdgcn_readfirstlane(s_row >> 4);
-  const uint32_t pos_bytes = static_cast<uint32_t>(a.p.pos_stride * ES), lane_at = (s_row & 15) * pos_bytes + 16 * s_ch;
-  u32x4 kr[CPT], vr[CPT];
-  int page[CPT];
-  auto find = [&](int k0) {
-#pragma unroll
-    for (int i = 0; i < CPT; ++i) page[i] = table[min(k0 + i * RPP + 16 * s_block, last) >> a.p.shift];
-  };
+  // A wave moves the tile's block of 16 rows of its own, which lie in one page:
+  // lane l chunk l % CH of rows l / CH + i * RPL.
+  constexpr int RPL = 64 / CH, NL = 16 / RPL;
+  const uint32_t pos_bytes = a.pos_bytes;
+  const uint32_t lane_at = (lane / CH) * pos_bytes + 16 * (lane % CH);
+  const int s_row = 16 * wave + lane / CH;
+  const uint32_t k_write = s_row * KP + (lane % CH) * 16, v_write = s_row * VP + (lane % CH) * 16;
+  u32x4 kr[NL], vr[NL];
+  int page;
+  auto find = [&](int k0) { page = table[min(k0 + 16 * wave, last) >> a.p.shift]; };
   auto fetch = [&](int k0) {
+    const bool in_pool = static_cast<unsigned>(page) < static_cast<unsigned>(a.p.n_pages);
+    const int k = k0 + 16 * wave;
+    bad_pages |= !in_pool && k < end;
+    const char *at = head + block_offset(a, in_pool ? page : 0, k);
+    const __amdgpu_buffer_rsrc_t bk = block_of(at, end - k, pos_bytes), bv = block_of(at + kv_bytes, end - k, pos_bytes);
 #pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const bool in_pool = static_cast<unsigned>(page[i]) < static_cast<unsigned>(a.p.n_pages);
-      const int k = k0 + i * RPP + 16 * s_block;
-      bad_pages |= !in_pool && k < end;
-      const char *at = head + ((in_pool ? page[i] : 0) * a.p.page_stride + (k & ((1 << a.p.shift) - 1)) * a.p.pos_stride) * ES;
-      kr[i] = load_16<0>(block_of(at, end - k, pos_bytes), lane_at);
-      vr[i] = load_16<0>(block_of(at + kv_bytes, end - k, pos_bytes), lane_at);
-    }
+    for (int i = 0; i < NL; ++i) kr[i] = load_16<0>(bk, lane_at + i * RPL * pos_bytes);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) vr[i] = load_16<0>(bv, lane_at + i * RPL * pos_bytes);
   };
   auto stage = [&](int buf) {
+    char *to_k = s_k + (k_write + (buf ? KT * KP : 0)), *to_v = s_v + (v_write + (buf ? KT * VP : 0));
 #pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const int r = s_row + i * RPP;
-      *reinterpret_cast<u32x4 *>(s_k + (buf * KT + r) * KP + s_ch * 16) = kr[i];
-      *reinterpret_cast<u32x4 *>(s_v + (buf * KT + r) * VP + s_ch * 16) = vr[i];
-    }
+    for (int i = 0; i < NL; ++i) *reinterpret_cast<u32x4 *>(to_k + i * RPL * KP) = kr[i];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) *reinterpret_cast<u32x4 *>(to_v + i * RPL * VP) = vr[i];
   };
 
   float m = -INFINITY, l = 0.f;  // m: the running maximum less kShift
@@ -726,9 +731,10 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
   const uint32_t k_read = static_cast<uint32_t>(c * KP + h * 16);
   const int s16 = lane & 15;
   const uint32_t v_read = static_cast<uint32_t>((4 * h + s16 / 4) * VP + ((lane >> 4) & 1) * 32 + (s16 % 4) * 8);
-  auto *shared_v = (__attribute__((address_space(3))) char *)s_v;
 
   auto compute = [&](int buf, int k0) {
+    const char *from_k = s_k + (k_read + (buf ? KT * KP : 0));
+    auto *from_v = (__attribute__((address_space(3))) char *)s_v + (v_read + (buf ? KT * VP : 0));
     f32x16 s[NKB];
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb) s[kb] = f32x16{};
@@ -736,7 +742,7 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb)
-        s[kb] = M::mma32(*reinterpret_cast<const u32x4 *>(s_k + (buf * KT + kb * 32) * KP + k_read + j * 32), qf[j], s[kb]);
+        s[kb] = M::mma32(*reinterpret_cast<const u32x4 *>(from_k + kb * 32 * KP + j * 32), qf[j], s[kb]);
     if (k0 + KT > w_full) {
       const int left = lim - k0 - 4 * h;
 #pragma unroll
@@ -778,9 +784,8 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
     for (int ks = 0; ks < 2 * NKB; ++ks)
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        const uint32_t from = static_cast<uint32_t>((buf * KT + ks * 16) * VP + d * 64) + v_read;
-        const h4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_h4 *)(shared_v + from));
-        const h4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_h4 *)(shared_v + from + 8 * VP));
+        const h4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_h4 *)(from_v + ks * 16 * VP + d * 64));
+        const h4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_h4 *)(from_v + ks * 16 * VP + d * 64 + 8 * VP));
         acc[d] = M::mma32(__builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7)), p[ks], acc[d]);
       }
   };
@@ -991,6 +996,8 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   a->causal = p.causal ? 1 : 0;
   a->max_tokens = p.seqs.cu_tokens ? std::min(p.max_tokens, p.seqs.tokens) : a->p.each;
   a->max_seqlen = p.max_seqlen;
+  a->page_bytes = static_cast<uint32_t>(p.pool.page_stride * elem_bytes(p.pool.dtype));
+  a->pos_bytes = static_cast<uint32_t>(p.pool.pos_stride * elem_bytes(p.pool.dtype));
   a->scale_log2 = p.softmax_scale * 1.44269504f;
   const int64_t rows = static_cast<int64_t>(a->max_tokens) * a->group;
   if (rows > INT32_MAX - kTileRows) return fail(HEXKV_ERANGE, "%s: 2^31 rows or more", what);
