@@ -66,13 +66,13 @@ __device__ __forceinline__ float weight_of(float sum) { return sum == 0.f ? 0.f 
 // Tokens of sequence b as this call sees them, and the keys they attend.
 struct Rows {
   int32_t first, count;  // tokens
-  int64_t start;
+  int32_t start;
   int32_t total;  // keys of the last token
   bool cut;
 
   __device__ __forceinline__ int keys(const PagedAttendArgs &a, int i) const {
     if (!a.causal) return total;
-    return start < 0 ? 0 : static_cast<int>(min(start + i + 1, static_cast<int64_t>(a.max_seqlen)));
+    return start < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(start) + i + 1, static_cast<int64_t>(a.max_seqlen)));
   }
 };
 
@@ -94,6 +94,7 @@ __device__ __forceinline__ Rows rows_of(const PagedAttendArgs &a, int b) {
 // was 17000 workgroups, 200 us of them leaving at once.
 struct Place {
   int b, tile, part, hk;
+  Rows seq;
 };
 
 // The sequence that has the index-th of all tiles, and which of its own that is
@@ -111,12 +112,14 @@ __device__ __forceinline__ Place place_of(const PagedAttendArgs &a, int block, i
     p.b = each ? index / each : a.p.batch;
     p.tile = index - p.b * each;
     if (p.b >= a.p.batch) p.b = -1;
+    else p.seq = rows_of(a, p.b);
     return p;
   }
   const int lane = threadIdx.x & 63;
   for (int b0 = 0; b0 < a.p.batch; b0 += 64) {
     const int b = b0 + lane;
-    const int n = b < a.p.batch ? tiles(min(sequence_of(a.p, b).count, a.max_tokens)) : 0;
+    const Rows seq = rows_of(a, min(b, a.p.batch - 1));
+    const int n = b < a.p.batch ? tiles(seq.count) : 0;
     int upto = n;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -127,10 +130,15 @@ __device__ __forceinline__ Place place_of(const PagedAttendArgs &a, int block, i
     if (past) {
       const int j = __builtin_ctzll(past);
       p.b = __builtin_amdgcn_readfirstlane(b0 + j);
-      p.tile = __builtin_amdgcn_readfirstlane(index - __shfl(upto - n, j));
+      p.tile = index - __builtin_amdgcn_readlane(upto - n, j);
+      p.seq.first = __builtin_amdgcn_readlane(seq.first, j);
+      p.seq.count = __builtin_amdgcn_readlane(seq.count, j);
+      p.seq.start = __builtin_amdgcn_readlane(seq.start, j);
+      p.seq.total = __builtin_amdgcn_readlane(seq.total, j);
+      p.seq.cut = __builtin_amdgcn_readlane(static_cast<int>(seq.cut), j);
       return p;
     }
-    index -= __shfl(upto, 63);
+    index -= __builtin_amdgcn_readlane(upto, 63);
   }
   p.b = -1;
   p.tile = 0;
@@ -282,15 +290,19 @@ __device__ void exact_row(const PagedAttendArgs &a, const T *q, int b, int hk, i
   *l_out = sum_from<1>(l);
 }
 
+constexpr int kRowWaves = 4;
+
 // LDS bytes of the row path: V as its waves turn it, then their sums.
-template <typename T, int D, int W>
+template <typename T, int D>
 constexpr int rows_lds() {
+  constexpr int W = kRowWaves;
   const int v = std::is_same<T, float>::value ? 0 : W * 32 * (2 * D + 32), o = W * 16 * (D + 4) * 4;
   return (v > o ? v : o) + 2 * W * 16 * 4 + 16;
 }
 
-template <typename T, int D, int W>
+template <typename T, int D>
 __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, char *s_mem) {
+  constexpr int W = kRowWaves;
   constexpr bool F32 = std::is_same<T, float>::value;
   using M = Mma<T>;
   constexpr int KEYS = F32 ? 16 : 32;       // keys of a step
@@ -304,7 +316,7 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
   constexpr int KP = 2 * D + 16;            // 16-bit: LDS bytes of a K row: 16 rows' chunks over all banks
   constexpr int VP = 2 * D + 32;            // of a V row: the 16 rows of a transposed read in two passes
   constexpr int OP = D + 4;                 // floats of a row in the join
-  constexpr int kMl = rows_lds<T, D, W>() - 2 * W * 16 * 4 - 16;
+  constexpr int kMl = rows_lds<T, D>() - 2 * W * 16 * 4 - 16;
   float(*s_m)[16] = reinterpret_cast<float(*)[16]>(s_mem + kMl), (*s_l)[16] = s_m + W;
   int &s_bad = *reinterpret_cast<int *>(s_mem + kMl + 2 * W * 16 * 4);
 
@@ -316,7 +328,7 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
   const int b = mine.b, hk = mine.hk, part = mine.part, tile = mine.tile;
   if (b < 0) return;
   const int pair = b * a.kv_heads + hk;
-  const Rows seq = rows_of(a, b);
+  const Rows seq = mine.seq;
   const int rows = seq.count * a.group, row0 = tile * 16;
   if (seq.cut && threadIdx.x == 0 && part == 0 && tile == 0) raise_status(a.status, HEXKV_STATUS_LENGTH_CLAMPED);
   const int p0 = part * a.part;
@@ -342,7 +354,6 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
   constexpr int ES = static_cast<int>(sizeof(T));
   const char *head = static_cast<const char *>(a.pages) + hk * a.p.head_stride * ES;
   const ScalarTable table = scalar_table(a, b);
-  const int last = (max(end, 1) - 1) & ~15;
   const uint32_t pos_bytes = a.pos_bytes;
   const int64_t kv_bytes = a.p.kv_stride * ES;
   unsigned bad_pages = 0;
@@ -352,7 +363,7 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
     __amdgpu_buffer_rsrc_t k, v;
     bool in_pool;
   };
-  auto page_of = [&](int k) { return table[min(k, last) >> a.p.shift]; };
+  auto page_of = [&](int k) { return table[min(k >> a.p.shift, a.p.width - 1)]; };
   auto block_at = [&](int k, int page) {
     Block x;
     x.in_pool = static_cast<unsigned>(page) < static_cast<unsigned>(a.p.n_pages);
@@ -629,6 +640,7 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
 
 // ------------------------------------------------------------ tile path ---
 
+constexpr int kCus = 256;
 constexpr int kTileRows = 128, kTileKeys = 64;
 // A sequence of so many rows per KV head, or fewer, takes the row path.
 constexpr int kFewRows = 32;
@@ -668,7 +680,7 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
   });
   const int b = mine.b, hk = mine.hk, part = mine.part, tile = mine.tile;
   if (b < 0) return;
-  const Rows seq = rows_of(a, b);
+  const Rows seq = mine.seq;
   const int total = seq.count * a.group, row0 = tile * kTileRows;
   const int p0 = part * a.tile_part;
   const int t_last = (min(row0 + kTileRows, total) - 1) / a.group;
@@ -693,7 +705,6 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
   const char *head = static_cast<const char *>(a.pages) + hk * a.p.head_stride * ES;
   const int64_t kv_bytes = a.p.kv_stride * ES;
   const ScalarTable table = scalar_table(a, b);
-  const int last = (max(end, 1) - 1) & ~15;
   int bad_pages = 0;
   // A wave moves the tile's block of 16 rows of its own, which lie in one page:
   // lane l chunk l % CH of rows l / CH + i * RPL.
@@ -704,7 +715,7 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
   const uint32_t k_write = s_row * KP + (lane % CH) * 16, v_write = s_row * VP + (lane % CH) * 16;
   u32x4 kr[NL], vr[NL];
   int page;
-  auto find = [&](int k0) { page = table[min(k0 + 16 * wave, last) >> a.p.shift]; };
+  auto find = [&](int k0) { page = table[min((k0 + 16 * wave) >> a.p.shift, a.p.width - 1)]; };
   auto fetch = [&](int k0) {
     const bool in_pool = static_cast<unsigned>(page) < static_cast<unsigned>(a.p.n_pages);
     const int k = k0 + 16 * wave;
@@ -877,10 +888,10 @@ constexpr bool has_tiles() {
   return !std::is_same<T, float>::value && (D == 64 || D == 128);
 }
 
-template <typename T, int D, int W>
-__global__ __launch_bounds__(W * 64, D <= 128 ? 12 / W : 1) void paged_rows_kernel(const PagedAttendArgs a) {
-  __shared__ __attribute__((aligned(16))) char s_mem[rows_lds<T, D, W>()];
-  rows_path<T, D, W>(a, blockIdx.x, s_mem);
+template <typename T, int D>
+__global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void paged_rows_kernel(const PagedAttendArgs a) {
+  __shared__ __attribute__((aligned(16))) char s_mem[rows_lds<T, D>()];
+  rows_path<T, D>(a, blockIdx.x, s_mem);
 }
 
 template <typename T, int D>
@@ -892,38 +903,46 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedAttendArg
 // A call that may hold sequences of either kind: tiles first (they take longest).
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void paged_mixed_kernel(const PagedAttendArgs a) {
-  constexpr int kRows = rows_lds<T, D, 4>(), kTiles = TileLds<D>::kBytes;
+  constexpr int kRows = rows_lds<T, D>(), kTiles = TileLds<D>::kBytes;
   __shared__ __attribute__((aligned(16))) char s_mem[kRows > kTiles ? kRows : kTiles];
   const int block = blockIdx.x;
   if (block < a.tile_blocks) tile_path<T, D>(a, block, s_mem);
-  else rows_path<T, D, 4>(a, block - a.tile_blocks, s_mem);
+  else rows_path<T, D>(a, block - a.tile_blocks, s_mem);
 }
 
 // The partitions of a split row, joined: a wave a row.
 constexpr int kJoinThreads = 256;
-constexpr int kMaxParts = 64;  // a lane each
+constexpr int kMaxParts = 512;
 
 template <typename T, int D>
 __device__ __forceinline__ void join_row(const float *o_parts, const float *ml_parts, int parts, T *out) {
   const int lane = threadIdx.x & 63;
-  float2 ml{-INFINITY, 0.f};
-  if (lane < parts) ml = *reinterpret_cast<const float2 *>(ml_parts + lane * 2);
-  const float top = wave_max(ml.x);
-  const float w = ml.x == -INFINITY ? 0.f : exp2_of(ml.x - top);
-  const float sum = sum_from<1>(ml.y * w);
-  const float inv = weight_of(sum);
+  float top = -INFINITY;
+  for (int p = lane; p < parts; p += 64) top = fmaxf(top, ml_parts[p * 2]);
+  top = wave_max(top);
   constexpr int DPL = D >= 64 ? D / 64 : 1;
   typedef float vd __attribute__((ext_vector_type(DPL)));
   const int at = D >= 64 ? lane * DPL : lane & (D - 1);
   vd o = {};
+  float sum = 0.f;
   constexpr int kDepth = 8;  // parts in flight
   for (int p0 = 0; p0 < parts; p0 += kDepth) {
     vd v[kDepth];
+    float2 ml[kDepth];
 #pragma unroll
-    for (int k = 0; k < kDepth; ++k) v[k] = *reinterpret_cast<const vd *>(o_parts + min(p0 + k, parts - 1) * D + at);
+    for (int k = 0; k < kDepth; ++k) {
+      const int p = min(p0 + k, parts - 1);
+      v[k] = *reinterpret_cast<const vd *>(o_parts + p * D + at);
+      ml[k] = *reinterpret_cast<const float2 *>(ml_parts + p * 2);
+    }
 #pragma unroll
-    for (int k = 0; k < kDepth; ++k) o += v[k] * (p0 + k < parts ? __shfl(w, (p0 + k) & 63) : 0.f);
+    for (int k = 0; k < kDepth; ++k) {
+      const float w = p0 + k >= parts || ml[k].x == -INFINITY ? 0.f : exp2_of(ml[k].x - top);
+      o += v[k] * w;
+      sum = fmaf(ml[k].y, w, sum);
+    }
   }
+  const float inv = weight_of(sum);
   if (lane * DPL >= D) return;
 #pragma unroll
   for (int e = 0; e < DPL; ++e) out[at + e] = Elem<T>::from_float(o[e] * inv);
@@ -964,6 +983,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAtt
 
 // ------------------------------------------------------------------ host ---
 
+static int64_t ceil_div(int64_t n, int64_t by) { return (n + by - 1) / by; }
 static int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // Checks a call and fills its arguments but for addresses.
@@ -1014,19 +1034,27 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
     few_tiles = std::min(few_tiles, all_rows / 16 + std::min<int64_t>(batch, tokens));
     tiles = std::min(tiles, all_rows / kTileRows + std::min<int64_t>(batch, all_rows / (kFewRows + 1)));
   }
-  // Partitions, so that the workgroups of either path fill the CUs.
-  auto split = [&](int64_t blocks, int64_t want, int64_t least, int32_t *part, int32_t *parts) {
-    int64_t n = p.partition;
-    if (!n) {
-      const int64_t each = std::max<int64_t>(1, want / std::max<int64_t>(blocks, 1));
-      n = std::max(least, round_up((p.max_seqlen + each - 1) / each, 64));
-    }
-    if ((p.max_seqlen + n - 1) / n > kMaxParts) n = round_up((p.max_seqlen + kMaxParts - 1) / kMaxParts, 64);
-    *part = static_cast<int32_t>(std::min<int64_t>(n, 1 << 30));
-    *parts = static_cast<int32_t>(std::max<int64_t>(1, (p.max_seqlen + n - 1) / n));
-  };
-  split(few_tiles * a->kv_heads, 768, 256, &a->part, &a->max_parts);
-  split((all_rows + kTileRows - 1) / kTileRows * a->kv_heads, 512, 512, &a->tile_part, &a->tile_parts);
+  // Partitions.  A CU alone takes 55 GB/s whatever its waves, so a row's keys are spread
+  // over CUs, but for those of up to 128 KB of K, which end before a second
+  // launch would have joined them (a step of 128 keys of 128 16-bit dims takes 1.15 us, the
+  // join 2.7): one workgroup a CU where that leaves it 2048 keys or fewer, else
+  // partitions of 1024 keys, which even out ragged lengths (us, MI355X, 16-bit heads
+  // of 128: 8 pairs of 1024 keys 8.5 split in 8, 12.9 whole, of 512 8.2 and 8.6; 32 pairs of 4096
+  // keys 19.5, 17.0, 16.5, 18.2, 26.3 and 40 in partitions of 128, 256, 512, 1024, 2048 and
+  // whole; 512 ragged ones of up to 8192 191, 181, 177, 193 and 200 from 256 on).
+  const int64_t row_keys = few_tiles * a->kv_heads * p.max_seqlen, each = round_up((row_keys + kCus - 1) / kCus, 128);
+  int64_t part = p.partition ? p.partition : each <= 2048 ? std::max<int64_t>(each, 128) : 1024;
+  if (!p.partition && static_cast<int64_t>(p.max_seqlen) * d * elem_bytes(p.pool.dtype) <= 128 << 10) part = 1 << 30;
+  part = std::max(part, round_up((p.max_seqlen + kMaxParts - 1) / kMaxParts, 128));
+  a->part = static_cast<int32_t>(std::min<int64_t>(part, 1 << 30));
+  a->max_parts = static_cast<int32_t>(std::max<int64_t>(1, (p.max_seqlen + part - 1) / part));
+  // Tiles are split where there are fewer than CUs, and no shorter than 512 keys: a partition's sums
+  // are written and read once more.
+  const int64_t full = (all_rows + kTileRows - 1) / kTileRows * a->kv_heads;
+  part = p.partition ? p.partition : std::max<int64_t>(512, round_up(ceil_div(p.max_seqlen, std::max<int64_t>(1, kCus / std::max<int64_t>(full, 1))), 64));
+  part = std::max(part, round_up((p.max_seqlen + kMaxParts - 1) / kMaxParts, 64));
+  a->tile_part = static_cast<int32_t>(std::min<int64_t>(part, 1 << 30));
+  a->tile_parts = static_cast<int32_t>(std::max<int64_t>(1, (p.max_seqlen + part - 1) / part));
   if (!few) a->max_parts = 1;
   if (!tiled) a->tile_parts = 1;
   const int64_t row_blocks = few_tiles * a->kv_heads * a->max_parts, tile_blocks = tiles * a->kv_heads * a->tile_parts;
@@ -1057,7 +1085,7 @@ static void launch_attend(const PagedAttendArgs &a, hipStream_t s) {
     if (rows && tiles) paged_mixed_kernel<T, D><<<dim3(rows + tiles), 256, 0, s>>>(a);
     else if (tiles) paged_tile_kernel<T, D><<<dim3(tiles), 256, 0, s>>>(a);
   }
-  if (!tiles) paged_rows_kernel<T, D, 4><<<dim3(rows), 256, 0, s>>>(a);
+  if (!tiles) paged_rows_kernel<T, D><<<dim3(rows), 256, 0, s>>>(a);
   const int each = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(a.max_tokens) * a.group, a.row_tiles * 16));
   const int64_t few = a.max_parts > 1 ? static_cast<int64_t>(a.p.batch) * a.kv_heads * each : 0;
   const int64_t tile = a.tile_parts > 1 ? static_cast<int64_t>(a.p.tokens) * a.q_heads : 0;
