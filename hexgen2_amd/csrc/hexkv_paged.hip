@@ -207,8 +207,8 @@ struct PagedCopyArgs {
   int64_t table_stride;
   int64_t page_bytes, pos_bytes, kv_bytes, head_bytes;  // of the pool
   int32_t n_pages, shift;
-  int32_t heads2, chunks;   // 2 x KV heads; 16-byte vectors of one head's row
-  int32_t rows;             // rows per workgroup, a power of two up to 16
+  int32_t heads2, chunk_shift;  // 2 x KV heads; 16-byte vectors of one head's row: 2^chunk_shift
+  int32_t rows;             // rows per workgroup, a power of two that divides the page
   int32_t batch;
   int32_t cu[S + 1];        // packed row of each sequence's first
   int32_t blocks[S + 1];    // workgroup of each sequence's first rows
@@ -218,14 +218,16 @@ using WidePagedCopy = PagedCopyArgs<HEXKV_MAX_LAYERS_PER_LAUNCH, HEXKV_MAX_SEQS_
 using SmallPagedCopy = PagedCopyArgs<32, 16>;
 static_assert(sizeof(WidePagedCopy) <= 4096, "kernel arguments above 4 KiB");
 
-constexpr int kPagedCopyThreads = 256;
-constexpr int kPagedCopyUnroll = 4;
+// Workgroups as for the handoff of the other caches: 1024 threads of eight
+// vectors each, 128 KB, and 256 of four for copies below 128 MB.
+constexpr int kCopyThreads = 1024, kCopyUnroll = 8;
+constexpr int kSmallCopyThreads = 256, kSmallCopyUnroll = 4;
 
-// A workgroup moves `rows` positions of one page (they lie in one: rows
-// divides the page) of one layer.  Vectors are taken in the order of the side
-// that is written.
-template <bool PACK, typename A>
-__global__ __launch_bounds__(kPagedCopyThreads) void paged_copy_kernel(const A a) {
+// A workgroup moves `rows` positions of one page of one layer.  Vectors are
+// taken in the order of the side that is written: a row's heads one after another
+// when packing, a head's rows, K then V, when unpacking.
+template <bool PACK, typename A, int NT, int UN>
+__global__ __launch_bounds__(NT) void paged_copy_kernel(const A a) {
   const int block = blockIdx.x;
   int lo = 0, hi = a.batch;
   while (hi - lo > 1) {
@@ -239,44 +241,47 @@ __global__ __launch_bounds__(kPagedCopyThreads) void paged_copy_kernel(const A a
   if (bad && threadIdx.x == 0 && blockIdx.y == 0) raise_status(a.status, HEXKV_STATUS_PAGE);
   if (!PACK && bad) return;
   const int64_t in_page = (bad ? 0 : page) * a.page_bytes + (p0 & ((1 << a.shift) - 1)) * a.pos_bytes;
-  const int64_t row_bytes = static_cast<int64_t>(a.heads2) * a.chunks * 16;
+  const int64_t row_bytes = static_cast<int64_t>(a.heads2) << (a.chunk_shift + 4);
   const int64_t in_packed = (static_cast<int64_t>(a.cu[lo]) + p0) * row_bytes;
   const char *src = a.src[blockIdx.y] + (PACK ? in_page : in_packed);
   char *dst = a.dst[blockIdx.y] + (PACK ? in_packed : in_page);
-  const int total = n * a.heads2 * a.chunks, heads = a.heads2 / 2;
-  for (int v0 = threadIdx.x; v0 < total; v0 += kPagedCopyThreads * kPagedCopyUnroll) {
-    u32x4 r[kPagedCopyUnroll];
-    int64_t to[kPagedCopyUnroll];
+  // Chunk c of unit u = outer * inner + i: a head of a row; a thread's next
+  // unit is `step` further.
+  const int heads = a.heads2 >> 1, total = n * a.heads2, inner = PACK ? a.heads2 : n;
+  const int step = NT >> a.chunk_shift, d_outer = step / inner, d_i = step - d_outer * inner;
+  const int64_t c = (threadIdx.x & ((1 << a.chunk_shift) - 1)) * 16;
+  int u = static_cast<int>(threadIdx.x) >> a.chunk_shift, outer = u / inner, i = u - outer * inner;
+  while (u < total) {
+    u32x4 r[UN];
+    int64_t to[UN];
+    const int first = u;
 #pragma unroll
-    for (int k = 0; k < kPagedCopyUnroll; ++k) {
-      const int v = min(v0 + k * kPagedCopyThreads, total - 1);
-      const int c = v % a.chunks, u = v / a.chunks;
-      int row, h2;
-      if (PACK) {
-        row = u / a.heads2;
-        h2 = u - row * a.heads2;
-      } else {
-        h2 = u / n;
-        row = u - h2 * n;
-        h2 = (h2 & 1) * heads + (h2 >> 1);  // a page holds a head's K and V together
-      }
-      const int64_t in_row = row * row_bytes + (static_cast<int64_t>(h2) * a.chunks + c) * 16;
-      const int kv = h2 >= heads, head = h2 - kv * heads;
-      const int64_t at = row * a.pos_bytes + kv * a.kv_bytes + head * a.head_bytes + c * 16;
-      to[k] = PACK ? in_row : at;
-      r[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + (PACK ? at : in_row)));
+    for (int k = 0; k < UN; ++k) {
+      const int row = PACK ? outer : i, h2 = PACK ? i : outer;
+      const int head = PACK ? (h2 >= heads ? h2 - heads : h2) : h2 >> 1, kv = PACK ? h2 >= heads : h2 & 1;
+      const int64_t packed = row * row_bytes + ((static_cast<int64_t>(kv ? heads : 0) + head) << (a.chunk_shift + 4)) + c;
+      const int64_t paged = row * a.pos_bytes + (kv ? a.kv_bytes : 0) + head * a.head_bytes + c;
+      to[k] = PACK ? packed : paged;
+      if (u < total) r[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + (PACK ? paged : packed)));
       if (PACK && bad) r[k] = u32x4{};
+      u += step;
+      i += d_i;
+      outer += d_outer;
+      if (i >= inner) {
+        i -= inner;
+        ++outer;
+      }
     }
 #pragma unroll
-    for (int k = 0; k < kPagedCopyUnroll; ++k)
-      if (v0 + k * kPagedCopyThreads < total) __builtin_nontemporal_store(r[k], reinterpret_cast<u32x4 *>(dst + to[k]));
+    for (int k = 0; k < UN; ++k)
+      if (first + k * step < total) __builtin_nontemporal_store(r[k], reinterpret_cast<u32x4 *>(dst + to[k]));
   }
 }
 
 template <typename A>
 static int launch_paged_copy(bool pack, const hexkv_pool &pool, const void *const *src, void *const *dst, int l0, int nl,
                              const int32_t *tables, int64_t table_stride, int nb, const int64_t *lens, int64_t packed_off,
-                             int rows, unsigned int *status, hipStream_t stream, const char *what) {
+                             int rows, bool small, unsigned int *status, hipStream_t stream, const char *what) {
   A a;
   const int es = elem_bytes(pool.dtype);
   a.tables = tables;
@@ -288,7 +293,7 @@ static int launch_paged_copy(bool pack, const hexkv_pool &pool, const void *cons
   a.n_pages = pool.n_pages;
   a.shift = __builtin_ctz(static_cast<unsigned>(pool.page_size));
   a.heads2 = 2 * pool.kv_heads;
-  a.chunks = pool.head_dim * es / 16;
+  a.chunk_shift = __builtin_ctz(static_cast<unsigned>(pool.head_dim * es / 16));
   a.rows = rows;
   a.batch = nb;
   a.status = status;
@@ -303,8 +308,15 @@ static int launch_paged_copy(bool pack, const hexkv_pool &pool, const void *cons
     a.dst[l] = static_cast<char *>(dst[l0 + l]) + (pack ? packed_off : 0);
   }
   const dim3 grid(static_cast<unsigned>(a.blocks[nb]), static_cast<unsigned>(nl));
-  if (pack) paged_copy_kernel<true, A><<<grid, kPagedCopyThreads, 0, stream>>>(a);
-  else paged_copy_kernel<false, A><<<grid, kPagedCopyThreads, 0, stream>>>(a);
+  if (small) {
+    constexpr int NT = kSmallCopyThreads, UN = kSmallCopyUnroll;
+    if (pack) paged_copy_kernel<true, A, NT, UN><<<grid, NT, 0, stream>>>(a);
+    else paged_copy_kernel<false, A, NT, UN><<<grid, NT, 0, stream>>>(a);
+  } else {
+    constexpr int NT = kCopyThreads, UN = kCopyUnroll;
+    if (pack) paged_copy_kernel<true, A, NT, UN><<<grid, NT, 0, stream>>>(a);
+    else paged_copy_kernel<false, A, NT, UN><<<grid, NT, 0, stream>>>(a);
+  }
   return check_launch(what);
 }
 
@@ -335,11 +347,12 @@ static int paged_copy(bool pack, const hexkv_pool *pool, const void *const *src,
   unsigned int *status = nullptr;
   rc = status_word(stream, &status, what);
   if (rc != HEXKV_OK) return rc;
-  // Rows of a workgroup: about 64 KB, so that it has enough in flight.
   const int64_t row_bytes = 2 * static_cast<int64_t>(pool->kv_heads) * pool->head_dim * elem_bytes(pool->dtype);
   if (row_bytes > INT64_C(1) << 26) return fail(HEXKV_ERANGE, "%s: rows of more than 2^26 bytes", what);
-  int rows = 16;
-  while (rows > 1 && rows * row_bytes > 65536) rows /= 2;
+  const bool small = total * row_bytes * n_layers < 128 << 20;
+  const int64_t share = small ? kSmallCopyThreads * kSmallCopyUnroll * 16 : kCopyThreads * kCopyUnroll * 16;
+  int rows = pool->page_size;
+  while (rows > 1 && rows * row_bytes > share) rows /= 2;
   int64_t base = 0;
   for (int b0 = 0; b0 < batch; b0 += HEXKV_MAX_SEQS_PER_LAUNCH) {
     const int nb = std::min(batch - b0, HEXKV_MAX_SEQS_PER_LAUNCH);
@@ -349,9 +362,9 @@ static int paged_copy(bool pack, const hexkv_pool *pool, const void *const *src,
       hipStream_t s = static_cast<hipStream_t>(stream);
       rc = nl <= 32 && nb <= 16
           ? launch_paged_copy<SmallPagedCopy>(pack, *pool, src, dst, l0, nl, t, table_stride, nb, lens + b0, base * row_bytes,
-                                              rows, status, s, what)
+                                              rows, small, status, s, what)
           : launch_paged_copy<WidePagedCopy>(pack, *pool, src, dst, l0, nl, t, table_stride, nb, lens + b0, base * row_bytes,
-                                             rows, status, s, what);
+                                             rows, small, status, s, what);
       if (rc != HEXKV_OK) return rc;
     }
     for (int b = 0; b < nb; ++b) base += lens[b0 + b];
