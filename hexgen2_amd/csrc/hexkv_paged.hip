@@ -390,7 +390,7 @@ extern "C" int hexkv_paged_append(const hexkv_paged_append_params *params, hexkv
   int rc = fill_tables(p.pool, p.seqs, &a.p, what);
   if (rc != HEXKV_OK) return rc;
   const int d = p.pool.head_dim, es = elem_bytes(p.pool.dtype), vec = 16 / es;
-  if (p.q_heads < 1 || p.q_heads > 1 << 16) return fail(HEXKV_EINVAL, "%s: %d query heads", what, p.q_heads);
+  if (p.q_heads < 0 || p.q_heads > 1 << 16) return fail(HEXKV_EINVAL, "%s: %d query heads", what, p.q_heads);
   if (p.rotary_dim < 0 || p.rotary_dim % 2 || p.rotary_dim > d)
     return fail(HEXKV_EINVAL, "%s: rotary_dim %d is not even or not in [0, %d]", what, p.rotary_dim, d);
   const int64_t q_row = static_cast<int64_t>(p.q_heads) * d, row = q_row + 2 * static_cast<int64_t>(p.pool.kv_heads) * d;
@@ -398,7 +398,7 @@ extern "C" int hexkv_paged_append(const hexkv_paged_append_params *params, hexkv
   if (p.qkv_stride < row && tokens > 1) return fail(HEXKV_EINVAL, "%s: qkv's rows overlap", what);
   if (p.q_stride < q_row && tokens > 1) return fail(HEXKV_EINVAL, "%s: q's rows overlap", what);
   if (tokens == 0 || p.seqs.batch == 0) return HEXKV_OK;
-  if (!p.qkv || !p.q || !p.pages || (p.rotary_dim && !p.inv_freq)) return fail(HEXKV_EINVAL, "%s: null tensor", what);
+  if (!p.qkv || (p.q_heads && !p.q) || !p.pages || (p.rotary_dim && !p.inv_freq)) return fail(HEXKV_EINVAL, "%s: null tensor", what);
   if (!aligned16(p.pages)) return fail(HEXKV_EINVAL, "%s: pages are not 16-byte aligned", what);
   // A thread writes the q that it read, so q may stand where it was; over
   // other rows, or over the pages, it may not.

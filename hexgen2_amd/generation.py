@@ -27,6 +27,10 @@ class InferenceParams:
     every sample's position.  ``kv_bits`` (an addition) 4 keeps the caches in
     four bits, ``[max_batch_size, max_sequence_len, row_bytes]`` (``fp4``); with
     ``attend_stored`` a prompt, too, attends its rows as they are stored there.
+    ``page_size`` (another) keeps each layer's cache in a pool of pages (``paged``):
+    ``key_value_memory_dict`` then maps to ``[n_pages, page_size, 2, kv_heads, head_dim]``
+    and ``page_tables`` (int32 ``[max_batch_size, width]``, device) says whose pages are
+    which; None: as many as ``max_sequence_len`` needs for each sequence, in order.
     """
     max_sequence_len: int
     max_batch_size: int = 1
@@ -37,6 +41,8 @@ class InferenceParams:
     lengths_per_sample: Optional[torch.Tensor] = None
     kv_bits: int = 16
     attend_stored: bool = False
+    page_size: int = 0
+    page_tables: Optional[torch.Tensor] = None
 
 
 # hexgen2/model.py:11-19 names the same record CacheState.

@@ -17,19 +17,24 @@ products are hexkv's too (``ops.norm_linear``, ``ops.norm_rope_linear``), with
 the norm before and the rotary or SwiGLU after them in the same launch.  Every
 KV byte moves through hexkv.  With ``weight_bits`` 4 the layers' matrices are
 rounded to four bits when the host is built and multiplied by ``fp4.linear``
-(the embedding, the norms and the LM head stay as they are).
+(the embedding, the norms and the LM head stay as they are).  With
+``page_size`` the caches are pools of pages, and a layer's rotation, append and
+attention two launches (``forward_pages``, which also takes single tokens and
+chunks of prompts of several sequences in one call).
 """
 from __future__ import annotations
 
 import json
 from dataclasses import dataclass
 from pathlib import Path
+from typing import Optional, Sequence
 
 import torch
 import torch.nn.functional as F
 
-from . import fp4, ops
-from .mha import FlashCrossAttention, _apply_rotary_single_query_attention, _update_kv_cache, update_and_attend
+from . import fp4, ops, paged, rotary
+from .mha import (FlashCrossAttention, _apply_rotary_single_query_attention, _page_size, _update_kv_cache, layer_pages,
+                  paged_sequences, update_and_attend)
 
 
 @dataclass
@@ -44,6 +49,7 @@ class LlamaShape:
     rope_theta: float = 10000.0
     max_position_embeddings: int = 2048
     tie_word_embeddings: bool = False
+    rope_scaling: Optional[dict] = None
 
     @property
     def head_dim(self) -> int:
@@ -51,8 +57,11 @@ class LlamaShape:
 
     @classmethod
     def from_config(cls, config: dict) -> "LlamaShape":
-        if config.get("model_type") != "llama" or config.get("rope_scaling") is not None:
-            raise ValueError("This baseline supports Llama architecture without RoPE scaling")
+        if config.get("model_type") != "llama":
+            raise ValueError("This baseline supports Llama architecture")
+        scaling = config.get("rope_scaling") or config.get("rope_parameters")
+        if rotary.kind_of(scaling) == "default":
+            scaling = None
         theta = config.get("rope_theta")
         if theta is None:
             theta = (config.get("rope_parameters") or {}).get("rope_theta", 10000.0)
@@ -63,7 +72,7 @@ class LlamaShape:
                    num_key_value_heads=config.get("num_key_value_heads") or config["num_attention_heads"],
                    rms_norm_eps=config.get("rms_norm_eps", 1e-6), rope_theta=float(theta),
                    max_position_embeddings=config.get("max_position_embeddings", 2048),
-                   tie_word_embeddings=bool(config.get("tie_word_embeddings", False)))
+                   tie_word_embeddings=bool(config.get("tie_word_embeddings", False)), rope_scaling=scaling)
 
 
 def read_config(model_dir) -> dict:
@@ -108,9 +117,15 @@ class LlamaHost:
                     layer[name] = fp4.quantize(layer[name])
             del w
         d = shape.head_dim
-        self.inv_freq = 1.0 / (shape.rope_theta ** (torch.arange(0, d, 2, device=self.device,
-                                                                  dtype=torch.float32) / d))
-        self.scale = d ** -0.5  # gpt.py:72
+        if shape.rope_scaling is None:
+            self.inv_freq = 1.0 / (shape.rope_theta ** (torch.arange(0, d, 2, device=self.device,
+                                                                      dtype=torch.float32) / d))
+            turned = 1.0
+        else:
+            self.inv_freq, turned = rotary.frequencies(d, shape.rope_theta, shape.rope_scaling,
+                                                       shape.max_position_embeddings, self.device)
+        # gpt.py:72.  All dims of q and k turn, so that a factor on sines and cosines is its square on the scores.
+        self.scale = d ** -0.5 * turned ** 2
         self.attn = FlashCrossAttention(causal=True, softmax_scale=self.scale)
 
     @classmethod
@@ -163,6 +178,12 @@ class LlamaHost:
             b0 = inference_params.batch_size_offset
             positions = inference_params.lengths_per_sample[b0:b0 + batch].to(torch.int32).contiguous()
         heads, kv_heads = s.num_attention_heads, s.num_key_value_heads
+        if inference_params.fused_ft_kernel and s.rope_scaling is not None:
+            raise ValueError("the FT caches' attention rotates by its base alone, without RoPE scaling")
+        if _page_size(inference_params):
+            tables, starts, bound = paged_sequences(inference_params, batch, seqlen, self.device)
+            pages = [layer_pages(inference_params, i, kv_heads, d, self.dtype, self.device) for i in range(len(self.layers))]
+            return self.forward_pages(input_ids, pages, tables, starts, max_seqlen=bound, last_token_only=last_token_only)
         h = F.embedding(input_ids, self.embed)
         y = None  # the block output still to be added to h
         for i, layer in enumerate(self.layers):
@@ -189,5 +210,31 @@ class LlamaHost:
             x, h = self._norm_linear(h, y, layer["ln2"], layer["gate_up"], glu=True)
             y = self._linear(x, layer["down"])
         if last_token_only:
+            h, y = h[:, -1], None if y is None else y[:, -1]
+        return self._norm_linear(h, y, self.norm, self.lm_head, keep_sum=False)[0]
+
+    @torch.inference_mode()
+    def forward_pages(self, input_ids: torch.Tensor, pages: Sequence[torch.Tensor], tables: torch.Tensor,
+                      starts: torch.Tensor, *, max_seqlen: int, cu_tokens: Optional[torch.Tensor] = None,
+                      max_tokens: int = 1, last_token_only: bool = False, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Logits of new tokens over paged caches, one pool a layer: ``input_ids [batch,
+        tokens]``, or with ``cu_tokens`` ``[1, tokens]`` of the sequences it bounds, at
+        the positions from ``starts`` on (all as in ``paged``).  ``last_token_only``: of each
+        row's last token; ``rows``: of these tokens (indices into the flattened ``input_ids``)."""
+        s = self.shape
+        h = F.embedding(input_ids, self.embed)
+        y = None  # the block output still to be added to h
+        for layer, pool in zip(self.layers, pages):
+            qkv, h = self._norm_linear(h, y, layer["ln1"], layer["wqkv"])
+            q = paged.append(qkv, pool, tables, starts, q_heads=s.num_attention_heads, cu_tokens=cu_tokens,
+                             inv_freq=self.inv_freq)
+            context = paged.attention(q, pool, tables, starts, max_seqlen=max_seqlen, cu_tokens=cu_tokens,
+                                      max_tokens=max_tokens, softmax_scale=self.scale, out=q)
+            y = self._linear(context.flatten(-2), layer["wo"])
+            x, h = self._norm_linear(h, y, layer["ln2"], layer["gate_up"], glu=True)
+            y = self._linear(x, layer["down"])
+        if rows is not None:
+            h, y = h.flatten(0, -2)[rows], None if y is None else y.flatten(0, -2)[rows]
+        elif last_token_only:
             h, y = h[:, -1], None if y is None else y[:, -1]
         return self._norm_linear(h, y, self.norm, self.lm_head, keep_sum=False)[0]

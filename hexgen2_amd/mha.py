@@ -23,7 +23,7 @@ from typing import Optional
 import torch
 from torch import nn
 
-from . import fp4, ops
+from . import fp4, ops, paged
 
 
 def inference_cache(batch_size: int, max_seqlen: int, num_heads_kv: int, head_dim: int,
@@ -53,6 +53,8 @@ def inference_cache(batch_size: int, max_seqlen: int, num_heads_kv: int, head_di
 _SEQLENS_ATTR = "_hexkv_seqlens"
 # Attribute of a 4-bit cache view: its KV heads, which its shape does not tell.
 _HEADS_ATTR = "_hexkv_kv_heads"
+# Attribute of a pool of pages _update_kv_cache returns: (tables, starts, bound) of its sequences.
+_PAGES_ATTR = "_hexkv_pages"
 
 
 def _sample_positions(inference_params, batch_start: int, batch_end: int) -> Optional[torch.Tensor]:
@@ -79,6 +81,55 @@ def _sample_positions(inference_params, batch_start: int, batch_end: int) -> Opt
 def _kv_bits(inference_params) -> int:
     """Bits of the caches (the reference's own ``InferenceParams`` has no such field)."""
     return getattr(inference_params, "kv_bits", 16)
+
+
+def _page_size(inference_params) -> int:
+    """Positions of a page, 0 for caches that are not paged."""
+    return getattr(inference_params, "page_size", 0)
+
+
+def paged_sequences(inference_params, batch: int, tokens: int, device):
+    """``(tables, starts, bound)`` of a step that brings ``tokens`` new tokens to
+    each of ``batch`` sequences: their rows of ``page_tables`` (made, in order, on first
+    use), the positions their tokens start at (``lengths_per_sample`` after
+    the prompt, else ``sequence_len_offset`` for all) and the most rows one may have."""
+    if inference_params.fused_ft_kernel or _kv_bits(inference_params) != 16:
+        raise ValueError("paged caches hold the data type, in pages of their own (no FT layout, no four bits)")
+    start, end = inference_params.batch_size_offset, inference_params.batch_size_offset + batch
+    bound = inference_params.sequence_len_offset + tokens
+    assert end <= inference_params.max_batch_size and bound <= inference_params.max_sequence_len
+    if inference_params.page_tables is None:
+        width = paged.pages_for(inference_params.max_sequence_len, _page_size(inference_params))
+        inference_params.page_tables = torch.arange(inference_params.max_batch_size * width, dtype=torch.int32,
+                                                    device=device).view(-1, width)
+    starts = _sample_positions(inference_params, start, end)
+    if starts is None:
+        starts = torch.full((batch,), inference_params.sequence_len_offset, dtype=torch.int32, device=device)
+    return _batch_rows(inference_params.page_tables, start, end), starts, bound
+
+
+def layer_pages(inference_params, layer_idx: int, num_heads_kv: int, head_dim: int, dtype: torch.dtype, device):
+    """Layer ``layer_idx``'s pool of pages, allocated on first use with as many pages
+    as the tables of ``max_batch_size`` sequences of ``max_sequence_len`` name."""
+    pages = inference_params.key_value_memory_dict.get(layer_idx)
+    if pages is None:
+        count = inference_params.max_batch_size * paged.pages_for(inference_params.max_sequence_len,
+                                                                  _page_size(inference_params))
+        pages = paged.kv_pages(count, _page_size(inference_params), num_heads_kv, head_dim, dtype, device)
+        inference_params.key_value_memory_dict[layer_idx] = pages
+    return pages
+
+
+def _update_pages(kv: torch.Tensor, inference_params, layer_idx: int) -> torch.Tensor:
+    """``_update_kv_cache`` into a paged cache: the layer's pool, with what
+    ``FlashCrossAttention`` needs to attend these sequences' rows in it."""
+    batch, seqlen, _, num_heads, head_dim = kv.shape
+    tables, starts, bound = paged_sequences(inference_params, batch, seqlen, kv.device)
+    pages = layer_pages(inference_params, layer_idx, num_heads, head_dim, kv.dtype, kv.device)
+    paged.append(kv.contiguous().view(batch, seqlen, -1), pages, tables, starts, q_heads=0)
+    view = pages[:]
+    setattr(view, _PAGES_ATTR, (tables, starts, bound))
+    return view
 
 
 def _batch_rows(cache: torch.Tensor, start: int, end: int) -> torch.Tensor:
@@ -110,7 +161,13 @@ def _update_kv_cache(kv: torch.Tensor, inference_params, layer_idx: int) -> torc
     the view is the 4-bit cache's, which ``FlashCrossAttention`` attends as
     it attends the other; the prompt (``sequence_len_offset`` 0) gets ``kv``
     back, as on the FT path: it attends its own keys as they were computed
-    (with ``attend_stored``: the view, as they were stored)."""
+    (with ``attend_stored``: the view, as they were stored).
+
+    With ``page_size`` the rows go into the layer's pool of pages, which is
+    returned and attended likewise; chunks of a prompt may follow one another
+    (``sequence_len_offset`` > 0 with several tokens)."""
+    if _page_size(inference_params):
+        return _update_pages(kv, inference_params, layer_idx)
     kv_bits = _kv_bits(inference_params)
     if inference_params.fused_ft_kernel and kv_bits == 16:
         return _update_ft_cache(kv, inference_params, layer_idx)
@@ -238,6 +295,12 @@ class FlashCrossAttention(nn.Module):
             raise NotImplementedError("variable-length (cu_seqlens) attention is not supported")
         causal = self.causal if causal is None else causal
         batch_size = q.shape[0]
+        sequences = getattr(kv, _PAGES_ATTR, None)
+        if sequences is not None:  # a pool of pages
+            tables, starts, bound = sequences
+            assert seqlens_k is None and tables.shape[0] == batch_size
+            return paged.attention(q.contiguous(), kv, tables, starts, max_seqlen=bound,
+                                   causal=bool(causal) and q.shape[1] > 1, softmax_scale=self.softmax_scale)
         seqlen_k = kv.shape[1]
         heads_k = getattr(kv, _HEADS_ATTR, None)  # (set: a 4-bit cache)
         assert kv.shape[0] == batch_size and (heads_k is not None or kv.shape[4] == q.shape[3])
@@ -278,7 +341,12 @@ def update_and_attend(q: torch.Tensor, kv: torch.Tensor, inference_params, layer
     kv (B, 1, 2, H_k, D).  With ``lengths_per_sample`` set, row b is written
     at ``lengths_per_sample[b]`` and attends that many keys plus the new one;
     ``sequence_len_offset`` bounds every sample's position (checked on the
-    device, reported by ``check_kv_status``)."""
+    device, reported by ``check_kv_status``).  Into pages (``page_size``) it is two launches."""
+    if _page_size(inference_params):
+        assert kv.shape[1] == 1 and q.shape[1] == 1
+        view = _update_pages(kv, inference_params, layer_idx)
+        tables, starts, bound = getattr(view, _PAGES_ATTR)
+        return paged.attention(q.contiguous(), view, tables, starts, max_seqlen=bound, softmax_scale=softmax_scale)
     cache = inference_params.key_value_memory_dict[layer_idx]
     batch_start = inference_params.batch_size_offset
     batch_end = batch_start + kv.shape[0]

@@ -140,7 +140,7 @@ def _append_form(qkv, pages, tables, starts, cu_tokens, q_heads, inv_freq, inter
     pool = _check_pages(pages, True)
     device, d = qkv.device, pool.head_dim
     width = (q_heads + 2 * pool.kv_heads) * d
-    if qkv.dtype != pages.dtype or device != pages.device or qkv.dim() < 1 or q_heads < 1 or qkv.shape[-1] != width:
+    if qkv.dtype != pages.dtype or device != pages.device or qkv.dim() < 1 or q_heads < 0 or qkv.shape[-1] != width:
         raise ValueError(f"qkv must be [..., {width}] ({q_heads} + 2 x {pool.kv_heads} heads of {d}) like the pages, got "
                          f"{tuple(qkv.shape)} {qkv.dtype} on {device}")
     p = _lib.PagedAppendParams()
@@ -169,7 +169,8 @@ def append(qkv: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, starts:
     """Rotate the new tokens' q and k heads to their positions, write k and v into
     the pages and return q, ``[..., q_heads, head_dim]`` (one launch).
 
-    ``qkv [..., (q_heads + 2 kv_heads) * head_dim]`` are the joined product's rows.
+    ``qkv [..., (q_heads + 2 kv_heads) * head_dim]`` are the joined product's rows
+    (``q_heads`` 0: k and v alone).
     The first ``2 * len(inv_freq)`` dims of a head turn (None: no rotation), pair j by
     ``position * inv_freq[j]``, in pairs (j, j + half) or with ``interleaved`` (2j, 2j + 1); sines
     and cosines are multiplied by ``rotary_scale``.  (``rotary.frequencies`` makes these
@@ -186,7 +187,7 @@ def append(qkv: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, starts:
     p = _lib.PagedAppendParams.from_buffer_copy(form[0])
     if out is None:
         out = qkv.new_empty(form[1])
-    p.qkv, p.q, p.pages = qkv.data_ptr(), out.data_ptr(), pages.data_ptr()
+    p.qkv, p.q, p.pages = qkv.data_ptr(), out.data_ptr() if q_heads else None, pages.data_ptr()
     seqs = p.seqs
     seqs.tables, seqs.starts = tables.data_ptr(), starts.data_ptr()
     if cu_tokens is not None:
@@ -230,7 +231,7 @@ def attention(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, starts
     ``max_tokens`` its new tokens: both are host values that size the launch.
     Softmax sums are fp32.  ``out`` may be ``q``; tokens of no sequence are left as they
     were in it, those of a sequence not in use become zero.  ``partition``: rows
-    per partition of a split row, a multiple of 128 (0: the library's choice); ``workspace``:
+    per partition of a split row, a multiple of 64 (0: the library's choice); ``workspace``:
     scratch that no overlapping call shares (default: one of this call's own)."""
     _require_device(q, pages, tables, starts)
     softmax_scale = None if softmax_scale is None else float(softmax_scale)

@@ -166,7 +166,8 @@ class Pilot:
         self.handoff = "host wire" if args.wire else "device memory (IPC)"
         self.channel = None if args.wire else IpcChannel()
         self.engine = Engine(args.model_dir, args.engine, "cuda", args.dtype, fused_append=args.fused_append,
-                             kv_bits=args.kv_bits, weight_bits=args.weight_bits)
+                             kv_bits=args.kv_bits, weight_bits=args.weight_bits, page_size=args.page_size,
+                             prefill_chunk=args.prefill_chunk)
         cfg = self.engine.config
         self.requests = read_trace(args.trace, args.model_dir, cfg.max_position_embeddings, cfg.vocab_size)
 
@@ -174,7 +175,8 @@ class Pilot:
         """What both ranks must agree on before the first request."""
         trace = json.dumps([asdict(r) for r in self.requests], sort_keys=True)
         settings = {k: getattr(self.args, k) for k in ("engine", "dtype", "seed", "warmup", "profile_first",
-                                                        "fused_append", "kv_bits", "weight_bits", "logprobs", "wire")}
+                                                        "fused_append", "kv_bits", "weight_bits", "page_size", "prefill_chunk",
+                                                        "logprobs", "wire")}
         settings["trace_sha256"] = hashlib.sha256(trace.encode()).hexdigest()
         settings["model"] = self.engine.identity["sha256"]
         return hashlib.sha256(json.dumps(settings, sort_keys=True).encode()).hexdigest()
@@ -295,6 +297,10 @@ def parse_args(argv=None):
                     help="keep and hand over the caches in the data type or in four bits")
     ap.add_argument("--weight-bits", type=int, choices=[16, 4], default=16,
                     help="hold the layers' matrices in the data type or in four bits")
+    ap.add_argument("--page-size", type=int, default=0,
+                    help="keep the caches in pages of so many positions (a power of two from 16 on)")
+    ap.add_argument("--prefill-chunk", type=int, default=0,
+                    help="with --page-size: prefill a prompt in chunks of so many tokens")
     ap.add_argument("--logprobs", action="store_true",
                     help="record the decoded tokens' log-probabilities and entropies")
     ap.add_argument("--wire", action="store_true",

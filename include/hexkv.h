@@ -809,7 +809,7 @@ typedef struct hexkv_paged_batch {
 typedef struct hexkv_paged_append_params {
   hexkv_pool pool;
   hexkv_paged_batch seqs;
-  int q_heads;
+  int q_heads;            /* 0: qkv holds k and v alone */
   const void *qkv;        /* [tokens] rows of (q_heads + 2 kv_heads) heads: q, k, v */
   int64_t qkv_stride;     /* elements from row to row */
   void *q;                /* [tokens][q_heads][head_dim], rotated; may be the q heads of qkv themselves */
@@ -843,7 +843,7 @@ typedef struct hexkv_paged_attend_params {
   void *out;              /* like q, and may be q */
   int64_t out_stride;
   const void *pages;
-  int32_t partition;      /* rows per partition of a split row, a multiple of 128; 0: the library's choice */
+  int32_t partition;      /* rows per partition of a split row, a multiple of 64; 0: the library's choice */
 } hexkv_paged_attend_params;
 
 /*

@@ -237,14 +237,14 @@ def check_attend(device, dtype, geometry, new, starts, page, causal=True, unifor
 def test_decode_rows(device, dtype, geometry):
     check_attend(device, dtype, geometry, [1] * 9, [0, 1, 14, 15, 16, 31, 32, 100, 255], 16, uniform=True)
     check_attend(device, dtype, geometry, [1, 1, 1], [640, 0, 333], 64, order="rows", seed=5)
-    check_attend(device, dtype, geometry, [1, 1, 1], [640, 0, 333], 128, order="apart", seed=6, partition=128)
+    check_attend(device, dtype, geometry, [1, 1, 1], [640, 0, 333], 128, order="apart", seed=6, partition=64)
 
 
 @pytest.mark.parametrize("dtype,geometry", itertools.product(DTYPES, GEOMETRIES))
 @pytest.mark.parametrize("causal", [True, False])
 def test_chunks(device, dtype, geometry, causal):
     check_attend(device, dtype, geometry, [3, 1, 40, 2], [0, 20, 5, 99], 16, causal)
-    check_attend(device, dtype, geometry, [37, 5], [0, 300], 32, causal, order="rows", partition=128)
+    check_attend(device, dtype, geometry, [37, 5], [0, 300], 32, causal, order="rows", partition=64)
     check_attend(device, dtype, geometry, [8, 8], [33, 0], 16, causal, uniform=True, order="apart")
 
 
@@ -254,8 +254,8 @@ def test_long_chunks(device, dtype, geometry):
     """Chunks of more rows than a tile, over keys that end inside pages and tiles."""
     check_attend(device, dtype, geometry, [150, 1, 65], [0, 200, 77], 16)
     check_attend(device, dtype, geometry, [129, 130], [63, 321], 128, order="rows")
-    check_attend(device, dtype, geometry, [140, 3, 1], [250, 130, 31], 32, partition=128)
-    check_attend(device, dtype, geometry, [140], [250], 32, causal=False, partition=128)
+    check_attend(device, dtype, geometry, [140, 3, 1], [250, 130, 31], 32, partition=64)
+    check_attend(device, dtype, geometry, [140], [250], 32, causal=False, partition=64)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -551,12 +551,12 @@ def test_calls_on_another_stream(device):
     pool = make_pool((hq, h, d), page, count, 2, torch.bfloat16, device)
     q = randn((2, hq, d), 3, torch.bfloat16, device)
     starts = int32([499, 299], device)
-    want = paged.attention(q, pool, tables, starts, max_seqlen=500, partition=128)
+    want = paged.attention(q, pool, tables, starts, max_seqlen=500, partition=64)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        parts = [paged.attention(q, pool, tables, starts, max_seqlen=500, partition=128) for _ in range(8)]
-    here = [paged.attention(q, pool, tables, starts, max_seqlen=500, partition=128) for _ in range(8)]
+        parts = [paged.attention(q, pool, tables, starts, max_seqlen=500, partition=64) for _ in range(8)]
+    here = [paged.attention(q, pool, tables, starts, max_seqlen=500, partition=64) for _ in range(8)]
     side.synchronize()
     assert all(torch.equal(t, want) for t in parts + here)
 
