@@ -58,4 +58,10 @@ inline int elem_bytes(int dtype) { return dtype == HEXKV_F32 ? 4 : 2; }
 // Bytes from the pool's base to the end of its last element.
 int64_t pool_bytes(const hexkv_pool &pool);
 
+// Whether [a, a + a_bytes) and [b, b + b_bytes) share a byte.
+inline bool overlap(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
+  const intptr_t x = reinterpret_cast<intptr_t>(a), y = reinterpret_cast<intptr_t>(b);
+  return a_bytes > 0 && b_bytes > 0 && x < y + b_bytes && y < x + a_bytes;
+}
+
 }  // namespace hexkv

@@ -39,7 +39,8 @@ int64_t pool_bytes(const hexkv_pool &pool) {
 static int check_table(const int32_t *tables, int64_t stride, int width, int batch, int page_size, const char *what) {
   if (batch < 0 || width < 0) return fail(HEXKV_EINVAL, "%s: negative batch or table width", what);
   if (batch && width && !tables) return fail(HEXKV_EINVAL, "%s: null tables", what);
-  if (batch > 1 && stride < width) return fail(HEXKV_EINVAL, "%s: table rows overlap", what);
+  // (stride 0: one table for all)
+  if (batch > 1 && stride != 0 && stride < width) return fail(HEXKV_EINVAL, "%s: table rows overlap", what);
   if (static_cast<int64_t>(width) * page_size > INT64_C(1) << 30)
     return fail(HEXKV_ERANGE, "%s: tables of more than 2^30 positions", what);
   return HEXKV_OK;
@@ -370,12 +371,6 @@ static int paged_copy(bool pack, const hexkv_pool *pool, const void *const *src,
     for (int b = 0; b < nb; ++b) base += lens[b0 + b];
   }
   return HEXKV_OK;
-}
-
-// Whether [a, a + a_bytes) and [b, b + b_bytes) share a byte.
-static bool overlap(const void *a, int64_t a_bytes, const void *b, int64_t b_bytes) {
-  const intptr_t x = reinterpret_cast<intptr_t>(a), y = reinterpret_cast<intptr_t>(b);
-  return a_bytes > 0 && b_bytes > 0 && x < y + b_bytes && y < x + a_bytes;
 }
 
 }  // namespace hexkv

@@ -1124,10 +1124,23 @@ extern "C" int hexkv_paged_attend(const hexkv_paged_attend_params *params, void 
   if (a.p.tokens == 0 || a.p.batch == 0 || a.max_tokens == 0) return HEXKV_OK;
   if (!a.q || !a.out || !a.pages) return fail(HEXKV_EINVAL, "%s: null tensor", what);
   if (!aligned16(a.q) || !aligned16(a.pages)) return fail(HEXKV_EINVAL, "%s: q or pages are not 16-byte aligned", what);
-  const int d = params->pool.head_dim;
+  const int d = params->pool.head_dim, es = elem_bytes(params->pool.dtype);
+  // A workgroup reads its rows of q before it writes them: out may be q, or lie
+  // beside it in the same rows, but not over other rows' q.
+  const int64_t row = static_cast<int64_t>(a.q_heads) * d, last = a.p.tokens - 1;
+  const int64_t q_bytes = (last * a.q_stride + row) * es, o_bytes = (last * a.o_stride + row) * es, pool = pool_bytes(params->pool);
+  if (overlap(a.out, o_bytes, a.q, q_bytes) && (last || a.out != a.q)) {
+    const int64_t step = a.q_stride * es, apart = static_cast<const char *>(a.out) - static_cast<const char *>(a.q);
+    const int64_t shift = last ? (apart % step + step) % step : 0;
+    if (!last || a.q_stride != a.o_stride || (apart && (shift < row * es || step - shift < row * es)))
+      return fail(HEXKV_EINVAL, "%s: out overlaps other rows of q", what);
+  }
+  if (overlap(a.out, o_bytes, a.pages, pool)) return fail(HEXKV_EINVAL, "%s: out overlaps the pages", what);
   const size_t need = attend_workspace(a, d);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(HEXKV_EWORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", what, need, workspace_bytes);
+  if (overlap(workspace, need, a.q, q_bytes) || overlap(workspace, need, a.out, o_bytes) || overlap(workspace, need, a.pages, pool))
+    return fail(HEXKV_EINVAL, "%s: the workspace overlaps a tensor", what);
   if (need) {
     const int64_t few = few_slots(a), tile = tile_slots(a);
     a.ws_o = static_cast<float *>(workspace);

@@ -799,7 +799,7 @@ typedef struct hexkv_pool {
  */
 typedef struct hexkv_paged_batch {
   const int32_t *tables;   /* device, [batch] rows of table_width entries */
-  int64_t table_stride;    /* entries from row to row */
+  int64_t table_stride;    /* entries from row to row (0: one for all) */
   int32_t table_width, batch;
   const int32_t *starts;   /* device, [batch] */
   const int32_t *cu_tokens; /* device, [batch + 1], or NULL */
@@ -840,7 +840,7 @@ typedef struct hexkv_paged_attend_params {
   int32_t max_seqlen;     /* bound on a sequence's rows, its new ones included */
   const void *q;          /* [tokens][q_heads][head_dim], rows 16-byte aligned */
   int64_t q_stride;       /* elements from row to row */
-  void *out;              /* like q, and may be q */
+  void *out;              /* like q, and may be q; else apart from q's elements and the pages */
   int64_t out_stride;
   const void *pages;
   int32_t partition;      /* rows per partition of a split row, a multiple of 64; 0: the library's choice */
@@ -861,7 +861,10 @@ size_t hexkv_paged_attend_workspace_bytes(const hexkv_paged_attend_params *param
  * hexkv_pack / hexkv_unpack for pools: rows [0, lens[b]) of every sequence of
  * every layer between the pages and [sum(lens)][2][kv_heads][head_dim] per
  * layer, one launch for up to HEXKV_MAX_LAYERS_PER_LAUNCH layers that share
- * the tables.  `pages` and `packed` are host arrays of device addresses.
+ * the tables.  `pages` and `packed` are host arrays of device addresses; what is
+ * written must not overlap what is read, and no two sequences of an unpack share a
+ * page below their lengths.  Rows of a page outside the pool are packed as zeros,
+ * not unpacked, and flagged HEXKV_STATUS_PAGE.
  */
 int hexkv_paged_pack(const hexkv_pool *pool, const void *const *pages, void *const *packed, int n_layers,
                      const int32_t *tables_dev, int64_t table_stride, int table_width, int batch, const int64_t *lens,

@@ -226,6 +226,20 @@ def test_append_refuses(changes, code, match):
     (dict(partition=32), _lib.HEXKV_EINVAL, "multiple of 64"),
     (dict(partition=-64), _lib.HEXKV_EINVAL, "multiple of 64"),
     (dict(out=None), _lib.HEXKV_EINVAL, "null"),
+    (dict(out=Q + 64), _lib.HEXKV_EINVAL, "rows of q"),
+    (dict(out=Q + 2 * 4 * 64), _lib.HEXKV_EINVAL, "rows of q"),
+    (dict(out=Q - 2 * 4 * 64), _lib.HEXKV_EINVAL, "rows of q"),
+    (dict(out=Q, out_stride=8 * 64), _lib.HEXKV_EINVAL, "rows of q"),
+    (dict(out=Q + 2 * 4 * 64 - 2, q_stride=8 * 64, out_stride=8 * 64), _lib.HEXKV_EINVAL, "rows of q"),
+    (dict(out=Q + 2 * 4 * 64 + 2, q_stride=8 * 64, out_stride=8 * 64), _lib.HEXKV_EINVAL, "rows of q"),
+    (dict(out=Q + 64, seqs=seqs(tokens=1, batch=1)), _lib.HEXKV_EINVAL, "rows of q"),
+    (dict(out=PAGES), _lib.HEXKV_EINVAL, "overlaps the pages"),
+    (dict(out=PAGES + 2 * 8 * 2 * 2 * 16 * 64 - 2), _lib.HEXKV_EINVAL, "overlaps the pages"),
+    # sizes past the launch's: 2^31 rows, 2^24 workgroups
+    (dict(pool=pool(kv_heads=1), q_heads=1 << 16, q_stride=64 << 16, out_stride=64 << 16, seqs=seqs(tokens=1 << 16), max_tokens=1 << 16),
+     _lib.HEXKV_ERANGE, "rows"),
+    (dict(pool=pool(kv_heads=1, dtype=_lib.HEXKV_F32), q_heads=1 << 10, q_stride=64 << 10, out_stride=64 << 10,
+          seqs=seqs(tokens=1 << 19), max_tokens=1 << 19), _lib.HEXKV_ERANGE, "workgroups"),
 ])
 def test_attention_refuses(changes, code, match):
     refused(lambda lib: lib.hexkv_paged_attend(ctypes.byref(attend_params(**changes)), None, 0, None), code, match)
@@ -240,6 +254,8 @@ def test_attention_refuses_a_missing_workspace():
     refused(lambda lib: lib.hexkv_paged_attend(ctypes.byref(p), None, 0, None), _lib.HEXKV_EWORKSPACE, "workspace")
     refused(lambda lib: lib.hexkv_paged_attend(ctypes.byref(p), QKV, need - 1, None), _lib.HEXKV_EWORKSPACE, "workspace")
     refused(lambda lib: lib.hexkv_paged_attend(ctypes.byref(p), QKV + 4, need, None), _lib.HEXKV_EWORKSPACE, "workspace")
+    for at in (Q, QKV, PAGES + 4096, Q - need + 16):
+        refused(lambda lib: lib.hexkv_paged_attend(ctypes.byref(p), at, need, None), _lib.HEXKV_EINVAL, "workspace overlaps")
     assert lib.hexkv_paged_attend_workspace_bytes(ctypes.byref(attend_params())) == 0  # short rows are not split
     assert lib.hexkv_paged_attend_workspace_bytes(ctypes.byref(attend_params(max_seqlen=65))) == 0
 
