@@ -14,16 +14,17 @@
 // 16-bit rows are loaded whole, 16 lanes a row, and pass through the wave's own
 // LDS (K, then V in the same place): loaded as K's operand takes it, in 64 bytes of
 // each of 16 rows, a line was asked for twice, and the loads could not be
-// nontemporal (Llama-3-8B decode batch 211 us, 224 nontemporal, against XXX).
+// nontemporal (Llama-3-8B decode batch 211 us, 224 nontemporal, against 185).
 // What bounds it: a decode row's K and V are read once, 4 D flops a key, so
 // memory.  Steps are loaded one ahead into registers, page numbers two ahead.
 //
 // Tile path (16-bit, head_dim 64 or 128, sequences of more than kFewRows rows):
-// 128 rows a workgroup, 32 a wave, which share tiles of 64 keys in LDS; the same
-// products on 32 x 32 x 16 matrix instructions.  What bounds it: the matrix cores, and
-// the softmax on the VALU beside them.  A probability enters P V as one 16-bit
-// term, rounded to nearest: an error of the order of the output's own rounding (that
-// of p averages over the keys), for two thirds of the matrix work.
+// 32 rows a wave, four or eight waves a workgroup (128 or 256 rows), which share tiles of
+// 16 keys a wave in LDS; the same products on 32 x 32 x 16 matrix instructions.  What
+// bounds it: the matrix cores, and the softmax on the VALU beside them.  A
+// probability enters P V as one 16-bit term, rounded to nearest: an error of the order
+// of the output's own rounding (that of p averages over the keys), for two thirds of
+// the matrix work.
 #include "hexkv_paged.h"
 
 #include <algorithm>
@@ -50,7 +51,7 @@ struct PagedAttendArgs {
   int32_t row_tiles, part, max_parts, row_blocks;
   // tile path: a bound on the tiles of all sequences, keys per partition and
   // partitions, and workgroups
-  int32_t tiles, tile_part, tile_parts, tile_blocks;
+  int32_t tiles, tile_part, tile_parts, tile_blocks, wide;
   // split rows: [pair][row][max_parts] and [token][head][tile_parts] of D sums, and of
   // (maximum, sum)
   float *ws_o, *ws_ml, *ws_tile_o, *ws_tile_ml;
@@ -147,7 +148,7 @@ __device__ __forceinline__ Place place_of(const PagedAttendArgs &a, int block, i
 
 // A sequence's table, read by scalar loads: a wave's lanes need the same page,
 // and a vector load's number would be waited for behind the rows loaded before it
-// (Llama-3-8B decode batch 217 us instead of XXX).
+// (Llama-3-8B decode batch 217 us instead of 185).
 typedef const __attribute__((address_space(4))) int32_t *ScalarTable;
 
 __device__ __forceinline__ ScalarTable scalar_table(const PagedAttendArgs &a, int b) {
@@ -290,19 +291,15 @@ __device__ void exact_row(const PagedAttendArgs &a, const T *q, int b, int hk, i
   *l_out = sum_from<1>(l);
 }
 
-constexpr int kRowWaves = 4;
-
 // LDS bytes of the row path: V as its waves turn it, then their sums.
-template <typename T, int D>
+template <typename T, int D, int W>
 constexpr int rows_lds() {
-  constexpr int W = kRowWaves;
   const int v = std::is_same<T, float>::value ? 0 : W * 32 * (2 * D + 32), o = W * 16 * (D + 4) * 4;
   return (v > o ? v : o) + 2 * W * 16 * 4 + 16;
 }
 
-template <typename T, int D>
+template <typename T, int D, int W>
 __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, char *s_mem) {
-  constexpr int W = kRowWaves;
   constexpr bool F32 = std::is_same<T, float>::value;
   using M = Mma<T>;
   constexpr int KEYS = F32 ? 16 : 32;       // keys of a step
@@ -316,7 +313,7 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
   constexpr int KP = 2 * D + 16;            // 16-bit: LDS bytes of a K row: 16 rows' chunks over all banks
   constexpr int VP = 2 * D + 32;            // of a V row: the 16 rows of a transposed read in two passes
   constexpr int OP = D + 4;                 // floats of a row in the join
-  constexpr int kMl = rows_lds<T, D>() - 2 * W * 16 * 4 - 16;
+  constexpr int kMl = rows_lds<T, D, W>() - 2 * W * 16 * 4 - 16;
   float(*s_m)[16] = reinterpret_cast<float(*)[16]>(s_mem + kMl), (*s_l)[16] = s_m + W;
   int &s_bad = *reinterpret_cast<int *>(s_mem + kMl + 2 * W * 16 * 4);
 
@@ -641,15 +638,19 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
 // ------------------------------------------------------------ tile path ---
 
 constexpr int kCus = 256;
-constexpr int kTileRows = 128, kTileKeys = 64;
 // A sequence of so many rows per KV head, or fewer, takes the row path.
 constexpr int kFewRows = 32;
 
-template <int D>
+// Rows a wave takes, and keys it computes at a time.
+constexpr int kWaveRows = 32, kStepKeys = 64;
+
+// W waves: 32 W rows, and tiles of 16 W keys, a block of 16 brought by each wave.
+template <int D, int W>
 struct TileLds {
+  static constexpr int KT = 16 * W;      // keys of a tile
   static constexpr int KP = 2 * D + 16;  // bytes per K row: 16 rows' chunks over all banks
   static constexpr int VP = 2 * D + 64;  // per V row: the 4 rows of a transposed read over all banks
-  static constexpr int kBytes = 2 * kTileKeys * (KP + VP) + 16;
+  static constexpr int kBytes = 2 * KT * (KP + VP) + 16;
 };
 
 // A wave, 32 rows, one per lane and half h:
@@ -659,15 +660,15 @@ struct TileLds {
 //   index of a 16-key step is key 4 h + e, then 8 + 4 h + e), V^T (A) comes from
 //   row-major LDS by transposing reads in the same order.
 // All of a lane's accumulators belong to its own row.
-template <typename T, int D>
+template <typename T, int D, int W>
 __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, char *s_mem) {
   using M = Mma<T>;
-  using L = TileLds<D>;
-  constexpr int KT = kTileKeys, NKB = KT / 32;
+  using L = TileLds<D, W>;
+  constexpr int KT = L::KT, NKB = kStepKeys / 32, kTileRows = kWaveRows * W;
   constexpr int NJ = D / 16;   // score steps
   constexpr int ND = D / 32;   // output blocks
   constexpr int CH = D / 8;    // 16-byte chunks of a head's row
-  static_assert(KT == 4 * 16, "a block of 16 rows a wave");
+  static_assert(KT % kStepKeys == 0, "whole steps");
   constexpr int KP = L::KP, VP = L::VP;
   char *s_k = s_mem, *s_v = s_mem + 2 * KT * KP;
   int &s_bad = *reinterpret_cast<int *>(s_mem + 2 * KT * (KP + VP));
@@ -690,7 +691,7 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
 
   // This wave's rows and this lane's; rows past the last repeat it.  A wave
   // without rows only stages.
-  const int wrow0 = row0 + wave * 32;
+  const int wrow0 = row0 + wave * kWaveRows;
   const bool idle = wrow0 >= total, live = wrow0 + c < total;
   const int row = min(wrow0 + c, total - 1), t = row / a.group, qh = hk * a.group + row - t * a.group;
   const int len = seq.keys(a, t), lim = min(len, p0 + a.tile_part);
@@ -743,9 +744,9 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
   const int s16 = lane & 15;
   const uint32_t v_read = static_cast<uint32_t>((4 * h + s16 / 4) * VP + ((lane >> 4) & 1) * 32 + (s16 % 4) * 8);
 
-  auto compute = [&](int buf, int k0) {
-    const char *from_k = s_k + (k_read + (buf ? KT * KP : 0));
-    auto *from_v = (__attribute__((address_space(3))) char *)s_v + (v_read + (buf ? KT * VP : 0));
+  auto compute = [&](int row, int k0) {  // keys at k0, rows of the LDS buffers from `row` on
+    const char *from_k = s_k + (k_read + row * KP);
+    auto *from_v = (__attribute__((address_space(3))) char *)s_v + (v_read + row * VP);
     f32x16 s[NKB];
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb) s[kb] = f32x16{};
@@ -754,7 +755,7 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb)
         s[kb] = M::mma32(*reinterpret_cast<const u32x4 *>(from_k + kb * 32 * KP + j * 32), qf[j], s[kb]);
-    if (k0 + KT > w_full) {
+    if (k0 + kStepKeys > w_full) {
       const int left = lim - k0 - 4 * h;
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb)
@@ -815,7 +816,9 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
         fetch(k0 + KT);
         find(k0 + 2 * KT);
       }
-      if (k0 < w_end) compute(buf, k0);
+#pragma unroll 1
+      for (int n = 0; n < KT; n += kStepKeys)
+        if (k0 + n < w_end) compute((buf ? KT : 0) + n, k0 + n);
       if (more) stage(buf ^ 1);
       buf ^= 1;
       __syncthreads();
@@ -890,24 +893,24 @@ constexpr bool has_tiles() {
 
 template <typename T, int D>
 __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void paged_rows_kernel(const PagedAttendArgs a) {
-  __shared__ __attribute__((aligned(16))) char s_mem[rows_lds<T, D>()];
-  rows_path<T, D>(a, blockIdx.x, s_mem);
+  __shared__ __attribute__((aligned(16))) char s_mem[rows_lds<T, D, 4>()];
+  rows_path<T, D, 4>(a, blockIdx.x, s_mem);
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void paged_tile_kernel(const PagedAttendArgs a) {
-  __shared__ __attribute__((aligned(16))) char s_mem[TileLds<D>::kBytes];
-  tile_path<T, D>(a, blockIdx.x, s_mem);
+template <typename T, int D, int W>
+__global__ __launch_bounds__(W * 64, 2) void paged_tile_kernel(const PagedAttendArgs a) {
+  __shared__ __attribute__((aligned(16))) char s_mem[TileLds<D, W>::kBytes];
+  tile_path<T, D, W>(a, blockIdx.x, s_mem);
 }
 
 // A call that may hold sequences of either kind: tiles first (they take longest).
-template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void paged_mixed_kernel(const PagedAttendArgs a) {
-  constexpr int kRows = rows_lds<T, D>(), kTiles = TileLds<D>::kBytes;
+template <typename T, int D, int W>
+__global__ __launch_bounds__(W * 64, 2) void paged_mixed_kernel(const PagedAttendArgs a) {
+  constexpr int kRows = rows_lds<T, D, W>(), kTiles = TileLds<D, W>::kBytes;
   __shared__ __attribute__((aligned(16))) char s_mem[kRows > kTiles ? kRows : kTiles];
   const int block = blockIdx.x;
-  if (block < a.tile_blocks) tile_path<T, D>(a, block, s_mem);
-  else rows_path<T, D>(a, block - a.tile_blocks, s_mem);
+  if (block < a.tile_blocks) tile_path<T, D, W>(a, block, s_mem);
+  else rows_path<T, D, W>(a, block - a.tile_blocks, s_mem);
 }
 
 // The partitions of a split row, joined: a wave a row.
@@ -986,6 +989,31 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAtt
 static int64_t ceil_div(int64_t n, int64_t by) { return (n + by - 1) / by; }
 static int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
+// Keys of a tile's partition.  A split fills the CUs evenly, and costs sums that
+// are written, read and joined.  A step of 64 keys (D = 128) takes a CU 1.42 us
+// for a lone tile of 128 rows, 2.25 for two at once, 2.0 for one of 256; a
+// partition's sums 0.026 us per 128 rows, the join 5.  With those, the least of
+// whole rows and of partitions that fill all CUs once to eight times: 512 rows of
+// 4 heads over 8192 keys on 8 KV heads 90 us in 4, 105 in 2, 173 whole; 1100 rows
+// over 31100 keys 606 for 878 whole; 1024 over 4096 whole 93, in two 99.  From two
+// tiles a CU on, causal rows' lengths even out by themselves (2500 rows over 4000
+// keys 150 whole, in two 204).
+static int64_t tile_partition(int64_t tiles, int64_t keys, bool wide) {
+  if (tiles >= 2 * kCus) return std::max<int64_t>(64, round_up(keys, 64));
+  const auto time = [&](int64_t parts) {
+    const int64_t steps = ceil_div(keys, 64 * parts) + 1, each = ceil_div(tiles * parts, kCus);
+    return steps * (wide ? each * 200 : each / 2 * 225 + each % 2 * 142) + (parts > 1 ? 500 + tiles * parts * (wide ? 52 : 26) / 10 : 0);
+  };
+  int64_t best = 1, least = time(1);
+  for (int64_t fill = 1; fill <= 8; ++fill) {
+    const int64_t parts = std::min(fill * kCus / std::max<int64_t>(tiles, 1), keys / 512);
+    if (parts < 2) continue;
+    const int64_t t = time(parts);
+    if (t < least) least = t, best = parts;
+  }
+  return std::max<int64_t>(64, round_up(ceil_div(keys, best), wide ? 128 : 64));
+}
+
 // Checks a call and fills its arguments but for addresses.
 static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs *a, const char *what) {
   if (!params) return fail(HEXKV_EINVAL, "%s: null argument", what);
@@ -1020,19 +1048,28 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   a->pos_bytes = static_cast<uint32_t>(p.pool.pos_stride * elem_bytes(p.pool.dtype));
   a->scale_log2 = p.softmax_scale * 1.44269504f;
   const int64_t rows = static_cast<int64_t>(a->max_tokens) * a->group;
-  if (rows > INT32_MAX - kTileRows) return fail(HEXKV_ERANGE, "%s: 2^31 rows or more", what);
+  if (rows > INT32_MAX - 256) return fail(HEXKV_ERANGE, "%s: 2^31 rows or more", what);
   // Which paths can have work: without cu_tokens every sequence has as many rows.
   const bool tiled = p.pool.dtype != HEXKV_F32 && (d == 64 || d == 128) && rows > kFewRows;
+  // Tiles of 256 rows read LDS and pages half as often, but one alone has a CU to
+  // itself from its first key to its last: chunks of 2048 over 8192 keys (32 heads
+  // on 8) 243 us for 252 with 128, of 512 84 for 90, of 8192 518 for 537; yet 2048
+  // rows from the first key on 66 for 59, 64 rows (256 of a KV head) over 8064 keys
+  // 31 for 25.  Workgroups of few rows are then one a CU too, so a call of more
+  // than four ragged sequences, which may be single tokens, keeps 128: a chunk of
+  // 2000 and 64 single tokens 804 us, with 256 rows a tile 829.
+  a->wide = tiled && d == 128 && rows >= 512 && p.max_seqlen >= 4096 && (!p.seqs.cu_tokens || p.seqs.batch <= 4);
+  const int64_t tile_rows = a->wide ? 256 : 128;
   const bool few = !tiled || p.seqs.cu_tokens;
   a->few_rows = tiled ? kFewRows : INT32_MAX;
   a->row_tiles = few ? static_cast<int32_t>((std::min<int64_t>(rows, a->few_rows) + 15) / 16) : 0;
   // Tiles of all sequences: without cu_tokens as they are, else at most one a
   // sequence more than full ones, of sequences with enough rows to have any.
   const int64_t batch = p.seqs.batch, all_rows = tokens * a->group;
-  int64_t few_tiles = batch * a->row_tiles, tiles = tiled ? batch * ((rows + kTileRows - 1) / kTileRows) : 0;
+  int64_t few_tiles = batch * a->row_tiles, tiles = tiled ? batch * ((rows + tile_rows - 1) / tile_rows) : 0;
   if (p.seqs.cu_tokens) {
     few_tiles = std::min(few_tiles, all_rows / 16 + std::min<int64_t>(batch, tokens));
-    tiles = std::min(tiles, all_rows / kTileRows + std::min<int64_t>(batch, all_rows / (kFewRows + 1)));
+    tiles = std::min(tiles, all_rows / tile_rows + std::min<int64_t>(batch, all_rows / (kFewRows + 1)));
   }
   // Partitions.  A CU alone takes 55 GB/s whatever its waves, so a row's keys are spread
   // over CUs, but for those of up to 128 KB of K, which end before a second
@@ -1048,10 +1085,10 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   part = std::max(part, round_up((p.max_seqlen + kMaxParts - 1) / kMaxParts, 128));
   a->part = static_cast<int32_t>(std::min<int64_t>(part, 1 << 30));
   a->max_parts = static_cast<int32_t>(std::max<int64_t>(1, (p.max_seqlen + part - 1) / part));
-  // Tiles are split where there are fewer than CUs, and no shorter than 512 keys: a partition's sums
-  // are written and read once more.
-  const int64_t full = (all_rows + kTileRows - 1) / kTileRows * a->kv_heads;
-  part = p.partition ? p.partition : std::max<int64_t>(512, round_up(ceil_div(p.max_seqlen, std::max<int64_t>(1, kCus / std::max<int64_t>(full, 1))), 64));
+  // Of ragged sequences, all but one taken for single tokens.
+  const int64_t long_rows = p.seqs.cu_tokens ? (std::max(tokens - batch, INT64_C(0)) + 1) * a->group : 0;
+  const int64_t full = (p.seqs.cu_tokens ? ceil_div(long_rows, tile_rows) : tiles) * a->kv_heads;
+  part = p.partition ? p.partition : tile_partition(full, p.max_seqlen, a->wide);
   part = std::max(part, round_up((p.max_seqlen + kMaxParts - 1) / kMaxParts, 64));
   a->tile_part = static_cast<int32_t>(std::min<int64_t>(part, 1 << 30));
   a->tile_parts = static_cast<int32_t>(std::max<int64_t>(1, (p.max_seqlen + part - 1) / part));
@@ -1082,8 +1119,12 @@ static void launch_attend(const PagedAttendArgs &a, hipStream_t s) {
   const unsigned rows = static_cast<unsigned>(a.row_blocks);
   const unsigned tiles = static_cast<unsigned>(a.tile_blocks);
   if constexpr (has_tiles<T, D>()) {
-    if (rows && tiles) paged_mixed_kernel<T, D><<<dim3(rows + tiles), 256, 0, s>>>(a);
-    else if (tiles) paged_tile_kernel<T, D><<<dim3(tiles), 256, 0, s>>>(a);
+    if constexpr (D == 128) {
+      if (a.wide && rows) paged_mixed_kernel<T, D, 8><<<dim3(rows + tiles), 512, 0, s>>>(a);
+      else if (a.wide) paged_tile_kernel<T, D, 8><<<dim3(tiles), 512, 0, s>>>(a);
+    }
+    if (tiles && rows && !a.wide) paged_mixed_kernel<T, D, 4><<<dim3(rows + tiles), 256, 0, s>>>(a);
+    else if (tiles && !a.wide) paged_tile_kernel<T, D, 4><<<dim3(tiles), 256, 0, s>>>(a);
   }
   if (!tiles) paged_rows_kernel<T, D><<<dim3(rows), 256, 0, s>>>(a);
   const int each = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(a.max_tokens) * a.group, a.row_tiles * 16));
