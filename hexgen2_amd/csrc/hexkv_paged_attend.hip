@@ -917,17 +917,16 @@ __global__ __launch_bounds__(W * 64, 2) void paged_mixed_kernel(const PagedAtten
 constexpr int kJoinThreads = 256;
 constexpr int kMaxParts = 512;
 
+// Sums are taken with the maximum as it rises, so that a row of up to kDepth
+// partitions waits for memory once.
 template <typename T, int D>
 __device__ __forceinline__ void join_row(const float *o_parts, const float *ml_parts, int parts, T *out) {
   const int lane = threadIdx.x & 63;
-  float top = -INFINITY;
-  for (int p = lane; p < parts; p += 64) top = fmaxf(top, ml_parts[p * 2]);
-  top = wave_max(top);
   constexpr int DPL = D >= 64 ? D / 64 : 1;
   typedef float vd __attribute__((ext_vector_type(DPL)));
   const int at = D >= 64 ? lane * DPL : lane & (D - 1);
   vd o = {};
-  float sum = 0.f;
+  float top = -INFINITY, sum = 0.f;
   constexpr int kDepth = 8;  // parts in flight
   for (int p0 = 0; p0 < parts; p0 += kDepth) {
     vd v[kDepth];
@@ -938,6 +937,13 @@ __device__ __forceinline__ void join_row(const float *o_parts, const float *ml_p
       v[k] = *reinterpret_cast<const vd *>(o_parts + p * D + at);
       ml[k] = *reinterpret_cast<const float2 *>(ml_parts + p * 2);
     }
+    float now = top;
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k) now = fmaxf(now, ml[k].x);
+    const float before = top == -INFINITY ? 0.f : exp2_of(top - now);
+    top = now;
+    o *= before;
+    sum *= before;
 #pragma unroll
     for (int k = 0; k < kDepth; ++k) {
       const float w = p0 + k >= parts || ml[k].x == -INFINITY ? 0.f : exp2_of(ml[k].x - top);
@@ -954,10 +960,10 @@ __device__ __forceinline__ void join_row(const float *o_parts, const float *ml_p
 // Rows of the row path first, `each` a sequence and KV head, then those of the tile
 // path, by token and head.
 template <typename T, int D>
-__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAttendArgs a, int64_t few, int each) {
-  int64_t id = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / 64) + (threadIdx.x >> 6);
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAttendArgs a, int few, int each) {
+  int id = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * (kJoinThreads / 64) + (threadIdx.x >> 6)));
   if (id < few) {
-    const int pair = static_cast<int>(id / each), row = static_cast<int>(id - static_cast<int64_t>(pair) * each);
+    const int pair = id / each, row = id - pair * each;
     const int b = pair / a.kv_heads, hk = pair - b * a.kv_heads;
     const Rows seq = rows_of(a, b);
     const int rows = seq.count * a.group;
@@ -970,7 +976,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAtt
     return;
   }
   id -= few;
-  const int token = static_cast<int>(id / a.q_heads), qh = static_cast<int>(id - static_cast<int64_t>(token) * a.q_heads);
+  const int token = id / a.q_heads, qh = id - token * a.q_heads;
   if (token >= a.p.tokens) return;
   const int b = a.p.cu ? token_sequence(a.p, token) : token / a.p.each;
   if (b < 0) return;
@@ -979,7 +985,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAtt
   if (t >= seq.count || seq.count * a.group <= a.few_rows) return;
   const int len = seq.keys(a, t);
   if (len <= a.tile_part) return;
-  const int64_t slot = id * a.tile_parts;
+  const int64_t slot = static_cast<int64_t>(id) * a.tile_parts;
   join_row<T, D>(a.ws_tile_o + slot * D, a.ws_tile_ml + slot * 2, (len + a.tile_part - 1) / a.tile_part,
                  static_cast<T *>(a.out) + token * a.o_stride + static_cast<int64_t>(qh) * D);
 }
@@ -1012,6 +1018,14 @@ static int64_t tile_partition(int64_t tiles, int64_t keys, bool wide) {
     if (t < least) least = t, best = parts;
   }
   return std::max<int64_t>(64, round_up(ceil_div(keys, best), wide ? 128 : 64));
+}
+
+// Split rows of either path.
+static int64_t split_few(const PagedAttendArgs &a) {
+  return a.max_parts > 1 ? static_cast<int64_t>(a.p.batch) * a.kv_heads * a.row_tiles * 16 : 0;
+}
+static int64_t split_tiled(const PagedAttendArgs &a) {
+  return a.tile_parts > 1 ? static_cast<int64_t>(a.p.tokens) * a.q_heads : 0;
 }
 
 // Checks a call and fills its arguments but for addresses.
@@ -1092,8 +1106,15 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   part = std::max(part, round_up((p.max_seqlen + kMaxParts - 1) / kMaxParts, 64));
   a->tile_part = static_cast<int32_t>(std::min<int64_t>(part, 1 << 30));
   a->tile_parts = static_cast<int32_t>(std::max<int64_t>(1, (p.max_seqlen + part - 1) / part));
-  if (!few) a->max_parts = 1;
+  // Where the tokens are so many that each sequence is a long one, unless some
+  // are left out, what few rows there may be are not split: no join is launched for
+  // them (5 us).
+  if (!few || (tiled && (tokens - (batch - 1) * a->max_tokens) * a->group > kFewRows)) {
+    a->part = 1 << 30;
+    a->max_parts = 1;
+  }
   if (!tiled) a->tile_parts = 1;
+  if (split_few(*a) + split_tiled(*a) > INT32_MAX) return fail(HEXKV_ERANGE, "%s: 2^31 split rows or more", what);
   const int64_t row_blocks = few_tiles * a->kv_heads * a->max_parts, tile_blocks = tiles * a->kv_heads * a->tile_parts;
   if (row_blocks + tile_blocks >= INT64_C(1) << 24) return fail(HEXKV_ERANGE, "%s: 2^24 workgroups or more", what);
   a->row_blocks = static_cast<int32_t>(row_blocks);
@@ -1102,13 +1123,9 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   return HEXKV_OK;
 }
 
-// Split rows of either path, each with its partitions' slots.
-static int64_t few_slots(const PagedAttendArgs &a) {
-  return a.max_parts > 1 ? static_cast<int64_t>(a.p.batch) * a.kv_heads * a.row_tiles * 16 * a.max_parts : 0;
-}
-static int64_t tile_slots(const PagedAttendArgs &a) {
-  return a.tile_parts > 1 ? static_cast<int64_t>(a.p.tokens) * a.q_heads * a.tile_parts : 0;
-}
+// ... each with its partitions' slots.
+static int64_t few_slots(const PagedAttendArgs &a) { return split_few(a) * a.max_parts; }
+static int64_t tile_slots(const PagedAttendArgs &a) { return split_tiled(a) * a.tile_parts; }
 
 static size_t attend_workspace(const PagedAttendArgs &a, int head_dim) {
   return static_cast<size_t>(few_slots(a) + tile_slots(a)) * (head_dim + 2) * sizeof(float);
@@ -1128,9 +1145,9 @@ static void launch_attend(const PagedAttendArgs &a, hipStream_t s) {
   }
   if (!tiles) paged_rows_kernel<T, D><<<dim3(rows), 256, 0, s>>>(a);
   const int each = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(a.max_tokens) * a.group, a.row_tiles * 16));
-  const int64_t few = a.max_parts > 1 ? static_cast<int64_t>(a.p.batch) * a.kv_heads * each : 0;
-  const int64_t tile = a.tile_parts > 1 ? static_cast<int64_t>(a.p.tokens) * a.q_heads : 0;
-  if (few + tile) paged_join_kernel<T, D><<<dim3(static_cast<unsigned>((few + tile + 3) / 4)), kJoinThreads, 0, s>>>(a, few, each);
+  const int few = a.max_parts > 1 ? a.p.batch * a.kv_heads * each : 0;
+  const int64_t joined = few + split_tiled(a);
+  if (joined) paged_join_kernel<T, D><<<dim3(static_cast<unsigned>((joined + 3) / 4)), kJoinThreads, 0, s>>>(a, few, each);
 }
 
 template <typename T>
