@@ -124,15 +124,13 @@ def _token_rows(shape, stride, dims: int, name: str):
 _FORMS: "OrderedDict[tuple, tuple]" = OrderedDict()
 
 
-def _form(key: tuple, make):
-    form = _FORMS.get(key)
-    if form is None:
-        form = _FORMS[key] = make()
-        while len(_FORMS) > 64:
-            try:
-                _FORMS.popitem(last=False)
-            except KeyError:  # another thread emptied it
-                break
+def _keep(key: tuple, form: tuple) -> tuple:
+    _FORMS[key] = form
+    while len(_FORMS) > 64:
+        try:
+            _FORMS.popitem(last=False)
+        except KeyError:  # another thread emptied it
+            break
     return form
 
 
@@ -178,12 +176,13 @@ def append(qkv: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, starts:
     lose nothing.  ``out`` may be q's part of ``qkv`` itself.  No two tokens may share a
     position of a page.  Tokens of no sequence, or of one not in use, are
     left as they were in ``out`` (and are not defined in a fresh one)."""
-    _require_device(qkv, pages, tables, starts)
     q_heads, rotary_scale = int(q_heads), float(rotary_scale)
     key = (_layout(qkv), _layout(pages), _layout(tables), _layout(starts), _layout(cu_tokens), _layout(inv_freq),
            _layout(out), q_heads, bool(interleaved), rotary_scale)
-    form = _form(key, lambda: _append_form(qkv, pages, tables, starts, cu_tokens, q_heads, inv_freq, interleaved,
-                                           rotary_scale, out))
+    form = _FORMS.get(key)
+    if form is None:
+        _require_device(qkv, pages, tables, starts)
+        form = _keep(key, _append_form(qkv, pages, tables, starts, cu_tokens, q_heads, inv_freq, interleaved, rotary_scale, out))
     p = _lib.PagedAppendParams.from_buffer_copy(form[0])
     if out is None:
         out = qkv.new_empty(form[1])
@@ -233,12 +232,13 @@ def attention(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, starts
     were in it, those of a sequence not in use become zero.  ``partition``: rows
     per partition of a split row, a multiple of 64 (0: the library's choice); ``workspace``:
     scratch that no overlapping call shares (default: one of this call's own)."""
-    _require_device(q, pages, tables, starts)
     softmax_scale = None if softmax_scale is None else float(softmax_scale)
     key = (_layout(q), _layout(pages), _layout(tables), _layout(starts), _layout(cu_tokens), _layout(out), int(max_tokens),
            bool(causal), softmax_scale, int(partition))
-    form = _form(key, lambda: _attend_form(q, pages, tables, starts, cu_tokens, max_tokens, causal, softmax_scale, out,
-                                           partition))
+    form = _FORMS.get(key)
+    if form is None:
+        _require_device(q, pages, tables, starts)
+        form = _keep(key, _attend_form(q, pages, tables, starts, cu_tokens, max_tokens, causal, softmax_scale, out, partition))
     p, needs = _lib.PagedAttendParams.from_buffer_copy(form[0]), form[1]
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
