@@ -653,6 +653,33 @@ struct TileLds {
   static constexpr int kBytes = 2 * KT * (KP + VP) + 16;
 };
 
+// The order of a block's matrix products and LDS reads.  Left alone the compiler reads a
+// product's operands just before it, into registers that the last product has freed,
+// and the matrix cores wait for each read (a chunk of 2048 over 8192 keys, its waves in
+// two phases as below, 341 us instead of 316).
+template <int N>
+__device__ __forceinline__ void order_reads() {
+  __builtin_amdgcn_sched_group_barrier(0x100, N, 0);
+}
+template <int N>
+__device__ __forceinline__ void order_products() {
+  __builtin_amdgcn_sched_group_barrier(0x008, N, 0);
+}
+template <int N, typename F>
+__device__ __forceinline__ void repeat(F f) {
+  if constexpr (N > 0) {
+    f();
+    repeat<N - 1>(f);
+  }
+}
+
+// A barrier that waits for this wave's LDS accesses and for nothing else.
+__device__ __forceinline__ void meet() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+}
+
 // A wave, 32 rows, one per lane and half h:
 //   S^T = K Q^T: K (A) from LDS, Q (B) in registers; lane (c, h) gets row c's
 //   scores of keys 8 i + 4 h + e.
@@ -744,10 +771,12 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
   const int s16 = lane & 15;
   const uint32_t v_read = static_cast<uint32_t>((4 * h + s16 / 4) * VP + ((lane >> 4) & 1) * 32 + (s16 % 4) * 8);
 
-  auto compute = [&](int row, int k0) {  // keys at k0, rows of the LDS buffers from `row` on
+  // A step, of the keys at k0, which are the LDS buffers' rows from `row` on: their
+  // scores, their probabilities, the sums of V.
+  f32x16 s[NKB];
+  u32x4 p[2 * NKB];
+  auto scores = [&](int row) {
     const char *from_k = s_k + (k_read + row * KP);
-    auto *from_v = (__attribute__((address_space(3))) char *)s_v + (v_read + row * VP);
-    f32x16 s[NKB];
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb) s[kb] = f32x16{};
 #pragma unroll
@@ -755,6 +784,8 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb)
         s[kb] = M::mma32(*reinterpret_cast<const u32x4 *>(from_k + kb * 32 * KP + j * 32), qf[j], s[kb]);
+  };
+  auto weigh = [&](int k0) {
     if (k0 + kStepKeys > w_full) {
       const int left = lim - k0 - 4 * h;
 #pragma unroll
@@ -781,7 +812,6 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
     }
     const float base = m == -INFINITY ? 0.f : -m;
     float l0 = 0.f, l1 = 0.f;
-    u32x4 p[2 * NKB];
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
@@ -792,6 +822,9 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
         p[2 * kb + i / 8][i % 8 / 2] = M::pair(e0, e1);
       }
     l += l0 + l1;
+  };
+  auto values = [&](int row) {
+    auto *from_v = (__attribute__((address_space(3))) char *)s_v + (v_read + row * VP);
 #pragma unroll
     for (int ks = 0; ks < 2 * NKB; ++ks)
 #pragma unroll
@@ -809,19 +842,72 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
     find(p0 + KT);
     stage(0);
     __syncthreads();
-    int buf = 0;
-    for (int k0 = p0; k0 < end; k0 += KT) {
-      const bool more = k0 + KT < end;
-      if (more) {
-        fetch(k0 + KT);
-        find(k0 + 2 * KT);
+    if constexpr (W == 4) {
+      int buf = 0;
+      for (int k0 = p0; k0 < end; k0 += KT) {
+        const bool more = k0 + KT < end;
+        if (more) {
+          fetch(k0 + KT);
+          find(k0 + 2 * KT);
+        }
+        if (k0 < w_end) {
+          scores(buf * KT);
+          order_reads<4>();
+          repeat<NKB * NJ - 4>([] { order_products<1>(), order_reads<1>(); });
+          order_products<4>();
+          weigh(k0);
+          values(buf * KT);
+          order_reads<2 * ND>();
+          repeat<(2 * NKB - 1) * ND>([] { order_products<1>(), order_reads<2>(); });
+          order_products<ND>();
+        }
+        if (more) stage(buf ^ 1);
+        buf ^= 1;
+        __syncthreads();
       }
+    } else {
+      // Waves w and w + 4 share a SIMD.  The second four run one phase behind, so that
+      // one of the two is at its products while the other is at its softmax (316 us for
+      // 324 with all in step; the products with their reads alone take 270, without reads 227):
+      // phase 2 i: products of step i (the last step's V, this one's scores), 2 i + 1: its
+      // softmax.  A tile is two steps; the next is staged with its second step's
+      // products, by when both halves are done with the buffer's V (in phases 4 t and 4 t +
+      // 1 of tile t), and before either reads it (from 4 t + 4 on).  All waves take all
+      // steps, as keys past a row's last weigh nothing.
+      const bool behind = wave >= W / 2;
+      if (behind) meet();
+      if (p0 + KT < end) {
+        fetch(p0 + KT);
+        find(p0 + 2 * KT);
+      }
+      scores(0);
+      meet();
+      weigh(p0);
+      meet();
+      int row = 0;
 #pragma unroll 1
-      for (int n = 0; n < KT; n += kStepKeys)
-        if (k0 + n < w_end) compute((buf ? KT : 0) + n, k0 + n);
-      if (more) stage(buf ^ 1);
-      buf ^= 1;
-      __syncthreads();
+      for (int k0 = p0 + kStepKeys; k0 < end; k0 += kStepKeys) {
+        const int last = row;
+        row = row + kStepKeys == 2 * KT ? 0 : row + kStepKeys;
+        const bool first = row % KT == 0;
+        const int next = k0 - row % KT + KT;  // the next tile
+        if (first && next < end) {
+          fetch(next);
+          find(next + KT);
+        }
+        values(last);
+        scores(row);
+        order_reads<2 * ND>();
+        repeat<(2 * NKB - 1) * ND>([] { order_reads<2>(), order_products<1>(); });
+        repeat<NKB * NJ>([] { order_reads<1>(), order_products<1>(); });
+        order_products<ND>();
+        if (!first && next < end) stage(row < KT);
+        meet();
+        weigh(k0);
+        meet();
+      }
+      values(row);
+      if (!behind) meet();
     }
   }
   if (bad_pages && lane == 0) {
