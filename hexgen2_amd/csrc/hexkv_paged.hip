@@ -345,15 +345,16 @@ static int paged_copy(bool pack, const hexkv_pool *pool, const void *const *src,
   for (int l = 0; l < n_layers; ++l)
     if (!src[l] || !dst[l] || !aligned16(src[l]) || !aligned16(dst[l]))
       return fail(HEXKV_EINVAL, "%s: layer %d's address is null or not 16-byte aligned", what, l);
-  unsigned int *status = nullptr;
-  rc = status_word(stream, &status, what);
-  if (rc != HEXKV_OK) return rc;
   const int64_t row_bytes = 2 * static_cast<int64_t>(pool->kv_heads) * pool->head_dim * elem_bytes(pool->dtype);
   if (row_bytes > INT64_C(1) << 26) return fail(HEXKV_ERANGE, "%s: rows of more than 2^26 bytes", what);
   const bool small = total * row_bytes * n_layers < 128 << 20;
   const int64_t share = small ? kSmallCopyThreads * kSmallCopyUnroll * 16 : kCopyThreads * kCopyUnroll * 16;
   int rows = pool->page_size;
   while (rows > 1 && rows * row_bytes > share) rows /= 2;
+  if (total / rows + batch >= 1 << 22) return fail(HEXKV_ERANGE, "%s: 2^22 workgroups a layer or more", what);
+  unsigned int *status = nullptr;
+  rc = status_word(stream, &status, what);
+  if (rc != HEXKV_OK) return rc;
   int64_t base = 0;
   for (int b0 = 0; b0 < batch; b0 += HEXKV_MAX_SEQS_PER_LAUNCH) {
     const int nb = std::min(batch - b0, HEXKV_MAX_SEQS_PER_LAUNCH);
@@ -392,6 +393,7 @@ extern "C" int hexkv_paged_append(const hexkv_paged_append_params *params, hexkv
   const int64_t tokens = p.seqs.tokens;
   if (p.qkv_stride < row && tokens > 1) return fail(HEXKV_EINVAL, "%s: qkv's rows overlap", what);
   if (p.q_stride < q_row && tokens > 1) return fail(HEXKV_EINVAL, "%s: q's rows overlap", what);
+  if (tokens >= 1 << 24) return fail(HEXKV_ERANGE, "%s: 2^24 tokens or more", what);
   if (tokens == 0 || p.seqs.batch == 0) return HEXKV_OK;
   if (!p.qkv || (p.q_heads && !p.q) || !p.pages || (p.rotary_dim && !p.inv_freq)) return fail(HEXKV_EINVAL, "%s: null tensor", what);
   if (!aligned16(p.pages)) return fail(HEXKV_EINVAL, "%s: pages are not 16-byte aligned", what);

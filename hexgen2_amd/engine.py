@@ -93,6 +93,8 @@ class Engine:
 
     @torch.inference_mode()
     def prefill(self, input_ids, max_new_tokens):
+        if self.page_size and not len(input_ids):
+            raise ValueError("prefill needs a token")
         ids = torch.tensor([input_ids], dtype=torch.long, device=self.device)
         state = CacheState(len(input_ids) + max_new_tokens, kv_bits=self.kv_bits, page_size=self.page_size)
         chunk = self.prefill_chunk or len(input_ids)

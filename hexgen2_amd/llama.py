@@ -222,6 +222,8 @@ class LlamaHost:
         the positions from ``starts`` on (all as in ``paged``).  ``last_token_only``: of each
         row's last token; ``rows``: of these tokens (indices into the flattened ``input_ids``)."""
         s = self.shape
+        if len(pages) != len(self.layers):
+            raise ValueError(f"pools of {len(pages)} layers for a model of {len(self.layers)}")
         h = F.embedding(input_ids, self.embed)
         y = None  # the block output still to be added to h
         for layer, pool in zip(self.layers, pages):

@@ -25,7 +25,9 @@ def kind_of(scaling: Optional[dict]) -> str:
 
 
 def _number(scaling: dict, name: str, default=None) -> float:
-    value = scaling.get(name, default)
+    value = scaling.get(name)
+    if value is None:
+        value = default
     if value is None or not float(value) > 0:
         raise ValueError(f"{scaling.get('rope_type', scaling.get('type'))} rotation needs a positive {name}, got {value!r}")
     return float(value)
@@ -64,6 +66,8 @@ def frequencies(dim: int, base: float = 10000.0, scaling: Optional[dict] = None,
     elif kind == "yarn":
         s, length = _number(scaling, "factor"), _number(scaling, "original_max_position_embeddings", max_positions)
         fast, slow = _number(scaling, "beta_fast", 32), _number(scaling, "beta_slow", 1)
+        if any(scaling.get(k) is not None for k in ("mscale", "mscale_all_dim")) or scaling.get("truncate") is False:
+            raise ValueError("yarn rotation with mscale, or with places that are not whole, is not supported")
 
         def pair(turns):  # the (fractional) pair that makes so many turns over L0
             return dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
@@ -71,5 +75,5 @@ def frequencies(dim: int, base: float = 10000.0, scaling: Optional[dict] = None,
         first, last = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), dim - 1)
         kept = 1 - ((torch.arange(dim // 2, dtype=torch.float64) - first) / max(last - first, 0.001)).clamp(0, 1)
         f = kept * f + (1 - kept) * f / s
-        scale = float(scaling.get("attention_factor") or (0.1 * math.log(s) + 1 if s > 1 else 1.0))
+        scale = _number(scaling, "attention_factor", 0.1 * math.log(s) + 1 if s > 1 else 1.0)
     return f.float().to(device), scale

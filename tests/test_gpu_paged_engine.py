@@ -152,6 +152,12 @@ def test_generate_refuses_what_cannot_run(device):
         engine.generate([[1], [2]], [4, 0])
     with pytest.raises(ValueError, match="step of 0"):
         engine.generate([[1]], 4, step_tokens=0)
+    with pytest.raises(ValueError, match="needs a token"):
+        engine.prefill([], 4)
+    pool = engine._pool(1)
+    with pytest.raises(ValueError, match="pools of 1 layers"):
+        engine.model.forward_pages(torch.tensor([[1]], device=device), pool[:1], torch.zeros((1, 1), dtype=torch.int32, device=device),
+                                   torch.zeros(1, dtype=torch.int32, device=device), max_seqlen=1)
     with pytest.raises(ValueError, match="page_size"):
         Engine(GOLDEN / "tiny_llama", "native", "cuda", "float16").generate([[1]], 4)
 

@@ -88,6 +88,22 @@ def test_hundreds_of_ragged_sequences(device, dtype):
     check_attend(device, dtype, (4, 2, 64), new, [5] * 130, 16)
 
 
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("lens", [[5000], [5000, 300]])
+def test_padded_chunks(device, dtype, lens):
+    """Token tensors much longer than what cu_tokens bounds: single tokens where the call
+    could hold chunks alone."""
+    hq, h, d, page, n = 8, 1, 128, 64, len(lens)
+    tables, count = make_tables([x + 1 for x in lens], page, 1, device)
+    pool = make_pool((hq, h, d), page, count, 2, dtype, device)
+    q = randn((70 * n, hq, d), 3, dtype, device)
+    out, cu = torch.full_like(q, 7.0), list(range(n + 1))
+    paged.attention(q, pool, tables, int32(lens, device), max_seqlen=5001, cu_tokens=int32(cu, device), max_tokens=70, out=out)
+    want, weight, reach = oracle.attend(wide(q), wide(pool), tables.tolist(), lens, cu)
+    assert (np.abs(wide(out) - want)[:n] <= tolerance(dtype, want, weight, reach, d, keys=5001)[:n]).all()
+    assert (out[n:] == 7).all()
+
+
 def test_the_smallest_calls(device):
     for dtype in DTYPES:
         check_attend(device, dtype, (1, 1, 16), [1], [0], 16, uniform=True)

@@ -89,6 +89,10 @@ def test_yarn_frequencies():
     assert scale == pytest.approx(0.1 * math.log(4) + 1)
     assert torch.allclose(f, torch.tensor([1.0, 0.1 * (0.5 + 0.5 / 4), 0.01 / 4, 0.001 / 4]))
     assert rotary.frequencies(8, 10000.0, dict(s, attention_factor=1.5))[1] == 1.5
+    assert rotary.frequencies(8, 10000.0, dict(s, attention_factor=None, mscale=None))[1] == scale
+    for more in (dict(mscale=0.7), dict(mscale_all_dim=1.0), dict(truncate=False), dict(attention_factor=-1.0)):
+        with pytest.raises(ValueError, match="yarn"):
+            rotary.frequencies(8, 10000.0, dict(s, **more))
 
 
 @pytest.mark.parametrize("scaling,match", [({"rope_type": "dynamic", "factor": 2.0}, "dynamic"), ({"rope_type": "linear"}, "factor"),
@@ -206,6 +210,7 @@ def refused(call, code, match):
     (dict(q=QKV, q_stride=4 * 64), _lib.HEXKV_EINVAL, "q overlaps"),
     (dict(qkv=PAGES + 4096), _lib.HEXKV_EINVAL, "pages overlap"),
     (dict(q=PAGES), _lib.HEXKV_EINVAL, "pages overlap"),
+    (dict(seqs=seqs(tokens=1 << 24)), _lib.HEXKV_ERANGE, "2\\^24 tokens"),
 ])
 def test_append_refuses(changes, code, match):
     refused(lambda lib: lib.hexkv_paged_append(ctypes.byref(append_params(**changes)), None), code, match)
@@ -285,6 +290,14 @@ def test_handoff_refuses(name, changes, code, match):
     ptr = lambda x: (ctypes.c_void_p * 1)(x)  # noqa: E731
     refused(lambda lib: getattr(lib, name)(ctypes.byref(a["pool"]), ptr(a["src"]), ptr(a["dst"]), a["layers"], a["tables"],
                                            a["stride"], 4, 2, (ctypes.c_int64 * 2)(*a["lens"]), None), code, match)
+
+
+@pytest.mark.parametrize("name", ["hexkv_paged_pack", "hexkv_paged_unpack"])
+def test_handoff_refuses_more_workgroups_than_a_launch_has(name):
+    ptr = lambda x: (ctypes.c_void_p * 1)(x)  # noqa: E731
+    p = pool(kv_heads=1, head_dim=16, pos_stride=16, kv_stride=16 * 16, head_stride=0, page_stride=2 * 16 * 16)
+    refused(lambda lib: getattr(lib, name)(ctypes.byref(p), ptr(QKV), ptr(PAGES), 1, TABLE, 1 << 23, 1 << 23, 1,
+                                           (ctypes.c_int64 * 1)(1 << 26), None), _lib.HEXKV_ERANGE, "2\\^22 workgroups")
 
 
 # -------------------------------------------------------- Python's checks ---
