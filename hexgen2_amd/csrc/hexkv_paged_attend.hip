@@ -977,8 +977,10 @@ constexpr bool has_tiles() {
   return !std::is_same<T, float>::value && (D == 64 || D == 128);
 }
 
+// (Three waves a SIMD, where the registers allow: fp32 heads of 128 spill at three, 105
+// us for 11 sequences of up to 4200 keys on 8 KV heads, and take 40 at two.)
 template <typename T, int D>
-__global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void paged_rows_kernel(const PagedAttendArgs a) {
+__global__ __launch_bounds__(256, D > 128 ? 1 : D * sizeof(T) > 256 ? 2 : 3) void paged_rows_kernel(const PagedAttendArgs a) {
   __shared__ __attribute__((aligned(16))) char s_mem[rows_lds<T, D, 4>()];
   rows_path<T, D, 4>(a, blockIdx.x, s_mem);
 }
@@ -1178,10 +1180,18 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   // partitions of 1024 keys, which even out ragged lengths (us, MI355X, 16-bit heads
   // of 128: 8 pairs of 1024 keys 8.5 split in 8, 12.9 whole, of 512 8.2 and 8.6; 32 pairs of 4096
   // keys 19.5, 17.0, 16.5, 18.2, 26.3 and 40 in partitions of 128, 256, 512, 1024, 2048 and
-  // whole; 512 ragged ones of up to 8192 191, 181, 177, 193 and 200 from 256 on).
-  const int64_t row_keys = few_tiles * a->kv_heads * p.max_seqlen, each = round_up((row_keys + kCus - 1) / kCus, 128);
-  int64_t part = p.partition ? p.partition : each <= 2048 ? std::max<int64_t>(each, 128) : 1024;
-  if (!p.partition && static_cast<int64_t>(p.max_seqlen) * d * elem_bytes(p.pool.dtype) <= 128 << 10) part = 1 << 30;
+  // whole; 512 ragged ones of up to 8192 191, 181, 177, 193 and 200 from 256 on).  More than half a
+  // workgroup a CU are not split for that: 144 pairs of 1100 keys 16.5 whole, 17.5 in
+  // partitions of 256, 19.2 of 512, 21.6 of 640; of up to 2000, 24 whole, 22 to 27 split.
+  const int64_t pairs = few_tiles * a->kv_heads;
+  const int64_t each = 2 * pairs > kCus ? p.max_seqlen : std::max<int64_t>(128, round_up(ceil_div(pairs * p.max_seqlen, kCus), 128));
+  int64_t part = p.partition ? p.partition : each <= 2048 ? std::max<int64_t>(each, 64) : 1024;
+  if (!p.partition && part < p.max_seqlen) {
+    // of one length, and where they save more than the join takes
+    part = round_up(ceil_div(p.max_seqlen, ceil_div(p.max_seqlen, part)), 128);
+    const int64_t key = static_cast<int64_t>(d) * elem_bytes(p.pool.dtype);
+    if (p.max_seqlen * key <= 128 << 10 || (p.max_seqlen - part) * key <= 96 << 10) part = 1 << 30;
+  }
   part = std::max(part, round_up((p.max_seqlen + kMaxParts - 1) / kMaxParts, 128));
   a->part = static_cast<int32_t>(std::min<int64_t>(part, 1 << 30));
   a->max_parts = static_cast<int32_t>(std::max<int64_t>(1, (p.max_seqlen + part - 1) / part));
