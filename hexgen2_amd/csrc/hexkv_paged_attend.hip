@@ -16,12 +16,13 @@
 // each of 16 rows, a line was asked for twice, and the loads could not be
 // nontemporal (Llama-3-8B decode batch 211 us, 224 nontemporal, against 185).
 // What bounds it: a decode row's K and V are read once, 4 D flops a key, so
-// memory.  Steps are loaded one ahead into registers, page numbers two ahead.
+// memory (64 sequences of 128 to 8192, 8 KV heads of 128: 1.10 GB in 181 us, 6.1 TB/s).  Steps are loaded one ahead into registers, page numbers two ahead.
 //
 // Tile path (16-bit, head_dim 64 or 128, sequences of more than kFewRows rows):
 // 32 rows a wave, four or eight waves a workgroup (128 or 256 rows), which share tiles of
 // 16 keys a wave in LDS; the same products on 32 x 32 x 16 matrix instructions.  What
-// bounds it: the matrix cores, and the softmax on the VALU beside them.  A
+// bounds it: the matrix cores, the LDS reads of their operands, and the softmax on the
+// VALU beside them (2048 rows over 8192 keys, 32 heads of 128 on 8: 316 us, 979 TFLOP/s).  A
 // probability enters P V as one 16-bit term, rounded to nearest: an error of the order
 // of the output's own rounding (that of p averages over the keys), for two thirds of
 // the matrix work.
