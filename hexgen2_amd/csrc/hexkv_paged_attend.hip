@@ -1086,27 +1086,29 @@ static int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; 
 
 // Keys of a tile's partition.  A split fills the CUs evenly, and costs sums that
 // are written, read and joined.  A step of 64 keys (D = 128) takes a CU 1.42 us
-// for a lone tile of 128 rows, 2.25 for two at once, 2.0 for one of 256; a
-// partition's sums 0.026 us per 128 rows, the join 5.  With those, the least of
+// for a lone tile of 128 rows, 2.25 for two at once, 2.0 for one of 256; with D = 64 two
+// thirds; a partition's sums 0.026 us per 128 rows, the join 5.  With those, the least of
 // whole rows and of partitions that fill all CUs once to eight times: 512 rows of
 // 4 heads over 8192 keys on 8 KV heads 90 us in 4, 105 in 2, 173 whole; 1100 rows
-// over 31100 keys 606 for 878 whole; 1024 over 4096 whole 93, in two 99.  From two
+// over 31100 keys 606 for 878 whole; 1024 over 4096 whole 93, in two 99; 250 rows of 8 heads on
+// one over 1050 keys 15.7 in partitions of 256, 20 of 512.  From two
 // tiles a CU on, causal rows' lengths even out by themselves (2500 rows over 4000
 // keys 150 whole, in two 204).
-static int64_t tile_partition(int64_t tiles, int64_t keys, bool wide) {
+static int64_t tile_partition(int64_t tiles, int64_t keys, int d, bool wide) {
   if (tiles >= 2 * kCus) return std::max<int64_t>(64, round_up(keys, 64));
   const auto time = [&](int64_t parts) {
     const int64_t steps = ceil_div(keys, 64 * parts) + 1, each = ceil_div(tiles * parts, kCus);
-    return steps * (wide ? each * 200 : each / 2 * 225 + each % 2 * 142) + (parts > 1 ? 500 + tiles * parts * (wide ? 52 : 26) / 10 : 0);
+    return steps * (wide ? each * 200 : each / 2 * 225 + each % 2 * 142) * (d + 64) / 192 +
+           (parts > 1 ? 500 + tiles * parts * (wide ? 52 : 26) * d / 1280 : 0);
   };
   int64_t best = 1, least = time(1);
   for (int64_t fill = 1; fill <= 8; ++fill) {
-    const int64_t parts = std::min(fill * kCus / std::max<int64_t>(tiles, 1), keys / 512);
+    const int64_t parts = std::min(fill * kCus / std::max<int64_t>(tiles, 1), keys / 192);
     if (parts < 2) continue;
     const int64_t t = time(parts);
     if (t < least) least = t, best = parts;
   }
-  return std::max<int64_t>(64, round_up(ceil_div(keys, best), wide ? 128 : 64));
+  return std::max<int64_t>(64, round_up(ceil_div(keys, best), 64));
 }
 
 // Split rows of either path.
@@ -1199,7 +1201,7 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   // Of ragged sequences, all but one taken for single tokens.
   const int64_t long_rows = p.seqs.cu_tokens ? (std::max(tokens - batch, INT64_C(0)) + 1) * a->group : 0;
   const int64_t full = (p.seqs.cu_tokens ? ceil_div(long_rows, tile_rows) : tiles) * a->kv_heads;
-  part = p.partition ? p.partition : tile_partition(full, p.max_seqlen, a->wide);
+  part = p.partition ? p.partition : tile_partition(full, p.max_seqlen, d, a->wide);
   part = std::max(part, round_up((p.max_seqlen + kMaxParts - 1) / kMaxParts, 64));
   a->tile_part = static_cast<int32_t>(std::min<int64_t>(part, 1 << 30));
   a->tile_parts = static_cast<int32_t>(std::max<int64_t>(1, (p.max_seqlen + part - 1) / part));
