@@ -18,7 +18,7 @@
 // What bounds it: a decode row's K and V are read once, 4 D flops a key, so
 // memory (64 sequences of 128 to 8192, 8 KV heads of 128: 1.10 GB in 181 us, 6.1 TB/s).  Steps are loaded one ahead into registers, page numbers two ahead.
 //
-// Tile path (16-bit, head_dim 64 or 128, sequences of more than kFewRows rows):
+// Tile path (16-bit, head_dim from 64 on, sequences of more than kFewRows rows):
 // 32 rows a wave, four or eight waves a workgroup (128 or 256 rows), which share tiles of
 // 16 keys a wave in LDS; the same products on 32 x 32 x 16 matrix instructions.  What
 // bounds it: the matrix cores, the LDS reads of their operands, and the softmax on the
@@ -975,7 +975,7 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
 
 template <typename T, int D>
 constexpr bool has_tiles() {
-  return !std::is_same<T, float>::value && (D == 64 || D == 128);
+  return !std::is_same<T, float>::value && D >= 64;
 }
 
 // (Three waves a SIMD, where the registers allow: fp32 heads of 128 spill at three, 105
@@ -987,14 +987,14 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : D * sizeof(T) > 256 ? 2 : 3) voi
 }
 
 template <typename T, int D, int W>
-__global__ __launch_bounds__(W * 64, 2) void paged_tile_kernel(const PagedAttendArgs a) {
+__global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void paged_tile_kernel(const PagedAttendArgs a) {
   __shared__ __attribute__((aligned(16))) char s_mem[TileLds<D, W>::kBytes];
   tile_path<T, D, W>(a, blockIdx.x, s_mem);
 }
 
 // A call that may hold sequences of either kind: tiles first (they take longest).
 template <typename T, int D, int W>
-__global__ __launch_bounds__(W * 64, 2) void paged_mixed_kernel(const PagedAttendArgs a) {
+__global__ __launch_bounds__(W * 64, D > 128 ? 1 : 2) void paged_mixed_kernel(const PagedAttendArgs a) {
   constexpr int kRows = rows_lds<T, D, W>(), kTiles = TileLds<D, W>::kBytes;
   __shared__ __attribute__((aligned(16))) char s_mem[kRows > kTiles ? kRows : kTiles];
   const int block = blockIdx.x;
@@ -1087,7 +1087,7 @@ static int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; 
 // Keys of a tile's partition.  A split fills the CUs evenly, and costs sums that
 // are written, read and joined.  A step of 64 keys (D = 128) takes a CU 1.42 us
 // for a lone tile of 128 rows, 2.25 for two at once, 2.0 for one of 256; with D = 64 two
-// thirds; a partition's sums 0.026 us per 128 rows, the join 5.  With those, the least of
+// thirds, with 256 (one at a time) five thirds; a partition's sums 0.026 us per 128 rows, the join 5.  With those, the least of
 // whole rows and of partitions that fill all CUs once to eight times: 512 rows of
 // 4 heads over 8192 keys on 8 KV heads 90 us in 4, 105 in 2, 173 whole; 1100 rows
 // over 31100 keys 606 for 878 whole; 1024 over 4096 whole 93, in two 99; 250 rows of 8 heads on
@@ -1098,7 +1098,7 @@ static int64_t tile_partition(int64_t tiles, int64_t keys, int d, bool wide) {
   if (tiles >= 2 * kCus) return std::max<int64_t>(64, round_up(keys, 64));
   const auto time = [&](int64_t parts) {
     const int64_t steps = ceil_div(keys, 64 * parts) + 1, each = ceil_div(tiles * parts, kCus);
-    return steps * (wide ? each * 200 : each / 2 * 225 + each % 2 * 142) * (d + 64) / 192 +
+    return steps * (wide ? each * 200 : d > 128 ? each * 142 : each / 2 * 225 + each % 2 * 142) * (d + 64) / 192 +
            (parts > 1 ? 500 + tiles * parts * (wide ? 52 : 26) * d / 1280 : 0);
   };
   int64_t best = 1, least = time(1);
@@ -1155,7 +1155,10 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   const int64_t rows = static_cast<int64_t>(a->max_tokens) * a->group;
   if (rows > INT32_MAX - 256) return fail(HEXKV_ERANGE, "%s: 2^31 rows or more", what);
   // Which paths can have work: without cu_tokens every sequence has as many rows.
-  const bool tiled = p.pool.dtype != HEXKV_F32 && (d == 64 || d == 128) && rows > kFewRows;
+  // Heads of 256 leave a CU one tile, of four waves: 2048 rows of 8 heads on one over 8000 keys 301 us, 1456 on
+  // the row path, 16 x 40 over 4000 32 for 86, but 40 over 1040 22.7 for 15.2.
+  const bool tiled = p.pool.dtype != HEXKV_F32 && rows > kFewRows &&
+                     (d == 64 || d == 128 || (d == 256 && static_cast<double>(tokens) * p.q_heads * p.max_seqlen >= 1 << 20));
   // Tiles of 256 rows read LDS and pages half as often, but one alone has a CU to
   // itself from its first key to its last: chunks of 2048 over 8192 keys (32 heads
   // on 8) 243 us for 252 with 128, of 512 84 for 90, of 8192 518 for 537; yet 2048

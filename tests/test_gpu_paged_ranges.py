@@ -68,6 +68,39 @@ def test_tiles_of_256_rows_skip_pages_outside_the_pool(device, dtype):
     assert (np.abs(wide(got) - want) <= tolerance(dtype, want, weight, reach, d, keys=start + new)).all()
 
 
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_tiles_of_heads_of_256(device, dtype, causal):
+    check_attend(device, dtype, (8, 1, 256), [260], [260], 16, causal, uniform=True)
+    check_attend(device, dtype, (8, 2, 256), [150, 1, 33, 9], [1001, 900, 0, 130], 32, causal, order="rows", extra=2)
+    check_attend(device, dtype, (4, 4, 256), [70, 64], [2000, 127], 64, causal, order="apart", partition=192)
+    for fill in (float("nan"), float("inf")):
+        check_attend(device, dtype, (8, 1, 256), [100, 3], [1300, 17], 64, causal, fill=fill)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+def test_tiles_of_heads_of_256_and_what_they_leave_out(device, dtype):
+    hq, h, d, page, start, new = 8, 1, 256, 64, 1300, 110
+    tables, count = make_tables([start + new], page, 1, device)
+    pool = make_pool((hq, h, d), page, count, 2, dtype, device)
+    q = randn((new, hq, d), 3, dtype, device)
+    clean = paged.attention(q, pool, tables, int32([start], device), max_seqlen=start + new)
+    at = start + 50
+    pool[tables[0, at // page].long(), at % page, 1, 0, 9] = float("nan")
+    got = paged.attention(q, pool, tables, int32([start], device), max_seqlen=start + new)
+    want = torch.ones((new, hq, d), dtype=torch.bool)
+    want[50:, :, 9] = False
+    assert torch.equal(torch.isfinite(got.cpu()), want)
+    assert torch.allclose(got[:50].float(), clean[:50].float(), rtol=4 * torch.finfo(dtype).eps, atol=4e-3)
+    pool[tables[0, at // page].long(), at % page, 1, 0, 9] = 0
+    tables[0, 3], tables[0, 20] = count, -1
+    ops.device_status(device)
+    got = paged.attention(q, pool, tables, int32([start], device), max_seqlen=start + new)
+    assert ops.device_status(device) == ops._lib.STATUS_PAGE
+    want, weight, reach = oracle.attend(wide(q), wide(pool), tables.tolist(), [start], None)
+    assert (np.abs(wide(got) - want) <= tolerance(dtype, want, weight, reach, d, keys=start + new)).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_of_many_partitions(device, dtype):
     """More partitions than a wave has lanes, and more keys than the most partitions
