@@ -118,7 +118,7 @@ def _token_rows(shape, stride, dims: int, name: str):
     return tokens, step
 
 
-# The checked parameter blocks of append and attention by what they depend on
+# The checked parameter blocks of append and attention, and the pools of the handoff, by what they depend on
 # (shapes, strides, types, devices and options, never an address), as
 # fp4.decode_attention keeps its own.
 _FORMS: "OrderedDict[tuple, tuple]" = OrderedDict()
@@ -277,28 +277,40 @@ def attend_workspace_bytes(q: torch.Tensor, pages: torch.Tensor, tables: torch.T
 def _copy_layers(pages_layers: TensorList, tables, lens, written: bool):
     """First layer, addresses, pool and checked lengths of a handoff call."""
     if isinstance(pages_layers, torch.Tensor):
-        if pages_layers.dim() != 6 or not pages_layers.shape[0]:
-            raise ValueError("stacked pages must be [n_layers, n_pages, page_size, 2, kv_heads, head_dim]")
-        _require_device(pages_layers)
-        pool = _pool_of(pages_layers.shape[1:], pages_layers.stride()[1:], pages_layers.dtype, written)
-        if written and pages_layers.shape[0] > 1 and pages_layers.stride(0) == 0:
-            raise ValueError("layers that are written must not share pages")
-        first, ptrs = pages_layers, _layer_ptrs(pages_layers)
-    else:
-        layers = _as_layers(pages_layers)
-        if not layers:
-            raise ValueError("no layers")
-        _require_device(*layers)
-        first = layers[0]
-        pool = _check_pages(first, written)
-        if any(t.shape != first.shape or t.stride() != first.stride() or t.dtype != first.dtype or t.device != first.device
-               for t in layers):
-            raise ValueError("all layers must share shape, strides, dtype and device")
-        ptrs = _ptr_array([t.data_ptr() for t in layers])
-    _require_device(tables)
+        key = (_layout(pages_layers), _layout(tables), written)
+        form = _FORMS.get(key)
+        if form is None:
+            if pages_layers.dim() != 6 or not pages_layers.shape[0]:
+                raise ValueError("stacked pages must be [n_layers, n_pages, page_size, 2, kv_heads, head_dim]")
+            _require_device(pages_layers, tables)
+            pool = _pool_of(pages_layers.shape[1:], pages_layers.stride()[1:], pages_layers.dtype, written)
+            if written and pages_layers.shape[0] > 1 and pages_layers.stride(0) == 0:
+                raise ValueError("layers that are written must not share pages")
+            _check_tables(tables, pages_layers.device)
+            form = _keep(key, (pool,))
+        return pages_layers, _layer_ptrs(pages_layers), form[0], _check_lens(lens, tables.shape[0])
+    layers = _as_layers(pages_layers)
+    if not layers:
+        raise ValueError("no layers")
+    _require_device(tables, *layers)
+    first = layers[0]
+    pool = _check_pages(first, written)
+    if any(t.shape != first.shape or t.stride() != first.stride() or t.dtype != first.dtype or t.device != first.device
+           for t in layers):
+        raise ValueError("all layers must share shape, strides, dtype and device")
     _check_tables(tables, first.device)
-    lens = _check_lens(lens, tables.shape[0])
-    return first, ptrs, pool, lens
+    return first, _ptr_array([t.data_ptr() for t in layers]), pool, _check_lens(lens, tables.shape[0])
+
+
+def _packed(packed: TensorList, n_layers: int, total: int, pool: _lib.Pool, first: torch.Tensor):
+    """Addresses of the packed layers, checked once a form where they are stacked."""
+    if not isinstance(packed, torch.Tensor):
+        return _packed_ptrs(packed, n_layers, total, 2 * pool.kv_heads * pool.head_dim, first.dtype, first.device)
+    key = (_layout(packed), n_layers, total, pool.kv_heads, pool.head_dim, first.dtype, first.get_device())
+    if key not in _FORMS:
+        _packed_ptrs(packed, n_layers, total, 2 * pool.kv_heads * pool.head_dim, first.dtype, first.device)
+        _keep(key, ())
+    return _layer_ptrs(packed)
 
 
 def _copy(name, pool, source, target, n_layers, tables, lens, first) -> None:
@@ -314,10 +326,11 @@ def pack_live(pages_layers: TensorList, tables: torch.Tensor, lens: Sequence[int
     head_dim]``, one launch.  ``pages_layers``: the layers' pools, a list or stacked,
     with one ``tables`` for all.  The rows of a page outside the pool come out as zeros."""
     first, ptrs, pool, lens = _copy_layers(pages_layers, tables, lens, False)
-    row = (2, pool.kv_heads, pool.head_dim)
     if out is None:
-        out = first.new_empty((len(ptrs), sum(lens), *row))
-    dst = _packed_ptrs(out, len(ptrs), sum(lens), 2 * pool.kv_heads * pool.head_dim, first.dtype, first.device)
+        out = first.new_empty((len(ptrs), sum(lens), 2, pool.kv_heads, pool.head_dim))
+        dst = _layer_ptrs(out)
+    else:
+        dst = _packed(out, len(ptrs), sum(lens), pool, first)
     _copy("hexkv_paged_pack", pool, ptrs, dst, len(ptrs), tables, lens, first)
     return out
 
@@ -327,5 +340,5 @@ def unpack_live(packed: TensorList, pages_layers: TensorList, tables: torch.Tens
     pages that ``tables`` names; all other rows are left untouched.  No two
     sequences may share a page here."""
     first, ptrs, pool, lens = _copy_layers(pages_layers, tables, lens, True)
-    src = _packed_ptrs(packed, len(ptrs), sum(lens), 2 * pool.kv_heads * pool.head_dim, first.dtype, first.device)
+    src = _packed(packed, len(ptrs), sum(lens), pool, first)
     _copy("hexkv_paged_unpack", pool, src, ptrs, len(ptrs), tables, lens, first)

@@ -158,6 +158,30 @@ def test_the_smallest_calls(device):
                             q_heads=4).shape == (0, 4, 64)
 
 
+def test_stacked_handoffs_of_changing_lengths(device):
+    """One stack of pools, other lengths and packets each time, none at all among them; refusals after good calls."""
+    pool = paged.kv_pages(8, 16, 2, 64, torch.float16, device, layers=3)
+    pool.copy_(randn(pool.shape, 1, torch.float16, device))
+    tables = int32([[0, 1, 2, 3], [4, 5, 6, 7]], device)
+    for lens in ([0, 0], [5, 60], [64, 0], [5, 60], [1, 1]):
+        got = paged.pack_live(pool, tables, lens)
+        for i in range(3):
+            assert np.array_equal(wide(got[i]), oracle.pack(wide(pool[i]), tables.tolist(), lens))
+        out = torch.empty_like(got)
+        assert paged.pack_live(pool, tables, lens, out=out) is out and torch.equal(out, got)
+        target = torch.zeros_like(pool)
+        paged.unpack_live(got, target, tables, lens)
+        assert torch.equal(paged.pack_live(target, tables, lens), got)
+    for bad in (torch.empty((3, 3, 2, 2, 64), dtype=torch.float16, device=device), got[:2], got.float(), got.cpu()):
+        with pytest.raises(ValueError):
+            paged.unpack_live(bad, pool, tables, [1, 1])
+        with pytest.raises(ValueError):
+            paged.pack_live(pool, tables, [1, 1], out=bad)
+    for wrong in (tables.cpu(), tables.long(), tables[:1]):
+        with pytest.raises(ValueError):
+            paged.pack_live(pool, wrong, [1, 1])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_sequences_that_share_a_prefix(device, dtype):
     """The same page in several tables, and twice in one, is read like any other."""
