@@ -22,10 +22,10 @@
 // 32 rows a wave, four or eight waves a workgroup (128 or 256 rows), which share tiles of
 // 16 keys a wave in LDS; the same products on 32 x 32 x 16 matrix instructions.  What
 // bounds it: the matrix cores, the LDS reads of their operands, and the softmax on the
-// VALU beside them (2048 rows over 8192 keys, 32 heads of 128 on 8: 316 us, 979 TFLOP/s).  A
-// probability enters P V as one 16-bit term, rounded to nearest: an error of the order
-// of the output's own rounding (that of p averages over the keys), for two thirds of
-// the matrix work.
+// VALU beside them (2048 rows over 8192 keys, 32 heads of 128 on 8: 432 us, 715 TFLOP/s,
+// the second terms' products not counted).  A probability enters P V as hi + lo here too:
+// one rounded term takes 316 us, but its error is half a step of the type, as much as the
+// output's own rounding.
 #include "hexkv_paged.h"
 
 #include <algorithm>
@@ -179,8 +179,8 @@ __device__ __forceinline__ u32x4 load_16(__amdgpu_buffer_rsrc_t block, uint32_t 
 
 // The matrix products of one type.  A probability is held at 2^kShift of the
 // running maximum, which moves when a score exceeds it by kSlack more (log2
-// units), and enters P V as hi + lo, two 16-bit terms: what bounds the kernel
-// is memory, and one term would double the error of a 16-bit output.  fp16
+// units), and enters P V as hi + lo, two 16-bit terms: one would double the
+// error of a 16-bit output.  fp16
 // ends at 2^-24, so that at scale 1 many small probabilities would be lost;
 // 2^(11 + 4) still lies below its largest.
 template <typename T>
@@ -196,9 +196,6 @@ struct Mma<__bf16> {
   }
   __device__ __forceinline__ static f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
-  }
-  __device__ __forceinline__ static unsigned int pair(float p0, float p1) {
-    return __builtin_bit_cast(unsigned int, v2{static_cast<__bf16>(p0), static_cast<__bf16>(p1)});
   }
   __device__ __forceinline__ static void split(float p0, float p1, unsigned int *hi, unsigned int *lo) {
     const v2 h = {static_cast<__bf16>(p0), static_cast<__bf16>(p1)};
@@ -218,9 +215,6 @@ struct Mma<_Float16> {
   }
   __device__ __forceinline__ static f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
-  }
-  __device__ __forceinline__ static unsigned int pair(float p0, float p1) {
-    return __builtin_bit_cast(unsigned int, v2{static_cast<_Float16>(p0), static_cast<_Float16>(p1)});
   }
   __device__ __forceinline__ static void split(float p0, float p1, unsigned int *hi, unsigned int *lo) {
     const v2 h = {static_cast<_Float16>(p0), static_cast<_Float16>(p1)};
@@ -639,7 +633,8 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
 // ------------------------------------------------------------ tile path ---
 
 constexpr int kCus = 256;
-// A sequence of so many rows per KV head, or fewer, takes the row path.
+// A sequence of so many rows per KV head, or fewer, takes the row path (16 sequences of
+// 40 rows over 4000 keys of 128 dims 19.0 us on tiles, 29.5 on rows; one alone 15.5 and 12.5).
 constexpr int kFewRows = 32;
 
 // Rows a wave takes, and keys it computes at a time.
@@ -657,7 +652,7 @@ struct TileLds {
 // The order of a block's matrix products and LDS reads.  Left alone the compiler reads a
 // product's operands just before it, into registers that the last product has freed,
 // and the matrix cores wait for each read (a chunk of 2048 over 8192 keys, its waves in
-// two phases as below, 341 us instead of 316).
+// two phases as below, 447 us instead of 429).
 template <int N>
 __device__ __forceinline__ void order_reads() {
   __builtin_amdgcn_sched_group_barrier(0x100, N, 0);
@@ -775,7 +770,7 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
   // A step, of the keys at k0, which are the LDS buffers' rows from `row` on: their
   // scores, their probabilities, the sums of V.
   f32x16 s[NKB];
-  u32x4 p[2 * NKB];
+  u32x4 hi[2 * NKB], lo[2 * NKB];
   auto scores = [&](int row) {
     const char *from_k = s_k + (k_read + row * KP);
 #pragma unroll
@@ -820,7 +815,10 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
         const float e0 = exp2_of(fmaf(s[kb][i], a.scale_log2, base)), e1 = exp2_of(fmaf(s[kb][i + 1], a.scale_log2, base));
         l0 += e0;
         l1 += e1;
-        p[2 * kb + i / 8][i % 8 / 2] = M::pair(e0, e1);
+        unsigned int x, y;
+        M::split(e0, e1, &x, &y);
+        hi[2 * kb + i / 8][i % 8 / 2] = x;
+        lo[2 * kb + i / 8][i % 8 / 2] = y;
       }
     l += l0 + l1;
   };
@@ -832,7 +830,9 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
       for (int d = 0; d < ND; ++d) {
         const h4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_h4 *)(from_v + ks * 16 * VP + d * 64));
         const h4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_h4 *)(from_v + ks * 16 * VP + d * 64 + 8 * VP));
-        acc[d] = M::mma32(__builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7)), p[ks], acc[d]);
+        const u32x4 v = __builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        acc[d] = M::mma32(v, hi[ks], acc[d]);
+        acc[d] = M::mma32(v, lo[ks], acc[d]);
       }
   };
 
@@ -859,8 +859,8 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
           weigh(k0);
           values(buf * KT);
           order_reads<2 * ND>();
-          repeat<(2 * NKB - 1) * ND>([] { order_products<1>(), order_reads<2>(); });
-          order_products<ND>();
+          repeat<(2 * NKB - 1) * ND>([] { order_products<2>(), order_reads<2>(); });
+          order_products<2 * ND>();
         }
         if (more) stage(buf ^ 1);
         buf ^= 1;
@@ -868,8 +868,8 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
       }
     } else {
       // Waves w and w + 4 share a SIMD.  The second four run one phase behind, so that
-      // one of the two is at its products while the other is at its softmax (316 us for
-      // 324 with all in step; the products with their reads alone take 270, without reads 227):
+      // one of the two is at its products while the other is at its softmax (429 us for
+      // 495 with all in step):
       // phase 2 i: products of step i (the last step's V, this one's scores), 2 i + 1: its
       // softmax.  A tile is two steps; the next is staged with its second step's
       // products, by when both halves are done with the buffer's V (in phases 4 t and 4 t +
@@ -899,9 +899,9 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
         values(last);
         scores(row);
         order_reads<2 * ND>();
-        repeat<(2 * NKB - 1) * ND>([] { order_reads<2>(), order_products<1>(); });
+        repeat<(2 * NKB - 1) * ND>([] { order_reads<2>(), order_products<2>(); });
         repeat<NKB * NJ>([] { order_reads<1>(), order_products<1>(); });
-        order_products<ND>();
+        order_products<2 * ND>();
         if (!first && next < end) stage(row < KT);
         meet();
         weigh(k0);
@@ -1085,20 +1085,20 @@ static int64_t ceil_div(int64_t n, int64_t by) { return (n + by - 1) / by; }
 static int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // Keys of a tile's partition.  A split fills the CUs evenly, and costs sums that
-// are written, read and joined.  A step of 64 keys (D = 128) takes a CU 1.42 us
-// for a lone tile of 128 rows, 2.25 for two at once, 2.0 for one of 256; with D = 64 two
-// thirds, with 256 (one at a time) five thirds; a partition's sums 0.026 us per 128 rows, the join 5.  With those, the least of
+// are written, read and joined.  A step of 64 keys (D = 128) takes a CU 1.89 us
+// for a lone tile of 128 rows, 3.0 for two at once, 2.68 for one of 256; with D = 64 0.62 of
+// that, with 256 (one at a time) 1.64; a partition's sums 0.026 us per 128 rows, the join 5.  With those, the least of
 // whole rows and of partitions that fill all CUs once to eight times: 512 rows of
-// 4 heads over 8192 keys on 8 KV heads 90 us in 4, 105 in 2, 173 whole; 1100 rows
-// over 31100 keys 606 for 878 whole; 1024 over 4096 whole 93, in two 99; 250 rows of 8 heads on
-// one over 1050 keys 15.7 in partitions of 256, 20 of 512.  From two
+// 4 heads over 8192 keys on 8 KV heads 111 us in 4, 153 in 2, 120 in 8, 266 whole; 1100 rows
+// over 31100 keys 793 for 986 whole; 1024 over 4096 111 in two, 138 whole; 250 rows of 8 heads on
+// one over 1050 keys 18.7 in partitions of 256, 23.6 of 512, 32.9 whole.  From two
 // tiles a CU on, causal rows' lengths even out by themselves (2500 rows over 4000
-// keys 150 whole, in two 204).
+// keys 190 whole, in two 248).
 static int64_t tile_partition(int64_t tiles, int64_t keys, int d, bool wide) {
   if (tiles >= 2 * kCus) return std::max<int64_t>(64, round_up(keys, 64));
   const auto time = [&](int64_t parts) {
     const int64_t steps = ceil_div(keys, 64 * parts) + 1, each = ceil_div(tiles * parts, kCus);
-    return steps * (wide ? each * 200 : d > 128 ? each * 142 : each / 2 * 225 + each % 2 * 142) * (d + 64) / 192 +
+    return steps * (wide ? each * 268 : d > 128 ? each * 189 : each / 2 * 300 + each % 2 * 189) * (d + 64) / 192 +
            (parts > 1 ? 500 + tiles * parts * (wide ? 52 : 26) * d / 1280 : 0);
   };
   int64_t best = 1, least = time(1);
@@ -1155,17 +1155,20 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   const int64_t rows = static_cast<int64_t>(a->max_tokens) * a->group;
   if (rows > INT32_MAX - 256) return fail(HEXKV_ERANGE, "%s: 2^31 rows or more", what);
   // Which paths can have work: without cu_tokens every sequence has as many rows.
-  // Heads of 256 leave a CU one tile, of four waves: 2048 rows of 8 heads on one over 8000 keys 301 us, 1456 on
-  // the row path, 16 x 40 over 4000 32 for 86, but 40 over 1040 22.7 for 15.2.
+  // Heads of 256 leave a CU one tile, of four waves (tokens of 8 heads on one, us on tiles and on rows): 2048 over
+  // 8048 keys 220 and 743, 16 x 40 over 4000 94 and 130; at the border 16 x 40 over 240 24 and 27, 100 over 1300 28 and 28,
+  // 150 over 950 28 and 21; 40 over 1040 26 and 16.
   const bool tiled = p.pool.dtype != HEXKV_F32 && rows > kFewRows &&
                      (d == 64 || d == 128 || (d == 256 && static_cast<double>(tokens) * p.q_heads * p.max_seqlen >= 1 << 20));
   // Tiles of 256 rows read LDS and pages half as often, but one alone has a CU to
   // itself from its first key to its last: chunks of 2048 over 8192 keys (32 heads
-  // on 8) 243 us for 252 with 128, of 512 84 for 90, of 8192 518 for 537; yet 2048
-  // rows from the first key on 66 for 59, 64 rows (256 of a KV head) over 8064 keys
-  // 31 for 25.  Workgroups of few rows are then one a CU too, so a call of more
+  // on 8) 429 us for 461 with 128, of 512 114 for 124, of 8192 from the first key on 736 for 777; at the
+  // borders 128 tokens (512 rows of a KV head) over 8128 keys 43 for 42, 2048 over 3548 146 for 145 and
+  // over 4108 170 for 172; yet 2048 from the first key on 80 for 71, 64 (256 rows) over 8064
+  // 35 for 29.  Workgroups of few rows are then one a CU too, so a call of more
   // than four ragged sequences, which may be single tokens, keeps 128: a chunk of
-  // 2000 and 64 single tokens 804 us, with 256 rows a tile 829.
+  // 2000 and 64 single tokens 478 us, with 256 rows a tile 534; 500 of 8 heads and 20 single ones 42, 56
+  // (and 3 single ones 41, 46; 2000 of 32 heads and 3 352, 336).
   a->wide = tiled && d == 128 && rows >= 512 && p.max_seqlen >= 4096 && (!p.seqs.cu_tokens || p.seqs.batch <= 4);
   const int64_t tile_rows = a->wide ? 256 : 128;
   const bool few = !tiled || p.seqs.cu_tokens;
