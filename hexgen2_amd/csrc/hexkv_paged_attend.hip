@@ -156,19 +156,22 @@ __device__ __forceinline__ ScalarTable scalar_table(const PagedAttendArgs &a, in
   return (ScalarTable)(a.p.tables + __builtin_amdgcn_readfirstlane(b) * a.p.table_stride);
 }
 
-// Bytes from the pool's base to position k's row in a page.
+// Bytes from the pool's base to position k's row in a page (in 64 bits: of a page's
+// positions some may lie 2^32 bytes from its first).
 __device__ __forceinline__ uint64_t block_offset(const PagedAttendArgs &a, int page, int k) {
   return static_cast<uint64_t>(static_cast<uint32_t>(page)) * a.page_bytes +
-         static_cast<uint32_t>(k & ((1 << a.p.shift) - 1)) * a.pos_bytes;
+         static_cast<uint64_t>(static_cast<uint32_t>(k & ((1 << a.p.shift) - 1))) * a.pos_bytes;
 }
 
 // 16 rows of one head in a page, as a buffer that ends behind the last row that
 // holds a key: rows past it (those of the page not yet written) and every row of
 // a page outside the pool read as zeros, and blocks past the end, which the
 // loads made ahead ask for, cost nothing.  (Addressed as memory the last block
-// was loaded again in their place: 512 keys of a partition moved 25% more.)
+// was loaded again in their place: 512 keys of a partition moved 25% more.)  Positions are up to
+// 2^28 bytes apart, so that 15 of them and a row fit the buffer's 32 bits.
+template <int ROW_BYTES>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t block_of(const char *at, int rows, uint32_t pos_bytes) {
-  const uint32_t bytes = rows >= 16 ? 16 * pos_bytes : rows > 0 ? rows * pos_bytes : 0;
+  const uint32_t bytes = rows >= 16 ? 15 * pos_bytes + ROW_BYTES : rows > 0 ? (rows - 1) * pos_bytes + ROW_BYTES : 0;
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(at), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00027000);
 }
 constexpr int kNontemporal = 2;  // a buffer load's cache policy
@@ -360,8 +363,8 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
     Block x;
     x.in_pool = static_cast<unsigned>(page) < static_cast<unsigned>(a.p.n_pages);
     const char *at = head + block_offset(a, x.in_pool ? page : 0, k);
-    x.k = block_of(at, x.in_pool ? end - k : 0, pos_bytes);
-    x.v = block_of(at + kv_bytes, x.in_pool ? end - k : 0, pos_bytes);
+    x.k = block_of<D * ES>(at, x.in_pool ? end - k : 0, pos_bytes);
+    x.v = block_of<D * ES>(at + kv_bytes, x.in_pool ? end - k : 0, pos_bytes);
     return x;
   };
   // 16-bit: lane l loads chunk l % CH of row l / CH + i * RPL, so that a load takes
@@ -745,7 +748,7 @@ __device__ __forceinline__ void tile_path(const PagedAttendArgs &a, int block, c
     const int k = k0 + 16 * wave;
     bad_pages |= !in_pool && k < end;
     const char *at = head + block_offset(a, in_pool ? page : 0, k);
-    const __amdgpu_buffer_rsrc_t bk = block_of(at, end - k, pos_bytes), bv = block_of(at + kv_bytes, end - k, pos_bytes);
+    const __amdgpu_buffer_rsrc_t bk = block_of<D * ES>(at, end - k, pos_bytes), bv = block_of<D * ES>(at + kv_bytes, end - k, pos_bytes);
 #pragma unroll
     for (int i = 0; i < NL; ++i) kr[i] = load_16<0>(bk, lane_at + i * RPL * pos_bytes);
 #pragma unroll

@@ -784,8 +784,8 @@ typedef struct hexkv_pool {
   int kv_heads, head_dim; /* head_dim 16, 32, 64, 128 or 256 */
   int32_t n_pages;        /* at least 1 */
   int32_t page_size;      /* a power of two from 16 to 2^20 */
-  /* Elements from page to page, position to position, K to V, head to head;
-   * whole numbers of 16 bytes, as the base address is. */
+  /* Elements from page to page (below 2^30), position to position (head_dim to
+   * 2^26), K to V, head to head; whole numbers of 16 bytes, as the base address is. */
   int64_t page_stride, pos_stride, kv_stride, head_stride;
 } hexkv_pool;
 
