@@ -98,6 +98,13 @@ def _sequences(seqs: _lib.PagedBatch, tables, starts, cu_tokens, tokens: int, de
     seqs.tokens = _int32(tokens, "tokens")
 
 
+def _set_sequences(seqs: _lib.PagedBatch, tables, starts, cu_tokens) -> None:
+    """Sets the addresses of a call's sequences."""
+    seqs.tables, seqs.starts = tables.data_ptr(), starts.data_ptr()
+    if cu_tokens is not None:
+        seqs.cu_tokens = cu_tokens.data_ptr()
+
+
 def _token_rows(shape, stride, dims: int, name: str):
     """``(tokens, elements from token to token)`` of a tensor whose last ``dims`` dims are a token's."""
     inner = 1
@@ -187,10 +194,7 @@ def append(qkv: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, starts:
     if out is None:
         out = qkv.new_empty(form[1])
     p.qkv, p.q, p.pages = qkv.data_ptr(), out.data_ptr() if q_heads else None, pages.data_ptr()
-    seqs = p.seqs
-    seqs.tables, seqs.starts = tables.data_ptr(), starts.data_ptr()
-    if cu_tokens is not None:
-        seqs.cu_tokens = cu_tokens.data_ptr()
+    _set_sequences(p.seqs, tables, starts, cu_tokens)
     if inv_freq is not None:
         p.inv_freq = inv_freq.data_ptr()
     _call("hexkv_paged_append", qkv, ctypes.byref(p))
@@ -243,10 +247,7 @@ def attention(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, starts
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     p.q, p.out, p.pages = q.data_ptr(), out.data_ptr(), pages.data_ptr()
-    seqs = p.seqs
-    seqs.tables, seqs.starts = tables.data_ptr(), starts.data_ptr()
-    if cu_tokens is not None:
-        seqs.cu_tokens = cu_tokens.data_ptr()
+    _set_sequences(p.seqs, tables, starts, cu_tokens)
     p.max_seqlen = _int32(max_seqlen, "max_seqlen")
     need = needs.get(p.max_seqlen)
     if need is None:
@@ -268,10 +269,15 @@ def attention(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, starts
 def attend_workspace_bytes(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, starts: torch.Tensor, *,
                            max_seqlen: int, cu_tokens: Optional[torch.Tensor] = None, max_tokens: int = 1,
                            causal: bool = True, partition: int = 0) -> int:
-    """Workspace bytes ``attention`` needs for this geometry and these bounds."""
+    """Workspace bytes ``attention`` needs for this geometry and these bounds (0: none)."""
     p, _ = _attend_form(q, pages, tables, starts, cu_tokens, max_tokens, causal, None, None, partition)
+    _set_sequences(p.seqs, tables, starts, cu_tokens)
     p.max_seqlen = _int32(max_seqlen, "max_seqlen")
-    return int(_lib.load().hexkv_paged_attend_workspace_bytes(ctypes.byref(p)))
+    lib = _lib.load()
+    need = int(lib.hexkv_paged_attend_workspace_bytes(ctypes.byref(p)))
+    if not need and lib.hexkv_last_error():  # bounds that attention refuses, too
+        raise ValueError(lib.hexkv_last_error().decode())
+    return need
 
 
 def _copy_layers(pages_layers: TensorList, tables, lens, written: bool):
