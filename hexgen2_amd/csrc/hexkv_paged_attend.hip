@@ -53,8 +53,10 @@ struct PagedAttendArgs {
   // tile path: a bound on the tiles of all sequences, keys per partition and
   // partitions, and workgroups
   int32_t tiles, tile_part, tile_parts, tile_blocks, wide;
-  // split rows: [pair][row][max_parts] and [token][head][tile_parts] of D sums, and of
-  // (maximum, sum)
+  // split rows: of the row path [sequence][KV head][pair_rows][max_parts], or where tokens times heads
+  // are fewer (pair_rows 0) [token][head][max_parts], of the tile path [token][head][tile_parts]; each of D
+  // sums, and of (maximum, sum)
+  int32_t pair_rows;
   float *ws_o, *ws_ml, *ws_tile_o, *ws_tile_ml;
   unsigned int *status;
 };
@@ -88,6 +90,13 @@ __device__ __forceinline__ Rows rows_of(const PagedAttendArgs &a, int b) {
   r.total = static_cast<int>(min(all, static_cast<int64_t>(a.max_seqlen)));
   r.cut = s.count > a.max_tokens || all > a.max_seqlen;
   return r;
+}
+
+// The place of the row path's split row `row` of sequence b and KV head hk (its token t and head qh), less
+// its partitions.
+__device__ __forceinline__ int64_t few_slot(const PagedAttendArgs &a, int b, int hk, int row, int first, int t, int qh) {
+  return a.pair_rows ? (static_cast<int64_t>(b) * a.kv_heads + hk) * a.pair_rows + row
+                     : static_cast<int64_t>(first + t) * a.q_heads + qh;
 }
 
 // Workgroups of either path are numbered by (tile, partition, KV head), the
@@ -322,7 +331,6 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
   });
   const int b = mine.b, hk = mine.hk, part = mine.part, tile = mine.tile;
   if (b < 0) return;
-  const int pair = b * a.kv_heads + hk;
   const Rows seq = mine.seq;
   const int rows = seq.count * a.group, row0 = tile * 16;
   if (seq.cut && threadIdx.x == 0 && part == 0 && tile == 0) raise_status(a.status, HEXKV_STATUS_LENGTH_CLAMPED);
@@ -606,7 +614,7 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
       o[n] *= weight_of(sum[n]);
       store4(static_cast<T *>(a.out) + (seq.first + tt) * a.o_stride + static_cast<int64_t>(hh) * D + 4 * c, o[n]);
     } else {
-      const int64_t slot = ((static_cast<int64_t>(pair) * a.row_tiles + tile) * 16 + rr) * a.max_parts + part;
+      const int64_t slot = few_slot(a, b, hk, rrow, seq.first, tt, hh) * a.max_parts + part;
       *reinterpret_cast<f32x4 *>(a.ws_o + slot * D + 4 * c) = o[n];
       if (c == 0) *reinterpret_cast<float2 *>(a.ws_ml + slot * 2) = float2{top[n], sum[n]};
     }
@@ -623,7 +631,7 @@ __device__ __forceinline__ void rows_path(const PagedAttendArgs &a, int block, c
     if (lane * DPL >= D) continue;
     const bool split = rlen > a.part;
     T *out = static_cast<T *>(a.out) + (seq.first + tt) * a.o_stride + static_cast<int64_t>(hh) * D + lane * DPL;
-    const int64_t slot = ((static_cast<int64_t>(pair) * a.row_tiles + tile) * 16 + rr) * a.max_parts + part;
+    const int64_t slot = few_slot(a, b, hk, rrow, seq.first, tt, hh) * a.max_parts + part;
 #pragma unroll
     for (int e = 0; e < DPL; ++e) {
       if (split) a.ws_o[slot * D + lane * DPL + e] = eo[e];
@@ -1049,37 +1057,43 @@ __device__ __forceinline__ void join_row(const float *o_parts, const float *ml_p
   for (int e = 0; e < DPL; ++e) out[at + e] = Elem<T>::from_float(o[e] * inv);
 }
 
-// Rows of the row path first, `each` a sequence and KV head, then those of the tile
-// path, by token and head.
+// Rows that are numbered by sequence and KV head first (`few` of them), then those that are by token
+// and head.
 template <typename T, int D>
-__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAttendArgs a, int few, int each) {
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const PagedAttendArgs a, int few) {
   int id = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * (kJoinThreads / 64) + (threadIdx.x >> 6)));
+  int b, hk, row, t, qh;
+  Rows seq;
   if (id < few) {
-    const int pair = id / each, row = id - pair * each;
-    const int b = pair / a.kv_heads, hk = pair - b * a.kv_heads;
-    const Rows seq = rows_of(a, b);
-    const int rows = seq.count * a.group;
-    if (row >= rows || rows > a.few_rows) return;
-    const int t = row / a.group, qh = hk * a.group + row - t * a.group, len = seq.keys(a, t);
-    if (len <= a.part) return;
-    const int64_t slot = (static_cast<int64_t>(pair) * a.row_tiles * 16 + row) * a.max_parts;
-    join_row<T, D>(a.ws_o + slot * D, a.ws_ml + slot * 2, (len + a.part - 1) / a.part,
-                   static_cast<T *>(a.out) + (seq.first + t) * a.o_stride + static_cast<int64_t>(qh) * D);
-    return;
+    const int pair = id / a.pair_rows;
+    row = id - pair * a.pair_rows;
+    b = pair / a.kv_heads;
+    hk = pair - b * a.kv_heads;
+    seq = rows_of(a, b);
+    t = row / a.group;
+    qh = hk * a.group + row - t * a.group;
+    if (seq.count * a.group > a.few_rows) return;
+  } else {
+    id -= few;
+    const int token = id / a.q_heads;
+    if (token >= a.p.tokens) return;
+    qh = id - token * a.q_heads;
+    b = a.p.cu ? token_sequence(a.p, token) : token / a.p.each;
+    if (b < 0) return;
+    seq = rows_of(a, b);
+    t = token - seq.first;
+    hk = qh / a.group;
+    row = t * a.group + qh - hk * a.group;
+    if (a.pair_rows && seq.count * a.group <= a.few_rows) return;
   }
-  id -= few;
-  const int token = id / a.q_heads, qh = id - token * a.q_heads;
-  if (token >= a.p.tokens) return;
-  const int b = a.p.cu ? token_sequence(a.p, token) : token / a.p.each;
-  if (b < 0) return;
-  const Rows seq = rows_of(a, b);
-  const int t = token - seq.first;
-  if (t >= seq.count || seq.count * a.group <= a.few_rows) return;
-  const int len = seq.keys(a, t);
-  if (len <= a.tile_part) return;
-  const int64_t slot = static_cast<int64_t>(id) * a.tile_parts;
-  join_row<T, D>(a.ws_tile_o + slot * D, a.ws_tile_ml + slot * 2, (len + a.tile_part - 1) / a.tile_part,
-                 static_cast<T *>(a.out) + token * a.o_stride + static_cast<int64_t>(qh) * D);
+  if (t >= seq.count) return;
+  const bool tile = seq.count * a.group > a.few_rows;
+  const int len = seq.keys(a, t), part = tile ? a.tile_part : a.part;
+  if (len <= part) return;
+  const int64_t slot = tile ? (static_cast<int64_t>(seq.first + t) * a.q_heads + qh) * a.tile_parts
+                            : few_slot(a, b, hk, row, seq.first, t, qh) * a.max_parts;
+  join_row<T, D>((tile ? a.ws_tile_o : a.ws_o) + slot * D, (tile ? a.ws_tile_ml : a.ws_ml) + slot * 2, (len + part - 1) / part,
+                 static_cast<T *>(a.out) + (seq.first + t) * a.o_stride + static_cast<int64_t>(qh) * D);
 }
 
 // ------------------------------------------------------------------ host ---
@@ -1114,13 +1128,17 @@ static int64_t tile_partition(int64_t tiles, int64_t keys, int d, bool wide) {
   return std::max<int64_t>(64, round_up(ceil_div(keys, best), 64));
 }
 
-// Split rows of either path.
+// Rows of either path that may be split.
 static int64_t split_few(const PagedAttendArgs &a) {
-  return a.max_parts > 1 ? static_cast<int64_t>(a.p.batch) * a.kv_heads * a.row_tiles * 16 : 0;
+  if (a.max_parts <= 1) return 0;
+  return a.pair_rows ? static_cast<int64_t>(a.p.batch) * a.kv_heads * a.pair_rows : static_cast<int64_t>(a.p.tokens) * a.q_heads;
 }
 static int64_t split_tiled(const PagedAttendArgs &a) {
   return a.tile_parts > 1 ? static_cast<int64_t>(a.p.tokens) * a.q_heads : 0;
 }
+// Waves of the join: those numbered by sequence, and those by token.
+static int64_t joined_pairs(const PagedAttendArgs &a) { return a.pair_rows ? split_few(a) : 0; }
+static int64_t joined_tokens(const PagedAttendArgs &a) { return a.pair_rows ? split_tiled(a) : std::max(split_few(a), split_tiled(a)); }
 
 // Checks a call and fills its arguments but for addresses.
 static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs *a, const char *what) {
@@ -1185,6 +1203,7 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
     few_tiles = std::min(few_tiles, all_rows / 16 + std::min<int64_t>(batch, tokens));
     tiles = std::min(tiles, all_rows / tile_rows + std::min<int64_t>(batch, all_rows / (kFewRows + 1)));
   }
+  if ((few_tiles + tiles) * a->kv_heads >= INT64_C(1) << 24) return fail(HEXKV_ERANGE, "%s: 2^24 workgroups or more", what);
   // Partitions.  A CU alone takes 55 GB/s whatever its waves, so a row's keys are spread
   // over CUs, but for those of up to 128 KB of K, which end before a second
   // launch would have joined them (a step of 128 keys of 128 16-bit dims takes 1.15 us, the
@@ -1222,7 +1241,12 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
     a->max_parts = 1;
   }
   if (!tiled) a->tile_parts = 1;
-  if (split_few(*a) + split_tiled(*a) > INT32_MAX) return fail(HEXKV_ERANGE, "%s: 2^31 split rows or more", what);
+  // The row path's split rows by sequence, with room for the longest of them, or by token,
+  // with room for all: a chunk beside many single tokens (fp32, 32 heads on 8, 2048 tokens beside 63)
+  // has 67 552 rows, which by sequence would take 4.2 million places.
+  const int64_t by_token = tokens * p.q_heads, most = std::min<int64_t>(rows, a->few_rows);
+  a->pair_rows = batch * p.pool.kv_heads <= by_token && batch * p.pool.kv_heads * most <= by_token ? static_cast<int32_t>(most) : 0;
+  if (joined_pairs(*a) + joined_tokens(*a) >= INT64_C(1) << 26) return fail(HEXKV_ERANGE, "%s: 2^26 split rows or more", what);
   const int64_t row_blocks = few_tiles * a->kv_heads * a->max_parts, tile_blocks = tiles * a->kv_heads * a->tile_parts;
   if (row_blocks + tile_blocks >= INT64_C(1) << 24) return fail(HEXKV_ERANGE, "%s: 2^24 workgroups or more", what);
   a->row_blocks = static_cast<int32_t>(row_blocks);
@@ -1252,10 +1276,9 @@ static void launch_attend(const PagedAttendArgs &a, hipStream_t s) {
     else if (tiles && !a.wide) paged_tile_kernel<T, D, 4><<<dim3(tiles), 256, 0, s>>>(a);
   }
   if (!tiles) paged_rows_kernel<T, D><<<dim3(rows), 256, 0, s>>>(a);
-  const int each = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(a.max_tokens) * a.group, a.row_tiles * 16));
-  const int few = a.max_parts > 1 ? a.p.batch * a.kv_heads * each : 0;
-  const int64_t joined = few + split_tiled(a);
-  if (joined) paged_join_kernel<T, D><<<dim3(static_cast<unsigned>((joined + 3) / 4)), kJoinThreads, 0, s>>>(a, few, each);
+  const int64_t few = joined_pairs(a), joined = few + joined_tokens(a);
+  if (joined)
+    paged_join_kernel<T, D><<<dim3(static_cast<unsigned>((joined + 3) / 4)), kJoinThreads, 0, s>>>(a, static_cast<int>(few));
 }
 
 template <typename T>

@@ -27,6 +27,25 @@ def test_split_rows_have_a_workspace():
     assert sized(32, 8, 128, torch.bfloat16, [512], 8192, uniform=True, partition=4096) >= 512 * 32 * 2 * 130 * 4
 
 
+@pytest.mark.parametrize("hq,h,d,dtype", [(32, 8, 128, torch.float32), (32, 8, 32, torch.bfloat16), (8, 1, 16, torch.float16),
+                                          (32, 8, 128, torch.bfloat16), (4, 4, 256, torch.float16)])
+@pytest.mark.parametrize("new", [[2048] + [1] * 63, [512] + [1] * 63, [4096], [3, 700, 1, 1, 90], [1] * 300, [9] * 40])
+def test_the_workspace_grows_with_the_tokens(hq, h, d, dtype, new):
+    """Every row of every token split, on both of a launch's paths, is the most that is taken, however
+    long the longest sequence is; and of single tokens no more than they are."""
+    for options, parts in ((dict(partition=1024), 8), ({}, 32)):
+        paths = 2 if d >= 64 and dtype != torch.float32 and max(new) > 1 else 1
+        assert sized(hq, h, d, dtype, new, 8192, **options) <= paths * sum(new) * hq * parts * (d + 2) * 4
+
+
+def test_more_split_rows_than_a_launch_joins_are_refused():
+    # 2^21 tokens of 32 heads: 2^26 rows, a wave each, are 2^32 lanes
+    with pytest.raises(ValueError, match="2\\^26 split rows"):
+        sized(32, 2, 16, torch.float16, [1 << 21], 256, uniform=True, partition=128)
+    assert sized(32, 2, 16, torch.float16, [1 << 20], 256, uniform=True, partition=128) == (1 << 25) * 2 * 18 * 4
+
+
+
 def test_bounds_that_attention_refuses_have_no_size():
     with pytest.raises(ValueError, match="max_seqlen"):
         sized(8, 2, 64, torch.float16, [1], -1)
