@@ -1046,9 +1046,11 @@ __device__ __forceinline__ void join_row(const float *o_parts, const float *ml_p
     sum *= before;
 #pragma unroll
     for (int k = 0; k < kDepth; ++k) {
-      const float w = p0 + k >= parts || ml[k].x == -INFINITY ? 0.f : exp2_of(ml[k].x - top);
-      o += v[k] * w;
-      sum = fmaf(ml[k].y, w, sum);
+      // (copies of the last are left out, not weighed by 0, which makes a NaN of an infinite sum)
+      const bool part = p0 + k < parts;
+      const float w = !part || ml[k].x == -INFINITY ? 0.f : exp2_of(ml[k].x - top);
+      o += part ? v[k] * w : vd{};
+      sum = part ? fmaf(ml[k].y, w, sum) : sum;
     }
   }
   const float inv = weight_of(sum);
