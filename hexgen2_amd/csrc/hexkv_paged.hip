@@ -9,6 +9,7 @@
 #include "hexkv_paged.h"
 
 #include <algorithm>
+#include <vector>
 
 namespace hexkv {
 
@@ -327,6 +328,27 @@ static int launch_paged_copy(bool pack, const hexkv_pool &pool, const void *cons
   return check_launch(what);
 }
 
+// Whether layers of `read_bytes` from the addresses `read` and layers of `written_bytes` from those in
+// `written` lie apart, and the written ones from each other (pools, whose pages may lie in turn: whether they
+// start apart).
+static bool layers_apart(const void *const *read, int64_t read_bytes, void *const *written, int64_t written_bytes, int n, bool pack) {
+  std::vector<uintptr_t> r(n), w(n);
+  for (int l = 0; l < n; ++l) {
+    r[l] = reinterpret_cast<uintptr_t>(read[l]);
+    w[l] = reinterpret_cast<uintptr_t>(written[l]);
+  }
+  std::sort(r.begin(), r.end());
+  std::sort(w.begin(), w.end());
+  for (int l = 1; l < n; ++l)
+    if (w[l] - w[l - 1] < static_cast<uintptr_t>(pack ? written_bytes : 1)) return false;
+  for (int i = 0, j = 0; i < n && j < n;) {
+    if (r[i] + read_bytes <= w[j]) ++i;
+    else if (w[j] + written_bytes <= r[i]) ++j;
+    else return false;
+  }
+  return true;
+}
+
 static int paged_copy(bool pack, const hexkv_pool *pool, const void *const *src, void *const *dst, int n_layers,
                       const int32_t *tables, int64_t table_stride, int table_width, int batch, const int64_t *lens,
                       hexkv_stream_t stream) {
@@ -358,6 +380,9 @@ static int paged_copy(bool pack, const hexkv_pool *pool, const void *const *src,
   int rows = pool->page_size;
   while (rows > 1 && rows * row_bytes > share) rows /= 2;
   if (total / rows + batch >= 1 << 22) return fail(HEXKV_ERANGE, "%s: 2^22 workgroups a layer or more", what);
+  const int64_t pool_size = pool_bytes(*pool), packed_size = total * row_bytes;
+  if (!layers_apart(src, pack ? pool_size : packed_size, dst, pack ? packed_size : pool_size, n_layers, pack))
+    return fail(HEXKV_EINVAL, "%s: a layer that is written overlaps another, or one that is read", what);
   unsigned int *status = nullptr;
   rc = status_word(stream, &status, what);
   if (rc != HEXKV_OK) return rc;

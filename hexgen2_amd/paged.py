@@ -330,7 +330,8 @@ def pack_live(pages_layers: TensorList, tables: torch.Tensor, lens: Sequence[int
     """``ops.pack_live`` of a paged cache: rows ``[0, lens[b])`` of every sequence
     of every layer into the handoff layout ``[n_layers, sum(lens), 2, kv_heads,
     head_dim]``, one launch.  ``pages_layers``: the layers' pools, a list or stacked,
-    with one ``tables`` for all.  The rows of a page outside the pool come out as zeros."""
+    with one ``tables`` for all.  The rows of a page outside the pool come out as zeros.
+    ``out`` must not overlap the pools."""
     first, ptrs, pool, lens = _copy_layers(pages_layers, tables, lens, False)
     if out is None:
         out = first.new_empty((len(ptrs), sum(lens), 2, pool.kv_heads, pool.head_dim))

@@ -861,9 +861,10 @@ size_t hexkv_paged_attend_workspace_bytes(const hexkv_paged_attend_params *param
  * hexkv_pack / hexkv_unpack for pools: rows [0, lens[b]) of every sequence of
  * every layer between the pages and [sum(lens)][2][kv_heads][head_dim] per
  * layer, one launch for up to HEXKV_MAX_LAYERS_PER_LAUNCH layers that share
- * the tables.  `pages` and `packed` are host arrays of device addresses; what is
- * written must not overlap what is read, and no two sequences of an unpack share a
- * page below their lengths.  Rows of a page outside the pool are packed as zeros,
+ * the tables.  `pages` and `packed` are host arrays of device addresses.  A layer that
+ * is written and overlaps another, or one that is read, is refused (each counted from its first
+ * byte to its last; pools that are written may lie in turn, page by page, but not start at the same
+ * address); no two sequences of an unpack share a page below their lengths.  Rows of a page outside the pool are packed as zeros,
  * not unpacked, and flagged HEXKV_STATUS_PAGE.
  */
 int hexkv_paged_pack(const hexkv_pool *pool, const void *const *pages, void *const *packed, int n_layers,
