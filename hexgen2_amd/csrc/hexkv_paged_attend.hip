@@ -1250,7 +1250,8 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   a->pair_rows = batch * p.pool.kv_heads <= by_token && batch * p.pool.kv_heads * most <= by_token ? static_cast<int32_t>(most) : 0;
   if (joined_pairs(*a) + joined_tokens(*a) >= INT64_C(1) << 26) return fail(HEXKV_ERANGE, "%s: 2^26 split rows or more", what);
   const int64_t row_blocks = few_tiles * a->kv_heads * a->max_parts, tile_blocks = tiles * a->kv_heads * a->tile_parts;
-  if (row_blocks + tile_blocks >= INT64_C(1) << 24) return fail(HEXKV_ERANGE, "%s: 2^24 workgroups or more", what);
+  if ((row_blocks + tile_blocks) * (a->wide ? 512 : 256) >= INT64_C(1) << 32)
+    return fail(HEXKV_ERANGE, "%s: workgroups of 2^32 lanes or more", what);
   a->row_blocks = static_cast<int32_t>(row_blocks);
   a->tiles = static_cast<int32_t>(tiles);
   a->tile_blocks = static_cast<int32_t>(tile_blocks);
