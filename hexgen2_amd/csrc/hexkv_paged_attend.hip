@@ -1151,7 +1151,9 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   const int d = p.pool.head_dim, vec = 16 / elem_bytes(p.pool.dtype);
   if (p.q_heads < 1 || p.q_heads > 1 << 16 || p.q_heads % p.pool.kv_heads)
     return fail(HEXKV_EINVAL, "%s: %d query heads on %d KV heads", what, p.q_heads, p.pool.kv_heads);
-  if (!(p.softmax_scale > 0.f) || p.softmax_scale > 3e38f) return fail(HEXKV_EINVAL, "%s: softmax_scale is not positive", what);
+  a->scale_log2 = p.softmax_scale * 1.44269504f;
+  if (!(p.softmax_scale > 0.f) || a->scale_log2 > 3e38f)
+    return fail(HEXKV_EINVAL, "%s: softmax_scale is not positive, or above 2e38", what);
   if (p.max_seqlen < 0 || p.max_seqlen > static_cast<int64_t>(p.seqs.table_width) * p.pool.page_size)
     return fail(HEXKV_ERANGE, "%s: max_seqlen %d outside the tables' [0, %lld]", what, p.max_seqlen,
                 static_cast<long long>(p.seqs.table_width) * p.pool.page_size);
@@ -1174,7 +1176,6 @@ static int fill_attend(const hexkv_paged_attend_params *params, PagedAttendArgs 
   a->max_seqlen = p.max_seqlen;
   a->page_bytes = static_cast<uint32_t>(p.pool.page_stride * elem_bytes(p.pool.dtype));
   a->pos_bytes = static_cast<uint32_t>(p.pool.pos_stride * elem_bytes(p.pool.dtype));
-  a->scale_log2 = p.softmax_scale * 1.44269504f;
   const int64_t rows = static_cast<int64_t>(a->max_tokens) * a->group;
   if (rows > INT32_MAX - 256) return fail(HEXKV_ERANGE, "%s: 2^31 rows or more", what);
   // Which paths can have work: without cu_tokens every sequence has as many rows.

@@ -835,7 +835,7 @@ typedef struct hexkv_paged_attend_params {
   hexkv_paged_batch seqs;
   int q_heads;            /* a multiple of kv_heads */
   int causal;             /* 1: token i of a sequence sees its first starts + i + 1 rows; 0: all of starts + count */
-  float softmax_scale;    /* above 0 */
+  float softmax_scale;    /* above 0, up to 2e38 */
   int32_t max_tokens;     /* bound on a sequence's new tokens (with cu_tokens) */
   int32_t max_seqlen;     /* bound on a sequence's rows, its new ones included */
   const void *q;          /* [tokens][q_heads][head_dim], rows 16-byte aligned */

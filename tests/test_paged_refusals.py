@@ -1,6 +1,8 @@
 """Calls of attention over pages that are refused before anything runs."""
 import ctypes
 
+import pytest
+
 from hexgen2_amd import _lib
 from tests.test_paged_host import attend_params, pool, refused, seqs
 
@@ -13,3 +15,10 @@ def test_launches_of_2_to_the_32_lanes_and_more_are_refused():
     refused(lambda lib: lib.hexkv_paged_attend(ctypes.byref(p), None, 0, None), _lib.HEXKV_ERANGE, "2\\^32 lanes")
     p.partition = 128
     refused(lambda lib: lib.hexkv_paged_attend(ctypes.byref(p), None, 0, None), _lib.HEXKV_EWORKSPACE, "workspace")
+
+
+@pytest.mark.parametrize("scale", [3.4e38, 2.4e38, 2.36e38])
+def test_scales_that_no_float_holds_in_powers_of_two_are_refused(scale):
+    """Scores are taken in powers of two: a scale whose product with log2(e) is infinite would make every score so."""
+    refused(lambda lib: lib.hexkv_paged_attend(ctypes.byref(attend_params(softmax_scale=scale)), None, 0, None),
+            _lib.HEXKV_EINVAL, "softmax_scale")
