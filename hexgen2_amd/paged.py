@@ -232,8 +232,9 @@ def attention(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor, starts
     Token i of a sequence sees its first ``starts + i + 1`` rows, without ``causal``
     all that the sequence has.  ``max_seqlen`` bounds a sequence's rows and, with ``cu_tokens``,
     ``max_tokens`` its new tokens: both are host values that size the launch.
-    Softmax sums are fp32.  ``out`` may be ``q``; tokens of no sequence are left as they
-    were in it, those of a sequence not in use become zero.  ``partition``: rows
+    Softmax sums are fp32.  ``out`` may be ``q``; tokens of no sequence, and those past
+    ``max_tokens`` of one (flagged, but for ``max_tokens`` 0, which launches nothing), are left as they
+    were in it (and are not defined in a fresh one), those of a sequence not in use become zero.  ``partition``: rows
     per partition of a split row, a multiple of 64 (0: the library's choice); ``workspace``:
     scratch that no overlapping call shares (default: one of this call's own)."""
     softmax_scale = None if softmax_scale is None else float(softmax_scale)

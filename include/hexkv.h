@@ -850,8 +850,9 @@ typedef struct hexkv_paged_attend_params {
  * Attention of the new tokens over their sequences' rows in the pages, their
  * own (already appended) included: decode rows, chunks of prompts and both in
  * one call.  A sequence with more than max_tokens tokens or max_seqlen rows is
- * cut to them and flagged HEXKV_STATUS_LENGTH_CLAMPED.  A row that attends
- * nothing, or only scores of -infinity, is zero.
+ * cut to them and flagged HEXKV_STATUS_LENGTH_CLAMPED; what out holds for the tokens cut
+ * off is left as it was.  A row that attends nothing, or only scores of -infinity, is zero.
+ * With tokens, batch or max_tokens 0 there are no tokens: nothing is launched, and nothing flagged.
  */
 int hexkv_paged_attend(const hexkv_paged_attend_params *params, void *workspace, size_t workspace_bytes,
                        hexkv_stream_t stream);
