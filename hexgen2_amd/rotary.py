@@ -2,7 +2,9 @@
 and ``ops.norm_rope_linear`` turn q and k by.
 
 The reference rotates by ``1 / base ** (2 j / dim)`` alone and refuses scaled
-rotation (hexgen2/model.py:37-38); long-context models scale it.
+rotation (hexgen2/model.py:37-38); long-context models scale it.  ``paged.append``
+takes the angle of a far position in 64 bits; ``ops.rope_split`` and
+``ops.norm_rope_linear`` take position * frequency in fp32, off by up to 2^-24 of it.
 """
 from __future__ import annotations
 
