@@ -9,7 +9,8 @@
 #include "hexkv_paged.h"
 
 #include <algorithm>
-#include <vector>
+#include <memory>
+#include <new>
 
 namespace hexkv {
 
@@ -330,15 +331,15 @@ static int launch_paged_copy(bool pack, const hexkv_pool &pool, const void *cons
 
 // Whether layers of `read_bytes` from the addresses `read` and layers of `written_bytes` from those in
 // `written` lie apart, and the written ones from each other (pools, whose pages may lie in turn: whether they
-// start apart).
-static bool layers_apart(const void *const *read, int64_t read_bytes, void *const *written, int64_t written_bytes, int n, bool pack) {
-  std::vector<uintptr_t> r(n), w(n);
+// start apart).  r, w: room for n addresses each.
+static bool layers_apart(const void *const *read, int64_t read_bytes, void *const *written, int64_t written_bytes, int n, bool pack,
+                         uintptr_t *r, uintptr_t *w) {
   for (int l = 0; l < n; ++l) {
     r[l] = reinterpret_cast<uintptr_t>(read[l]);
     w[l] = reinterpret_cast<uintptr_t>(written[l]);
   }
-  std::sort(r.begin(), r.end());
-  std::sort(w.begin(), w.end());
+  std::sort(r, r + n);
+  std::sort(w, w + n);
   for (int l = 1; l < n; ++l)
     if (w[l] - w[l - 1] < static_cast<uintptr_t>(pack ? written_bytes : 1)) return false;
   for (int i = 0, j = 0; i < n && j < n;) {
@@ -381,7 +382,15 @@ static int paged_copy(bool pack, const hexkv_pool *pool, const void *const *src,
   while (rows > 1 && rows * row_bytes > share) rows /= 2;
   if (total / rows + batch >= 1 << 22) return fail(HEXKV_ERANGE, "%s: 2^22 workgroups a layer or more", what);
   const int64_t pool_size = pool_bytes(*pool), packed_size = total * row_bytes;
-  if (!layers_apart(src, pack ? pool_size : packed_size, dst, pack ? packed_size : pool_size, n_layers, pack))
+  uintptr_t few[2 * HEXKV_MAX_LAYERS_PER_LAUNCH];
+  std::unique_ptr<uintptr_t[]> many;
+  if (n_layers > HEXKV_MAX_LAYERS_PER_LAUNCH) {
+    many.reset(new (std::nothrow) uintptr_t[2 * static_cast<size_t>(n_layers)]);
+    if (!many) return fail(HEXKV_ERANGE, "%s: no memory for the addresses of %d layers", what, n_layers);
+  }
+  uintptr_t *sorted = many ? many.get() : few;
+  if (!layers_apart(src, pack ? pool_size : packed_size, dst, pack ? packed_size : pool_size, n_layers, pack, sorted,
+                    sorted + n_layers))
     return fail(HEXKV_EINVAL, "%s: a layer that is written overlaps another, or one that is read", what);
   unsigned int *status = nullptr;
   rc = status_word(stream, &status, what);

@@ -35,6 +35,13 @@ def test_layers_that_are_written_must_lie_apart():
     refused(copy("hexkv_paged_unpack", [PAGES, PAGES + POOL, PAGES], [QKV] * 3), _lib.HEXKV_EINVAL, "overlaps")
 
 
+@pytest.mark.parametrize("name", ["hexkv_paged_pack", "hexkv_paged_unpack"])
+def test_overlaps_among_more_layers_than_a_launch_takes(name):
+    pages = [PAGES + (i * 73 % 200) * POOL for i in range(200)]
+    packed = [QKV + i * PACKED for i in range(199)]
+    refused(copy(name, pages, packed + [PAGES + 150 * POOL + 16]), _lib.HEXKV_EINVAL, "overlaps")
+
+
 @pytest.mark.gpu
 def test_layers_side_by_side_and_on_top_of_each_other(device):
     """One allocation holds pools and packets: next to each other they are copied, a byte over they are refused."""
