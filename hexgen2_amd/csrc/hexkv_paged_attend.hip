@@ -22,7 +22,7 @@
 // 32 rows a wave, four or eight waves a workgroup (128 or 256 rows), which share tiles of
 // 16 keys a wave in LDS; the same products on 32 x 32 x 16 matrix instructions.  What
 // bounds it: the matrix cores, the LDS reads of their operands, and the softmax on the
-// VALU beside them (2048 rows over 8192 keys, 32 heads of 128 on 8: 432 us, 715 TFLOP/s,
+// VALU beside them (2048 rows over 8192 keys, 32 heads of 128 on 8: 424 us, 729 TFLOP/s,
 // the second terms' products not counted).  A probability enters P V as hi + lo here too:
 // one rounded term takes 316 us, but its error is half a step of the type, as much as the
 // output's own rounding.
